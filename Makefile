@@ -8,8 +8,9 @@ ROCM     ?= /opt/rocm
 CXXFLAGS  = -O3 -std=c++17 -fPIC -fopenmp -Wall -Wextra -Wno-unused-parameter \
             -Icpp/include -MMD -MP
 HIPFLAGS  = --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Icpp/include -Wall \
+            -Xclang -target-feature -Xclang -packed-fp32-ops \
             -Wno-unused-parameter -MMD -MP
-LDFLAGS   = -shared -fopenmp -L$(ROCM)/lib -Wl,-rpath,$(ROCM)/lib
+LDFLAGS   = -shared -fopenmp -Wl,-rpath,$(ROCM)/lib
 
 BUILD    := build
 LIBDIR   := lightgbm_amd/lib
@@ -26,8 +27,14 @@ ifeq ($(strip $(HIP_OBJS)),)
   LINKER = $(CXX)
   EXTRA_LIBS =
 else
-  LINKER = $(HIPCC)
-  EXTRA_LIBS = -lamdhip64 -lrccl
+  # The HIP and HSA runtimes are needed by their plain names, as torch's libraries need theirs:
+  # whichever is loaded first serves both, in either order of import. With the versioned names
+  # a process that imports torch second would hold two runtimes, of which the later one finds
+  # no device. Empty libraries without a soname stand in for them at link time.
+  LINKER = $(HIPCC) -no-hip-rt
+  STUBS = $(BUILD)/stub/libamdhip64.so $(BUILD)/stub/libhsa-runtime64.so
+  EXTRA_LIBS = -Wl,--no-as-needed -L$(BUILD)/stub -lamdhip64 -lhsa-runtime64 \
+               -L$(ROCM)/lib -lrccl
 endif
 
 CLI := lightgbm_amd/bin/migbm
@@ -48,7 +55,11 @@ $(BUILD)/%.o: cpp/src/%.cpp | $(BUILD)
 $(BUILD)/hip/%.o: cpp/src/hip/%.hip.cpp | $(BUILD)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
-$(TARGET): $(HOST_OBJS) $(HIP_OBJS) | $(BUILD)
+$(STUBS): | $(BUILD)
+	mkdir -p $(BUILD)/stub
+	$(CXX) -shared -nostdlib -x c /dev/null -o $@
+
+$(TARGET): $(HOST_OBJS) $(HIP_OBJS) $(STUBS) | $(BUILD)
 	$(LINKER) $(LDFLAGS) $(HOST_OBJS) $(HIP_OBJS) $(EXTRA_LIBS) -o $@
 
 # ---- ASAN lane: host-only (no HIP) CLI under AddressSanitizer.
