@@ -24,6 +24,9 @@ typedef void* BoosterHandle;
 #define C_API_DTYPE_FLOAT64 (1)
 #define C_API_DTYPE_INT32 (2)
 #define C_API_DTYPE_INT64 (3)
+/* class-score operators only */
+#define C_API_DTYPE_FLOAT16 (4)
+#define C_API_DTYPE_BFLOAT16 (5)
 
 #define C_API_PREDICT_NORMAL (0)
 #define C_API_PREDICT_RAW_SCORE (1)
@@ -326,5 +329,66 @@ LIGHTGBM_C_EXPORT int LGBM_NetworkFree();
 LIGHTGBM_C_EXPORT int LGBM_NetworkInitWithFunctions(int num_machines, int rank,
                                                     void* reduce_scatter_ext_fun,
                                                     void* allgather_ext_fun);
+
+// ---- operators over class scores (no counterpart in the reference)
+/*! a strided array: strides count elements; data == NULL where an optional one is absent.
+ *  Of a two-dimensional array stride[2] is not read, of a vector stride[1] neither. */
+typedef struct {
+  void* data;
+  int64_t stride[3];
+  int32_t type;  // C_API_DTYPE_*
+  int32_t reserved;
+} LGBM_Array;
+
+typedef struct {
+  int64_t rows;
+  int32_t classes;
+  int32_t k;            // 1 .. min(classes, 256)
+  double temperature;   // of log_rest
+  LGBM_Array scores;    // [rows, classes], a floating type
+  LGBM_Array top_class; // out [rows, k], int32
+  LGBM_Array top_logit; // out [rows, k], the scores' type
+  LGBM_Array log_rest;  // out [rows], optional; float64 for float64 scores, else float32
+} LGBM_TopLogitsArgs;
+
+typedef struct {
+  int64_t rows;
+  int32_t classes;
+  int32_t k;                // teacher slots a row, 1 .. 256
+  double temperature;
+  double alpha;             // weight of the teacher's term; 1 - alpha is the labels'
+  LGBM_Array scores;        // [rows, classes], a floating type
+  LGBM_Array teacher_class; // [rows, k], int32 or int64; outside 0..classes-1: an empty slot
+  LGBM_Array teacher_logit; // [rows, k], a floating type
+  LGBM_Array teacher_rest;  // [rows], optional
+  LGBM_Array label;         // [rows], integer or float32; needed where alpha < 1
+  LGBM_Array weight;        // [rows], optional, a floating type
+  LGBM_Array loss;          // out [rows], optional; float64 for float64 scores, else float32
+  LGBM_Array gradient;      // out [rows, classes], optional; float32 for float64 scores,
+  LGBM_Array hessian;       // else the scores' type
+} LGBM_DistillArgs;
+
+typedef struct {
+  int64_t rows;             // sequences
+  int32_t classes;
+  int32_t drafts;           // drafted classes a sequence at most, 1 .. 1024
+  LGBM_Array target;        // [rows, drafts + 1, classes] probabilities, a floating type
+  LGBM_Array draft_prob;    // [rows, drafts, classes], optional, the target's type
+  LGBM_Array draft_class;   // [rows, drafts], int32 or int64
+  LGBM_Array accept;        // [rows, drafts] uniform numbers, float32 or float64
+  LGBM_Array sample;        // [rows] uniform numbers, float32 or float64
+  LGBM_Array length;        // [rows], optional, int32 or int64: drafts of each sequence
+  LGBM_Array out_class;     // out [rows, drafts + 1], int32
+  LGBM_Array out_accepted;  // out [rows], int32
+  void* workspace;          // LGBM_VerifyDraftsWorkspace bytes on the device
+  int64_t workspace_bytes;
+} LGBM_VerifyArgs;
+
+/*! All three: device < 0 takes host memory, otherwise every array is in that HIP device's
+ *  memory and the work is enqueued on `stream` (a hipStream_t) without waiting. */
+LIGHTGBM_C_EXPORT int LGBM_TopLogits(const LGBM_TopLogitsArgs* args, int device, void* stream);
+LIGHTGBM_C_EXPORT int LGBM_Distill(const LGBM_DistillArgs* args, int device, void* stream);
+LIGHTGBM_C_EXPORT int LGBM_VerifyDrafts(const LGBM_VerifyArgs* args, int device, void* stream);
+LIGHTGBM_C_EXPORT int LGBM_VerifyDraftsWorkspace(const LGBM_VerifyArgs* args, int64_t* out_bytes);
 
 #endif  // MIGBM_C_API_H_

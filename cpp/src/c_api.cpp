@@ -12,6 +12,8 @@
 #include "migbm/network.h"
 #include "migbm/objective.h"
 
+#include "migbm/class_ops.h"
+
 #include <mutex>
 #include <string>
 
@@ -1598,6 +1600,30 @@ void AllgatherBridge(const char* input, int input_size, char* output) {
                   output, input_size * world);
 }
 }  // namespace
+
+int LGBM_TopLogits(const LGBM_TopLogitsArgs* args, int device, void* stream) {
+  API_BEGIN();
+  class_ops::TopLogits(*args, device, stream);
+  API_END();
+}
+
+int LGBM_Distill(const LGBM_DistillArgs* args, int device, void* stream) {
+  API_BEGIN();
+  class_ops::Distill(*args, device, stream);
+  API_END();
+}
+
+int LGBM_VerifyDrafts(const LGBM_VerifyArgs* args, int device, void* stream) {
+  API_BEGIN();
+  class_ops::VerifyDrafts(*args, device, stream);
+  API_END();
+}
+
+int LGBM_VerifyDraftsWorkspace(const LGBM_VerifyArgs* args, int64_t* out_bytes) {
+  API_BEGIN();
+  *out_bytes = class_ops::VerifyWorkspace(*args);
+  API_END();
+}
 
 int LGBM_NetworkInit(const char* machines, int local_listen_port, int listen_time_out,
                      int num_machines) {

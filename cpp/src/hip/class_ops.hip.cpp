@@ -1,0 +1,691 @@
+/*!
+ * Device operators over class scores for MI355X (gfx950): top logits, the distillation loss
+ * with its gradient, and the verification of drafted classes.
+ *
+ * A workgroup owns a row (or a sequence). Everything is held in 32 bits (64 for float64
+ * scores); exponentials are taken to base two of one fused multiply-add,
+ *   exp((z - high) / T) = 2^(z * s - high * s),  s = log2(e) / T,
+ * whose rounding of high * s is a factor common to the row and cancels in every quotient.
+ */
+#include <hip/hip_runtime.h>
+
+#include "migbm/class_ops.h"
+#include "migbm/common.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace migbm {
+namespace class_ops {
+namespace {
+
+#define OPS_HIP_OK(call)                                                                 \
+  do {                                                                                   \
+    hipError_t _e = (call);                                                              \
+    if (_e != hipSuccess)                                                                \
+      ::migbm::Log::Fatal("HIP error %s at %s:%d", hipGetErrorString(_e), __FILE__,      \
+                          __LINE__);                                                     \
+  } while (0)
+
+// ------------------------------------------------------------------ elements
+/*! what a row of T is computed in: 64 bits for float64 scores, 32 for the others */
+template <typename T> using Acc = std::conditional_t<std::is_same_v<T, double>, double, float>;
+/*! the type of gradients: the framework's 32-bit gradient for float64 scores */
+template <typename T> using Out = std::conditional_t<std::is_same_v<T, double>, float, T>;
+
+template <typename A> __device__ __forceinline__ A NegInf() { return -static_cast<A>(INFINITY); }
+__device__ __forceinline__ float Exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ double Exp2(double x) { return exp2(x); }
+__device__ __forceinline__ float Log2(float x) { return log2f(x); }
+__device__ __forceinline__ double Log2(double x) { return log2(x); }
+__device__ __forceinline__ float Fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double Fma(double a, double b, double c) { return fma(a, b, c); }
+__device__ __forceinline__ float Max(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double Max(double a, double b) { return fmax(a, b); }
+
+template <typename T> __device__ __forceinline__ T At(const LGBM_Array& a, int64_t at) {
+  return static_cast<const T*>(a.data)[at];
+}
+
+/*! one of the small arrays (teacher, weights): its type is the same for the whole launch */
+template <typename A> __device__ __forceinline__ A LoadFloat(const LGBM_Array& a, int64_t at) {
+  switch (a.type) {
+    case C_API_DTYPE_FLOAT64: return static_cast<A>(At<double>(a, at));
+    case C_API_DTYPE_FLOAT32: return static_cast<A>(At<float>(a, at));
+    case C_API_DTYPE_FLOAT16: return static_cast<A>(At<_Float16>(a, at));
+    default: return static_cast<A>(static_cast<float>(At<__bf16>(a, at)));
+  }
+}
+
+/*! a class id in 0..classes-1, or -1; float32 labels are whole numbers held in a float */
+__device__ __forceinline__ int LoadClass(const LGBM_Array& a, int64_t at, int classes) {
+  int64_t v;
+  if (a.type == C_API_DTYPE_INT32) {
+    v = At<int32_t>(a, at);
+  } else if (a.type == C_API_DTYPE_INT64) {
+    v = At<int64_t>(a, at);
+  } else {
+    const float f = At<float>(a, at);
+    v = f >= 0.0f && f < 4e9f ? static_cast<int64_t>(f) : -1;
+  }
+  return v >= 0 && v < classes ? static_cast<int>(v) : -1;
+}
+
+template <typename A>
+__device__ __forceinline__ void StoreFloat(const LGBM_Array& a, int64_t at, A v) {
+  if (a.type == C_API_DTYPE_FLOAT64) static_cast<double*>(a.data)[at] = v;
+  else static_cast<float*>(a.data)[at] = static_cast<float>(v);
+}
+
+// ------------------------------------------------------------------ reductions
+constexpr int kWave = 64;
+
+template <typename A> __device__ __forceinline__ A WaveSum(A v) {
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+template <typename A> __device__ __forceinline__ A WaveMax(A v) {
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) v = Max(v, __shfl_xor(v, d));
+  return v;
+}
+
+/*! sums (maxima) over the workgroup, known to every thread, always in the same order.
+ *  `lds` has one place a wave; it may be used again after the next barrier. */
+template <int kBlock, typename A> __device__ __forceinline__ A BlockSum(A v, A* lds) {
+  v = WaveSum(v);
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  A s = lds[0];
+#pragma unroll
+  for (int i = 1; i < kBlock / kWave; ++i) s += lds[i];
+  return s;
+}
+template <int kBlock, typename A> __device__ __forceinline__ A BlockMax(A v, A* lds) {
+  v = WaveMax(v);
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  A s = lds[0];
+#pragma unroll
+  for (int i = 1; i < kBlock / kWave; ++i) s = Max(s, lds[i]);
+  return s;
+}
+
+// ------------------------------------------------------------------ distillation, any strides
+constexpr double kLog2e = 1.4426950408889634074;
+constexpr double kLn2 = 0.69314718055994530942;
+
+/*! where the student's share of the unnamed classes is below this, it is summed again
+ *  against its own maximum: 2^-100 of the row's largest term is near the end of 32 bits */
+template <typename A> __device__ __forceinline__ A SmallRest() { return static_cast<A>(0x1p-100); }
+
+/*!
+ * One workgroup a row, the row read from memory in each of its passes: maximum, sums,
+ * gradients. With the teacher's slots (class c_j, logit t_j) and, where given, the
+ * logarithm r of what it gives to all other classes,
+ *   P = softmax(t_1 / T, .., t_k / T, r),  Q = softmax(z / T),  rho = sum of Q over the others,
+ *   loss = w * (alpha T^2 (sum_j P_j log(P_j / Q_cj) + P_r log(P_r / rho))
+ *               + (1 - alpha) (-log softmax(z)_y)),
+ *   dloss / dz_c = w * (alpha T (Q_c - P_c) + (1 - alpha)(softmax(z)_c - [c = y])),
+ *     where P_c = P_r Q_c / rho for a class without a slot,
+ *   hessian_c = w * C / (C - 1) * (alpha Q_c (1 - Q_c) + (1 - alpha) p_c (1 - p_c)).
+ * The slots' classes are bits in LDS, so that the sum over the others is taken directly and
+ * not as a difference, which a confident student would cancel to nothing. The first slot of
+ * a class counts.
+ */
+template <typename T, int kBlock>
+__global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
+  using A = Acc<T>;
+  extern __shared__ uint32_t mark[];
+  __shared__ int s_cls[kMaxTop];
+  __shared__ A s_red[6][kBlock / kWave];
+  __shared__ int s_dup;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, c = a.classes, k = a.k;
+  const T* z = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+  const int64_t zs = a.scores.stride[1];
+  using O = Out<T>;
+  O* grad = a.gradient.data ? static_cast<O*>(a.gradient.data) + row * a.gradient.stride[0]
+                            : nullptr;
+  O* hess = a.hessian.data ? static_cast<O*>(a.hessian.data) + row * a.hessian.stride[0]
+                           : nullptr;
+  const int64_t gs = a.gradient.stride[1], hs = a.hessian.stride[1];
+  const A w = a.weight.data ? LoadFloat<A>(a.weight, row * a.weight.stride[0]) : A(1);
+  const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
+  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
+
+  for (int i = tid; i < (c + 31) / 32; i += kBlock) mark[i] = 0;
+  if (tid == 0) s_dup = 0;
+  A high = NegInf<A>();
+  bool nan = false;
+  if (w != A(0)) {
+    for (int i = tid; i < c; i += kBlock) {
+      const A v = static_cast<A>(z[i * zs]);
+      high = Max(high, v);
+      nan |= v != v;
+    }
+  }
+  high = BlockMax<kBlock>(high, s_red[0]);
+  nan = __syncthreads_or(nan);
+  // a row without weight, or with every class masked, has no loss and no gradient
+  if (w == A(0) || (high == NegInf<A>() && !nan)) {
+    if (a.loss.data && tid == 0) StoreFloat(a.loss, row * a.loss.stride[0], A(0));
+    for (int i = tid; i < c; i += kBlock) {
+      if (grad) grad[i * gs] = static_cast<O>(0.0f);
+      if (hess) hess[i * hs] = static_cast<O>(0.0f);
+    }
+    return;
+  }
+  if (high == NegInf<A>()) high = A(0);
+
+  // the slots, one a thread
+  int cls = -1;
+  if (tid < k) {
+    cls = LoadClass(a.teacher_class,
+                    row * a.teacher_class.stride[0] + tid * a.teacher_class.stride[1], c);
+    if (cls >= 0 && (atomicOr(&mark[cls >> 5], 1u << (cls & 31)) >> (cls & 31) & 1u)) s_dup = 1;
+    s_cls[tid] = cls;
+  }
+  __syncthreads();
+  if (s_dup && tid < k) {
+    for (int i = 0; i < tid; ++i)
+      if (s_cls[i] == cls) cls = -1;
+  }
+  const A logit = cls >= 0 ? scale * LoadFloat<A>(a.teacher_logit,
+                                                  row * a.teacher_logit.stride[0] +
+                                                      tid * a.teacher_logit.stride[1])
+                           : NegInf<A>();
+  const bool rest = a.teacher_rest.data != nullptr;
+  const A r = rest ? scale1 * LoadFloat<A>(a.teacher_rest, row * a.teacher_rest.stride[0])
+                   : NegInf<A>();
+  const A t_high_or = BlockMax<kBlock>(Max(logit, r), s_red[1]);
+  const bool t_nan = __syncthreads_or(logit != logit || r != r);
+  const bool taught = alpha > A(0) && (t_high_or > NegInf<A>() || t_nan);
+  const A t_high = t_high_or > NegInf<A>() ? t_high_or : A(0);
+
+  // sums
+  const A off = -high * scale, off1 = -high * scale1;
+  const A z_slot = cls >= 0 ? static_cast<A>(z[cls * zs]) : NegInf<A>();
+  const A log_e = Fma(z_slot, scale, off);
+  const A e_slot = cls >= 0 ? Exp2(log_e) : A(0);
+  A left = 0, total1 = 0;
+  for (int i = tid; i < c; i += kBlock) {
+    const A v = static_cast<A>(z[i * zs]);
+    if (!(mark[i >> 5] >> (i & 31) & 1u)) left += Exp2(Fma(v, scale, off));
+    if (alpha < A(1)) total1 += Exp2(Fma(v, scale1, off1));
+  }
+  left = BlockSum<kBlock>(left, s_red[0]);
+  const A total = left + BlockSum<kBlock>(e_slot, s_red[2]);
+  if (alpha < A(1)) total1 = BlockSum<kBlock>(total1, s_red[3]);
+  const A u = logit > NegInf<A>() || logit != logit ? Exp2(logit - t_high) : A(0);
+  const A u_rest = rest ? Exp2(r - t_high) : A(0);
+  const A t_sum = BlockSum<kBlock>(u, s_red[4]) + u_rest;
+  const A log_total = Log2(total);
+  const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
+  A log_left = Log2(left), rest_off = off;
+  bool again = rest && left < SmallRest<A>();
+  if (again) {
+    A own = NegInf<A>();
+    for (int i = tid; i < c; i += kBlock)
+      if (!(mark[i >> 5] >> (i & 31) & 1u)) own = Max(own, static_cast<A>(z[i * zs]));
+    own = BlockMax<kBlock>(own, s_red[1]);
+    again = own > NegInf<A>();
+    if (again) {
+      rest_off = -own * scale;
+      left = 0;
+      for (int i = tid; i < c; i += kBlock)
+        if (!(mark[i >> 5] >> (i & 31) & 1u))
+          left += Exp2(Fma(static_cast<A>(z[i * zs]), scale, rest_off));
+      left = BlockSum<kBlock>(left, s_red[5]);
+      log_left = Log2(left) - rest_off + off;
+    }
+  }
+  const int y = alpha < A(1) ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
+
+  if (a.loss.data) {
+    A kl = 0;
+    if (cls >= 0 && !(p == A(0)))
+      kl = p * (logit - t_high - Log2(t_sum) - (log_e - log_total));
+    __syncthreads();
+    kl = BlockSum<kBlock>(kl, s_red[0]);
+    if (tid == 0) {
+      if (rest && !(share == A(0)))
+        kl += share * (r - t_high - Log2(t_sum) - (log_left - log_total));
+      A v = taught ? alpha * temp * temp * (kl * static_cast<A>(kLn2)) : A(0);
+      if (y >= 0)
+        v += (A(1) - alpha) * static_cast<A>(kLn2) *
+             (Log2(total1) - Fma(static_cast<A>(z[y * zs]), scale1, off1));
+      StoreFloat(a.loss, row * a.loss.stride[0], v * w);
+    }
+  }
+  if (!grad && !hess) return;
+  const A soft = taught ? alpha : A(0), hard = y >= 0 ? A(1) - alpha : A(0);
+  const A inv = A(1) / total, inv1 = hard > A(0) ? A(1) / total1 : A(0);
+  const A spread = rest && left > A(0) ? share / left : A(0);
+  const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
+  // P_c of the classes without a slot is written with the row, that of a slot by its thread
+  auto put = [&](int i, A v, A want, bool spread_it) {
+    const A e = Exp2(Fma(v, scale, off));
+    const A q = e * inv;
+    if (spread_it) want = spread * (again ? Exp2(Fma(v, scale, rest_off)) : e);
+    A g = soft > A(0) ? soft * temp * (q - want) : A(0);
+    A h = soft > A(0) ? soft * q * (A(1) - q) : A(0);
+    if (hard > A(0)) {
+      const A q1 = Exp2(Fma(v, scale1, off1)) * inv1;
+      g += hard * (q1 - (i == y ? A(1) : A(0)));
+      h += hard * q1 * (A(1) - q1);
+    }
+    if (grad) grad[i * gs] = static_cast<O>(g * w);
+    if (hess) hess[i * hs] = static_cast<O>(h * factor * w);
+  };
+  for (int i = tid; i < c; i += kBlock)
+    if (!(mark[i >> 5] >> (i & 31) & 1u)) put(i, static_cast<A>(z[i * zs]), A(0), true);
+  if (cls >= 0) put(cls, z_slot, p, false);
+}
+
+// ------------------------------------------------------------------ top logits, any strides
+/*! keys order as the values do, zeros of both signs alike; 0: never chosen (NaN, -inf) */
+__device__ __forceinline__ uint32_t KeyOf(float v) {
+  if (!(v > -INFINITY)) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t KeyOf(double v) {
+  if (!(v > -INFINITY)) return 0ull;
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+  return b >> 63 ? ~b : b | (1ull << 63);
+}
+template <typename T> using Key = std::conditional_t<std::is_same_v<T, double>, uint64_t, uint32_t>;
+
+/*!
+ * The `take` largest of a digit's counts: the digit at which the count from the largest
+ * digit down reaches `take`, and how many of it are still to be taken. One wave's work.
+ */
+__device__ __forceinline__ void PickDigit(const int* hist, int take, int* digit, int* left) {
+  // lane l holds the four digits 255-4l .. 252-4l, largest first
+  const int lane = threadIdx.x % kWave;
+  int own[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum += own[i] = hist[255 - 4 * lane - i];
+  int before = sum;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int o = __shfl_up(before, d);
+    if (lane >= d) before += o;
+  }
+  before -= sum;
+  if (before < take && take <= before + sum) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (before < take && take <= before + own[i]) {
+        *digit = 255 - 4 * lane - i;
+        *left = take - before;
+      }
+      before += own[i];
+    }
+  }
+}
+
+/*!
+ * One workgroup a row, in any strides and with any ties: the k-th largest key is found
+ * digit by digit (eight bits a pass, counted in LDS), its equals are cut by class the same
+ * way, and what is chosen is put in order by counting how many precede it.
+ */
+template <typename T, int kBlock>
+__global__ void __launch_bounds__(kBlock) k_top_any(LGBM_TopLogitsArgs a) {
+  using A = Acc<T>;
+  using K = Key<T>;
+  __shared__ int hist[256];
+  __shared__ int s_digit, s_left, s_count;
+  __shared__ K s_key[kMaxTop];
+  __shared__ int s_cls[kMaxTop];
+  __shared__ A s_red[2][kBlock / kWave];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, c = a.classes;
+  const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+  const int64_t xs = a.scores.stride[1];
+  auto value = [&](int i) { return static_cast<A>(x[i * xs]); };
+
+  int valid = 0;
+  for (int i = tid; i < c; i += kBlock) valid += KeyOf(value(i)) != 0;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  if (valid) atomicAdd(&s_count, valid);
+  __syncthreads();
+  valid = s_count;
+  const int take = min(a.k, valid);
+  __syncthreads();
+  if (tid == 0) s_count = 0;
+
+  K edge = 0;   // the take-th largest key
+  int cut = c;  // of the keys equal to it, the classes below this are chosen
+  if (take > 0) {
+    int left = take;
+    for (int shift = sizeof(K) * 8 - 8; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += kBlock) hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < c; i += kBlock) {
+        const K key = KeyOf(value(i));
+        // the digits above are the edge's; the last shift is all of the key
+        const bool same = shift == sizeof(K) * 8 - 8 || (key >> (shift + 8)) == (edge >> (shift + 8));
+        if (key != 0 && same) atomicAdd(&hist[static_cast<int>(key >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (tid < kWave) PickDigit(hist, left, &s_digit, &s_left);
+      __syncthreads();
+      edge |= static_cast<K>(s_digit) << shift;
+      left = s_left;
+    }
+    // `left` of the classes whose key is the edge: the lowest, that is the largest of ~class
+    int high = 0;
+    for (int shift = 16; shift >= 0; shift -= 8) {
+      __syncthreads();
+      for (int i = tid; i < 256; i += kBlock) hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < c; i += kBlock) {
+        const int turned = 0xffffff - i;
+        if (KeyOf(value(i)) == edge && (shift == 16 || (turned >> (shift + 8)) == (high >> (shift + 8))))
+          atomicAdd(&hist[(turned >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (tid < kWave) PickDigit(hist, left, &s_digit, &s_left);
+      __syncthreads();
+      high |= s_digit << shift;
+      left = s_left;
+    }
+    cut = 0xffffff - high + 1;
+  }
+  __syncthreads();
+  // what is chosen, and the largest and the sum of what is not
+  A other = NegInf<A>();
+  for (int i = tid; i < c; i += kBlock) {
+    const A v = value(i);
+    const K key = KeyOf(v);
+    if (key == 0) continue;
+    if (take > 0 && (key > edge || (key == edge && i < cut))) {
+      const int at = atomicAdd(&s_count, 1);
+      s_key[at] = key;
+      s_cls[at] = i;
+    } else {
+      other = Max(other, v);
+    }
+  }
+  __syncthreads();
+  if (tid < take) {
+    const K key = s_key[tid];
+    const int cls = s_cls[tid];
+    int rank = 0;
+    for (int i = 0; i < take; ++i) rank += s_key[i] > key || (s_key[i] == key && s_cls[i] < cls);
+    static_cast<int32_t*>(a.top_class.data)[row * a.top_class.stride[0] +
+                                            rank * a.top_class.stride[1]] = cls;
+    static_cast<T*>(a.top_logit.data)[row * a.top_logit.stride[0] + rank * a.top_logit.stride[1]] =
+        x[cls * xs];
+  } else if (tid < a.k) {
+    static_cast<int32_t*>(a.top_class.data)[row * a.top_class.stride[0] +
+                                            tid * a.top_class.stride[1]] = -1;
+    static_cast<T*>(a.top_logit.data)[row * a.top_logit.stride[0] + tid * a.top_logit.stride[1]] =
+        static_cast<T>(-INFINITY);
+  }
+  if (a.log_rest.data == nullptr) return;
+  const A scale = static_cast<A>(kLog2e / a.temperature);
+  other = BlockMax<kBlock>(other, s_red[0]);
+  A sum = 0;
+  if (other > NegInf<A>() && other < static_cast<A>(INFINITY)) {
+    for (int i = tid; i < c; i += kBlock) {
+      const A v = value(i);
+      const K key = KeyOf(v);
+      if (key != 0 && !(take > 0 && (key > edge || (key == edge && i < cut))))
+        sum += Exp2((v - other) * scale);
+    }
+    sum = BlockSum<kBlock>(sum, s_red[1]);
+  }
+  if (tid == 0)
+    StoreFloat(a.log_rest, row * a.log_rest.stride[0],
+               sum > A(0) ? other / static_cast<A>(a.temperature) + Log2(sum) * static_cast<A>(kLn2)
+                          : other);
+}
+
+// ------------------------------------------------------------------ verification
+/*! what counts as probability: NaN, infinities and negative values are none */
+template <typename T> __device__ __forceinline__ double Mass(T x) {
+  const double v = static_cast<double>(static_cast<Acc<T>>(x));
+  return v > 0.0 && v < static_cast<double>(INFINITY) ? v : 0.0;
+}
+
+__device__ __forceinline__ double Uniform(const LGBM_Array& a, int64_t at) {
+  return a.type == C_API_DTYPE_FLOAT64 ? At<double>(a, at) : static_cast<double>(At<float>(a, at));
+}
+
+/*! drafts of sequence `row`, 0..drafts */
+__device__ __forceinline__ int Length(const LGBM_VerifyArgs& a, int64_t row) {
+  if (a.length.data == nullptr) return a.drafts;
+  const int64_t at = row * a.length.stride[0];
+  const int64_t v = a.length.type == C_API_DTYPE_INT64 ? At<int64_t>(a.length, at)
+                                                       : At<int32_t>(a.length, at);
+  return static_cast<int>(min(max(v, int64_t{0}), static_cast<int64_t>(a.drafts)));
+}
+
+template <typename T>
+__device__ __forceinline__ const T* TargetRow(const LGBM_VerifyArgs& a, int64_t row, int64_t s) {
+  return static_cast<const T*>(a.target.data) + row * a.target.stride[0] + s * a.target.stride[1];
+}
+template <typename T>
+__device__ __forceinline__ const T* DraftRow(const LGBM_VerifyArgs& a, int64_t row, int64_t s) {
+  return static_cast<const T*>(a.draft_prob.data) + row * a.draft_prob.stride[0] +
+         s * a.draft_prob.stride[1];
+}
+
+/*! whether draft s (class x) of the sequence stands: u q(x) < p(x), in 64 bits, where the
+ *  product of 32-bit numbers is exact */
+template <typename T>
+__device__ __forceinline__ bool Stands(const LGBM_VerifyArgs& a, int64_t row, int s, int x) {
+  if (x < 0) return false;
+  const double u = Uniform(a.accept, row * a.accept.stride[0] + s * a.accept.stride[1]);
+  const double p = Mass(TargetRow<T>(a, row, s)[x * a.target.stride[2]]);
+  const double q = a.draft_prob.data ? Mass(DraftRow<T>(a, row, s)[x * a.draft_prob.stride[2]])
+                                     : 1.0;
+  return u * q < p;
+}
+
+/*! how many drafts of the sequence stand; one wave's work, known to all its lanes */
+template <typename T>
+__device__ __forceinline__ int Accepted(const LGBM_VerifyArgs& a, int64_t row, int length) {
+  const int lane = threadIdx.x % kWave;
+  for (int s0 = 0; s0 < length; s0 += kWave) {
+    const int s = s0 + lane;
+    bool refused = false;
+    if (s < length) {
+      const int x = LoadClass(a.draft_class, row * a.draft_class.stride[0] +
+                                                 s * a.draft_class.stride[1], a.classes);
+      refused = !Stands<T>(a, row, s, x);
+    }
+    const unsigned long long who = __ballot(refused);
+    if (who) return s0 + __ffsll(who) - 1;
+  }
+  return length;
+}
+
+/*! what class c weighs in the draw of the class that follows the accepted ones */
+template <typename T> struct Residual {
+  const T* p;
+  const T* q;        // nullptr: nothing is taken away, but for class `gone`
+  int64_t ps, qs;
+  int gone;
+  __device__ __forceinline__ double operator()(int c) const {
+    const double v = Mass(p[c * ps]);
+    if (q != nullptr) return fmax(v - Mass(q[c * qs]), 0.0);
+    return c == gone ? 0.0 : v;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ Residual<T> ResidualOf(const LGBM_VerifyArgs& a, int64_t row,
+                                                  int accepted, int length) {
+  Residual<T> f{TargetRow<T>(a, row, accepted), nullptr, a.target.stride[2],
+                a.draft_prob.stride[2], -1};
+  if (accepted < length) {
+    if (a.draft_prob.data) {
+      f.q = DraftRow<T>(a, row, accepted);
+    } else {
+      f.gone = LoadClass(a.draft_class, row * a.draft_class.stride[0] +
+                                            accepted * a.draft_class.stride[1], a.classes);
+    }
+  }
+  return f;
+}
+
+/*!
+ * The first class at which the running sum of `mass` over [base, base + len) exceeds
+ * `goal`; the last one with any mass where rounding keeps the sum from it, -1 where there
+ * is none. The range is cut into one segment a wave, the segment that holds the goal into
+ * as many again, down to one class a lane: all but the first cut read a fraction of it.
+ * Whole workgroup; `sums` has one place a wave.
+ */
+template <int kBlock, typename F>
+__device__ __forceinline__ int FindClass(const F& mass, int base, int len, double goal,
+                                         double* sums) {
+  constexpr int kWaves = kBlock / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  while (len > kWave) {
+    const int seg = ((len + kWaves - 1) / kWaves + kWave - 1) / kWave * kWave;
+    double own = 0;
+    for (int i = wave * seg + lane; i < min(len, (wave + 1) * seg); i += kWave)
+      own += mass(base + i);
+    own = WaveSum(own);
+    __syncthreads();
+    if (lane == 0) sums[wave] = own;
+    __syncthreads();
+    int found = -1;
+    double before = 0, reach = 0;
+    for (int i = 0; i < kWaves; ++i) {
+      if (!(sums[i] > 0)) continue;
+      found = i;
+      before = reach;
+      reach += sums[i];
+      if (reach > goal) break;
+    }
+    if (found < 0) return -1;
+    goal -= before;
+    base += found * seg;
+    len = min(len - found * seg, seg);
+  }
+  const double own = lane < len ? mass(base + lane) : 0.0;
+  double reach = own;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const double o = __shfl_up(reach, d);
+    if (lane >= d) reach += o;
+  }
+  const unsigned long long some = __ballot(own > 0), over = __ballot(own > 0 && reach > goal);
+  if (over) return base + __ffsll(over) - 1;
+  return some ? base + 63 - __clzll(some) : -1;
+}
+
+/*! one workgroup a sequence */
+template <typename T, int kBlock>
+__global__ void __launch_bounds__(kBlock) k_verify_any(LGBM_VerifyArgs a) {
+  __shared__ double sums[kBlock / kWave];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, c = a.classes;
+  const int length = Length(a, row);
+  const int n = Accepted<T>(a, row, length);  // every wave finds the same
+  Residual<T> mass = ResidualOf<T>(a, row, n, length);
+  double total = 0;
+  for (int round = 0; round < 2; ++round) {
+    total = 0;
+    for (int i = tid; i < c; i += kBlock) total += mass(i);
+    __syncthreads();
+    total = BlockSum<kBlock>(total, sums);
+    if (total > 0) break;
+    // nothing is left of the target: the draw is from the target itself
+    mass.q = nullptr;
+    mass.gone = -1;
+  }
+  const double goal = Uniform(a.sample, row * a.sample.stride[0]) * total;
+  const int drawn = FindClass<kBlock>(mass, 0, c, goal, sums);
+  int32_t* out = static_cast<int32_t*>(a.out_class.data) + row * a.out_class.stride[0];
+  for (int s = tid; s <= a.drafts; s += kBlock) {
+    int x = -1;
+    if (s < n) x = LoadClass(a.draft_class, row * a.draft_class.stride[0] +
+                                                s * a.draft_class.stride[1], c);
+    else if (s == n) x = drawn;
+    out[s * a.out_class.stride[1]] = x;
+  }
+  if (tid == 0)
+    static_cast<int32_t*>(a.out_accepted.data)[row * a.out_accepted.stride[0]] = n;
+}
+
+// ------------------------------------------------------------------ launches
+/*! the calling thread's device is `device` while this lives */
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    OPS_HIP_OK(hipGetDevice(&before_));
+    if (device != before_) {
+      OPS_HIP_OK(hipSetDevice(device));
+      moved_ = true;
+    }
+  }
+  ~OnDevice() {
+    if (moved_) (void)hipSetDevice(before_);
+  }
+
+ private:
+  int before_ = 0;
+  bool moved_ = false;
+};
+
+template <typename F> void ByType(int type, F&& f) {
+  switch (type) {
+    case C_API_DTYPE_FLOAT64: f(double{}); break;
+    case C_API_DTYPE_FLOAT32: f(float{}); break;
+    case C_API_DTYPE_FLOAT16: f(_Float16{}); break;
+    default: f(__bf16{}); break;
+  }
+}
+
+void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
+  OnDevice on(device);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<uint32_t>(a.rows));
+  ByType(a.scores.type, [&](auto t) {
+    hipLaunchKernelGGL((k_top_any<decltype(t), 256>), grid, dim3(256), 0, s, a);
+  });
+  OPS_HIP_OK(hipGetLastError());
+}
+
+void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
+  OnDevice on(device);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<uint32_t>(a.rows));
+  const size_t lds = sizeof(uint32_t) * ((a.classes + 31) / 32);
+  ByType(a.scores.type, [&](auto t) {
+    auto kernel = k_distill_any<decltype(t), 256>;
+    if (lds > 32768)
+      OPS_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(lds)));
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, a);
+  });
+  OPS_HIP_OK(hipGetLastError());
+}
+
+int64_t VerifyWorkspaceDevice(const LGBM_VerifyArgs&) { return 0; }
+
+void VerifyDevice(const LGBM_VerifyArgs& a, int device, void* stream) {
+  OnDevice on(device);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<uint32_t>(a.rows));
+  ByType(a.target.type, [&](auto t) {
+    hipLaunchKernelGGL((k_verify_any<decltype(t), 256>), grid, dim3(256), 0, s, a);
+  });
+  OPS_HIP_OK(hipGetLastError());
+}
+
+const DeviceOps kOps{TopLogitsDevice, DistillDevice, VerifyDevice, VerifyWorkspaceDevice};
+const bool kRegistered = (g_device_ops = &kOps, true);
+
+}  // namespace
+}  // namespace class_ops
+}  // namespace migbm

@@ -8,6 +8,7 @@ from .basic import Booster, Dataset, LightGBMError, Sequence, register_logger
 from .callback import EarlyStopException, early_stopping, log_evaluation, \
     record_evaluation, reset_parameter
 from .engine import CVBooster, cv, train
+from . import ops
 
 try:
     from .sklearn import LGBMClassifier, LGBMModel, LGBMRanker, LGBMRegressor
@@ -35,5 +36,5 @@ __all__ = [
     "Dataset", "Booster", "LightGBMError", "register_logger", "Sequence",
     "train", "cv", "CVBooster",
     "early_stopping", "log_evaluation", "record_evaluation", "reset_parameter",
-    "EarlyStopException",
+    "EarlyStopException", "ops",
 ] + _SKLEARN_EXPORTS + _DASK_EXPORTS + _PLOT_EXPORTS

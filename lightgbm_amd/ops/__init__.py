@@ -1,1 +1,310 @@
-"""HIP/CDNA4 kernel extension helpers (device learner build metadata lives here)."""
+"""Operators over class scores and class probabilities, on the host or on a HIP device.
+
+`top_logits` selects what a teacher has to say about a row, `distill_loss` and
+`distill_gradients` are the objective that trains a student on it (the `distill` objective of
+`train` runs the same code), and `verify_drafts` turns classes that a student drafted into
+classes distributed as the target's probabilities say.
+
+Arrays are numpy arrays or torch tensors. Tensors on a HIP device are used where they are: the
+work goes to the current stream of their device, nothing is copied and nothing waits, and the
+results are tensors of that device. Everything else is computed on the host. Any strides will
+do. The functions record nothing for automatic differentiation: `distill_gradients` is the
+backward pass of `distill_loss`.
+"""
+import ctypes
+import struct
+import sys
+from typing import Any, NamedTuple, Optional
+
+import numpy as np
+
+from ..basic import _LIB, LightGBMError, _safe_call
+
+__all__ = ["TopLogits", "DistillGradients", "VerifiedDrafts", "top_logits", "distill_loss",
+           "distill_gradients", "verify_drafts"]
+
+
+class TopLogits(NamedTuple):
+    """The top logits of a teacher.
+
+    classes: [rows, k] integers; an id outside 0..num_classes-1 (top_logits writes -1) is an
+        empty slot, whose logit is not looked at. Of a class named twice in a row the first
+        slot counts.
+    logits: [rows, k].
+    log_rest: [rows] or None, the log-sum-exp at the loss's temperature of the teacher's logits
+        of all other classes. Without it the teacher's probabilities are normalised over the
+        slots; a row of -inf, with empty slots, has no teacher.
+    """
+    classes: Any
+    logits: Any
+    log_rest: Optional[Any] = None
+
+
+class DistillGradients(NamedTuple):
+    gradient: Any
+    hessian: Optional[Any] = None
+    loss: Optional[Any] = None
+
+
+class VerifiedDrafts(NamedTuple):
+    """classes: [sequences, drafts + 1] int32, the accepted drafts, the class drawn after them,
+    then -1. accepted: [sequences] int32, how many drafts were accepted."""
+    classes: Any
+    accepted: Any
+
+
+_F32, _F64, _I32, _I64, _F16, _BF16 = range(6)
+_NUMPY_TYPES = {"f4": _F32, "f8": _F64, "i4": _I32, "i8": _I64, "f2": _F16}
+_NUMPY_OF = {_F32: np.float32, _F64: np.float64, _I32: np.int32, _F16: np.float16}
+_TORCH_TYPES = {}
+_TORCH_OF = {}
+
+# LGBM_Array: data, three strides, type, reserved
+_TOP = struct.Struct("@qiid" + "Pqqqii" * 4)
+_DISTILL = struct.Struct("@qiidd" + "Pqqqii" * 9)
+_VERIFY = struct.Struct("@qii" + "Pqqqii" * 8 + "Pq")
+_NONE = (0, 0, 0, 0, 0, 0)
+
+for _f in (_LIB.LGBM_TopLogits, _LIB.LGBM_Distill, _LIB.LGBM_VerifyDrafts):
+    _f.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
+_LIB.LGBM_VerifyDraftsWorkspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]
+
+
+def _torch_of(x):
+    """The torch module if x is one of its tensors."""
+    torch = sys.modules.get("torch")
+    if torch is None or not isinstance(x, torch.Tensor):
+        return None
+    if not _TORCH_TYPES:
+        for code, dtype in ((_F32, torch.float32), (_F64, torch.float64), (_I32, torch.int32),
+                            (_I64, torch.int64), (_F16, torch.float16), (_BF16, torch.bfloat16)):
+            _TORCH_TYPES[dtype] = code
+            _TORCH_OF[code] = dtype
+    return torch
+
+
+class _Place:
+    """Where a call runs, and how its results are made: as its first array is."""
+
+    def __init__(self, x):
+        self.torch = torch = _torch_of(x)
+        self.device = -1
+        self.on = None
+        if torch is not None:
+            self.on = x.device
+            if self.on.type == "cuda":
+                self.device = self.on.index
+            elif self.on.type != "cpu":
+                raise LightGBMError(f"tensors on {self.on} are not supported")
+
+    def stream(self):
+        return self.torch.cuda.current_stream(self.on).cuda_stream if self.device >= 0 else None
+
+    def empty(self, shape, code, class_major=False):
+        if self.torch is not None:
+            if class_major:
+                return self.torch.empty(shape[::-1], dtype=_TORCH_OF[code], device=self.on).t()
+            return self.torch.empty(shape, dtype=_TORCH_OF[code], device=self.on)
+        return np.empty(shape, dtype=_NUMPY_OF[code], order="F" if class_major else "C")
+
+    def check(self, x, name, shape):
+        """x as an array of this place, of this shape (None: any length)."""
+        torch = _torch_of(x)
+        if self.device >= 0:
+            if torch is None or x.device != self.on:
+                raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
+        elif torch is not None:
+            if x.device.type != "cpu":
+                raise LightGBMError(f"{name} is on {x.device}, the first array is on the host")
+        elif not isinstance(x, np.ndarray):
+            x = np.asarray(x)
+        got = x.shape
+        if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
+            want = ", ".join("*" if w is None else str(w) for w in shape)
+            raise LightGBMError(f"{name} must have the shape [{want}], got {list(got)}")
+        return x
+
+
+def _array(x, name):
+    """The six fields of an LGBM_Array."""
+    if x is None:
+        return _NONE
+    if isinstance(x, np.ndarray):
+        dtype = x.dtype
+        code = _NUMPY_TYPES.get(dtype.kind + str(dtype.itemsize)) if dtype.isnative else None
+        if code is not None:
+            size = dtype.itemsize
+            steps = x.strides
+            if any(s % size for s in steps):
+                raise LightGBMError(f"{name} has strides that are no multiple of its elements")
+            steps = [s // size for s in steps]
+            at = x.__array_interface__["data"][0]
+    else:
+        code = _TORCH_TYPES.get(x.dtype)
+        steps = x.stride()
+        at = x.data_ptr()
+        dtype = x.dtype
+    if code is None:
+        raise LightGBMError(f"{name} has the type {dtype}, which is not supported")
+    n = len(steps)
+    if n == 2:
+        return (at, steps[0], steps[1], 0, code, 0)
+    if n == 1:
+        return (at, steps[0], 0, 0, code, 0)
+    return (at, steps[0], steps[1], steps[2], code, 0)
+
+
+def _host(x):
+    """Whatever is no tensor, as a numpy array."""
+    return x if _torch_of(x) is not None or isinstance(x, np.ndarray) else np.asarray(x)
+
+
+def _two_dim(x, name, dims=2):
+    x = _host(x)
+    if len(x.shape) != dims:
+        raise LightGBMError(f"{name} must have {dims} dimensions, got {list(x.shape)}")
+    return x
+
+
+def top_logits(scores, k, temperature=1.0, rest=True):
+    """The k largest scores of each row, largest first, with the log-sum-exp of the others.
+
+    scores: [rows, classes] float64, float32, float16 or bfloat16, at most 1048576 classes.
+    k: 1..min(classes, 256).
+    temperature: what the scores are divided by in log_rest; the logits stay as they are.
+    rest: whether log_rest is computed; it is float64 for float64 scores, else float32.
+
+    Equal scores go to the lowest class first. NaN and -inf are never selected: a row with
+    fewer than k other scores ends in class -1 with logit -inf. log_rest leaves NaN out.
+    """
+    scores = _two_dim(scores, "scores")
+    rows, classes = scores.shape
+    where = _Place(scores)
+    x = _array(scores, "scores")
+    code = x[4]
+    k = int(k)
+    out_class = where.empty((rows, max(k, 0)), _I32)
+    out_logit = where.empty((rows, max(k, 0)), code)
+    log_rest = where.empty((rows,), _F64 if code == _F64 else _F32) if rest else None
+    _safe_call(_LIB.LGBM_TopLogits(
+        _TOP.pack(rows, classes, k, temperature, *x, *_array(out_class, ""),
+                  *_array(out_logit, ""), *_array(log_rest, "")),
+        where.device, where.stream()))
+    return TopLogits(out_class, out_logit, log_rest)
+
+
+def _distill(scores, teacher, labels, weight, temperature, alpha, loss, gradient, hessian):
+    scores = _two_dim(scores, "scores")
+    rows, classes = scores.shape
+    where = _Place(scores)
+    if not 2 <= len(teacher) <= 3:
+        raise LightGBMError("teacher must be (classes, logits) or (classes, logits, log_rest)")
+    t_class = _two_dim(teacher[0], "teacher classes")
+    k = t_class.shape[1]
+    t_class = where.check(t_class, "teacher classes", (rows, None))
+    t_logit = where.check(teacher[1], "teacher logits", (rows, k))
+    t_rest = teacher[2] if len(teacher) == 3 else None
+    if t_rest is not None:
+        t_rest = where.check(t_rest, "teacher log_rest", (rows,))
+    if alpha == 1.0:
+        labels = None
+    if labels is not None:
+        labels = where.check(labels, "labels", (rows,))
+    if weight is not None:
+        weight = where.check(weight, "weight", (rows,))
+    x = _array(scores, "scores")
+    code = x[4]
+    out = _F32 if code == _F64 else code
+    class_major = x[1] == 1 and x[2] != 1
+    made_loss = where.empty((rows,), _F64 if code == _F64 else _F32) if loss else None
+    made_grad = where.empty((rows, classes), out, class_major) if gradient else None
+    made_hess = where.empty((rows, classes), out, class_major) if hessian else None
+    _safe_call(_LIB.LGBM_Distill(
+        _DISTILL.pack(rows, classes, k, temperature, alpha, *x,
+                      *_array(t_class, "teacher classes"), *_array(t_logit, "teacher logits"),
+                      *_array(t_rest, "teacher log_rest"), *_array(labels, "labels"),
+                      *_array(weight, "weight"), *_array(made_loss, ""), *_array(made_grad, ""),
+                      *_array(made_hess, "")),
+        where.device, where.stream()))
+    return made_loss, made_grad, made_hess
+
+
+def distill_loss(scores, teacher, labels=None, weight=None, temperature=1.0, alpha=1.0):
+    """The distillation loss of each row, [rows] (float64 for float64 scores, else float32).
+
+    With Q = softmax(scores / T) and P the teacher's probabilities at the same temperature,
+
+        weight * (alpha * T**2 * KL(P || Q) + (1 - alpha) * -log softmax(scores)[label])
+
+    where the classes that the teacher does not name are one event: P of it comes from
+    log_rest, Q of it is the sum of theirs.
+
+    scores: [rows, classes], the student's.
+    teacher: TopLogits, or a tuple of its two or three arrays; 1..256 slots a row.
+    labels: [rows] integers or float32, needed where alpha < 1; a label outside
+        0..classes-1 leaves its row without that term.
+    weight: [rows]. A row of weight zero, and a row whose scores are all -inf, has no loss and
+        no gradient, whatever else stands in it.
+    """
+    return _distill(scores, teacher, labels, weight, temperature, alpha, True, False, False)[0]
+
+
+def distill_gradients(scores, teacher, labels=None, weight=None, temperature=1.0, alpha=1.0,
+                      hessian=False, loss=False):
+    """The gradient of the sum of distill_loss with respect to the scores, [rows, classes], and
+    in the same pass, where asked for, the diagonal of the hessian as the multiclass objective
+    has it (classes / (classes - 1) * q * (1 - q)) and the loss.
+
+    The scores' type and order (float32 for float64 scores, as all gradients of the framework).
+    """
+    made = _distill(scores, teacher, labels, weight, temperature, alpha, loss, True, hessian)
+    return DistillGradients(made[1], made[2], made[0])
+
+
+def verify_drafts(target_prob, drafts, draft_prob, accept_uniform, sample_uniform, lengths=None):
+    """Accept or replace drafted classes so that the results are distributed as the target's.
+
+    target_prob: [sequences, drafts + 1, classes], the target's probabilities at each drafted
+        place and at the one after; float64, float32, float16 or bfloat16.
+    drafts: [sequences, drafts] int32 or int64, at most 1024 a sequence.
+    draft_prob: [sequences, drafts, classes], the target's type: the probabilities that the
+        drafts were drawn from, or None for drafts that were not drawn (probability one).
+    accept_uniform: [sequences, drafts] and
+    sample_uniform: [sequences], uniform numbers in [0, 1), float32 or float64.
+    lengths: [sequences] int32 or int64, how many drafts a sequence has, all where None.
+
+    A draft x stands while accept * q(x) < p(x), compared in 64 bits. After the last that
+    stands one class is drawn: from max(p - q, 0) at the first refused place, from p after the
+    last draft; the smallest class with mass whose running sum exceeds sample times the whole. NaN,
+    infinite and negative entries weigh nothing, a draft outside 0..classes-1 is refused. Where
+    the difference has no mass the draw is from p, where p has none the class is -1.
+    """
+    target_prob = _two_dim(target_prob, "target_prob", 3)
+    rows, places, classes = target_prob.shape
+    where = _Place(target_prob)
+    t = places - 1
+    drafts = where.check(drafts, "drafts", (rows, t))
+    if draft_prob is not None:
+        draft_prob = where.check(draft_prob, "draft_prob", (rows, t, classes))
+    accept = where.check(accept_uniform, "accept_uniform", (rows, t))
+    sample = where.check(sample_uniform, "sample_uniform", (rows,))
+    if lengths is not None:
+        lengths = where.check(lengths, "lengths", (rows,))
+    out_class = where.empty((rows, places), _I32)
+    out_accepted = where.empty((rows,), _I32)
+    fields = (rows, classes, t, *_array(target_prob, "target_prob"),
+              *_array(draft_prob, "draft_prob"), *_array(drafts, "drafts"),
+              *_array(accept, "accept_uniform"), *_array(sample, "sample_uniform"),
+              *_array(lengths, "lengths"), *_array(out_class, ""), *_array(out_accepted, ""))
+    scratch, size = None, 0
+    if where.device >= 0:
+        need = ctypes.c_int64(0)
+        _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_VERIFY.pack(*fields, 0, 0),
+                                                   ctypes.byref(need)))
+        size = need.value
+        if size:
+            scratch = where.torch.empty((size,), dtype=where.torch.uint8, device=where.on)
+    _safe_call(_LIB.LGBM_VerifyDrafts(
+        _VERIFY.pack(*fields, scratch.data_ptr() if size else 0, size),
+        where.device, where.stream()))
+    return VerifiedDrafts(out_class, out_accepted)

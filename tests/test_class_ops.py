@@ -1,0 +1,667 @@
+"""Operators over class scores against plain 64-bit numpy, on the host and on the GPU.
+
+Tolerances. The device takes exponentials of z * s - high * s with s = log2(e) / T in 32 bits
+(64 for float64 scores), eps = 2^-24 (2^-53) being half a step. One term of a softmax with
+exponent x (base two) is off by at most eps * (2 |x| + 4) of itself: the rounding of s, that of
+the fused product, and one step of the exponential; as 2^-x (2 |x| + 4) <= 4.2, that is below
+8 eps of the row's largest term, and below (2 * 64 + 4) eps of the term for every term above
+2^-64. The rounding of high * s is common to the row. A sum of n terms adds at most one
+rounding for each addition along its longest chain: n / 64 + 32 (a lane's own terms, then the
+tree). `_rel` is the sum of these; a result's own rounding to its type is added where it is
+compared.
+"""
+import math
+
+import numpy as np
+import pytest
+
+import lightgbm_amd as lgb
+from lightgbm_amd import ops
+from lightgbm_amd.basic import LightGBMError
+
+torch = pytest.importorskip("torch")
+
+PLACES = ["numpy", "torch", pytest.param("gpu", marks=pytest.mark.gpu)]
+INF = math.inf
+HALF_STEP = {"f64": 2.0 ** -53, "f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f64": 0.0, "f32": 2.0 ** -126, "f16": 2.0 ** -25, "bf16": 2.0 ** -126}
+TORCH = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float16,
+         "bf16": torch.bfloat16, "i32": torch.int32, "i64": torch.int64}
+
+
+def _rel(classes, dtype):
+    return (2 * 64 + 4 + 2 * (classes / 64 + 32)) * HALF_STEP["f64" if dtype == "f64" else "f32"]
+
+
+def _round(x, dtype):
+    """x (float64) rounded to a type, as float64."""
+    return torch.from_numpy(np.ascontiguousarray(x)).to(TORCH[dtype]).double().numpy()
+
+
+def _put(place, x, dtype=None, order="C", pad=0):
+    """A numpy array as an array of the place, row- or class-major; `pad` columns of NaN (or -7)
+    stand between its rows."""
+    if x is None:
+        return None
+    x = np.asarray(x)
+    if pad and x.ndim == 2:
+        wide = np.full((x.shape[0], x.shape[1] + pad), np.nan if x.dtype.kind == "f" else -7,
+                       dtype=x.dtype)
+        wide[:, :x.shape[1]] = x
+        return _put(place, wide, dtype, order)[:, :x.shape[1]]
+    if place == "numpy":
+        kind = {"f64": np.float64, "f32": np.float32, "f16": np.float16, "i32": np.int32,
+                "i64": np.int64, None: x.dtype}[dtype]
+        return np.array(x, dtype=kind, order=order)
+    t = torch.from_numpy(np.array(x))
+    if dtype is not None:
+        t = t.to(TORCH[dtype])
+    if order == "F":
+        t = t.t().contiguous().t()
+    return t.cuda() if place == "gpu" else t
+
+
+def _get(x):
+    if x is None or isinstance(x, np.ndarray):
+        return x
+    x = x.cpu()
+    return (x.double() if x.dtype.is_floating_point else x).numpy()
+
+
+def _types(place):
+    return ["f64", "f32", "f16"] + ([] if place == "numpy" else ["bf16"])
+
+
+# ------------------------------------------------------------------ plain forms, 64 bits
+def _lse(v):
+    v = np.asarray(v, dtype=np.float64)
+    high = v.max() if v.size else -INF
+    if not np.isfinite(high):
+        return high
+    return high + math.log(np.exp(v - high).sum())
+
+
+def _plain_top(x, k, t):
+    n, c = x.shape
+    classes = np.full((n, k), -1)
+    logits = np.full((n, k), -INF)
+    rest = np.empty(n)
+    for i in range(n):
+        able = [j for j in range(c) if x[i, j] > -INF]
+        order = sorted(able, key=lambda j: (-x[i, j], j))
+        classes[i, :len(order[:k])] = order[:k]
+        logits[i, :len(order[:k])] = x[i, order[:k]]
+        rest[i] = _lse([x[i, j] / t for j in order[k:]])
+    return classes, logits, rest
+
+
+def _plain_distill(z, classes, logits, rest, labels, weight, t, alpha):
+    """loss, gradient, hessian, and the scale that the gradient's error is relative to."""
+    n, c = z.shape
+    loss, grad, hess = np.zeros(n), np.zeros((n, c)), np.zeros((n, c))
+    size_l, size_g = np.zeros(n), np.zeros((n, c))
+    factor = c / (c - 1) if c > 1 else 1.0
+    for i in range(n):
+        w = 1.0 if weight is None else weight[i]
+        if w == 0 or z[i].max() == -INF:
+            continue
+        with np.errstate(all="ignore"):
+            # against the row's maximum: of z = 5000 alone, 64 bits keep 5e-13
+            d = z[i] - (z[i].max() if z[i].max() < INF else 0.0)
+            log_q = d / t - _lse(d / t)
+            log_1 = d - _lse(d)
+        q, q1 = np.exp(log_q), np.exp(log_1)
+        slot = {}
+        for j in range(classes.shape[1]):
+            if 0 <= classes[i, j] < c:
+                slot.setdefault(int(classes[i, j]), logits[i, j] / t)
+        r = -INF if rest is None else rest[i]
+        norm = _lse(list(slot.values()) + [r])
+        others = np.array([j not in slot for j in range(c)])
+        if norm > -INF and alpha > 0:
+            log_rho = _lse(log_q[others])
+            want = np.zeros(c)
+            total = 0.0
+            spread = 0.0
+            for j, v in slot.items():
+                lp = v - norm
+                want[j] = math.exp(lp)
+                if want[j] > 0:
+                    total += want[j] * (lp - log_q[j])
+                    spread += want[j] * (abs(lp) + abs(log_q[j]))
+            share = math.exp(r - norm)
+            if share > 0:
+                total += share * (r - norm - log_rho)
+                spread += share * (abs(r - norm) + abs(log_rho))
+                if log_rho > -INF:
+                    want[others] = share * np.exp(log_q[others] - log_rho)
+            loss[i] += alpha * t * t * total
+            size_l[i] += alpha * t * t * (2 + spread)
+            grad[i] += alpha * t * (q - want)
+            size_g[i] += alpha * t * (q + want)
+            hess[i] += alpha * q * (1 - q)
+        if alpha < 1 and 0 <= labels[i] < c:
+            y = int(labels[i])
+            loss[i] -= (1 - alpha) * log_1[y]
+            size_l[i] += (1 - alpha) * (2 + abs(log_1[y]))
+            grad[i] += (1 - alpha) * (q1 - (np.arange(c) == y))
+            size_g[i] += (1 - alpha) * (q1 + (np.arange(c) == y))
+            hess[i] += (1 - alpha) * q1 * (1 - q1)
+        loss[i] *= w
+        size_l[i] *= abs(w)
+        grad[i] *= w
+        size_g[i] *= abs(w)
+        hess[i] *= w * factor
+    return loss, grad, hess, size_l, size_g
+
+
+def _plain_verify(p, drafts, q, u, v, lengths):
+    b, t1, c = p.shape
+    mass = lambda a: np.where((a > 0) & np.isfinite(a), a, 0.0)  # noqa: E731
+    p = mass(p)
+    q = None if q is None else mass(q)
+    classes = np.full((b, t1), -1)
+    accepted = np.zeros(b, dtype=int)
+    for i in range(b):
+        length = t1 - 1 if lengths is None else min(max(int(lengths[i]), 0), t1 - 1)
+        s = 0
+        while s < length:
+            x = int(drafts[i, s])
+            if not 0 <= x < c:
+                break
+            if not u[i, s] * (1.0 if q is None else q[i, s, x]) < p[i, s, x]:
+                break
+            classes[i, s] = x
+            s += 1
+        left = p[i, s].copy()
+        if s < length:
+            if q is not None:
+                left = np.maximum(left - q[i, s], 0)
+            elif 0 <= drafts[i, s] < c:
+                left[drafts[i, s]] = 0
+        if left.sum() == 0:
+            left = p[i, s]
+        accepted[i] = s
+        if left.sum() > 0:
+            reach = np.cumsum(left)
+            # a class without mass is never drawn, not for a sample below zero either
+            over = np.nonzero((reach > v[i] * reach[-1]) & (left > 0))[0]
+            classes[i, s] = over[0] if len(over) else np.nonzero(left)[0][-1]
+    return classes, accepted
+
+
+# ------------------------------------------------------------------ top logits
+def _top_case(place, x, dtype, k, t=1.0, order="C", pad=0):
+    x = _round(x, dtype)
+    got = ops.top_logits(_put(place, x, dtype, order, pad), k, temperature=t)
+    classes, logits, rest = _plain_top(x, k, t)
+    np.testing.assert_array_equal(_get(got.classes), classes)
+    np.testing.assert_array_equal(_get(got.logits), logits)
+    out = "f64" if dtype == "f64" else "f32"
+    where = np.isfinite(rest)
+    # the maximum over T is rounded, and scaled by a rounded s
+    far = _rel(x.shape[1], dtype) * (1 + np.abs(rest[where]))
+    assert np.all(np.abs(_get(got.log_rest)[where] - rest[where]) <=
+                  far + 2 * HALF_STEP[out] * np.abs(rest[where]))
+    np.testing.assert_array_equal(_get(got.log_rest)[~where], rest[~where])
+    return got
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("rows,classes,k", [
+    (1, 1, 1), (3, 2, 1), (5, 7, 3), (70, 10, 10), (130, 33, 4), (3, 64, 64), (2, 65, 20),
+    (4, 257, 256), (9, 1000, 17), (2, 1025, 100), (3, 4099, 64), (2, 20011, 256), (1, 70001, 33)])
+def test_top_logits_sizes(place, rows, classes, k):
+    rng = np.random.default_rng(rows * classes + k)
+    for dtype in _types(place):
+        _top_case(place, 3 * rng.standard_normal((rows, classes)), dtype, k, t=1.7)
+        _top_case(place, 3 * rng.standard_normal((rows, classes)), dtype, k, order="F", pad=1)
+        _top_case(place, 3 * rng.standard_normal((rows, classes)), dtype, k, t=0.5, pad=3)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 100, 300, 5000, 40001])
+def test_top_logits_ties(place, classes):
+    """Constant rows, rows of few values, signed zeros, sorted rows: the lowest classes win."""
+    rng = np.random.default_rng(classes)
+    k = min(50, classes - 1)
+    rows = [np.zeros(classes), np.full(classes, -3.25), np.arange(classes) * 0.0 - 0.0,
+            rng.integers(0, 3, classes).astype(float), np.arange(classes) / 8.0,
+            -np.arange(classes) / 8.0, np.where(np.arange(classes) % 2, 0.0, -0.0),
+            np.where(np.arange(classes) == classes - 1, 50.0, -80.0),
+            np.minimum(np.arange(classes), 7.0)]
+    for dtype in _types(place):
+        for order in "CF":
+            _top_case(place, np.stack(rows), dtype, k, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [5, 90, 3000, 33000])
+def test_top_logits_masked(place, classes):
+    rng = np.random.default_rng(classes)
+    x = rng.standard_normal((8, classes))
+    x[0] = -INF
+    x[1] = np.nan
+    x[2, 1:] = -INF
+    x[3, ::2] = np.nan
+    x[4, 3:] = -INF
+    x[5, -1] = INF
+    x[6, :classes // 2] = np.finfo(np.float16).min
+    x[7, :] = np.where(np.arange(classes) < 2, x[7], np.nan)
+    for dtype in _types(place):
+        for order in "CF":
+            _top_case(place, x, dtype, 4, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_top_logits_confident(place):
+    """What is left stands far below the best: it is summed against its own maximum."""
+    for classes in (12, 400, 9000):
+        x = np.random.default_rng(1).standard_normal((3, classes))
+        x[:, 2] = 400.0
+        x[1, 3] = 300.0
+        for dtype in _types(place):
+            _top_case(place, x, dtype, 1)
+            _top_case(place, x, dtype, 2, t=0.25)
+
+
+# ------------------------------------------------------------------ distillation
+def _teacher(rng, rows, classes, k, rest, masked=False):
+    ids = np.stack([rng.permutation(max(classes, k))[:k] for _ in range(rows)])
+    logits = np.sort(8 * rng.random((rows, k)), axis=1)[:, ::-1].astype(np.float32)
+    ids = np.where(ids < classes, ids, -1)
+    r = (1 + 3 * rng.random(rows)).astype(np.float32) if rest else None
+    if masked:
+        ids[::3, (k + 1) // 2:] = -1
+        logits = np.where(ids < 0, np.nan, logits).astype(np.float32)
+        ids[1::5] = -1
+        if rest:
+            r[1::5] = -INF
+    return ids, logits, r
+
+
+def _distill_case(place, z, teacher, dtype, labels=None, weight=None, t=1.0, alpha=1.0,
+                  order="C", pad=0, int_type="i32"):
+    z = _round(z, dtype)
+    ids, logits, rest = teacher
+    put_teacher = ops.TopLogits(_put(place, ids, int_type), _put(place, logits, "f32"),
+                                _put(place, rest, "f32"))
+    args = (_put(place, z, dtype, order, pad), put_teacher)
+    mix = {"labels": _put(place, labels, int_type), "weight": _put(place, weight, "f32"),
+           "temperature": t, "alpha": alpha}
+    w = None if weight is None else np.asarray(weight, np.float32).astype(np.float64)
+    loss, grad, hess, size_l, size_g = _plain_distill(
+        z, ids, logits.astype(np.float64), None if rest is None else rest.astype(np.float64),
+        labels, w, t, alpha)
+    rel = _rel(z.shape[1], dtype)
+    out = "f32" if dtype == "f64" else dtype
+    got_loss = _get(ops.distill_loss(*args, **mix))
+    got = ops.distill_gradients(*args, hessian=True, loss=True, **mix)
+    alone = ops.distill_gradients(*args, **mix)
+    with np.errstate(invalid="ignore"):
+        close = np.abs(got_loss - loss) <= 3 * rel * size_l + HALF_STEP[
+            "f64" if dtype == "f64" else "f32"] * np.abs(loss)
+    same = (got_loss == loss) | (np.isnan(got_loss) & np.isnan(loss))
+    assert np.all(close | same)
+    np.testing.assert_array_equal(got_loss, _get(got.loss))
+    np.testing.assert_array_equal(_get(got.gradient), _get(alone.gradient))
+    assert alone.hessian is None and alone.loss is None
+    for a, b, size in ((_get(got.gradient), grad, size_g), (_get(got.hessian), hess, size_g)):
+        # a hessian q (1 - q) is off by what q is, relative to q at most
+        far = 3 * rel * size * (z.shape[1] / max(1, z.shape[1] - 1)) / min(t, 1.0)
+        far = far + (1 + rel) * HALF_STEP[out] * np.abs(b) + TINY[out]
+        with np.errstate(invalid="ignore"):
+            close = np.abs(a - b) <= far
+        assert np.all(close | (np.isnan(a) & np.isnan(b))), np.nanmax(np.abs(a - b) - far)
+    return got
+
+
+SIZES = [(1, 1, 1), (2, 2, 1), (5, 3, 2), (70, 7, 3), (200, 10, 10), (65, 33, 9), (3, 64, 20),
+         (66, 65, 64), (3, 300, 150), (4, 1000, 8), (2, 1025, 256), (3, 4099, 50), (2, 20011, 17),
+         (1, 70001, 64)]
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("rows,classes,k", SIZES)
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_sizes(place, rows, classes, k, rest):
+    rng = np.random.default_rng(rows + classes + k)
+    teacher = _teacher(rng, rows, classes, k, rest and classes > k)
+    labels = rng.integers(0, classes, rows)
+    for dtype in _types(place):
+        z = 3 * rng.standard_normal((rows, classes))
+        _distill_case(place, z, teacher, dtype, t=2.0)
+        _distill_case(place, z, teacher, dtype, labels=labels, t=1.0, alpha=0.25, order="F",
+                      int_type="i64")
+        _distill_case(place, z, teacher, dtype, labels=labels, t=3.0, alpha=0.5, pad=3)
+        _distill_case(place, z, teacher, dtype, labels=labels, t=1.5, alpha=0.0, order="F", pad=1)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [9, 130, 1500, 17000])
+def test_distill_masked(place, classes):
+    """Masked classes, rows with nothing in them, padding of any contents, empty slots, rows
+    without a teacher or a label, the same class twice, ids out of range."""
+    rng = np.random.default_rng(classes)
+    rows, k = 21, 6
+    ids, logits, rest = _teacher(rng, rows, classes, k, True, masked=True)
+    ids[6, 2] = ids[6, 0] = 1
+    ids[6, 1] = 2
+    logits[6] = [1, 2, 3, 4, 5, 6]
+    ids[9] = [3, 3, 3, 3, 3, 3]
+    logits[9] = [0, 1, np.nan, INF, 2, 3]
+    ids[12] = [classes, -5, 2 ** 31 - 1, 0, -1, 1]
+    logits[12] = [9, 9, 9, 1, np.nan, 2]
+    z = 2 * rng.standard_normal((rows, classes))
+    z[rng.random((rows, classes)) < 0.2] = -INF
+    np.put_along_axis(z, np.clip(ids, 0, classes - 1), 0.5, axis=1)
+    z[10] = -INF
+    z[13, classes // 2:] = np.finfo(np.float16).min
+    weight = rng.random(rows).astype(np.float32) + 0.5
+    weight[4] = 0.0
+    z[4] = np.nan
+    weight[5] = -1.5
+    labels = rng.integers(0, classes, rows)
+    labels[2], labels[3], labels[8] = -1, classes, -100
+    z[np.arange(rows), np.clip(labels, 0, classes - 1)] = np.where(
+        np.arange(rows) == 4, np.nan, 1.0)
+    z[10] = -INF
+    for dtype in _types(place):
+        for order in "CF":
+            for r in (rest, None):
+                _distill_case(place, z, (ids, logits, r), dtype, labels=labels, weight=weight,
+                              t=2.0, alpha=0.5, order=order)
+                _distill_case(place, z, (ids, logits, r), dtype, weight=weight, t=1.0,
+                              order=order, pad=2)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [8, 200, 6000])
+def test_distill_far_apart(place, classes):
+    """A student sure of its class: the others' share underflows, and is summed again."""
+    rng = np.random.default_rng(3)
+    z = rng.standard_normal((4, classes))
+    z[:, 2] = 30.0
+    z[1, 2] = 120.0
+    z[2, 2] = 900.0
+    z[3] += 5000.0
+    ids = np.full((4, 3), -1)
+    ids[:, 0] = 2
+    logits = np.zeros((4, 3), np.float32)
+    rest = np.zeros(4, np.float32)
+    for dtype in _types(place):
+        for order in "CF":
+            _distill_case(place, z, (ids, logits, rest), dtype, order=order)
+            _distill_case(place, z, (ids, logits, rest), dtype, t=0.5, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 150, 5000])
+def test_distill_infinite(place, classes):
+    """A teacher's class that the student masks costs an infinite loss and a finite gradient;
+    NaN and +inf among the scores make NaN of their row alone."""
+    rng = np.random.default_rng(4)
+    z = rng.standard_normal((5, classes))
+    z[0, 1] = -INF
+    z[1, 4] = np.nan
+    z[2, 4] = INF
+    z[3, 3:] = -INF
+    ids = np.tile([1, 0, 2], (5, 1))
+    logits = np.tile(np.float32([3, 2, 1]), (5, 1))
+    rest = np.float32([0.5, 0.5, 0.5, 0.5, 0.5])
+    for dtype in _types(place):
+        for order in "CF":
+            args = (_put(place, z, dtype, order),
+                    ops.TopLogits(_put(place, ids, "i32"), _put(place, logits, "f32"),
+                                  _put(place, rest, "f32")))
+            loss = _get(ops.distill_loss(*args))
+            grad = _get(ops.distill_gradients(*args).gradient)
+            assert loss[0] == INF and loss[3] == INF and np.isfinite(loss[4])
+            assert np.isnan(loss[1]) and np.isnan(loss[2])
+            assert np.all(np.isfinite(grad[[0, 3, 4]]))
+            assert np.all(np.isnan(grad[[1, 2]]))
+            assert grad[0, 1] < 0 and np.all(grad[3, 3:] == 0)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("order", ["C", "F"])
+@pytest.mark.parametrize("classes", [5, 140])
+def test_distill_gradient_is_the_slope(place, order, classes):
+    """Central differences of the float64 loss: the third derivative of the loss is at most
+    2 alpha / T + 1, so a step h leaves h^2 / 3 and the loss's rounding over h. The gradient
+    itself is rounded to 32 bits."""
+    rng = np.random.default_rng(11)
+    rows, k, h = 4, 3, 1e-5
+    ids, logits, rest = _teacher(rng, rows, classes, k, True)
+    labels = rng.integers(0, classes, rows)
+    weight = np.float32([1.0, 0.5, 2.0, 1.0])
+    z = rng.standard_normal((rows, classes))
+    teacher = ops.TopLogits(_put(place, ids, "i32"), _put(place, logits, "f32"),
+                            _put(place, rest, "f32"))
+    mix = {"labels": _put(place, labels, "i32"), "weight": _put(place, weight, "f32"),
+           "temperature": 2.0, "alpha": 0.6}
+    grad = _get(ops.distill_gradients(_put(place, z, "f64", order), teacher, **mix).gradient)
+    loss = lambda x: _get(ops.distill_loss(_put(place, x, "f64", order), teacher, **mix))  # noqa: E731
+    top = np.abs(loss(z)).max()
+    for c in range(0, classes, max(1, classes // 7)):
+        up, down = z.copy(), z.copy()
+        up[:, c] += h
+        down[:, c] -= h
+        slope = (loss(up) - loss(down)) / (2 * h)
+        far = 2 * 3 * h * h + 2 * 3 * _rel(classes, "f64") * (10 + top) / h
+        assert np.all(np.abs(slope - grad[:, c]) <= far + HALF_STEP["f32"] * np.abs(grad[:, c]))
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_distill_broadcast_and_strides(place):
+    """One row of scores for all teachers, teachers in any order of memory, every second row."""
+    rng = np.random.default_rng(5)
+    ids, logits, rest = _teacher(rng, 6, 40, 5, True)
+    z = np.float32(rng.standard_normal((1, 40)))
+    many = np.repeat(z, 6, 0)
+    want = ops.distill_gradients(_put(place, many, "f32"), ops.TopLogits(
+        _put(place, ids, "i32"), _put(place, logits, "f32"), _put(place, rest, "f32")), loss=True)
+    if place == "numpy":
+        one = np.broadcast_to(z, (6, 40))
+    else:
+        one = _put(place, z, "f32").expand(6, 40)
+    twice = _put(place, np.repeat(ids, 2, 0), "i64")[::2]
+    got = ops.distill_gradients(one, (twice, _put(place, logits, "f32", "F"),
+                                      _put(place, rest, "f64")), loss=True)
+    np.testing.assert_array_equal(_get(got.gradient), _get(want.gradient))
+    np.testing.assert_array_equal(_get(got.loss), _get(want.loss))
+
+
+# ------------------------------------------------------------------ verification
+def _softmax(x):
+    e = np.exp(x - x.max(-1, keepdims=True))
+    return e / e.sum(-1, keepdims=True)
+
+
+def _verify_case(place, p, drafts, q, u, v, lengths, dtype, int_type="i32", uniform="f32"):
+    p = _round(p, dtype)
+    q = None if q is None else _round(q, dtype)
+    u, v = _round(u, uniform), _round(v, uniform)
+    got = ops.verify_drafts(_put(place, p, dtype), _put(place, drafts, int_type),
+                            _put(place, q, dtype), _put(place, u, uniform),
+                            _put(place, v, uniform), lengths=_put(place, lengths, int_type))
+    classes, accepted = _plain_verify(p, drafts, q, u, v, lengths)
+    np.testing.assert_array_equal(_get(got.accepted), accepted)
+    np.testing.assert_array_equal(_get(got.classes), classes)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("rows,t,classes", [
+    (1, 1, 1), (1, 4, 2), (300, 3, 10), (67, 1, 63), (40, 5, 64), (33, 2, 65), (20, 70, 130),
+    (9, 3, 1000), (5, 2, 4099), (3, 4, 20011), (2, 1, 70001), (1, 2, 131072)])
+def test_verify_sizes(place, rows, t, classes):
+    rng = np.random.default_rng(rows + t + classes)
+    x = 2 * rng.standard_normal((rows, t + 1, classes))
+    p = _softmax(x)
+    q = _softmax(x[:, :t] + 0.7 * rng.standard_normal((rows, t, classes)))
+    drafts = (q / rng.exponential(size=q.shape)).argmax(-1)
+    u, v = rng.random((rows, t)), rng.random(rows)
+    lengths = rng.integers(0, t + 1, rows)
+    for dtype in _types(place):
+        _verify_case(place, p, drafts, q, u, v, None, dtype)
+        _verify_case(place, p, drafts, q, u, v, lengths, dtype, "i64", "f64")
+        _verify_case(place, p, p[:, :t].argmax(-1), None, u, v, lengths, dtype)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [4, 70, 5000])
+def test_verify_borders(place, classes):
+    """Sums that are exact in every order, numbers that stand on a border or outside [0, 1),
+    entries that are no probability, lengths and ids out of range, rows with no mass."""
+    rows, t = 16, 2
+    p = np.zeros((rows, t + 1, classes))
+    p[..., 1], p[..., 3], p[..., classes - 1] = 0.25, 0.25, 0.5
+    q = np.zeros((rows, t, classes))
+    q[..., 1], q[..., 3], q[..., 0] = 0.5, 0.25, 0.25
+    drafts = np.tile([1, 3], (rows, 1))
+    u = np.full((rows, t), 0.25)
+    v = np.zeros(rows)
+    lengths = np.full(rows, t)
+    u[0] = 0.5                # 0.5 * 0.5 < 0.25 is false: refused
+    u[1, 1] = 1.0             # 1 * 0.25 < 0.25 is false
+    v[2], v[3], v[4], v[5] = 0.25, 0.5, 1.0, 2.0
+    v[6] = np.nan
+    drafts[7, 0], drafts[8, 1] = -1, classes
+    lengths[9], lengths[10] = -3, 99
+    p[11, :, 1], q[11, :, 0] = np.nan, INF
+    p[12] = 0.0
+    q[13] = np.maximum(p[13, :t], q[13])   # nothing of the target is left
+    u[13] = 1.0
+    p[14, :, 0] = -1.0
+    v[15], u[15] = -0.5, np.nan
+    for dtype in _types(place):
+        for uniform in ("f32", "f64"):
+            _verify_case(place, p, drafts, q, u, v, lengths, dtype, uniform=uniform)
+            _verify_case(place, p, drafts, None, u, v, lengths, dtype, uniform=uniform)
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_verify_strides(place):
+    rng = np.random.default_rng(8)
+    p = _softmax(rng.standard_normal((6, 4, 50))).astype(np.float32)
+    q = _softmax(rng.standard_normal((6, 3, 50))).astype(np.float32)
+    drafts = rng.integers(0, 50, (6, 3))
+    u, v = rng.random((6, 3)).astype(np.float32), rng.random(6).astype(np.float32)
+    want = ops.verify_drafts(*[_put(place, x) for x in (p, drafts, q, u, v)])
+    turn = lambda x: _put(place, np.ascontiguousarray(x.transpose(2, 0, 1)))  # noqa: E731
+    moved = [turn(p), turn(q)]
+    moved = [x.transpose(1, 2, 0) if place == "numpy" else x.permute(1, 2, 0) for x in moved]
+    got = ops.verify_drafts(moved[0], _put(place, np.repeat(drafts, 2, 1))[:, ::2], moved[1],
+                            _put(place, u, order="F"), _put(place, np.repeat(v, 2))[::2])
+    np.testing.assert_array_equal(_get(got.classes), _get(want.classes))
+    np.testing.assert_array_equal(_get(got.accepted), _get(want.accepted))
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_verify_distribution(place):
+    """The first class of every sequence is distributed as the target, whatever the draft: over
+    n sequences a frequency is off by at most 5 standard deviations of sqrt(p (1 - p) / n)."""
+    rng = np.random.default_rng(9)
+    n, c = 40000, 8
+    p0 = _softmax(rng.standard_normal(c))
+    q0 = _softmax(rng.standard_normal(c))
+    p = np.broadcast_to(p0, (n, 2, c))
+    q = np.broadcast_to(q0, (n, 1, c))
+    drafts = (q / rng.exponential(size=(n, 1, c))).argmax(-1)
+    got = ops.verify_drafts(*[_put(place, np.ascontiguousarray(x)) for x in
+                              (p, drafts, q, rng.random((n, 1)), rng.random(n))])
+    seen = np.bincount(_get(got.classes)[:, 0], minlength=c) / n
+    assert np.all(np.abs(seen - p0) <= 5 * np.sqrt(p0 * (1 - p0) / n))
+
+
+# ------------------------------------------------------------------ the set together, refusals
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [12, 3000])
+def test_teacher_to_student(place, classes):
+    """A student that starts from zero scores follows its gradient to the teacher: its loss does
+    not rise, and a student that has the teacher's scores has no loss and no gradient."""
+    rng = np.random.default_rng(12)
+    scores = _put(place, 2 * rng.standard_normal((5, classes)).astype(np.float32))
+    teacher = ops.top_logits(scores, 5, temperature=2.0)
+    loss = _get(ops.distill_loss(scores, teacher, temperature=2.0))
+    # KL of two roundings of one distribution: first order terms cancel up to their error
+    assert np.all(np.abs(loss) <= 4 * 3 * _rel(classes, "f32") * 20)
+    grad = _get(ops.distill_gradients(scores, teacher, temperature=2.0).gradient)
+    assert np.all(np.abs(grad) <= 2 * 6 * _rel(classes, "f32"))
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_no_rows(place):
+    top = ops.top_logits(_put(place, np.zeros((0, 5), np.float32)), 2)
+    assert tuple(top.classes.shape) == (0, 2) and tuple(top.log_rest.shape) == (0,)
+    z = _put(place, np.zeros((0, 5), np.float32))
+    got = ops.distill_gradients(z, top, hessian=True, loss=True)
+    assert tuple(got.gradient.shape) == (0, 5) and tuple(got.loss.shape) == (0,)
+    p = _put(place, np.zeros((0, 3, 5), np.float32))
+    got = ops.verify_drafts(p, _put(place, np.zeros((0, 2), np.int32)), None,
+                            _put(place, np.zeros((0, 2), np.float32)),
+                            _put(place, np.zeros(0, np.float32)))
+    assert tuple(got.classes.shape) == (0, 3)
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_refusals(place):
+    f = lambda *shape: _put(place, np.ones(shape, np.float32))  # noqa: E731
+    i = lambda *shape: _put(place, np.ones(shape, np.int32))  # noqa: E731
+    teacher = (i(3, 2), f(3, 2))
+    bad = [
+        lambda: ops.top_logits(f(3, 4), 0),
+        lambda: ops.top_logits(f(3, 4), 5),
+        lambda: ops.top_logits(f(3, 400), 257),
+        lambda: ops.top_logits(f(4), 1),
+        lambda: ops.top_logits(f(3, 0), 1),
+        lambda: ops.top_logits(i(3, 4), 1),
+        lambda: ops.top_logits(f(3, 4), 1, temperature=0.0),
+        lambda: ops.top_logits(f(3, 4), 1, temperature=-1.0),
+        lambda: ops.top_logits(f(3, 4), 1, temperature=math.nan),
+        lambda: ops.top_logits(f(3, 4), 1, temperature=math.inf),
+        lambda: ops.distill_loss(f(3, 4), (i(2, 2), f(2, 2))),
+        lambda: ops.distill_loss(f(3, 4), (i(3, 2), f(3, 3))),
+        lambda: ops.distill_loss(f(3, 4), (f(3, 2), f(3, 2))),
+        lambda: ops.distill_loss(f(3, 4), (i(3, 2), i(3, 2))),
+        lambda: ops.distill_loss(f(3, 4), (i(3, 2),)),
+        lambda: ops.distill_loss(f(3, 4), (i(3, 2), f(3, 2), f(3, 1))),
+        lambda: ops.distill_loss(f(3, 4), (i(3, 257), f(3, 257))),
+        lambda: ops.distill_loss(f(3, 4), (i(3, 0), f(3, 0))),
+        lambda: ops.distill_loss(f(3, 4), teacher, alpha=0.5),
+        lambda: ops.distill_loss(f(3, 4), teacher, alpha=1.5),
+        lambda: ops.distill_loss(f(3, 4), teacher, alpha=math.nan),
+        lambda: ops.distill_loss(f(3, 4), teacher, temperature=0.0),
+        lambda: ops.distill_loss(f(3, 4), teacher, labels=i(2), alpha=0.5),
+        lambda: ops.distill_loss(f(3, 4), teacher, weight=f(4)),
+        lambda: ops.distill_loss(f(3, 4), teacher, weight=i(3)),
+        lambda: ops.distill_gradients(f(3, 4, 1), teacher),
+        lambda: ops.verify_drafts(f(2, 1, 4), i(2, 0), None, f(2, 0), f(2)),
+        lambda: ops.verify_drafts(f(2, 3, 4), i(2, 3), None, f(2, 3), f(2)),
+        lambda: ops.verify_drafts(f(2, 3, 4), i(2, 2), f(2, 3, 4), f(2, 2), f(2)),
+        lambda: ops.verify_drafts(f(2, 3, 4), f(2, 2), None, f(2, 2), f(2)),
+        lambda: ops.verify_drafts(f(2, 3, 4), i(2, 2), None, i(2, 2), f(2)),
+        lambda: ops.verify_drafts(f(2, 3, 4), i(2, 2), None, f(2, 2), f(3)),
+        lambda: ops.verify_drafts(f(2, 3, 4), i(2, 2), None, f(2, 2), f(2), lengths=f(2)),
+        lambda: ops.verify_drafts(f(2, 3), i(2, 2), None, f(2, 2), f(2)),
+    ]
+    for k, call in enumerate(bad):
+        with pytest.raises(LightGBMError):
+            call()
+            pytest.fail(f"call {k} was not refused")
+    other = ops.verify_drafts
+    with pytest.raises(LightGBMError):
+        other(f(2, 3, 4), i(2, 2), _put(place, np.ones((2, 2, 4))), f(2, 2), f(2))
+
+
+@pytest.mark.gpu
+def test_refuses_mixed_places():
+    z, ids, t = np.ones((3, 4), np.float32), np.ones((3, 2), np.int32), np.ones((3, 2), np.float32)
+    with pytest.raises(LightGBMError):
+        ops.distill_loss(_put("gpu", z), (ids, t))
+    with pytest.raises(LightGBMError):
+        ops.distill_loss(_put("torch", z), (_put("gpu", ids), _put("torch", t)))
+
+
+def test_lgb_exports_ops():
+    assert lgb.ops is ops
