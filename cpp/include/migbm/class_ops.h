@@ -10,6 +10,7 @@
 #define MIGBM_CLASS_OPS_H_
 
 #include "c_api.h"
+#include "dataset.h"
 
 namespace migbm {
 namespace class_ops {
@@ -42,6 +43,16 @@ void Check(const LGBM_VerifyArgs& a);
 void TopLogits(const LGBM_TopLogitsArgs& a, int device, void* stream);
 void Distill(const LGBM_DistillArgs& a, int device, void* stream);
 void VerifyDrafts(const LGBM_VerifyArgs& a, int device, void* stream);
+/*!
+ * The distillation arguments of a dataset in the boosting engine's layout: class-major
+ * float64 scores, float32 gradients, and the dataset's teacher, labels and weights in host
+ * memory. The caller sets the outputs.
+ */
+LGBM_DistillArgs DistillArgsOf(const Metadata& meta, data_size_t num_data, int num_class,
+                               double temperature, double alpha, const double* score);
+inline LGBM_Array ArrayOf(const void* data, int type, int64_t s0, int64_t s1 = 0) {
+  return LGBM_Array{const_cast<void*>(data), {s0, s1, 0}, type, 0};
+}
 /*! bytes of device scratch memory that VerifyDrafts needs (0: none) */
 int64_t VerifyWorkspace(const LGBM_VerifyArgs& a);
 

@@ -146,6 +146,8 @@ struct Config {
   int lambdarank_truncation_level = 30;
   bool lambdarank_norm = true;
   double lambdarank_position_bias_regularization = 0.0;
+  double distill_temperature = 1.0;  // of the distill objective and metric
+  double distill_alpha = 1.0;        // weight of the teacher's term; the labels have the rest
   std::vector<double> label_gain;
   int objective_seed = 5;
 

@@ -29,6 +29,11 @@ class Metadata {
   void SetQueryBoundaries(std::vector<data_size_t> boundaries);
   void SetInitScore(const double* s, int64_t n);
   void SetPosition(const int32_t* p, data_size_t n);
+  /*! a teacher's top logits, `n` = rows * slots values in row order; the three arrays are
+   *  set on their own and agree only once all are there (CheckTeacher) */
+  void SetTeacherClass(const int32_t* p, int64_t n);
+  void SetTeacherLogit(const float* p, int64_t n);
+  void SetTeacherRest(const float* p, int64_t n);
 
   data_size_t num_data() const { return num_data_; }
   const label_t* label() const { return label_.data(); }
@@ -45,6 +50,22 @@ class Metadata {
   const double* init_score() const { return init_score_.empty() ? nullptr : init_score_.data(); }
   int64_t num_init_score() const { return static_cast<int64_t>(init_score_.size()); }
   const int32_t* positions() const { return positions_.empty() ? nullptr : positions_.data(); }
+  /*! slots of the teacher's top logits a row (0: no teacher) */
+  int teacher_slots() const {
+    return num_data_ > 0 ? static_cast<int>(teacher_class_.size() / num_data_) : 0;
+  }
+  const int32_t* teacher_class() const {
+    return teacher_class_.empty() ? nullptr : teacher_class_.data();
+  }
+  const float* teacher_logit() const {
+    return teacher_logit_.empty() ? nullptr : teacher_logit_.data();
+  }
+  const float* teacher_rest() const {
+    return teacher_rest_.empty() ? nullptr : teacher_rest_.data();
+  }
+  int64_t num_teacher_logit() const { return static_cast<int64_t>(teacher_logit_.size()); }
+  /*! throws unless there are as many classes as logits, in whole rows */
+  void CheckTeacher() const;
 
   std::vector<label_t>& mutable_label() { return label_; }
 
@@ -83,6 +104,9 @@ class Metadata {
   std::vector<label_t> query_weights_;
   std::vector<double> init_score_;
   std::vector<int32_t> positions_;
+  std::vector<int32_t> teacher_class_;
+  std::vector<float> teacher_logit_;
+  std::vector<float> teacher_rest_;
   std::vector<int32_t> streamed_query_ids_;
 };
 

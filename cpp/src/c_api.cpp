@@ -870,10 +870,14 @@ int LGBM_DatasetSetField(DatasetHandle handle, const char* field_name, const voi
     else if (name == "group" || name == "query") d->metadata().SetQuery(nullptr, 0);
     else if (name == "init_score") d->metadata().SetInitScore(nullptr, 0);
     else if (name == "position") d->metadata().SetPosition(nullptr, 0);
+    else if (name == "teacher_class") d->metadata().SetTeacherClass(nullptr, 0);
+    else if (name == "teacher_logit") d->metadata().SetTeacherLogit(nullptr, 0);
+    else if (name == "teacher_log_rest") d->metadata().SetTeacherRest(nullptr, 0);
     else Log::Fatal("Unknown field %s", field_name);
     return 0;
   }
-  if ((name == "label" || name == "weight" || name == "position") &&
+  if ((name == "label" || name == "weight" || name == "position" ||
+       name == "teacher_log_rest") &&
       num_element != d->num_data()) {
     Log::Fatal("Length of %s (%d) differs from the number of rows (%d)", field_name,
                num_element, d->num_data());
@@ -900,6 +904,14 @@ int LGBM_DatasetSetField(DatasetHandle handle, const char* field_name, const voi
   } else if (name == "position") {
     MIGBM_CHECK(type == C_API_DTYPE_INT32);
     d->metadata().SetPosition(static_cast<const int32_t*>(field_data), num_element);
+  } else if (name == "teacher_class") {
+    MIGBM_CHECK(type == C_API_DTYPE_INT32);
+    d->metadata().SetTeacherClass(static_cast<const int32_t*>(field_data), num_element);
+  } else if (name == "teacher_logit" || name == "teacher_log_rest") {
+    MIGBM_CHECK(type == C_API_DTYPE_FLOAT32);
+    const float* p = static_cast<const float*>(field_data);
+    if (name == "teacher_logit") d->metadata().SetTeacherLogit(p, num_element);
+    else d->metadata().SetTeacherRest(p, num_element);
   } else {
     Log::Fatal("Unknown field %s", field_name);
   }
@@ -931,6 +943,18 @@ int LGBM_DatasetGetField(DatasetHandle handle, const char* field_name, int* out_
     *out_ptr = d->metadata().positions();
     *out_len = *out_ptr ? d->num_data() : 0;
     *out_type = C_API_DTYPE_INT32;
+  } else if (name == "teacher_class") {
+    *out_ptr = d->metadata().teacher_class();
+    *out_len = d->metadata().teacher_slots() * d->num_data();
+    *out_type = C_API_DTYPE_INT32;
+  } else if (name == "teacher_logit") {
+    *out_ptr = d->metadata().teacher_logit();
+    *out_len = static_cast<int>(d->metadata().num_teacher_logit());
+    *out_type = C_API_DTYPE_FLOAT32;
+  } else if (name == "teacher_log_rest") {
+    *out_ptr = d->metadata().teacher_rest();
+    *out_len = *out_ptr ? d->num_data() : 0;
+    *out_type = C_API_DTYPE_FLOAT32;
   } else {
     Log::Fatal("Unknown field %s", field_name);
   }

@@ -453,6 +453,24 @@ void Distill(const LGBM_DistillArgs& a, int device, void* stream) {
   else Device().distill(a, device, stream);
 }
 
+LGBM_DistillArgs DistillArgsOf(const Metadata& meta, data_size_t num_data, int num_class,
+                               double temperature, double alpha, const double* score) {
+  meta.CheckTeacher();
+  LGBM_DistillArgs a{};
+  a.rows = num_data;
+  a.classes = num_class;
+  a.k = meta.teacher_slots();
+  a.temperature = temperature;
+  a.alpha = alpha;
+  a.scores = ArrayOf(score, C_API_DTYPE_FLOAT64, 1, num_data);
+  a.teacher_class = ArrayOf(meta.teacher_class(), C_API_DTYPE_INT32, a.k, 1);
+  a.teacher_logit = ArrayOf(meta.teacher_logit(), C_API_DTYPE_FLOAT32, a.k, 1);
+  a.teacher_rest = ArrayOf(meta.teacher_rest(), C_API_DTYPE_FLOAT32, 1);
+  a.label = ArrayOf(meta.label(), C_API_DTYPE_FLOAT32, 1);
+  a.weight = ArrayOf(meta.weights(), C_API_DTYPE_FLOAT32, 1);
+  return a;
+}
+
 int64_t VerifyWorkspace(const LGBM_VerifyArgs& a) {
   Check(a);
   return a.rows == 0 || g_device_ops == nullptr ? 0 : g_device_ops->verify_workspace(a);

@@ -296,6 +296,8 @@ void Config::Set(const std::unordered_map<std::string, std::string>& params_in) 
     else if (k == "pred_early_stop_margin") pred_early_stop_margin = ParseDouble(v);
     else if (k == "lambdarank_position_bias_regularization")
       lambdarank_position_bias_regularization = ParseDouble(v);
+    else if (k == "distill_temperature") distill_temperature = ParseDouble(v);
+    else if (k == "distill_alpha") distill_alpha = ParseDouble(v);
     // unknown keys are kept in raw only (tolerated, like the reference's pass-through)
   }
 
@@ -326,6 +328,7 @@ void Config::Set(const std::unordered_map<std::string, std::string>& params_in) 
   if (objective == "multiclassova" || objective == "multiclass_ova" || objective == "ova" || objective == "ovr")
     objective = "multiclassova";
   if (objective == "softmax") objective = "multiclass";
+  if (objective == "distillation") objective = "distill";
   if (objective == "cross_entropy" || objective == "xentropy") objective = "cross_entropy";
   if (objective == "cross_entropy_lambda" || objective == "xentlambda") objective = "cross_entropy_lambda";
 

@@ -58,6 +58,40 @@ void Metadata::SetPosition(const int32_t* p, data_size_t n) {
   positions_.assign(p, p + n);
 }
 
+static void CheckTeacherLength(const char* what, int64_t n, data_size_t rows) {
+  if (rows <= 0 || n % rows != 0)
+    Log::Fatal("Length of %s (%lld) is no multiple of the number of rows (%d)", what,
+               static_cast<long long>(n), rows);
+}
+
+void Metadata::SetTeacherClass(const int32_t* p, int64_t n) {
+  if (p == nullptr || n == 0) { teacher_class_.clear(); return; }
+  CheckTeacherLength("teacher_class", n, num_data_);
+  teacher_class_.assign(p, p + n);
+}
+
+void Metadata::SetTeacherLogit(const float* p, int64_t n) {
+  if (p == nullptr || n == 0) { teacher_logit_.clear(); return; }
+  CheckTeacherLength("teacher_logit", n, num_data_);
+  teacher_logit_.assign(p, p + n);
+}
+
+void Metadata::SetTeacherRest(const float* p, int64_t n) {
+  if (p == nullptr || n == 0) { teacher_rest_.clear(); return; }
+  MIGBM_CHECK_EQ(n, num_data_);
+  teacher_rest_.assign(p, p + n);
+}
+
+void Metadata::CheckTeacher() const {
+  if (teacher_class_.empty())
+    Log::Fatal("The distill objective and the distill_loss metric need a teacher's top logits "
+               "(Dataset.set_teacher)");
+  if (teacher_class_.size() != teacher_logit_.size())
+    Log::Fatal("The teacher has %lld classes but %lld logits",
+               static_cast<long long>(teacher_class_.size()),
+               static_cast<long long>(teacher_logit_.size()));
+}
+
 // ------------------------------------------------------------------ Dataset
 void Dataset::FinishBinMappers(const Config&) {
   hist_offsets_.resize(bin_mappers_.size());
@@ -1037,6 +1071,23 @@ std::unique_ptr<Dataset> Dataset::Subset(const data_size_t* indices, data_size_t
     for (data_size_t i = 0; i < n; ++i) pos[i] = metadata_.positions()[indices[i]];
     d->metadata_.SetPosition(pos.data(), n);
   }
+  if (const int k = metadata_.teacher_slots(); k > 0) {
+    metadata_.CheckTeacher();
+    std::vector<int32_t> cls(static_cast<size_t>(n) * k);
+    std::vector<float> logit(cls.size());
+    for (data_size_t i = 0; i < n; ++i) {
+      const size_t from = static_cast<size_t>(indices[i]) * k, to = static_cast<size_t>(i) * k;
+      std::copy_n(metadata_.teacher_class() + from, k, cls.begin() + to);
+      std::copy_n(metadata_.teacher_logit() + from, k, logit.begin() + to);
+    }
+    d->metadata_.SetTeacherClass(cls.data(), static_cast<int64_t>(cls.size()));
+    d->metadata_.SetTeacherLogit(logit.data(), static_cast<int64_t>(logit.size()));
+    if (metadata_.teacher_rest() != nullptr) {
+      std::vector<float> rest(n);
+      for (data_size_t i = 0; i < n; ++i) rest[i] = metadata_.teacher_rest()[indices[i]];
+      d->metadata_.SetTeacherRest(rest.data(), n);
+    }
+  }
   return d;
 }
 
@@ -1252,6 +1303,17 @@ void Dataset::SaveBinaryFile(const char* filename) const {
     fwrite(&nq, sizeof(nq), 1, fp);
     fwrite(metadata_.query_boundaries(), sizeof(data_size_t), nq + 1, fp);
   }
+  // a teacher follows where there is one: slots a row, whether the rest is known, the arrays
+  if (const int32_t slots = metadata_.teacher_slots(); slots > 0) {
+    metadata_.CheckTeacher();
+    const uint8_t has_rest = metadata_.teacher_rest() != nullptr;
+    const size_t n = static_cast<size_t>(slots) * num_data_;
+    fwrite(&slots, sizeof(slots), 1, fp);
+    fwrite(&has_rest, 1, 1, fp);
+    fwrite(metadata_.teacher_class(), sizeof(int32_t), n, fp);
+    fwrite(metadata_.teacher_logit(), sizeof(float), n, fp);
+    if (has_rest) fwrite(metadata_.teacher_rest(), sizeof(float), num_data_, fp);
+  }
   fclose(fp);
 }
 
@@ -1338,6 +1400,25 @@ std::unique_ptr<Dataset> Dataset::LoadFromBinFile(const char* filename) {
     MIGBM_CHECK_EQ(fread(qb.data(), sizeof(data_size_t), nq + 1, fp),
                    static_cast<size_t>(nq + 1));
     d->metadata_.SetQueryBoundaries(std::move(qb));
+  }
+  int32_t slots = 0;
+  if (fread(&slots, sizeof(slots), 1, fp) == 1) {
+    MIGBM_CHECK(slots > 0 && slots <= 256);
+    uint8_t has_rest;
+    MIGBM_CHECK_EQ(fread(&has_rest, 1, 1, fp), 1u);
+    const size_t n = static_cast<size_t>(slots) * d->num_data_;
+    std::vector<int32_t> cls(n);
+    std::vector<float> logit(n);
+    MIGBM_CHECK_EQ(fread(cls.data(), sizeof(int32_t), n, fp), n);
+    MIGBM_CHECK_EQ(fread(logit.data(), sizeof(float), n, fp), n);
+    d->metadata_.SetTeacherClass(cls.data(), static_cast<int64_t>(n));
+    d->metadata_.SetTeacherLogit(logit.data(), static_cast<int64_t>(n));
+    if (has_rest) {
+      std::vector<float> rest(d->num_data_);
+      MIGBM_CHECK_EQ(fread(rest.data(), sizeof(float), d->num_data_, fp),
+                     static_cast<size_t>(d->num_data_));
+      d->metadata_.SetTeacherRest(rest.data(), d->num_data_);
+    }
   }
   fclose(fp);
   return d;

@@ -319,7 +319,7 @@ std::string GBDT::ModelToIfElse(int num_iteration) const {
       obj == "multiclassova" || obj == "ova") {
     ss << "  for (int k = 0; k < MIGBM_NUM_CLASSES; ++k)\n"
        << "    output[k] = 1.0 / (1.0 + std::exp(-" << sigmoid << " * output[k]));\n";
-  } else if (obj == "multiclass" || obj == "softmax") {
+  } else if (obj == "multiclass" || obj == "softmax" || obj == "distill") {
     ss << "  double wmax = output[0];\n"
        << "  for (int k = 1; k < MIGBM_NUM_CLASSES; ++k) if (output[k] > wmax) wmax = output[k];\n"
        << "  double wsum = 0.0;\n"

@@ -26,6 +26,7 @@
 #include "migbm/tree_learner.h"
 #include "migbm/objective.h"
 #include "migbm/network.h"
+#include "migbm/class_ops.h"
 
 #include <algorithm>
 #include <condition_variable>
@@ -2527,7 +2528,7 @@ class HIPTreeLearner : public TreeLearner {
       if (name == r) return !config_->reg_sqrt;
     }
     if (name == "binary" || name == "cross_entropy" || name == "cross_entropy_lambda" ||
-        name == "multiclass" || name == "multiclassova")
+        name == "multiclass" || name == "multiclassova" || name == "distill")
       return true;
     if (name == "lambdarank") return rank_ok_;
     return false;
@@ -2641,6 +2642,11 @@ class HIPTreeLearner : public TreeLearner {
   int num_queries_ = 0;
   DevBuf<double> d_score_;
   DevBuf<float> d_label_, d_weight_;
+  // the distill objective's teacher, as it was when the training data was uploaded
+  DevBuf<int32_t> d_teacher_class_;
+  DevBuf<float> d_teacher_logit_, d_teacher_rest_;
+  int teacher_slots_ = 0;
+  bool teacher_rest_ = false;
   DevBuf<uint32_t> d_idx_, d_idx_tmp_;
   DevBuf<uint8_t> d_marks_;
   DevBuf<int> d_block_cnt_, d_block_loff_, d_block_roff_;
@@ -2985,6 +2991,24 @@ void HIPTreeLearner::Init(const Dataset* train_data, bool is_constant_hessian) {
   d_label_.Alloc(num_data_);
   HIP_OK(hipMemcpy(d_label_.ptr, train_data->metadata().label(), sizeof(float) * num_data_,
                    hipMemcpyHostToDevice));
+  const Metadata& meta = train_data->metadata();
+  teacher_slots_ = meta.teacher_slots();
+  teacher_rest_ = meta.teacher_rest() != nullptr;
+  if (teacher_slots_ > 0) {
+    meta.CheckTeacher();
+    const size_t count = static_cast<size_t>(num_data_) * teacher_slots_;
+    d_teacher_class_.Alloc(count);
+    d_teacher_logit_.Alloc(count);
+    HIP_OK(hipMemcpy(d_teacher_class_.ptr, meta.teacher_class(), sizeof(int32_t) * count,
+                     hipMemcpyHostToDevice));
+    HIP_OK(hipMemcpy(d_teacher_logit_.ptr, meta.teacher_logit(), sizeof(float) * count,
+                     hipMemcpyHostToDevice));
+    if (teacher_rest_) {
+      d_teacher_rest_.Alloc(num_data_);
+      HIP_OK(hipMemcpy(d_teacher_rest_.ptr, meta.teacher_rest(), sizeof(float) * num_data_,
+                       hipMemcpyHostToDevice));
+    }
+  }
   weights_present_ = train_data->metadata().weights() != nullptr;
   if (weights_present_) {
     d_weight_.Alloc(num_data_);
@@ -3170,6 +3194,23 @@ void HIPTreeLearner::DeviceBoosting(const ObjectiveFunction* obj) {
     hipLaunchKernelGGL(hipk::k_grad_multiclass, g, b, 0, stream_, d_score_.ptr,
                        d_label_.ptr, weights_present_ ? d_weight_.ptr : nullptr, n,
                        num_class_score_, d_grad_.ptr, d_hess_.ptr);
+  } else if (name == "distill") {
+    const Metadata& meta = train_data_->metadata();
+    LGBM_DistillArgs a = class_ops::DistillArgsOf(meta, n, num_class_score_,
+                                                  config_->distill_temperature,
+                                                  config_->distill_alpha, d_score_.ptr);
+    if (a.k != teacher_slots_ || (a.teacher_rest.data != nullptr) != teacher_rest_)
+      Log::Fatal("The teacher was changed after the training data was uploaded");
+    a.teacher_class.data = d_teacher_class_.ptr;
+    a.teacher_logit.data = d_teacher_logit_.ptr;
+    if (teacher_rest_) a.teacher_rest.data = d_teacher_rest_.ptr;
+    a.label.data = d_label_.ptr;
+    a.weight.data = weights_present_ ? d_weight_.ptr : nullptr;
+    a.gradient = class_ops::ArrayOf(d_grad_.ptr, C_API_DTYPE_FLOAT32, 1, n);
+    a.hessian = class_ops::ArrayOf(d_hess_.ptr, C_API_DTYPE_FLOAT32, 1, n);
+    int device = 0;
+    HIP_OK(hipGetDevice(&device));
+    class_ops::Distill(a, device, stream_);
   } else if (name == "multiclassova") {
     hipLaunchKernelGGL(hipk::k_grad_multiclass_ova, g, b, 0, stream_, d_score_.ptr,
                        d_label_.ptr, weights_present_ ? d_weight_.ptr : nullptr, n,

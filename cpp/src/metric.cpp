@@ -1,5 +1,6 @@
 /*! migbm metrics: regression family, binary (logloss/error/auc/ap), multiclass, ranking
  *  (ndcg@/map@), cross-entropy. Parity target: reference src/metric/*. */
+#include "migbm/class_ops.h"
 #include "migbm/metric.h"
 #include "migbm/network.h"
 
@@ -279,6 +280,45 @@ class BinaryLoglossMetric : public Metric {
   const label_t* label_ = nullptr;
   const label_t* weights_ = nullptr;
   double sum_w_ = 0;
+};
+
+/*! mean of the distill objective's loss over the dataset's teacher and labels */
+class DistillLossMetric : public Metric {
+ public:
+  explicit DistillLossMetric(const Config& cfg)
+      : names_({"distill_loss"}),
+        nc_(cfg.num_class),
+        temperature_(cfg.distill_temperature),
+        alpha_(cfg.distill_alpha) {}
+  void Init(const Metadata& meta, data_size_t num_data) override {
+    num_data_ = num_data;
+    meta_ = &meta;
+    meta.CheckTeacher();
+    sum_w_ = num_data_;
+    if (meta.weights()) {
+      sum_w_ = 0;
+      for (data_size_t i = 0; i < num_data_; ++i) sum_w_ += meta.weights()[i];
+    }
+  }
+  const std::vector<std::string>& GetName() const override { return names_; }
+  double factor_to_bigger_better() const override { return 1.0; }
+  std::vector<double> Eval(const double* score, const ObjectiveFunction*) const override {
+    std::vector<double> loss(num_data_);
+    LGBM_DistillArgs a =
+        class_ops::DistillArgsOf(*meta_, num_data_, nc_, temperature_, alpha_, score);
+    a.loss = class_ops::ArrayOf(loss.data(), C_API_DTYPE_FLOAT64, 1);
+    class_ops::Distill(a, -1, nullptr);
+    double sum = 0;
+    for (double v : loss) sum += v;
+    return {GlobalAvg(sum, sum_w_)};
+  }
+
+ private:
+  std::vector<std::string> names_;
+  data_size_t num_data_ = 0;
+  int nc_;
+  double temperature_, alpha_, sum_w_ = 0;
+  const Metadata* meta_ = nullptr;
 };
 
 class MultiLoglossMetric : public Metric {
@@ -694,6 +734,8 @@ Metric* Metric::Create(const std::string& name, const Config& cfg) {
   if (name == "multi_logloss" || name == "softmax" || name == "multiclass" ||
       name == "multiclassova")
     return new MultiLoglossMetric(cfg.num_class);
+  if (name == "distill_loss" || name == "distill" || name == "distillation")
+    return new DistillLossMetric(cfg);
   if (name == "multi_error") return new MultiErrorMetric(cfg.num_class, cfg.multi_error_top_k);
   if (name == "auc_mu") return new AucMuMetric(cfg);
   if (name == "ndcg" || name == "lambdarank" || name == "rank_xendcg") return new NDCGMetric(cfg);

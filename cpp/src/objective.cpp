@@ -1,6 +1,7 @@
 /*! migbm objective functions: regression family, binary, multiclass, cross-entropy,
  *  lambdarank, rank_xendcg. Gradient formulas per the published algorithms (parity target:
  *  reference src/objective/*). */
+#include "migbm/class_ops.h"
 #include "migbm/objective.h"
 
 #include <algorithm>
@@ -446,6 +447,100 @@ class MulticlassSoftmax : public ObjectiveFunction {
   std::vector<data_size_t> class_counts_;
 };
 
+// ------------------------------------------------------------------ distillation
+/*! softmax regression on a teacher's top logits, mixed with the labels: the teacher comes
+ *  with the dataset (no counterpart in the reference; beside MulticlassSoftmax) */
+class Distill : public ObjectiveFunction {
+ public:
+  explicit Distill(const Config& cfg)
+      : num_class_(cfg.num_class),
+        temperature_(cfg.distill_temperature),
+        alpha_(cfg.distill_alpha) {}
+  void Init(const Metadata& meta, data_size_t num_data) override {
+    num_data_ = num_data;
+    meta_ = &meta;  // its arrays are looked up anew in each iteration, as they may be set again
+    LGBM_DistillArgs a = Args(nullptr);
+    a.scores.data = a.loss.data = &a;  // checked for presence alone
+    a.loss.type = C_API_DTYPE_FLOAT64;
+    class_ops::Check(a);
+    // where the boosting starts: the mean over the rows of what the scores are to reach. What
+    // the teacher leaves unnamed is shared evenly, a row without a teacher counts evenly too.
+    start_.assign(num_class_, 0.0);
+    std::vector<double> p(a.k);
+    std::vector<char> named(num_class_);
+    double sum_w = 0;
+    for (data_size_t i = 0; i < num_data_; ++i) {
+      const double w = meta.weights() ? meta.weights()[i] : 1.0;
+      const int32_t* cls = meta.teacher_class() + static_cast<size_t>(i) * a.k;
+      const float* logit = meta.teacher_logit() + static_cast<size_t>(i) * a.k;
+      double high = meta.teacher_rest() ? meta.teacher_rest()[i] : kMinScore;
+      std::fill(named.begin(), named.end(), 0);
+      int n = 0;
+      for (int j = 0; j < a.k; ++j) {
+        p[j] = -1.0;
+        if (cls[j] < 0 || cls[j] >= num_class_ || named[cls[j]]) continue;
+        named[cls[j]] = 1;
+        p[j] = 0.0;
+        ++n;
+        high = std::max(high, logit[j] / temperature_);
+      }
+      double rest = 1.0, sum = 1.0;
+      if (high > kMinScore) {
+        rest = meta.teacher_rest() ? std::exp(meta.teacher_rest()[i] - high) : 0.0;
+        sum = rest;
+        for (int j = 0; j < a.k; ++j)
+          if (p[j] == 0.0) sum += p[j] = std::exp(logit[j] / temperature_ - high);
+      }
+      if (!(sum > 0) || !std::isfinite(sum)) continue;
+      sum_w += w;
+      for (int j = 0; j < a.k; ++j)
+        if (p[j] > 0) start_[cls[j]] += w * alpha_ * p[j] / sum;
+      const int others = num_class_ - n;
+      if (others > 0)
+        for (int c = 0; c < num_class_; ++c)
+          if (!named[c]) start_[c] += w * alpha_ * rest / sum / others;
+      const int y = alpha_ < 1.0 ? static_cast<int>(meta.label()[i]) : -1;
+      if (y >= 0 && y < num_class_) start_[y] += w * (1.0 - alpha_);
+    }
+    for (double& s : start_)
+      s = std::log(std::max(kEpsilon, sum_w > 0 ? s / sum_w : 1.0 / num_class_));
+  }
+  void GetGradients(const double* score, score_t* grad, score_t* hess) const override {
+    LGBM_DistillArgs a = Args(score);
+    a.gradient = class_ops::ArrayOf(grad, C_API_DTYPE_FLOAT32, 1, num_data_);
+    a.hessian = class_ops::ArrayOf(hess, C_API_DTYPE_FLOAT32, 1, num_data_);
+    class_ops::Distill(a, -1, nullptr);
+  }
+  double BoostFromScore(int class_id) const override { return start_[class_id]; }
+  int NumModelPerIteration() const override { return num_class_; }
+  int NumPredictOneRow() const override { return num_class_; }
+  void ConvertOutput(const double* in, double* out) const override {
+    const double mx = *std::max_element(in, in + num_class_);
+    double sum = 0;
+    for (int c = 0; c < num_class_; ++c) sum += out[c] = std::exp(in[c] - mx);
+    for (int c = 0; c < num_class_; ++c) out[c] /= sum;
+  }
+  const char* GetName() const override { return "distill"; }
+  std::string ToString() const override {
+    std::stringstream ss;
+    ss.precision(17);
+    ss << "distill num_class:" << num_class_ << " distill_temperature:" << temperature_
+       << " distill_alpha:" << alpha_;
+    return ss.str();
+  }
+
+ private:
+  LGBM_DistillArgs Args(const double* score) const {
+    return class_ops::DistillArgsOf(*meta_, num_data_, num_class_, temperature_, alpha_, score);
+  }
+
+  data_size_t num_data_ = 0;
+  int num_class_;
+  double temperature_, alpha_;
+  const Metadata* meta_ = nullptr;
+  std::vector<double> start_;
+};
+
 class MulticlassOVA : public ObjectiveFunction {
  public:
   explicit MulticlassOVA(const Config& cfg) : num_class_(cfg.num_class), sigmoid_(cfg.sigmoid) {}
@@ -828,6 +923,7 @@ ObjectiveFunction* ObjectiveFunction::Create(const std::string& name, const Conf
   if (name == "tweedie") return new RegressionTweedieLoss(cfg);
   if (name == "binary") return new BinaryLogloss(cfg);
   if (name == "multiclass") return new MulticlassSoftmax(cfg);
+  if (name == "distill") return new Distill(cfg);
   if (name == "multiclassova") return new MulticlassOVA(cfg);
   if (name == "cross_entropy") return new CrossEntropy(cfg);
   if (name == "cross_entropy_lambda") return new CrossEntropyLambda(cfg);

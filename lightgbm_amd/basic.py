@@ -282,7 +282,7 @@ class Dataset:
 
     def __init__(self, data, label=None, reference=None, weight=None, group=None,
                  init_score=None, feature_name="auto", categorical_feature="auto",
-                 params=None, free_raw_data=True, position=None):
+                 params=None, free_raw_data=True, position=None, teacher=None):
         self.data = data
         self.label = label
         self.reference = reference
@@ -290,6 +290,7 @@ class Dataset:
         self.group = group
         self.init_score = init_score
         self.position = position
+        self.teacher = teacher
         self.feature_name = feature_name
         self.categorical_feature = categorical_feature
         self.params = dict(params) if params else {}
@@ -365,6 +366,8 @@ class Dataset:
             self.set_init_score(self.init_score)
         if self.position is not None:
             self.set_position(self.position)
+        if self.teacher is not None:
+            self.set_teacher(self.teacher)
         # feature names
         names = self._resolve_feature_names()
         if names is not None:
@@ -431,6 +434,14 @@ class Dataset:
             self.set_init_score(data)
         elif field_name == "position":
             self.set_position(data)
+        elif field_name in ("teacher_class", "teacher_logit", "teacher_log_rest"):
+            self.construct()
+            kind = np.int32 if field_name == "teacher_class" else np.float32
+            arr = np.ascontiguousarray(np.asarray(data).ravel(), dtype=kind)
+            _safe_call(_LIB.LGBM_DatasetSetField(
+                self._handle, _c_str(field_name), arr.ctypes.data_as(ctypes.c_void_p),
+                ctypes.c_int(len(arr)),
+                ctypes.c_int(_DTYPE_I32 if kind is np.int32 else _DTYPE_F32)))
         else:
             raise LightGBMError(f"Unknown field {field_name}")
         return self
@@ -502,6 +513,56 @@ class Dataset:
                 self._handle, _c_str("position"), arr.ctypes.data_as(ctypes.c_void_p),
                 ctypes.c_int(len(arr)), ctypes.c_int(_DTYPE_I32)))
         return self
+
+    def set_teacher(self, teacher):
+        """Give every row a teacher's top logits, for the distill objective and the
+        distill_loss metric: an ops.TopLogits or a tuple (classes, logits[, log_rest]) of
+        arrays of shape [rows, k], [rows, k] and [rows], log_rest at distill_temperature. The
+        dataset holds them in 32 bits. Tensors on a device are copied to the host. None takes the teacher away."""
+        self.teacher = teacher
+        if self._handle is None:
+            return self
+        if teacher is None:
+            for name in ("teacher_class", "teacher_logit", "teacher_log_rest"):
+                self.set_field(name, None)
+            return self
+        parts = [p.detach().cpu().float().numpy() if hasattr(p, "detach") and
+                 p.dtype.is_floating_point else p.cpu().numpy() if hasattr(p, "detach") else
+                 None if p is None else np.asarray(p) for p in teacher]
+        if not 2 <= len(parts) <= 3:
+            raise LightGBMError("teacher must be (classes, logits) or (classes, logits, log_rest)")
+        classes, logits = parts[0], parts[1]
+        rest = parts[2] if len(parts) == 3 else None
+        rows = self.num_data()
+        if classes.ndim != 2 or classes.shape[0] != rows or not 1 <= classes.shape[1] <= 256:
+            raise LightGBMError(f"teacher classes must have the shape [{rows}, 1..256], "
+                                f"got {list(classes.shape)}")
+        if classes.dtype.kind not in "iu":
+            raise LightGBMError("teacher classes must be integers")
+        if logits.shape != classes.shape:
+            raise LightGBMError(f"teacher logits must have the shape {list(classes.shape)}, "
+                                f"got {list(logits.shape)}")
+        if rest is not None and rest.shape != (rows,):
+            raise LightGBMError(f"teacher log_rest must have the shape [{rows}], "
+                                f"got {list(rest.shape)}")
+        # ids that 32 bits do not hold are no classes
+        big = np.iinfo(np.int32).max
+        classes = np.where((classes >= 0) & (classes <= big), classes, -1)
+        self.set_field("teacher_class", classes)
+        self.set_field("teacher_logit", logits)
+        self.set_field("teacher_log_rest", rest)
+        return self
+
+    def get_teacher(self):
+        """The teacher as ops.TopLogits of numpy arrays, or None."""
+        from .ops import TopLogits
+        classes = self.get_field("teacher_class")
+        if classes is None:
+            return None
+        rows = self.num_data()
+        return TopLogits(classes.reshape(rows, -1),
+                         self.get_field("teacher_logit").reshape(rows, -1),
+                         self.get_field("teacher_log_rest"))
 
     def set_init_score(self, init_score):
         self.init_score = init_score
@@ -609,10 +670,10 @@ class Dataset:
         return ds
 
     def create_valid(self, data, label=None, weight=None, group=None, init_score=None,
-                     params=None, position=None):
+                     params=None, position=None, teacher=None):
         return Dataset(data, label=label, reference=self, weight=weight, group=group,
                        init_score=init_score, params=params or dict(self.params),
-                       position=position)
+                       position=position, teacher=teacher)
 
     def get_feature_name(self):
         self.construct()
@@ -1030,6 +1091,34 @@ class Booster:
             res = res.astype(np.int32)
         return res
 
+    def top_logits(self, data, k, temperature=1.0, **kwargs):
+        """This booster as a teacher: ops.top_logits of its raw class scores for `data`, to be
+        given to a student's Dataset. kwargs go to predict."""
+        from .ops import top_logits
+        scores = self.predict(data, raw_score=True, **kwargs)
+        if scores.ndim != 2:
+            raise LightGBMError("top_logits needs a booster with several classes")
+        return top_logits(scores, k, temperature=temperature)
+
+    def verify_drafts(self, data, drafts, draft_prob, accept_uniform, sample_uniform,
+                      lengths=None, **kwargs):
+        """This booster as the target of ops.verify_drafts: `data` has drafts + 1 rows for each
+        sequence, one after the other, the features of each drafted place and of the one after.
+        drafts: [sequences, drafts]. kwargs go to predict."""
+        from .ops import verify_drafts
+        drafts = np.asarray(drafts)
+        if drafts.ndim != 2:
+            raise LightGBMError(f"drafts must have 2 dimensions, got {list(drafts.shape)}")
+        target = self.predict(data, **kwargs)
+        if target.ndim != 2:
+            raise LightGBMError("verify_drafts needs a booster with several classes")
+        places = drafts.shape[1] + 1
+        if target.shape[0] != drafts.shape[0] * places:
+            raise LightGBMError(f"data must have {drafts.shape[0]} * {places} rows, "
+                                f"got {target.shape[0]}")
+        return verify_drafts(target.reshape(drafts.shape[0], places, -1), drafts, draft_prob,
+                             accept_uniform, sample_uniform, lengths=lengths)
+
     def refit(self, data, label, decay_rate=0.9, **kwargs):
         leaf_preds = self.predict(data, pred_leaf=True)
         if leaf_preds.ndim == 1:
@@ -1037,7 +1126,8 @@ class Booster:
         nrow, ncol = leaf_preds.shape
         new_params = dict(self.params)
         new_params["refit_decay_rate"] = decay_rate
-        train_set = Dataset(data, label=label, params=new_params)
+        train_set = Dataset(data, label=label, params=new_params,
+                            teacher=kwargs.get("teacher"))
         new_booster = Booster(new_params, train_set)
         # copy model
         _safe_call(_LIB.LGBM_BoosterMerge(new_booster._handle, self._handle))
