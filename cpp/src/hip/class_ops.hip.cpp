@@ -284,6 +284,260 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
   if (cls >= 0) put(cls, z_slot, p, false);
 }
 
+// ------------------------------------------------------------------ distillation, few classes
+/*!
+ * The threads that share a row. kAcross: a class's rows stand next to each other in memory
+ * (a booster's scores), so neighbouring threads are neighbouring rows, and a row's L threads
+ * are R apart; otherwise a row's threads are L neighbours. Thread l of a row holds the
+ * classes e * L + l. R * L = 256.
+ */
+template <bool kAcross> struct Team {
+  int L, R, l, r;
+  __device__ explicit Team(int lanes) : L(lanes), R(256 / lanes) {
+    l = kAcross ? threadIdx.x / R : threadIdx.x % L;
+    r = kAcross ? threadIdx.x % R : threadIdx.x / L;
+  }
+  /*! of one thread a row nothing is shared */
+  __device__ void Sync() const {
+    if (!(kAcross && L == 1)) __syncthreads();
+  }
+  template <typename A, typename F> __device__ A Reduce(A v, A* lds, const F& f) const {
+    if (kAcross) {
+      if (L == 1) return v;
+      __syncthreads();
+      lds[threadIdx.x] = v;
+      __syncthreads();
+      v = lds[r];
+      for (int i = 1; i < L; ++i) v = f(v, lds[i * R + r]);
+      return v;
+    }
+    for (int d = L / 2; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
+    return v;
+  }
+  template <typename A> __device__ A Sum(A v, A* lds) const {
+    return Reduce(v, lds, [](A a, A b) { return a + b; });
+  }
+  template <typename A> __device__ A Max(A v, A* lds) const {
+    return Reduce(v, lds, [](A a, A b) { return class_ops::Max(a, b); });
+  }
+};
+
+template <typename A>
+using Word = std::conditional_t<std::is_same_v<A, double>, unsigned long long, unsigned int>;
+__device__ __forceinline__ unsigned int ToBits(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ unsigned long long ToBits(double v) { return __double_as_longlong(v); }
+__device__ __forceinline__ float FromBits(unsigned int v) { return __uint_as_float(v); }
+__device__ __forceinline__ double FromBits(unsigned long long v) { return __longlong_as_double(v); }
+
+/*! more than 32 KiB of dynamic LDS has to be asked for */
+template <typename F> void AllowLds(F* kernel, size_t bytes) {
+  if (bytes > 32768)
+    OPS_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(bytes)));
+}
+
+/*!
+ * Up to E * L classes: a row is read once and stays in its threads' registers. What the
+ * teacher wants of each class is a table in LDS, one word a class: first the lowest slot that
+ * names the class (with the sign bit set, kNone: none), then that slot's probability.
+ */
+template <typename T, int E, bool kAcross>
+__global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int lanes) {
+  using A = Acc<T>;
+  using O = Out<T>;
+  using W = Word<A>;
+  constexpr W kNone = ~W{0}, kSlot = W{1} << (sizeof(W) * 8 - 1);
+  extern __shared__ unsigned long long tile_lds[];
+  W* want = reinterpret_cast<W*>(tile_lds);  // R * classes
+  __shared__ A red[256];
+  const Team<kAcross> team(lanes);
+  const int c = a.classes, k = a.k, L = team.L, R = team.R;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * R + team.r;
+  const bool there = row < a.rows;
+  auto place = [&](int cls) { return kAcross ? cls * R + team.r : team.r * c + cls; };
+
+  const A w = !there ? A(0) : a.weight.data ? LoadFloat<A>(a.weight, row * a.weight.stride[0])
+                                            : A(1);
+  A z[E];
+  {
+    const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int cls = e * L + team.l;
+      const bool read = w != A(0) && cls < c;
+      z[e] = read ? static_cast<A>(x[cls * a.scores.stride[1]]) : NegInf<A>();
+      if (cls < c) want[place(cls)] = kNone;
+    }
+  }
+  team.Sync();
+  auto load_class = [&](int j) {
+    return LoadClass(a.teacher_class,
+                     row * a.teacher_class.stride[0] + j * a.teacher_class.stride[1], c);
+  };
+  const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
+  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
+  auto load_logit = [&](int j) {
+    return scale * LoadFloat<A>(a.teacher_logit,
+                                row * a.teacher_logit.stride[0] + j * a.teacher_logit.stride[1]);
+  };
+  const bool teach = w != A(0) && alpha > A(0);
+  if (teach) {
+    for (int j = team.l; j < k; j += L) {
+      const int cls = load_class(j);
+      if (cls >= 0) atomicMin(&want[place(cls)], kSlot | static_cast<W>(j));
+    }
+  }
+  A high = NegInf<A>();
+#pragma unroll
+  for (int e = 0; e < E; ++e) high = Max(high, z[e]);
+  high = team.Max(high, red);
+  if (!(high > NegInf<A>())) high = A(0);
+  team.Sync();
+
+  // the teacher's distribution, in logarithms to base two
+  const bool rest = a.teacher_rest.data != nullptr;
+  const A r = rest && teach ? scale1 * LoadFloat<A>(a.teacher_rest, row * a.teacher_rest.stride[0])
+                            : NegInf<A>();
+  A t_high = r;
+  A t_nan = r != r ? A(1) : A(0);
+  auto for_slots = [&](auto&& f) {  // the slots that count
+    if (!teach) return;
+    for (int j = team.l; j < k; j += L) {
+      const int cls = load_class(j);
+      if (cls < 0) continue;
+      W* at = &want[place(cls)];
+      if (*at == (kSlot | static_cast<W>(j))) f(j, cls, at);
+    }
+  };
+  for_slots([&](int j, int, W*) {
+    const A t = load_logit(j);
+    t_high = Max(t_high, t);
+    if (t != t) t_nan = A(1);
+  });
+  t_high = team.Max(t_high, red);
+  t_nan = team.Max(t_nan, red);
+  const bool taught = teach && (t_high > NegInf<A>() || t_nan > A(0));
+  if (!(t_high > NegInf<A>())) t_high = A(0);
+  A t_sum = 0;
+  for_slots([&](int j, int, W*) { t_sum += Exp2(load_logit(j) - t_high); });
+  const A u_rest = rest ? Exp2(r - t_high) : A(0);
+  t_sum = team.Sum(t_sum, red) + u_rest;
+  const A t_inv = taught ? A(1) / t_sum : A(0), t_log = t_high + Log2(t_sum);
+  const A share = taught ? u_rest * t_inv : A(0);
+
+  // the student's: the classes without a slot are summed on their own
+  const A off = -high * scale, off1 = -high * scale1;
+  const bool two = alpha < A(1);
+  A ez[E], left = 0, named = 0, total1 = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int cls = e * L + team.l;
+    ez[e] = Exp2(Fma(z[e], scale, off));
+    if (cls < c && want[place(cls)] != kNone) named += ez[e];
+    else left += ez[e];
+    if (two) total1 += Exp2(Fma(z[e], scale1, off1));
+  }
+  left = team.Sum(left, red);
+  const A total = left + team.Sum(named, red);
+  if (two) total1 = team.Sum(total1, red);
+  const A log_total = Log2(total);
+  A log_left = Log2(left), rest_off = off;
+  const bool again = rest && left < SmallRest<A>();
+  if (__syncthreads_or(again)) {
+    A own = NegInf<A>();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int cls = e * L + team.l;
+      if (cls < c && want[place(cls)] == kNone) own = Max(own, z[e]);
+    }
+    own = team.Max(own, red);
+    const bool able = again && own > NegInf<A>();
+    const A own_off = -own * scale;
+    A sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int cls = e * L + team.l;
+      if (able && cls < c && want[place(cls)] == kNone) sum += Exp2(Fma(z[e], scale, own_off));
+    }
+    sum = team.Sum(sum, red);
+    if (able) {
+      left = sum;
+      rest_off = own_off;
+      log_left = Log2(left) - rest_off + off;
+    }
+  }
+  const bool live = w != A(0) && !(total == A(0));  // otherwise every class is masked
+  const int y = two && live ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
+
+  // the table's slots give way to their probabilities; every class has one such slot
+  A kl = 0;
+  const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+  team.Sync();
+  for_slots([&](int j, int cls, W* at) {
+    const A lp = load_logit(j) - t_log;
+    const A p = taught ? Exp2(lp) : A(0);
+    if (a.loss.data && !(p == A(0))) {
+      const A v = static_cast<A>(x[cls * a.scores.stride[1]]);
+      kl += p * (lp - (Fma(v, scale, off) - log_total));
+    }
+    *at = ToBits(p) & ~kSlot;
+  });
+  if (a.loss.data) {
+    kl = team.Sum(kl, red);
+    if (there && team.l == 0) {
+      A v = 0;
+      if (live) {
+        if (rest && !(share == A(0))) kl += share * (r - t_log - (log_left - log_total));
+        if (taught) v = alpha * temp * temp * (kl * static_cast<A>(kLn2));
+        if (y >= 0)
+          v += (A(1) - alpha) * static_cast<A>(kLn2) *
+               (Log2(total1) - Fma(static_cast<A>(x[y * a.scores.stride[1]]), scale1, off1));
+        v *= w;
+      }
+      StoreFloat(a.loss, row * a.loss.stride[0], v);
+    }
+  }
+  if (!a.gradient.data && !a.hessian.data) return;
+  team.Sync();
+  const A soft = taught ? alpha : A(0), hard = y >= 0 ? A(1) - alpha : A(0);
+  const A inv = A(1) / total, inv1 = hard > A(0) ? A(1) / total1 : A(0);
+  const A spread = rest && left > A(0) ? share / left : A(0);
+  const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
+  const bool moved = rest_off != off;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int cls = e * L + team.l;
+    if (!there || cls >= c) continue;
+    A g = 0, h = 0;
+    if (live) {
+      const A q = ez[e] * inv;
+      if (soft > A(0)) {
+        const W bits = want[place(cls)];
+        A p = FromBits(bits);
+        if (bits == kNone) {
+          p = A(0);
+          if (spread > A(0)) p = spread * (moved ? Exp2(Fma(z[e], scale, rest_off)) : ez[e]);
+          else if (spread != spread) p = spread;
+        }
+        g = soft * temp * (q - p);
+        h = soft * q * (A(1) - q);
+      }
+      if (hard > A(0)) {
+        const A q1 = Exp2(Fma(z[e], scale1, off1)) * inv1;
+        g += hard * (q1 - (cls == y ? A(1) : A(0)));
+        h += hard * q1 * (A(1) - q1);
+      }
+    }
+    if (a.gradient.data)
+      static_cast<O*>(a.gradient.data)[row * a.gradient.stride[0] + cls * a.gradient.stride[1]] =
+          static_cast<O>(g * w);
+    if (a.hessian.data)
+      static_cast<O*>(a.hessian.data)[row * a.hessian.stride[0] + cls * a.hessian.stride[1]] =
+          static_cast<O>(h * factor * w);
+  }
+}
+
 // ------------------------------------------------------------------ top logits, any strides
 /*! keys order as the values do, zeros of both signs alike; 0: never chosen (NaN, -inf) */
 __device__ __forceinline__ uint32_t KeyOf(float v) {
@@ -655,17 +909,45 @@ void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
   OPS_HIP_OK(hipGetLastError());
 }
 
+/*! the smallest power of two of threads that hold `classes` at `each` a thread */
+int LanesFor(int classes, int each) {
+  int lanes = 1;
+  while (lanes * each < classes) lanes *= 2;
+  return lanes;
+}
+
+template <typename T, int E, bool kAcross>
+void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
+  const int lanes = LanesFor(a.classes, E), rows = 256 / lanes;
+  const size_t lds = sizeof(Word<Acc<T>>) * rows * a.classes;  // at most 2048 * E bytes
+  auto kernel = k_distill_tile<T, E, kAcross>;
+  AllowLds(kernel, lds);
+  hipLaunchKernelGGL(kernel,
+                     dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256), lds, s, a,
+                     lanes);
+}
+
 void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
   OnDevice on(device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t row_step = std::abs(a.scores.stride[0]);  // 0: one row for all
+  const bool across = row_step != 0 && row_step < std::abs(a.scores.stride[1]);
+  if (a.classes <= (across ? 512 : 256)) {
+    ByType(a.scores.type, [&](auto t) {
+      using T = decltype(t);
+      if (!across) LaunchDistillTile<T, 4, false>(a, s);
+      else if (a.classes <= 8) LaunchDistillTile<T, 8, true>(a, s);
+      else if (a.classes <= 256) LaunchDistillTile<T, 16, true>(a, s);
+      else LaunchDistillTile<T, 32, true>(a, s);
+    });
+    OPS_HIP_OK(hipGetLastError());
+    return;
+  }
   const dim3 grid(static_cast<uint32_t>(a.rows));
   const size_t lds = sizeof(uint32_t) * ((a.classes + 31) / 32);
   ByType(a.scores.type, [&](auto t) {
     auto kernel = k_distill_any<decltype(t), 256>;
-    if (lds > 32768)
-      OPS_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                     hipFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(lds)));
+    AllowLds(kernel, lds);
     hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, a);
   });
   OPS_HIP_OK(hipGetLastError());
