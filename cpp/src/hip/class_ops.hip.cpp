@@ -538,6 +538,328 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   }
 }
 
+// ------------------------------------------------------------------ rows of many classes
+using Words = uint32_t __attribute__((ext_vector_type(4)));
+
+/*! sixteen bytes of a row: as many elements as they hold */
+template <typename T> struct Chunk {
+  static constexpr int kSize = 16 / sizeof(T);
+  T v[kSize];
+};
+
+/*!
+ * A row whose classes stand next to each other, as its workgroup holds it: the first
+ * kBlock * kCached chunks in registers, one chunk a thread in turn, further chunks read again
+ * in each pass, and the classes after the last whole chunk one a thread. Chunks are read at
+ * their elements' alignment: the hardware splits what crosses a line.
+ */
+template <typename T, int kBlock, int kCached> struct RowOf {
+  static constexpr int kSize = Chunk<T>::kSize;
+  using A = Acc<T>;
+  const T* x;
+  int chunks, tail;  // whole chunks, and the class of this thread after them (-1: none)
+  A tail_value;
+  Words raw[kCached];
+
+  __device__ __forceinline__ RowOf(const T* row, int classes)
+      : x(row), chunks(classes / kSize) {
+    tail = chunks * kSize + static_cast<int>(threadIdx.x);
+    if (tail >= classes) tail = -1;
+  }
+  __device__ __forceinline__ Words Read(int chunk) const {
+    Words got;
+    __builtin_memcpy(&got, x + static_cast<int64_t>(chunk) * kSize, sizeof(got));
+    return got;
+  }
+  __device__ __forceinline__ void Load() {
+#pragma unroll
+    for (int n = 0; n < kCached; ++n) {
+      const int chunk = n * kBlock + threadIdx.x;
+      raw[n] = chunk < chunks ? Read(chunk) : Words{};
+    }
+    tail_value = tail >= 0 ? static_cast<A>(x[tail]) : A(0);
+  }
+  template <typename F>
+  static __device__ __forceinline__ void Give(const Words& words, int chunk, const F& f) {
+    Chunk<T> got;
+    __builtin_memcpy(&got, &words, sizeof(got));
+    A v[kSize];
+#pragma unroll
+    for (int i = 0; i < kSize; ++i) v[i] = static_cast<A>(got.v[i]);
+    f(chunk * kSize, v);
+  }
+  /*! f(first class, values) of all that this thread holds, kSize or one at a time */
+  template <typename F> __device__ __forceinline__ void Each(const F& f) {
+#pragma unroll
+    for (int n = 0; n < kCached; ++n) {
+      // what a pass makes of the row is not kept for the next: the compiler would hold its
+      // conversions and exponentials in registers that are not there
+      asm volatile("" : "+v"(raw[n]));
+      const int chunk = n * kBlock + threadIdx.x;
+      if (chunk < chunks) Give(raw[n], chunk, f);
+    }
+#pragma unroll 4
+    for (int chunk = kCached * kBlock + threadIdx.x; chunk < chunks; chunk += kBlock)
+      Give(Read(chunk), chunk, f);
+    if (tail >= 0) {
+      const A v[1] = {tail_value};
+      f(tail, v);
+    }
+  }
+};
+
+template <typename V> constexpr int kSizeOf = std::extent_v<std::remove_reference_t<V>>;
+
+/*! kCount sums over the workgroup at once; `lds` has kCount * waves places */
+template <int kBlock, int kCount, typename A>
+__device__ __forceinline__ void BlockSums(A (&v)[kCount], A* lds) {
+  constexpr int kWaves = kBlock / kWave;
+#pragma unroll
+  for (int n = 0; n < kCount; ++n) {
+    v[n] = WaveSum(v[n]);
+    if (threadIdx.x % kWave == 0) lds[n * kWaves + threadIdx.x / kWave] = v[n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kCount; ++n) {
+    v[n] = lds[n * kWaves];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) v[n] += lds[n * kWaves + i];
+  }
+}
+
+/*!
+ * One workgroup a row of many classes: read once, as far as its registers reach, then the
+ * maximum, the sums and the gradients from there. A thread looks at the bits of its chunk's
+ * slots together, and leaves the fast path only where one is set.
+ */
+template <typename T, int kBlock, int kCached>
+__global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
+  using A = Acc<T>;
+  using O = Out<T>;
+  using Row = RowOf<T, kBlock, kCached>;
+  constexpr int kWaves = kBlock / kWave;
+  extern __shared__ uint32_t mark[];
+  __shared__ int s_cls[kMaxTop];
+  __shared__ A s_max[2][kWaves], s_sum[4 * kWaves], s_more[3][kWaves];
+  __shared__ int s_dup;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, c = a.classes, k = a.k;
+  O* grad = a.gradient.data ? static_cast<O*>(a.gradient.data) + row * a.gradient.stride[0]
+                            : nullptr;
+  O* hess = a.hessian.data ? static_cast<O*>(a.hessian.data) + row * a.hessian.stride[0]
+                           : nullptr;
+  const A w = a.weight.data ? LoadFloat<A>(a.weight, row * a.weight.stride[0]) : A(1);
+  auto put_zeros = [&] {
+    if (a.loss.data && tid == 0) StoreFloat(a.loss, row * a.loss.stride[0], A(0));
+    for (int i = tid; i < c; i += kBlock) {
+      if (grad) grad[i] = static_cast<O>(0.0f);
+      if (hess) hess[i] = static_cast<O>(0.0f);
+    }
+  };
+  if (w == A(0)) {
+    put_zeros();
+    return;
+  }
+  Row z(static_cast<const T*>(a.scores.data) + row * a.scores.stride[0], c);
+  z.Load();
+  for (int i = tid; i < (c + 31) / 32; i += kBlock) mark[i] = 0;
+  if (tid == 0) s_dup = 0;
+
+  // the slots, one a thread
+  const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
+  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
+  const bool rest = a.teacher_rest.data != nullptr, two = alpha < A(1);
+  int cls = -1;
+  A logit = NegInf<A>(), z_slot = NegInf<A>();
+  if (tid < k) {
+    cls = LoadClass(a.teacher_class,
+                    row * a.teacher_class.stride[0] + tid * a.teacher_class.stride[1], c);
+    if (cls >= 0) {
+      logit = scale * LoadFloat<A>(a.teacher_logit, row * a.teacher_logit.stride[0] +
+                                                        tid * a.teacher_logit.stride[1]);
+      z_slot = static_cast<A>(z.x[cls]);
+    }
+    s_cls[tid] = cls;
+  }
+  const A r = rest ? scale1 * LoadFloat<A>(a.teacher_rest, row * a.teacher_rest.stride[0])
+                   : NegInf<A>();
+  const int label = two ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
+  const A z_label = label >= 0 ? static_cast<A>(z.x[label]) : A(0);
+  __syncthreads();
+  if (cls >= 0 && (atomicOr(&mark[cls >> 5], 1u << (cls & 31)) >> (cls & 31) & 1u)) s_dup = 1;
+
+  A high = NegInf<A>();
+  z.Each([&](int, const auto& v) {
+#pragma unroll
+    for (int i = 0; i < kSizeOf<decltype(v)>; ++i) high = Max(high, v[i]);
+  });
+  high = WaveMax(high);
+  A t_high = WaveMax(Max(logit, r));
+  if (tid % kWave == 0) {
+    s_max[0][tid / kWave] = high;
+    s_max[1][tid / kWave] = t_high;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    high = Max(high, s_max[0][i]);
+    t_high = Max(t_high, s_max[1][i]);
+  }
+  if (s_dup) {  // the first slot of a class counts
+    for (int i = 0; i < tid && tid < k; ++i)
+      if (s_cls[i] == cls) cls = -1;
+    if (cls < 0) logit = z_slot = NegInf<A>();
+    t_high = BlockMax<kBlock>(Max(logit, r), s_more[0]);
+  }
+  if (!(high > NegInf<A>())) high = A(0);
+  const bool t_some = t_high > NegInf<A>();
+  if (!t_some) t_high = A(0);
+
+  const A off = -high * scale, off1 = -high * scale1;
+  auto bits_of = [&](int base, int size) {  // those of a chunk stand in one word
+    return mark[base >> 5] >> (base & 31) & ((1u << size) - 1u);
+  };
+  A left = 0, total1 = 0;
+  z.Each([&](int base, const auto& v) {
+    constexpr int kSize = kSizeOf<decltype(v)>;
+    const uint32_t bits = bits_of(base, kSize);
+    A e[kSize], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kSize; ++i) e[i] = Exp2(Fma(v[i], scale, off));
+    if (bits == 0) {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) sum += e[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) sum += bits >> i & 1u ? A(0) : e[i];
+    }
+    left += sum;
+    if (two) {
+      sum = 0;
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) sum += Exp2(Fma(v[i], scale1, off1));
+      total1 += sum;
+    }
+  });
+  const A log_e = Fma(z_slot, scale, off);
+  A sums[4] = {left, cls >= 0 ? Exp2(log_e) : A(0),
+               cls >= 0 && !(logit == NegInf<A>()) ? Exp2(logit - t_high) : A(0), total1};
+  const A u = sums[2];
+  BlockSums<kBlock>(sums, s_sum);
+  left = sums[0];
+  total1 = sums[3];
+  const A total = left + sums[1];
+  if (total == A(0)) {  // every class is masked
+    put_zeros();
+    return;
+  }
+  const A u_rest = rest ? Exp2(r - t_high) : A(0);
+  const A t_sum = sums[2] + u_rest;
+  const bool taught = alpha > A(0) && (t_some || t_sum != t_sum);
+  const A t_log = t_high + Log2(t_sum), log_total = Log2(total);
+  const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
+  A log_left = Log2(left), rest_off = off;
+  if (rest && left < SmallRest<A>()) {
+    A own = NegInf<A>();
+    z.Each([&](int base, const auto& v) {
+    constexpr int kSize = kSizeOf<decltype(v)>;
+      const uint32_t bits = bits_of(base, kSize);
+#pragma unroll
+      for (int i = 0; i < kSize; ++i)
+        if (!(bits >> i & 1u)) own = Max(own, v[i]);
+    });
+    own = BlockMax<kBlock>(own, s_more[1]);
+    if (own > NegInf<A>()) {
+      rest_off = -own * scale;
+      left = 0;
+      z.Each([&](int base, const auto& v) {
+    constexpr int kSize = kSizeOf<decltype(v)>;
+        const uint32_t bits = bits_of(base, kSize);
+#pragma unroll
+        for (int i = 0; i < kSize; ++i)
+          if (!(bits >> i & 1u)) left += Exp2(Fma(v[i], scale, rest_off));
+      });
+      left = BlockSum<kBlock>(left, s_more[2]);
+      log_left = Log2(left) - rest_off + off;
+    }
+  }
+
+  if (a.loss.data) {
+    A kl[1] = {cls >= 0 && !(p == A(0)) ? p * (logit - t_log - (log_e - log_total)) : A(0)};
+    __syncthreads();
+    BlockSums<kBlock>(kl, s_sum);
+    if (tid == 0) {
+      if (rest && !(share == A(0))) kl[0] += share * (r - t_log - (log_left - log_total));
+      A v = taught ? alpha * temp * temp * (kl[0] * static_cast<A>(kLn2)) : A(0);
+      if (label >= 0)
+        v += (A(1) - alpha) * static_cast<A>(kLn2) * (Log2(total1) - Fma(z_label, scale1, off1));
+      StoreFloat(a.loss, row * a.loss.stride[0], v * w);
+    }
+  }
+  if (!grad && !hess) return;
+  const A soft = taught ? alpha : A(0), hard = label >= 0 ? A(1) - alpha : A(0);
+  const A inv = A(1) / total, inv1 = hard > A(0) ? A(1) / total1 : A(0);
+  const A spread = rest && left > A(0) ? share / left : A(0);
+  const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
+  const bool moved = rest_off != off;
+  // a class without a slot: its gradient is one factor of each exponential
+  const A coef = soft > A(0) ? w * soft * temp * (moved ? inv : inv - spread) : A(0);
+  const A coef_rest = moved && soft > A(0) ? -w * soft * temp * spread : A(0);
+  const A coef1 = hard > A(0) ? w * hard * inv1 : A(0);
+  auto gradient_of = [&](A v) {
+    A g = coef * Exp2(Fma(v, scale, off));
+    if (hard > A(0)) g = Fma(coef1, Exp2(Fma(v, scale1, off1)), g);
+    if (moved) g = Fma(coef_rest, Exp2(Fma(v, scale, rest_off)), g);
+    return g;
+  };
+  auto hessian_of = [&](A v) {
+    const A q = Exp2(Fma(v, scale, off)) * inv;
+    A h = soft > A(0) ? soft * q * (A(1) - q) : A(0);
+    if (hard > A(0)) {
+      const A q1 = Exp2(Fma(v, scale1, off1)) * inv1;
+      h += hard * q1 * (A(1) - q1);
+    }
+    return h * factor * w;
+  };
+  z.Each([&](int base, const auto& v) {
+    constexpr int kSize = kSizeOf<decltype(v)>;
+    const uint32_t bits = bits_of(base, kSize);
+    O g[kSize], h[kSize];
+    if (grad) {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) g[i] = static_cast<O>(gradient_of(v[i]));
+    }
+    if (hess) {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) h[i] = static_cast<O>(hessian_of(v[i]));
+    }
+    if (bits == 0 &&
+        static_cast<unsigned>(label - base) >= static_cast<unsigned>(kSize)) {
+      if (grad) __builtin_memcpy(grad + base, &g, sizeof(O) * kSize);
+      if (hess) __builtin_memcpy(hess + base, &h, sizeof(O) * kSize);
+    } else {  // a slot's class is its thread's, below
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) {
+        if (bits >> i & 1u) continue;
+        if (grad)
+          grad[base + i] = base + i == label
+                               ? static_cast<O>(gradient_of(v[i]) - w * hard)
+                               : g[i];
+        if (hess) hess[base + i] = h[i];
+      }
+    }
+  });
+  if (cls >= 0) {
+    const A q = Exp2(log_e) * inv;
+    A g = soft > A(0) ? soft * temp * (q - p) : A(0);
+    if (hard > A(0))
+      g += hard * (Exp2(Fma(z_slot, scale1, off1)) * inv1 - (cls == label ? A(1) : A(0)));
+    if (grad) grad[cls] = static_cast<O>(g * w);
+    if (hess) hess[cls] = static_cast<O>(hessian_of(z_slot));
+  }
+}
+
 // ------------------------------------------------------------------ top logits, any strides
 /*! keys order as the values do, zeros of both signs alike; 0: never chosen (NaN, -inf) */
 __device__ __forceinline__ uint32_t KeyOf(float v) {
@@ -927,6 +1249,14 @@ void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
                      lanes);
 }
 
+template <typename T, int kBlock, int kCached>
+void LaunchDistillRow(const LGBM_DistillArgs& a, hipStream_t s) {
+  auto kernel = k_distill_row<T, kBlock, kCached>;
+  const size_t lds = sizeof(uint32_t) * ((a.classes + 31) / 32);
+  AllowLds(kernel, lds);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(kBlock), lds, s, a);
+}
+
 void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
   OnDevice on(device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -939,6 +1269,24 @@ void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
       else if (a.classes <= 8) LaunchDistillTile<T, 8, true>(a, s);
       else if (a.classes <= 256) LaunchDistillTile<T, 16, true>(a, s);
       else LaunchDistillTile<T, 32, true>(a, s);
+    });
+    OPS_HIP_OK(hipGetLastError());
+    return;
+  }
+  if (a.scores.stride[1] == 1 && a.scores.type != C_API_DTYPE_FLOAT64 &&
+      (!a.gradient.data || a.gradient.stride[1] == 1) &&
+      (!a.hessian.data || a.hessian.stride[1] == 1)) {
+    ByType(a.scores.type, [&](auto t) {
+      using T = decltype(t);
+      if constexpr (!std::is_same_v<T, double>) {
+        constexpr int kSize = Chunk<T>::kSize;
+        const int chunks = (a.classes + kSize - 1) / kSize;
+        if (chunks <= 256) LaunchDistillRow<T, 256, 1>(a, s);
+        else if (chunks <= 1024) LaunchDistillRow<T, 256, 4>(a, s);
+        else if (chunks <= 4096) LaunchDistillRow<T, 512, 8>(a, s);
+        else if (chunks <= 8192) LaunchDistillRow<T, 1024, 8>(a, s);
+        else LaunchDistillRow<T, 1024, 12>(a, s);
+      }
     });
     OPS_HIP_OK(hipGetLastError());
     return;
