@@ -13,6 +13,7 @@
 #include "migbm/common.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace migbm {
@@ -909,7 +910,7 @@ __device__ __forceinline__ void PickDigit(const int* hist, int take, int* digit,
  * way, and what is chosen is put in order by counting how many precede it.
  */
 template <typename T, int kBlock>
-__global__ void __launch_bounds__(kBlock) k_top_any(LGBM_TopLogitsArgs a) {
+__device__ __forceinline__ void TopAny(const LGBM_TopLogitsArgs& a, int64_t row) {
   using A = Acc<T>;
   using K = Key<T>;
   __shared__ int hist[256];
@@ -917,7 +918,6 @@ __global__ void __launch_bounds__(kBlock) k_top_any(LGBM_TopLogitsArgs a) {
   __shared__ K s_key[kMaxTop];
   __shared__ int s_cls[kMaxTop];
   __shared__ A s_red[2][kBlock / kWave];
-  const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, c = a.classes;
   const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
   const int64_t xs = a.scores.stride[1];
@@ -1020,6 +1020,292 @@ __global__ void __launch_bounds__(kBlock) k_top_any(LGBM_TopLogitsArgs a) {
     StoreFloat(a.log_rest, row * a.log_rest.stride[0],
                sum > A(0) ? other / static_cast<A>(a.temperature) + Log2(sum) * static_cast<A>(kLn2)
                           : other);
+}
+
+template <typename T, int kBlock>
+__global__ void __launch_bounds__(kBlock) k_top_any(LGBM_TopLogitsArgs a) {
+  TopAny<T, kBlock>(a, blockIdx.x);
+}
+
+// ------------------------------------------------------------------ top logits, few classes
+/*!
+ * Up to E * L classes, in the registers of their row's threads (Team): k times the largest
+ * that is left, by comparison with all others. Of equals the lowest class is met first.
+ */
+template <typename T, int E, bool kAcross>
+__global__ void __launch_bounds__(256) k_top_tile(LGBM_TopLogitsArgs a, int lanes) {
+  using A = Acc<T>;
+  __shared__ A red[256];
+  __shared__ int red_cls[256];
+  const Team<kAcross> team(lanes);
+  const int c = a.classes, L = team.L, R = team.R;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * R + team.r;
+  const bool there = row < a.rows;
+  A z[E];
+  const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int cls = e * L + team.l;
+    z[e] = there && cls < c ? static_cast<A>(x[cls * a.scores.stride[1]]) : NegInf<A>();
+  }
+  uint32_t left = ~0u;  // of this thread's classes
+  int32_t* out_class = static_cast<int32_t*>(a.top_class.data) + row * a.top_class.stride[0];
+  T* out_logit = static_cast<T*>(a.top_logit.data) + row * a.top_logit.stride[0];
+  for (int j = 0; j < a.k; ++j) {
+    A best = NegInf<A>();
+    int cls = -1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if ((left >> e & 1u) && z[e] > best) {
+        best = z[e];
+        cls = e * L + team.l;
+      }
+    }
+    auto other = [&](A v, int o) {
+      if (o >= 0 && (cls < 0 || v > best || (v == best && o < cls))) {
+        best = v;
+        cls = o;
+      }
+    };
+    if (kAcross) {
+      if (L > 1) {
+        __syncthreads();
+        red[threadIdx.x] = best;
+        red_cls[threadIdx.x] = cls;
+        __syncthreads();
+        for (int i = 0; i < L; ++i) other(red[i * R + team.r], red_cls[i * R + team.r]);
+      }
+    } else {
+      for (int d = L / 2; d > 0; d >>= 1) {
+        const A v = __shfl_xor(best, d);
+        const int o = __shfl_xor(cls, d);
+        other(v, o);
+      }
+    }
+    if (cls >= 0 && (cls & (L - 1)) == team.l) left &= ~(1u << (cls / L));
+    if (there && team.l == 0) {
+      out_class[j * a.top_class.stride[1]] = cls;
+      out_logit[j * a.top_logit.stride[1]] = static_cast<T>(best);
+    }
+  }
+  if (a.log_rest.data == nullptr) return;
+  A high = NegInf<A>();
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (left >> e & 1u) high = Max(high, z[e]);
+  high = team.Max(high, red);
+  const A scale = static_cast<A>(kLog2e / a.temperature);
+  const bool able = high > NegInf<A>() && high < static_cast<A>(INFINITY);
+  A sum = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (able && (left >> e & 1u) && z[e] > NegInf<A>()) sum += Exp2((z[e] - high) * scale);
+  sum = team.Sum(sum, red);
+  if (there && team.l == 0)
+    StoreFloat(a.log_rest, row * a.log_rest.stride[0],
+               sum > A(0) ? high / static_cast<A>(a.temperature) + Log2(sum) * static_cast<A>(kLn2)
+                          : high);
+}
+
+// ------------------------------------------------------------------ top logits, many classes
+constexpr int kTopBins = 512;         // of the threads' maxima
+constexpr int kTopCandidates = 1024;  // of a row at most, or it goes the slow way
+
+/*!
+ * One workgroup a row. Every thread takes the maxima of four parts of what it holds: the k-th
+ * largest of these 4 * kBlock values, or anything below it, has at least k scores above or
+ * equal to it, and seldom many more. A histogram of the maxima gives such a value; a second
+ * pass over the registers picks the scores that reach it (candidates) and sums the
+ * exponentials of the others; the candidates are put in order by counting. Rows with more
+ * candidates than fit, of many equal scores for instance, are done digit by digit (TopAny).
+ */
+template <typename T, int kBlock, int kCached>
+__global__ void __launch_bounds__(kBlock) k_top_row(LGBM_TopLogitsArgs a) {
+  using A = Acc<T>;
+  constexpr int kWaves = kBlock / kWave;
+  static_assert(std::is_same_v<A, float>, "keys of 32 bits");
+  __shared__ int hist[kTopBins];
+  __shared__ A s_low[kWaves], s_high[kWaves], s_sum[kWaves];
+  __shared__ int s_bin, s_count, s_valid;
+  __shared__ uint32_t s_edge;
+  __shared__ A s_value[kTopCandidates];
+  __shared__ int s_cls[kTopCandidates];
+  __shared__ A s_rest[kTopCandidates];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, k = a.k;
+  RowOf<T, kBlock, kCached> z(
+      static_cast<const T*>(a.scores.data) + row * a.scores.stride[0], a.classes);
+  z.Load();
+  for (int i = tid; i < kTopBins; i += kBlock) hist[i] = 0;
+  if (tid == 0) {
+    s_count = s_valid = s_bin = 0;
+    s_edge = ~0u;
+  }
+  A part[4] = {NegInf<A>(), NegInf<A>(), NegInf<A>(), NegInf<A>()};
+  z.Each([&](int, const auto& v) {
+#pragma unroll
+    for (int i = 0; i < kSizeOf<decltype(v)>; ++i) part[i & 3] = Max(part[i & 3], v[i]);
+  });
+  A high = NegInf<A>(), low = -NegInf<A>();
+  int valid = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    high = Max(high, part[i]);
+    if (part[i] > NegInf<A>()) {
+      low = fminf(low, part[i]);
+      ++valid;
+    }
+  }
+  high = WaveMax(high);
+  low = -WaveMax(-low);
+  valid = WaveSum(valid);
+  __syncthreads();
+  if (tid % kWave == 0) {
+    s_high[tid / kWave] = high;
+    s_low[tid / kWave] = low;
+    atomicAdd(&s_valid, valid);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    high = Max(high, s_high[i]);
+    low = fminf(low, s_low[i]);
+  }
+  const bool bounded = s_valid >= k;  // otherwise every score may be among the k largest
+  const A range = high - low;
+  if (!(range < static_cast<A>(INFINITY)) || !(high > NegInf<A>())) {
+    TopAny<T, kBlock>(a, row);  // infinite scores, or none at all
+    return;
+  }
+  // bins order as the maxima do; where rounding puts equals into one, it is for all alike
+  const A per = range > A(0) ? static_cast<A>(kTopBins - 1) / range : A(0);
+  auto bin_of = [&](A v) {
+    return min(static_cast<int>(fminf((v - low) * per, static_cast<A>(kTopBins - 1))),
+               kTopBins - 1);
+  };
+  if (bounded) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (part[i] > NegInf<A>()) atomicAdd(&hist[bin_of(part[i])], 1);
+    __syncthreads();
+    if (tid < kWave) {
+      // lane l holds the bins 511 - 8 l .. 504 - 8 l, largest first
+      constexpr int kEach = kTopBins / kWave;
+      int own[kEach], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += own[i] = hist[kTopBins - 1 - kEach * tid - i];
+      int before = sum;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(before, d);
+        if (tid >= d) before += o;
+      }
+      before -= sum;
+      if (before < k && k <= before + sum) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          if (before < k && k <= before + own[i]) s_bin = kTopBins - 1 - kEach * tid - i;
+          before += own[i];
+        }
+      }
+    }
+    __syncthreads();
+    const int bin = s_bin;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (part[i] > NegInf<A>() && bin_of(part[i]) >= bin) atomicMin(&s_edge, KeyOf(part[i]));
+    __syncthreads();
+  }
+  // the smallest of the maxima in the bins down to the k-th
+  A edge = bounded ? __uint_as_float(s_edge & 0x80000000u ? s_edge & 0x7fffffffu : ~s_edge)
+                   : -FLT_MAX;
+  const A scale = static_cast<A>(kLog2e / a.temperature);
+  A off = bounded ? -edge * scale : A(0);  // unbounded, nothing but -inf is below the edge
+  const bool rest = a.log_rest.data != nullptr;
+  A sum = 0;
+  z.Each([&](int base, const auto& v) {
+    constexpr int kSize = kSizeOf<decltype(v)>;
+    A top = v[0];
+#pragma unroll
+    for (int i = 1; i < kSize; ++i) top = Max(top, v[i]);
+    if (top >= edge) {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) {
+        if (!(v[i] >= edge)) continue;
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kTopCandidates) {
+          s_value[at] = v[i];
+          s_cls[at] = base + i;
+        }
+      }
+    }
+    if (rest) {
+      A own = 0;
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) own += v[i] < edge ? Exp2(Fma(v[i], scale, off)) : A(0);
+      sum += own;
+    }
+  });
+  __syncthreads();
+  const int n = s_count;
+  if (n > kTopCandidates) {
+    TopAny<T, kBlock>(a, row);
+    return;
+  }
+  int32_t* out_class = static_cast<int32_t*>(a.top_class.data) + row * a.top_class.stride[0];
+  T* out_logit = static_cast<T*>(a.top_logit.data) + row * a.top_logit.stride[0];
+  for (int i = tid; i < n; i += kBlock) {
+    const A v = s_value[i];
+    const int cls = s_cls[i];
+    int rank = 0;
+    for (int o = 0; o < n; ++o) {
+      const A u = s_value[o];
+      rank += u > v || (u == v && s_cls[o] < cls);
+    }
+    if (rank < k) {
+      out_class[rank * a.top_class.stride[1]] = cls;
+      out_logit[rank * a.top_logit.stride[1]] = static_cast<T>(v);
+    } else {
+      s_rest[rank - k] = v;  // in order, so that their sum is the same every time
+    }
+  }
+  for (int i = n + tid; i < k; i += kBlock) {
+    out_class[i * a.top_class.stride[1]] = -1;
+    out_logit[i * a.top_logit.stride[1]] = static_cast<T>(-INFINITY);
+  }
+  if (!rest) return;
+  // two sums, each against a value near its own: of what is below the edge, and of the
+  // candidates that were not chosen
+  sum = BlockSum<kBlock>(sum, s_sum);
+  if (n <= k && sum < SmallRest<A>()) {  // far below the edge: against its own maximum
+    A own = NegInf<A>();
+    z.Each([&](int, const auto& v) {
+#pragma unroll
+      for (int i = 0; i < kSizeOf<decltype(v)>; ++i) own = Max(own, v[i] < edge ? v[i] : own);
+    });
+    own = BlockMax<kBlock>(own, s_low);
+    sum = 0;
+    if (own > NegInf<A>()) {
+      off = -own * scale;
+      z.Each([&](int, const auto& v) {
+#pragma unroll
+        for (int i = 0; i < kSizeOf<decltype(v)>; ++i)
+          sum += v[i] < edge ? Exp2(Fma(v[i], scale, off)) : A(0);
+      });
+      sum = BlockSum<kBlock>(sum, s_high);
+    }
+  }
+  A log_rest = sum > A(0) ? Log2(sum) - off : NegInf<A>();
+  if (n > k) {
+    const A next = s_rest[0];
+    A more = 0;
+    for (int i = tid; i < n - k; i += kBlock) more += Exp2((s_rest[i] - next) * scale);
+    more = BlockSum<kBlock>(more, s_high);
+    const A log_more = Fma(next, scale, Log2(more)), top = Max(log_rest, log_more);
+    log_rest = top + Log2(Exp2(log_rest - top) + Exp2(log_more - top));
+  }
+  if (tid == 0)
+    StoreFloat(a.log_rest, row * a.log_rest.stride[0], log_rest * static_cast<A>(kLn2));
 }
 
 // ------------------------------------------------------------------ verification
@@ -1221,16 +1507,6 @@ template <typename F> void ByType(int type, F&& f) {
   }
 }
 
-void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
-  OnDevice on(device);
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<uint32_t>(a.rows));
-  ByType(a.scores.type, [&](auto t) {
-    hipLaunchKernelGGL((k_top_any<decltype(t), 256>), grid, dim3(256), 0, s, a);
-  });
-  OPS_HIP_OK(hipGetLastError());
-}
-
 /*! the smallest power of two of threads that hold `classes` at `each` a thread */
 int LanesFor(int classes, int each) {
   int lanes = 1;
@@ -1249,6 +1525,55 @@ void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
                      lanes);
 }
 
+/*! whether the rows of a class stand closer together than the classes of a row */
+bool ClassMajor(const LGBM_Array& scores) {
+  const int64_t row_step = std::abs(scores.stride[0]);  // 0: one row for all
+  return row_step != 0 && row_step < std::abs(scores.stride[1]);
+}
+
+template <typename T, int E, bool kAcross>
+void LaunchTopTile(const LGBM_TopLogitsArgs& a, hipStream_t s) {
+  const int lanes = LanesFor(a.classes, E), rows = 256 / lanes;
+  hipLaunchKernelGGL((k_top_tile<T, E, kAcross>),
+                     dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256), 0, s, a,
+                     lanes);
+}
+
+template <typename T, int kBlock, int kCached>
+void LaunchTopRow(const LGBM_TopLogitsArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_top_row<T, kBlock, kCached>), dim3(static_cast<uint32_t>(a.rows)),
+                     dim3(kBlock), 0, s, a);
+}
+
+void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
+  OnDevice on(device);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool across = ClassMajor(a.scores);
+  ByType(a.scores.type, [&](auto t) {
+    using T = decltype(t);
+    if (a.classes <= (across ? 512 : 256)) {
+      if (!across) LaunchTopTile<T, 4, false>(a, s);
+      else if (a.classes <= 8) LaunchTopTile<T, 8, true>(a, s);
+      else if (a.classes <= 256) LaunchTopTile<T, 16, true>(a, s);
+      else LaunchTopTile<T, 32, true>(a, s);
+      return;
+    }
+    if constexpr (!std::is_same_v<T, double>) {
+      if (a.scores.stride[1] == 1) {
+        const int chunks = a.classes / Chunk<T>::kSize;
+        if (chunks <= 256) LaunchTopRow<T, 256, 1>(a, s);
+        else if (chunks <= 1024) LaunchTopRow<T, 256, 4>(a, s);
+        else if (chunks <= 4096) LaunchTopRow<T, 512, 8>(a, s);
+        else LaunchTopRow<T, 1024, 8>(a, s);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((k_top_any<T, 256>), dim3(static_cast<uint32_t>(a.rows)), dim3(256), 0, s,
+                       a);
+  });
+  OPS_HIP_OK(hipGetLastError());
+}
+
 template <typename T, int kBlock, int kCached>
 void LaunchDistillRow(const LGBM_DistillArgs& a, hipStream_t s) {
   auto kernel = k_distill_row<T, kBlock, kCached>;
@@ -1260,8 +1585,7 @@ void LaunchDistillRow(const LGBM_DistillArgs& a, hipStream_t s) {
 void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
   OnDevice on(device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t row_step = std::abs(a.scores.stride[0]);  // 0: one row for all
-  const bool across = row_step != 0 && row_step < std::abs(a.scores.stride[1]);
+  const bool across = ClassMajor(a.scores);
   if (a.classes <= (across ? 512 : 256)) {
     ByType(a.scores.type, [&](auto t) {
       using T = decltype(t);
