@@ -1444,6 +1444,21 @@ __device__ __forceinline__ int FindClass(const F& mass, int base, int len, doubl
   return some ? base + 63 - __clzll(some) : -1;
 }
 
+/*! writes a sequence's results; `who` and `many` are the threads that do it */
+__device__ __forceinline__ void PutVerified(const LGBM_VerifyArgs& a, int64_t row, int accepted,
+                                            int drawn, int who, int many) {
+  int32_t* out = static_cast<int32_t*>(a.out_class.data) + row * a.out_class.stride[0];
+  for (int s = who; s <= a.drafts; s += many) {
+    int x = s == accepted ? drawn : -1;
+    if (s < accepted)
+      x = LoadClass(a.draft_class, row * a.draft_class.stride[0] + s * a.draft_class.stride[1],
+                    a.classes);
+    out[s * a.out_class.stride[1]] = x;
+  }
+  if (who == 0)
+    static_cast<int32_t*>(a.out_accepted.data)[row * a.out_accepted.stride[0]] = accepted;
+}
+
 /*! one workgroup a sequence */
 template <typename T, int kBlock>
 __global__ void __launch_bounds__(kBlock) k_verify_any(LGBM_VerifyArgs a) {
@@ -1466,16 +1481,193 @@ __global__ void __launch_bounds__(kBlock) k_verify_any(LGBM_VerifyArgs a) {
   }
   const double goal = Uniform(a.sample, row * a.sample.stride[0]) * total;
   const int drawn = FindClass<kBlock>(mass, 0, c, goal, sums);
-  int32_t* out = static_cast<int32_t*>(a.out_class.data) + row * a.out_class.stride[0];
-  for (int s = tid; s <= a.drafts; s += kBlock) {
-    int x = -1;
-    if (s < n) x = LoadClass(a.draft_class, row * a.draft_class.stride[0] +
-                                                s * a.draft_class.stride[1], c);
-    else if (s == n) x = drawn;
-    out[s * a.out_class.stride[1]] = x;
+  PutVerified(a, row, n, drawn, tid, kBlock);
+}
+
+// ------------------------------------------------------------------ verification, few classes
+constexpr int kFewEach = 4;                    // classes a lane
+constexpr int kFewClasses = kWave * kFewEach;  // at most
+
+/*! `lanes` (a power of two) lanes a sequence, each with four neighbouring classes */
+template <typename T>
+__global__ void __launch_bounds__(256) k_verify_few(LGBM_VerifyArgs a, int lanes) {
+  const int l = threadIdx.x % lanes;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
+  const bool there = at < a.rows;
+  const int64_t row = there ? at : a.rows - 1;  // so that every lane takes part in the shuffles
+  const int length = Length(a, row);
+  int n = length;
+  for (int s = l; s < length; s += lanes) {
+    const int x = LoadClass(a.draft_class,
+                            row * a.draft_class.stride[0] + s * a.draft_class.stride[1], a.classes);
+    if (!Stands<T>(a, row, s, x)) {
+      n = s;
+      break;
+    }
   }
-  if (tid == 0)
-    static_cast<int32_t*>(a.out_accepted.data)[row * a.out_accepted.stride[0]] = n;
+  for (int d = lanes / 2; d > 0; d >>= 1) n = min(n, __shfl_xor(n, d));
+  Residual<T> mass = ResidualOf<T>(a, row, n, length);
+  double own[kFewEach], sum, total;
+  for (int round = 0; round < 2; ++round) {
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kFewEach; ++i) {
+      const int c = l * kFewEach + i;
+      own[i] = c < a.classes ? mass(c) : 0.0;
+      sum += own[i];
+    }
+    total = sum;
+    for (int d = lanes / 2; d > 0; d >>= 1) total += __shfl_xor(total, d);
+    if (!(total > 0)) {  // nothing is left of the target: the draw is from the target itself
+      mass.q = nullptr;
+      mass.gone = -1;
+    }
+    if (!__any(!(total > 0))) break;
+  }
+  double reach = sum;
+  for (int d = 1; d < lanes; d <<= 1) {
+    const double o = __shfl_up(reach, d, lanes);
+    if (l >= d) reach += o;
+  }
+  reach -= sum;
+  const double goal = Uniform(a.sample, row * a.sample.stride[0]) * total;
+  int first = a.classes, last = -1;
+#pragma unroll
+  for (int i = 0; i < kFewEach; ++i) {
+    if (!(own[i] > 0)) continue;
+    reach += own[i];
+    last = l * kFewEach + i;
+    if (reach > goal) first = min(first, last);
+  }
+  for (int d = lanes / 2; d > 0; d >>= 1) {
+    first = min(first, __shfl_xor(first, d));
+    last = max(last, __shfl_xor(last, d));
+  }
+  if (there) PutVerified(a, row, n, first < a.classes ? first : last, l, lanes);
+}
+
+// ------------------------------------------------------------------ verification, many classes
+constexpr int kSplitBlock = 256;
+constexpr int kSplitWaves = kSplitBlock / kWave;
+constexpr int kMostSplits = 64;  // workgroups a sequence
+
+/*! classes of one wave's segment: whole turns of the wave over its chunks */
+template <typename T> __host__ __device__ inline int SegmentOf(int classes, int splits) {
+  const int turn = kWave * Chunk<T>::kSize, waves = splits * kSplitWaves;
+  return ((classes + waves - 1) / waves + turn - 1) / turn * turn;
+}
+
+/*! Mass of a value of at most 32 bits, in as many */
+template <typename T> __device__ __forceinline__ float Mass32(T x) {
+  const float v = fmaxf(static_cast<float>(x), 0.0f);  // NaN gives zero
+  return v < INFINITY ? v : 0.0f;
+}
+__device__ __forceinline__ double MassOf(double x) { return Mass(x); }
+__device__ __forceinline__ double MassOf(float x) { return Mass32(x); }
+__device__ __forceinline__ double MassOf(_Float16 x) { return Mass32(x); }
+__device__ __forceinline__ double MassOf(__bf16 x) { return Mass32(x); }
+
+/*! the mass of classes [begin, end) of a row whose classes stand next to each other; one wave */
+template <typename T>
+__device__ __forceinline__ double WaveMass(const Residual<T>& f, int begin, int end) {
+  constexpr int kSize = Chunk<T>::kSize;
+  const int lane = threadIdx.x % kWave;
+  double sum = 0;
+  const int whole = begin + (end - begin) / kSize * kSize;
+#pragma unroll 4
+  for (int c = begin + lane * kSize; c < whole; c += kWave * kSize) {
+    Chunk<T> p, q;
+    __builtin_memcpy(&p, f.p + c, sizeof(p));
+    if (f.q != nullptr) __builtin_memcpy(&q, f.q + c, sizeof(q));
+#pragma unroll
+    for (int i = 0; i < kSize; ++i) {
+      double v = MassOf(p.v[i]);
+      if (f.q != nullptr) v = fmax(v - MassOf(q.v[i]), 0.0);
+      else if (c + i == f.gone) v = 0.0;
+      sum += v;
+    }
+  }
+  if (whole + lane < end) sum += f(whole + lane);
+  return WaveSum(sum);
+}
+
+/*!
+ * Each wave of `splits` workgroups a sequence sums one segment of the row that the class is
+ * drawn from. Which row that is, every workgroup finds for itself: a few gathers, instead of
+ * a launch before this one.
+ */
+template <typename T>
+__global__ void __launch_bounds__(kSplitBlock) k_verify_sums(LGBM_VerifyArgs a) {
+  const int64_t row = blockIdx.y;
+  const int length = Length(a, row), n = Accepted<T>(a, row, length);
+  const Residual<T> mass = ResidualOf<T>(a, row, n, length);
+  const int seg = SegmentOf<T>(a.classes, gridDim.x);
+  const int at = blockIdx.x * kSplitWaves + threadIdx.x / kWave;
+  const int begin = min(a.classes, at * seg), end = min(a.classes, begin + seg);
+  const double sum = WaveMass(mass, begin, end);
+  if (threadIdx.x % kWave == 0)
+    static_cast<double*>(a.workspace)[row * gridDim.x * kSplitWaves + at] = sum;
+}
+
+/*! one workgroup a sequence: the segment that holds the goal, then the class in it */
+template <typename T>
+__global__ void __launch_bounds__(kSplitBlock) k_verify_draw(LGBM_VerifyArgs a, int splits) {
+  __shared__ double sums[kSplitWaves];
+  const int64_t row = blockIdx.x;
+  const int segments = splits * kSplitWaves;
+  static_assert(kMostSplits * kSplitWaves <= 4 * kWave, "four segments a lane");
+  const double* part = static_cast<const double*>(a.workspace) + row * segments;
+  const int length = Length(a, row), n = Accepted<T>(a, row, length);
+  Residual<T> mass = ResidualOf<T>(a, row, n, length);
+  const double v = Uniform(a.sample, row * a.sample.stride[0]);
+  // every wave does the same with the segments' sums: lane l has those of 4 l .. 4 l + 3
+  const int lane = threadIdx.x % kWave;
+  double own[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    own[i] = 4 * lane + i < segments ? part[4 * lane + i] : 0.0;
+    sum += own[i];
+  }
+  double reach = sum;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const double o = __shfl_up(reach, d);
+    if (lane >= d) reach += o;
+  }
+  const double total = __shfl(reach, kWave - 1);
+  reach -= sum;
+  int drawn;
+  if (total > 0) {
+    const double goal = v * total;
+    int found = -1, last = -1;
+    double before = 0, last_before = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!(own[i] > 0)) continue;
+      last = 4 * lane + i;
+      last_before = reach;
+      reach += own[i];
+      if (found < 0 && reach > goal) {
+        found = last;
+        before = last_before;
+      }
+    }
+    const unsigned long long over = __ballot(found >= 0), some = __ballot(last >= 0);
+    const int who = over ? __ffsll(over) - 1 : 63 - __clzll(some);
+    found = __shfl(over ? found : last, who);
+    before = __shfl(over ? before : last_before, who);
+    const int seg = SegmentOf<T>(a.classes, splits);
+    drawn = FindClass<kSplitBlock>(mass, found * seg, min(seg, a.classes - found * seg),
+                                   goal - before, sums);
+  } else {  // nothing is left of the target: the draw is from the target itself
+    mass.q = nullptr;
+    mass.gone = -1;
+    double whole = 0;
+    for (int i = threadIdx.x; i < a.classes; i += kSplitBlock) whole += mass(i);
+    whole = BlockSum<kSplitBlock>(whole, sums);
+    drawn = FindClass<kSplitBlock>(mass, 0, a.classes, v * whole, sums);
+  }
+  PutVerified(a, row, n, drawn, threadIdx.x, kSplitBlock);
 }
 
 // ------------------------------------------------------------------ launches
@@ -1625,14 +1817,39 @@ void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
   OPS_HIP_OK(hipGetLastError());
 }
 
-int64_t VerifyWorkspaceDevice(const LGBM_VerifyArgs&) { return 0; }
+/*! workgroups a sequence, 0 where the split kernels do not apply */
+int SplitsOf(const LGBM_VerifyArgs& a) {
+  if (a.classes <= kFewClasses || a.rows > 65535) return 0;  // a grid's second dimension
+  if (a.target.stride[2] != 1 || (a.draft_prob.data && a.draft_prob.stride[2] != 1)) return 0;
+  const int64_t wanted = (1024 + a.rows - 1) / a.rows, fitting = (a.classes + 2047) / 2048;
+  return static_cast<int>(std::min<int64_t>({wanted, fitting, kMostSplits}));
+}
+
+int64_t VerifyWorkspaceDevice(const LGBM_VerifyArgs& a) {
+  return a.rows * SplitsOf(a) * kSplitWaves * static_cast<int64_t>(sizeof(double));
+}
 
 void VerifyDevice(const LGBM_VerifyArgs& a, int device, void* stream) {
+  const int splits = SplitsOf(a);
+  if (splits > 0 && (a.workspace == nullptr || a.workspace_bytes < VerifyWorkspaceDevice(a)))
+    Log::Fatal("VerifyDrafts needs a workspace of %lld bytes, got %lld",
+               static_cast<long long>(VerifyWorkspaceDevice(a)),
+               static_cast<long long>(a.workspace ? a.workspace_bytes : 0));
   OnDevice on(device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<uint32_t>(a.rows));
+  const uint32_t rows = static_cast<uint32_t>(a.rows);
   ByType(a.target.type, [&](auto t) {
-    hipLaunchKernelGGL((k_verify_any<decltype(t), 256>), grid, dim3(256), 0, s, a);
+    using T = decltype(t);
+    if (a.classes <= kFewClasses) {
+      const int lanes = LanesFor(a.classes, kFewEach), each = 256 / lanes;
+      hipLaunchKernelGGL((k_verify_few<T>), dim3((rows + each - 1) / each), dim3(256), 0, s, a,
+                         lanes);
+    } else if (splits > 0) {
+      hipLaunchKernelGGL((k_verify_sums<T>), dim3(splits, rows), dim3(kSplitBlock), 0, s, a);
+      hipLaunchKernelGGL((k_verify_draw<T>), dim3(rows), dim3(kSplitBlock), 0, s, a, splits);
+    } else {
+      hipLaunchKernelGGL((k_verify_any<T, 256>), dim3(rows), dim3(256), 0, s, a);
+    }
   });
   OPS_HIP_OK(hipGetLastError());
 }

@@ -69,72 +69,80 @@ for _f in (_LIB.LGBM_TopLogits, _LIB.LGBM_Distill, _LIB.LGBM_VerifyDrafts):
     _f.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
 _LIB.LGBM_VerifyDraftsWorkspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]
 
+# torch is looked up when the first array that may be its is seen: the package works without
+_torch = None
+_Tensor = ()
 
-def _torch_of(x):
-    """The torch module if x is one of its tensors."""
-    torch = sys.modules.get("torch")
-    if torch is None or not isinstance(x, torch.Tensor):
-        return None
-    if not _TORCH_TYPES:
-        for code, dtype in ((_F32, torch.float32), (_F64, torch.float64), (_I32, torch.int32),
-                            (_I64, torch.int64), (_F16, torch.float16), (_BF16, torch.bfloat16)):
-            _TORCH_TYPES[dtype] = code
-            _TORCH_OF[code] = dtype
-    return torch
+
+def _is_tensor(x):
+    global _torch, _Tensor
+    if _torch is None:
+        _torch = sys.modules.get("torch")
+        if _torch is None:
+            return False
+        _Tensor = _torch.Tensor
+        for code, name in ((_F32, "float32"), (_F64, "float64"), (_I32, "int32"),
+                           (_I64, "int64"), (_F16, "float16"), (_BF16, "bfloat16")):
+            _TORCH_TYPES[getattr(_torch, name)] = code
+            _TORCH_OF[code] = getattr(_torch, name)
+    return isinstance(x, _Tensor)
+
+
+def _stream_of(device):
+    """The current stream of a device, as a pointer."""
+    return _torch.cuda.current_stream(device).cuda_stream
 
 
 class _Place:
     """Where a call runs, and how its results are made: as its first array is."""
 
+    __slots__ = ("tensor", "device", "on")
+
     def __init__(self, x):
-        self.torch = torch = _torch_of(x)
         self.device = -1
         self.on = None
-        if torch is not None:
+        self.tensor = _is_tensor(x)
+        if self.tensor:
             self.on = x.device
-            if self.on.type == "cuda":
+            if x.is_cuda:
                 self.device = self.on.index
             elif self.on.type != "cpu":
                 raise LightGBMError(f"tensors on {self.on} are not supported")
 
     def stream(self):
-        return self.torch.cuda.current_stream(self.on).cuda_stream if self.device >= 0 else None
+        return _stream_of(self.on) if self.device >= 0 else None
 
     def empty(self, shape, code, class_major=False):
-        if self.torch is not None:
+        if self.tensor:
             if class_major:
-                return self.torch.empty(shape[::-1], dtype=_TORCH_OF[code], device=self.on).t()
-            return self.torch.empty(shape, dtype=_TORCH_OF[code], device=self.on)
+                return _torch.empty(shape[::-1], dtype=_TORCH_OF[code], device=self.on).t()
+            return _torch.empty(shape, dtype=_TORCH_OF[code], device=self.on)
         return np.empty(shape, dtype=_NUMPY_OF[code], order="F" if class_major else "C")
 
-    def check(self, x, name, shape):
-        """x as an array of this place, of this shape (None: any length)."""
-        torch = _torch_of(x)
-        if self.device >= 0:
-            if torch is None or x.device != self.on:
-                raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
-        elif torch is not None:
-            if x.device.type != "cpu":
-                raise LightGBMError(f"{name} is on {x.device}, the first array is on the host")
+    def array(self, x, name, shape):
+        """The six fields of an LGBM_Array of x, which has to be of this place and shape."""
+        if x is None:
+            return _NONE
+        if _is_tensor(x):
+            if (x.device != self.on) if self.tensor else x.is_cuda:
+                raise LightGBMError(f"{name} is on {x.device}, the first array on "
+                                    f"{self.on or 'the host'}")
+        elif self.device >= 0:
+            raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
         elif not isinstance(x, np.ndarray):
             x = np.asarray(x)
-        got = x.shape
-        if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
-            want = ", ".join("*" if w is None else str(w) for w in shape)
-            raise LightGBMError(f"{name} must have the shape [{want}], got {list(got)}")
-        return x
+        if tuple(x.shape) != shape:
+            raise LightGBMError(f"{name} must have the shape {list(shape)}, got {list(x.shape)}")
+        return _fields(x, name)
 
 
-def _array(x, name):
-    """The six fields of an LGBM_Array."""
-    if x is None:
-        return _NONE
+def _fields(x, name):
     if isinstance(x, np.ndarray):
         dtype = x.dtype
         code = _NUMPY_TYPES.get(dtype.kind + str(dtype.itemsize)) if dtype.isnative else None
+        steps = x.strides
         if code is not None:
             size = dtype.itemsize
-            steps = x.strides
             if any(s % size for s in steps):
                 raise LightGBMError(f"{name} has strides that are no multiple of its elements")
             steps = [s // size for s in steps]
@@ -143,9 +151,8 @@ def _array(x, name):
         code = _TORCH_TYPES.get(x.dtype)
         steps = x.stride()
         at = x.data_ptr()
-        dtype = x.dtype
     if code is None:
-        raise LightGBMError(f"{name} has the type {dtype}, which is not supported")
+        raise LightGBMError(f"{name} has the type {x.dtype}, which is not supported")
     n = len(steps)
     if n == 2:
         return (at, steps[0], steps[1], 0, code, 0)
@@ -154,16 +161,14 @@ def _array(x, name):
     return (at, steps[0], steps[1], steps[2], code, 0)
 
 
-def _host(x):
-    """Whatever is no tensor, as a numpy array."""
-    return x if _torch_of(x) is not None or isinstance(x, np.ndarray) else np.asarray(x)
-
-
-def _two_dim(x, name, dims=2):
-    x = _host(x)
-    if len(x.shape) != dims:
-        raise LightGBMError(f"{name} must have {dims} dimensions, got {list(x.shape)}")
-    return x
+def _shaped(x, name, dims=2):
+    """x as an array, with its shape, which has to have so many dimensions."""
+    if not isinstance(x, np.ndarray) and not _is_tensor(x):
+        x = np.asarray(x)
+    shape = x.shape
+    if len(shape) != dims:
+        raise LightGBMError(f"{name} must have {dims} dimensions, got {list(shape)}")
+    return x, shape
 
 
 def top_logits(scores, k, temperature=1.0, rest=True):
@@ -177,54 +182,46 @@ def top_logits(scores, k, temperature=1.0, rest=True):
     Equal scores go to the lowest class first. NaN and -inf are never selected: a row with
     fewer than k other scores ends in class -1 with logit -inf. log_rest leaves NaN out.
     """
-    scores = _two_dim(scores, "scores")
-    rows, classes = scores.shape
+    scores, (rows, classes) = _shaped(scores, "scores")
     where = _Place(scores)
-    x = _array(scores, "scores")
+    x = _fields(scores, "scores")
     code = x[4]
     k = int(k)
     out_class = where.empty((rows, max(k, 0)), _I32)
     out_logit = where.empty((rows, max(k, 0)), code)
     log_rest = where.empty((rows,), _F64 if code == _F64 else _F32) if rest else None
     _safe_call(_LIB.LGBM_TopLogits(
-        _TOP.pack(rows, classes, k, temperature, *x, *_array(out_class, ""),
-                  *_array(out_logit, ""), *_array(log_rest, "")),
+        _TOP.pack(rows, classes, k, temperature, *x, *_fields(out_class, ""),
+                  *_fields(out_logit, ""), *(_fields(log_rest, "") if rest else _NONE)),
         where.device, where.stream()))
     return TopLogits(out_class, out_logit, log_rest)
 
 
 def _distill(scores, teacher, labels, weight, temperature, alpha, loss, gradient, hessian):
-    scores = _two_dim(scores, "scores")
-    rows, classes = scores.shape
+    scores, (rows, classes) = _shaped(scores, "scores")
     where = _Place(scores)
     if not 2 <= len(teacher) <= 3:
         raise LightGBMError("teacher must be (classes, logits) or (classes, logits, log_rest)")
-    t_class = _two_dim(teacher[0], "teacher classes")
-    k = t_class.shape[1]
-    t_class = where.check(t_class, "teacher classes", (rows, None))
-    t_logit = where.check(teacher[1], "teacher logits", (rows, k))
-    t_rest = teacher[2] if len(teacher) == 3 else None
-    if t_rest is not None:
-        t_rest = where.check(t_rest, "teacher log_rest", (rows,))
-    if alpha == 1.0:
-        labels = None
-    if labels is not None:
-        labels = where.check(labels, "labels", (rows,))
-    if weight is not None:
-        weight = where.check(weight, "weight", (rows,))
-    x = _array(scores, "scores")
+    t_class, (_, k) = _shaped(teacher[0], "teacher classes")
+    # every row of the results; what is not asked for, or not looked at, is absent
+    row, slots = (rows,), (rows, k)
+    x = _fields(scores, "scores")
     code = x[4]
     out = _F32 if code == _F64 else code
     class_major = x[1] == 1 and x[2] != 1
-    made_loss = where.empty((rows,), _F64 if code == _F64 else _F32) if loss else None
+    fields = (rows, classes, k, temperature, alpha, *x,
+              *where.array(t_class, "teacher classes", slots),
+              *where.array(teacher[1], "teacher logits", slots),
+              *where.array(teacher[2] if len(teacher) == 3 else None, "teacher log_rest", row),
+              *where.array(None if alpha == 1.0 else labels, "labels", row),
+              *where.array(weight, "weight", row))
+    made_loss = where.empty(row, _F64 if code == _F64 else _F32) if loss else None
     made_grad = where.empty((rows, classes), out, class_major) if gradient else None
     made_hess = where.empty((rows, classes), out, class_major) if hessian else None
     _safe_call(_LIB.LGBM_Distill(
-        _DISTILL.pack(rows, classes, k, temperature, alpha, *x,
-                      *_array(t_class, "teacher classes"), *_array(t_logit, "teacher logits"),
-                      *_array(t_rest, "teacher log_rest"), *_array(labels, "labels"),
-                      *_array(weight, "weight"), *_array(made_loss, ""), *_array(made_grad, ""),
-                      *_array(made_hess, "")),
+        _DISTILL.pack(*fields, *(_fields(made_loss, "") if loss else _NONE),
+                      *(_fields(made_grad, "") if gradient else _NONE),
+                      *(_fields(made_hess, "") if hessian else _NONE)),
         where.device, where.stream()))
     return made_loss, made_grad, made_hess
 
@@ -279,32 +276,29 @@ def verify_drafts(target_prob, drafts, draft_prob, accept_uniform, sample_unifor
     infinite and negative entries weigh nothing, a draft outside 0..classes-1 is refused. Where
     the difference has no mass the draw is from p, where p has none the class is -1.
     """
-    target_prob = _two_dim(target_prob, "target_prob", 3)
-    rows, places, classes = target_prob.shape
+    target_prob, (rows, places, classes) = _shaped(target_prob, "target_prob", 3)
     where = _Place(target_prob)
     t = places - 1
-    drafts = where.check(drafts, "drafts", (rows, t))
-    if draft_prob is not None:
-        draft_prob = where.check(draft_prob, "draft_prob", (rows, t, classes))
-    accept = where.check(accept_uniform, "accept_uniform", (rows, t))
-    sample = where.check(sample_uniform, "sample_uniform", (rows,))
-    if lengths is not None:
-        lengths = where.check(lengths, "lengths", (rows,))
+    fields = (rows, classes, t, *_fields(target_prob, "target_prob"),
+              *where.array(draft_prob, "draft_prob", (rows, t, classes)),
+              *where.array(drafts, "drafts", (rows, t)),
+              *where.array(accept_uniform, "accept_uniform", (rows, t)),
+              *where.array(sample_uniform, "sample_uniform", (rows,)),
+              *where.array(lengths, "lengths", (rows,)))
     out_class = where.empty((rows, places), _I32)
     out_accepted = where.empty((rows,), _I32)
-    fields = (rows, classes, t, *_array(target_prob, "target_prob"),
-              *_array(draft_prob, "draft_prob"), *_array(drafts, "drafts"),
-              *_array(accept, "accept_uniform"), *_array(sample, "sample_uniform"),
-              *_array(lengths, "lengths"), *_array(out_class, ""), *_array(out_accepted, ""))
-    scratch, size = None, 0
+    fields += (*_fields(out_class, ""), *_fields(out_accepted, ""))
+    scratch = 0
+    size = 0
     if where.device >= 0:
         need = ctypes.c_int64(0)
         _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_VERIFY.pack(*fields, 0, 0),
                                                    ctypes.byref(need)))
         size = need.value
         if size:
-            scratch = where.torch.empty((size,), dtype=where.torch.uint8, device=where.on)
-    _safe_call(_LIB.LGBM_VerifyDrafts(
-        _VERIFY.pack(*fields, scratch.data_ptr() if size else 0, size),
-        where.device, where.stream()))
+            # freed to the caching allocator, which gives it out again in the stream's order
+            space = _torch.empty((size,), dtype=_torch.uint8, device=where.on)
+            scratch = space.data_ptr()
+    _safe_call(_LIB.LGBM_VerifyDrafts(_VERIFY.pack(*fields, scratch, size), where.device,
+                                      where.stream()))
     return VerifiedDrafts(out_class, out_accepted)
