@@ -342,158 +342,180 @@ template <typename F> void AllowLds(F* kernel, size_t bytes) {
  * Up to E * L classes: a row is read once and stays in its threads' registers. What the
  * teacher wants of each class is a table in LDS, one word a class: first the lowest slot that
  * names the class (with the sign bit set, kNone: none), then that slot's probability.
+ * The statistics are held in S: float64 scores have their loss in 64 bits, and their 32-bit
+ * gradients from exponents that are formed in 64 bits and rounded to 32, which moves a
+ * gradient by about its own rounding and takes a third off a booster's (185 -> 125 us for two
+ * million rows of seven classes with hessians, where 64-bit exponentials are the bound).
  */
-template <typename T, int E, bool kAcross>
+template <typename T, typename S, int E, bool kAcross>
 __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int lanes) {
   using A = Acc<T>;
   using O = Out<T>;
-  using W = Word<A>;
+  using W = Word<S>;
   constexpr W kNone = ~W{0}, kSlot = W{1} << (sizeof(W) * 8 - 1);
   extern __shared__ unsigned long long tile_lds[];
   W* want = reinterpret_cast<W*>(tile_lds);  // R * classes
-  __shared__ A red[256];
+  __shared__ A red_high[kAcross ? 256 : 1];
+  __shared__ S red[kAcross ? 256 : 1];
   const Team<kAcross> team(lanes);
   const int c = a.classes, k = a.k, L = team.L, R = team.R;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * R + team.r;
   const bool there = row < a.rows;
   auto place = [&](int cls) { return kAcross ? cls * R + team.r : team.r * c + cls; };
 
-  const A w = !there ? A(0) : a.weight.data ? LoadFloat<A>(a.weight, row * a.weight.stride[0])
-                                            : A(1);
-  A z[E];
-  {
-    const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+  const S w = !there ? S(0) : a.weight.data ? LoadFloat<S>(a.weight, row * a.weight.stride[0])
+                                            : S(1);
+  const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+  auto score = [&](int cls) { return static_cast<A>(x[cls * a.scores.stride[1]]); };
+  A z[E];  // not kept beyond the exponentials: the few that need a score later read it again
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int cls = e * L + team.l;
-      const bool read = w != A(0) && cls < c;
-      z[e] = read ? static_cast<A>(x[cls * a.scores.stride[1]]) : NegInf<A>();
-      if (cls < c) want[place(cls)] = kNone;
-    }
+  for (int e = 0; e < E; ++e) {
+    const int cls = e * L + team.l;
+    z[e] = w != S(0) && cls < c ? score(cls) : NegInf<A>();
+    if (cls < c) want[place(cls)] = kNone;
   }
   team.Sync();
+  const S temp = static_cast<S>(a.temperature), alpha = static_cast<S>(a.alpha);
+  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
+  // exponents are formed as the scores are held, and taken as the statistics are
+  auto exponent = [](A v, A by, A from) { return static_cast<S>(Fma(v, by, from)); };
+  const bool teach = w != S(0) && alpha > S(0);
+  // the slots of this thread: the first few stay in registers
+  constexpr int kHeld = 4;
+  int held_cls[kHeld];
+  S held_logit[kHeld];
   auto load_class = [&](int j) {
     return LoadClass(a.teacher_class,
                      row * a.teacher_class.stride[0] + j * a.teacher_class.stride[1], c);
   };
-  const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
-  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
   auto load_logit = [&](int j) {
-    return scale * LoadFloat<A>(a.teacher_logit,
-                                row * a.teacher_logit.stride[0] + j * a.teacher_logit.stride[1]);
+    return static_cast<S>(scale *
+                          LoadFloat<A>(a.teacher_logit, row * a.teacher_logit.stride[0] +
+                                                            j * a.teacher_logit.stride[1]));
   };
-  const bool teach = w != A(0) && alpha > A(0);
-  if (teach) {
-    for (int j = team.l; j < k; j += L) {
-      const int cls = load_class(j);
-      if (cls >= 0) atomicMin(&want[place(cls)], kSlot | static_cast<W>(j));
-    }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int j = team.l + i * L;
+    held_cls[i] = teach && j < k ? load_class(j) : -1;
+    held_logit[i] = held_cls[i] >= 0 ? load_logit(j) : S(0);
   }
+  // f(slot, class, logit) of all of them
+  auto all_slots = [&](auto&& f) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (held_cls[i] >= 0) f(team.l + i * L, held_cls[i], held_logit[i]);
+    if (!teach) return;
+    for (int j = team.l + kHeld * L; j < k; j += L) {
+      const int cls = load_class(j);
+      if (cls >= 0) f(j, cls, load_logit(j));
+    }
+  };
+  all_slots([&](int j, int cls, S) {
+    atomicMin(&want[place(cls)], kSlot | static_cast<W>(j));
+  });
   A high = NegInf<A>();
 #pragma unroll
   for (int e = 0; e < E; ++e) high = Max(high, z[e]);
-  high = team.Max(high, red);
+  high = team.Max(high, red_high);
   if (!(high > NegInf<A>())) high = A(0);
   team.Sync();
 
   // the teacher's distribution, in logarithms to base two
   const bool rest = a.teacher_rest.data != nullptr;
-  const A r = rest && teach ? scale1 * LoadFloat<A>(a.teacher_rest, row * a.teacher_rest.stride[0])
-                            : NegInf<A>();
-  A t_high = r;
-  A t_nan = r != r ? A(1) : A(0);
-  auto for_slots = [&](auto&& f) {  // the slots that count
-    if (!teach) return;
-    for (int j = team.l; j < k; j += L) {
-      const int cls = load_class(j);
-      if (cls < 0) continue;
+  const S r = rest && teach ? static_cast<S>(scale1 * LoadFloat<A>(a.teacher_rest,
+                                                                   row * a.teacher_rest.stride[0]))
+                            : NegInf<S>();
+  S t_high = r;
+  S t_nan = r != r ? S(1) : S(0);
+  auto for_slots = [&](auto&& f) {  // the slots that count, with their place in the table
+    all_slots([&](int j, int cls, S t) {
       W* at = &want[place(cls)];
-      if (*at == (kSlot | static_cast<W>(j))) f(j, cls, at);
-    }
+      if (*at == (kSlot | static_cast<W>(j))) f(cls, t, at);
+    });
   };
-  for_slots([&](int j, int, W*) {
-    const A t = load_logit(j);
+  for_slots([&](int, S t, W*) {
     t_high = Max(t_high, t);
-    if (t != t) t_nan = A(1);
+    if (t != t) t_nan = S(1);
   });
   t_high = team.Max(t_high, red);
   t_nan = team.Max(t_nan, red);
-  const bool taught = teach && (t_high > NegInf<A>() || t_nan > A(0));
-  if (!(t_high > NegInf<A>())) t_high = A(0);
-  A t_sum = 0;
-  for_slots([&](int j, int, W*) { t_sum += Exp2(load_logit(j) - t_high); });
-  const A u_rest = rest ? Exp2(r - t_high) : A(0);
+  const bool taught = teach && (t_high > NegInf<S>() || t_nan > S(0));
+  if (!(t_high > NegInf<S>())) t_high = S(0);
+  S t_sum = 0;
+  for_slots([&](int, S t, W*) { t_sum += Exp2(t - t_high); });
+  const S u_rest = rest ? Exp2(r - t_high) : S(0);
   t_sum = team.Sum(t_sum, red) + u_rest;
-  const A t_inv = taught ? A(1) / t_sum : A(0), t_log = t_high + Log2(t_sum);
-  const A share = taught ? u_rest * t_inv : A(0);
+  const S t_log = t_high + Log2(t_sum);
+  const S share = taught ? u_rest / t_sum : S(0);
 
   // the student's: the classes without a slot are summed on their own
   const A off = -high * scale, off1 = -high * scale1;
-  const bool two = alpha < A(1);
-  A ez[E], left = 0, named = 0, total1 = 0;
+  const bool hard_term = alpha < S(1), two = hard_term && scale != scale1;
+  S ez[E], e1[E], left = 0, named = 0, total1 = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int cls = e * L + team.l;
-    ez[e] = Exp2(Fma(z[e], scale, off));
+    ez[e] = Exp2(exponent(z[e], scale, off));
     if (cls < c && want[place(cls)] != kNone) named += ez[e];
     else left += ez[e];
-    if (two) total1 += Exp2(Fma(z[e], scale1, off1));
+    e1[e] = two ? Exp2(exponent(z[e], scale1, off1)) : ez[e];
+    total1 += e1[e];
   }
   left = team.Sum(left, red);
-  const A total = left + team.Sum(named, red);
-  if (two) total1 = team.Sum(total1, red);
-  const A log_total = Log2(total);
-  A log_left = Log2(left), rest_off = off;
-  const bool again = rest && left < SmallRest<A>();
+  const S total = left + team.Sum(named, red);
+  total1 = two ? team.Sum(total1, red) : total;
+  const S log_total = Log2(total);
+  S log_left = Log2(left);
+  A rest_off = off;
+  const bool again = rest && left < SmallRest<S>();
   if (__syncthreads_or(again)) {
     A own = NegInf<A>();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int cls = e * L + team.l;
-      if (cls < c && want[place(cls)] == kNone) own = Max(own, z[e]);
+      if (again && cls < c && want[place(cls)] == kNone) own = Max(own, score(cls));
     }
-    own = team.Max(own, red);
+    own = team.Max(own, red_high);
     const bool able = again && own > NegInf<A>();
     const A own_off = -own * scale;
-    A sum = 0;
+    S sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int cls = e * L + team.l;
-      if (able && cls < c && want[place(cls)] == kNone) sum += Exp2(Fma(z[e], scale, own_off));
+      if (able && cls < c && want[place(cls)] == kNone)
+        sum += Exp2(exponent(score(cls), scale, own_off));
     }
     sum = team.Sum(sum, red);
     if (able) {
       left = sum;
       rest_off = own_off;
-      log_left = Log2(left) - rest_off + off;
+      log_left = Log2(left) + static_cast<S>(off - rest_off);
     }
   }
-  const bool live = w != A(0) && !(total == A(0));  // otherwise every class is masked
-  const int y = two && live ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
+  const bool live = w != S(0) && !(total == S(0));  // otherwise every class is masked
+  const int y = hard_term && live ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
 
   // the table's slots give way to their probabilities; every class has one such slot
-  A kl = 0;
-  const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+  S kl = 0;
   team.Sync();
-  for_slots([&](int j, int cls, W* at) {
-    const A lp = load_logit(j) - t_log;
-    const A p = taught ? Exp2(lp) : A(0);
-    if (a.loss.data && !(p == A(0))) {
-      const A v = static_cast<A>(x[cls * a.scores.stride[1]]);
-      kl += p * (lp - (Fma(v, scale, off) - log_total));
+  for_slots([&](int cls, S t, W* at) {
+    const S lp = t - t_log;
+    const S p = taught ? Exp2(lp) : S(0);
+    if (a.loss.data && !(p == S(0))) {
+      kl += p * (lp - (exponent(score(cls), scale, off) - log_total));
     }
     *at = ToBits(p) & ~kSlot;
   });
   if (a.loss.data) {
     kl = team.Sum(kl, red);
     if (there && team.l == 0) {
-      A v = 0;
+      S v = 0;
       if (live) {
-        if (rest && !(share == A(0))) kl += share * (r - t_log - (log_left - log_total));
-        if (taught) v = alpha * temp * temp * (kl * static_cast<A>(kLn2));
+        if (rest && !(share == S(0))) kl += share * (r - t_log - (log_left - log_total));
+        if (taught) v = alpha * temp * temp * (kl * static_cast<S>(kLn2));
         if (y >= 0)
-          v += (A(1) - alpha) * static_cast<A>(kLn2) *
-               (Log2(total1) - Fma(static_cast<A>(x[y * a.scores.stride[1]]), scale1, off1));
+          v += (S(1) - alpha) * static_cast<S>(kLn2) *
+               (Log2(total1) - exponent(score(y), scale1, off1));
         v *= w;
       }
       StoreFloat(a.loss, row * a.loss.stride[0], v);
@@ -501,33 +523,33 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   }
   if (!a.gradient.data && !a.hessian.data) return;
   team.Sync();
-  const A soft = taught ? alpha : A(0), hard = y >= 0 ? A(1) - alpha : A(0);
-  const A inv = A(1) / total, inv1 = hard > A(0) ? A(1) / total1 : A(0);
-  const A spread = rest && left > A(0) ? share / left : A(0);
-  const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
+  const S soft = taught ? alpha : S(0), hard = y >= 0 ? S(1) - alpha : S(0);
+  const S inv = S(1) / total, inv1 = hard > S(0) ? S(1) / total1 : S(0);
+  const S spread = rest && left > S(0) ? share / left : S(0);
+  const S factor = c > 1 ? static_cast<S>(c) / static_cast<S>(c - 1) : S(1);
   const bool moved = rest_off != off;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int cls = e * L + team.l;
     if (!there || cls >= c) continue;
-    A g = 0, h = 0;
+    S g = 0, h = 0;
     if (live) {
-      const A q = ez[e] * inv;
-      if (soft > A(0)) {
+      const S q = ez[e] * inv;
+      if (soft > S(0)) {
         const W bits = want[place(cls)];
-        A p = FromBits(bits);
+        S p = FromBits(bits);
         if (bits == kNone) {
-          p = A(0);
-          if (spread > A(0)) p = spread * (moved ? Exp2(Fma(z[e], scale, rest_off)) : ez[e]);
+          p = S(0);
+          if (spread > S(0)) p = spread * (moved ? Exp2(exponent(score(cls), scale, rest_off)) : ez[e]);
           else if (spread != spread) p = spread;
         }
         g = soft * temp * (q - p);
-        h = soft * q * (A(1) - q);
+        h = soft * q * (S(1) - q);
       }
-      if (hard > A(0)) {
-        const A q1 = Exp2(Fma(z[e], scale1, off1)) * inv1;
-        g += hard * (q1 - (cls == y ? A(1) : A(0)));
-        h += hard * q1 * (A(1) - q1);
+      if (hard > S(0)) {
+        const S q1 = e1[e] * inv1;
+        g += hard * (q1 - (cls == y ? S(1) : S(0)));
+        h += hard * q1 * (S(1) - q1);
       }
     }
     if (a.gradient.data)
@@ -1594,7 +1616,7 @@ __device__ __forceinline__ double WaveMass(const Residual<T>& f, int begin, int 
 /*!
  * Each wave of `splits` workgroups a sequence sums one segment of the row that the class is
  * drawn from. Which row that is, every workgroup finds for itself: a few gathers, instead of
- * a launch before this one.
+ * a launch before this one. The first of them writes what is known already.
  */
 template <typename T>
 __global__ void __launch_bounds__(kSplitBlock) k_verify_sums(LGBM_VerifyArgs a) {
@@ -1607,38 +1629,50 @@ __global__ void __launch_bounds__(kSplitBlock) k_verify_sums(LGBM_VerifyArgs a) 
   const double sum = WaveMass(mass, begin, end);
   if (threadIdx.x % kWave == 0)
     static_cast<double*>(a.workspace)[row * gridDim.x * kSplitWaves + at] = sum;
+  if (blockIdx.x == 0) PutVerified(a, row, n, -1, threadIdx.x, kSplitBlock);
 }
 
-/*! one workgroup a sequence: the segment that holds the goal, then the class in it */
+/*!
+ * One workgroup a sequence: the segment that holds the goal, by the waves' sums; in it the
+ * run of neighbouring classes of one thread, by a scan over the threads' sums; in that the
+ * class. The row is read twice where the goal lies, and nowhere else.
+ */
 template <typename T>
 __global__ void __launch_bounds__(kSplitBlock) k_verify_draw(LGBM_VerifyArgs a, int splits) {
+  constexpr int kSize = Chunk<T>::kSize;
   __shared__ double sums[kSplitWaves];
+  __shared__ double s_goal;
+  __shared__ int s_base;
   const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int segments = splits * kSplitWaves;
   static_assert(kMostSplits * kSplitWaves <= 4 * kWave, "four segments a lane");
   const double* part = static_cast<const double*>(a.workspace) + row * segments;
-  const int length = Length(a, row), n = Accepted<T>(a, row, length);
+  const int length = Length(a, row);
+  const int n = static_cast<const int32_t*>(a.out_accepted.data)[row * a.out_accepted.stride[0]];
   Residual<T> mass = ResidualOf<T>(a, row, n, length);
   const double v = Uniform(a.sample, row * a.sample.stride[0]);
   // every wave does the same with the segments' sums: lane l has those of 4 l .. 4 l + 3
-  const int lane = threadIdx.x % kWave;
   double own[4], sum = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     own[i] = 4 * lane + i < segments ? part[4 * lane + i] : 0.0;
     sum += own[i];
   }
-  double reach = sum;
+  auto wave_scan = [&](double reach) {
 #pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const double o = __shfl_up(reach, d);
-    if (lane >= d) reach += o;
-  }
+    for (int d = 1; d < kWave; d <<= 1) {
+      const double o = __shfl_up(reach, d);
+      if (lane >= d) reach += o;
+    }
+    return reach;
+  };
+  double reach = wave_scan(sum);
   const double total = __shfl(reach, kWave - 1);
   reach -= sum;
   int drawn;
   if (total > 0) {
-    const double goal = v * total;
+    double goal = v * total;
     int found = -1, last = -1;
     double before = 0, last_before = 0;
 #pragma unroll
@@ -1655,19 +1689,62 @@ __global__ void __launch_bounds__(kSplitBlock) k_verify_draw(LGBM_VerifyArgs a, 
     const unsigned long long over = __ballot(found >= 0), some = __ballot(last >= 0);
     const int who = over ? __ffsll(over) - 1 : 63 - __clzll(some);
     found = __shfl(over ? found : last, who);
-    before = __shfl(over ? before : last_before, who);
+    goal -= __shfl(over ? before : last_before, who);
     const int seg = SegmentOf<T>(a.classes, splits);
-    drawn = FindClass<kSplitBlock>(mass, found * seg, min(seg, a.classes - found * seg),
-                                   goal - before, sums);
+    const int begin = found * seg, end = min(a.classes, begin + seg);
+    // this thread's run; whole chunks at first, the classes after the last of them one by one
+    const int each = (seg + kSplitBlock * kSize - 1) / (kSplitBlock * kSize) * kSize;
+    const int mine = min(end, begin + tid * each), stop = min(end, mine + each);
+    double run = 0;
+    int c = mine;
+    for (; c + kSize <= stop; c += kSize) {
+      Chunk<T> p, q;
+      __builtin_memcpy(&p, mass.p + c, sizeof(p));
+      if (mass.q != nullptr) __builtin_memcpy(&q, mass.q + c, sizeof(q));
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) {
+        double w = MassOf(p.v[i]);
+        if (mass.q != nullptr) w = fmax(w - MassOf(q.v[i]), 0.0);
+        else if (c + i == mass.gone) w = 0.0;
+        run += w;
+      }
+    }
+    for (; c < stop; ++c) run += mass(c);
+    double upto = wave_scan(run);
+    if (lane == kWave - 1) sums[wave] = upto;
+    __syncthreads();
+    // the first wave whose sums up to its end pass the goal, the last with any where none does
+    int chosen = -1;
+    double wave_before = 0, prefix = 0;
+    for (int i = 0; i < kSplitWaves; ++i) {
+      if (!(sums[i] > 0)) continue;
+      chosen = i;
+      wave_before = prefix;
+      prefix += sums[i];
+      if (prefix > goal) break;
+    }
+    upto += wave_before;
+    const unsigned long long pass = __ballot(run > 0 && upto > goal), any = __ballot(run > 0);
+    const int who_runs = pass ? __ffsll(pass) - 1 : 63 - __clzll(any | 1);
+    const bool here = wave == chosen && lane == who_runs;
+    if (here) {
+      s_base = mine;
+      s_goal = goal - (upto - run);
+    }
+    __syncthreads();
+    const int base = s_base;
+    drawn = FindClass<kSplitBlock>(mass, base, min(each, end - base), s_goal, sums);
   } else {  // nothing is left of the target: the draw is from the target itself
     mass.q = nullptr;
     mass.gone = -1;
     double whole = 0;
-    for (int i = threadIdx.x; i < a.classes; i += kSplitBlock) whole += mass(i);
+    for (int i = tid; i < a.classes; i += kSplitBlock) whole += mass(i);
     whole = BlockSum<kSplitBlock>(whole, sums);
     drawn = FindClass<kSplitBlock>(mass, 0, a.classes, v * whole, sums);
   }
-  PutVerified(a, row, n, drawn, threadIdx.x, kSplitBlock);
+  if (tid == 0)
+    static_cast<int32_t*>(a.out_class.data)[row * a.out_class.stride[0] +
+                                            n * a.out_class.stride[1]] = drawn;
 }
 
 // ------------------------------------------------------------------ launches
@@ -1706,15 +1783,22 @@ int LanesFor(int classes, int each) {
   return lanes;
 }
 
-template <typename T, int E, bool kAcross>
+template <typename T, typename S, int E, bool kAcross>
 void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
   const int lanes = LanesFor(a.classes, E), rows = 256 / lanes;
-  const size_t lds = sizeof(Word<Acc<T>>) * rows * a.classes;  // at most 2048 * E bytes
-  auto kernel = k_distill_tile<T, E, kAcross>;
+  const size_t lds = sizeof(Word<S>) * rows * a.classes;  // at most 2048 * E bytes
+  auto kernel = k_distill_tile<T, S, E, kAcross>;
   AllowLds(kernel, lds);
-  hipLaunchKernelGGL(kernel,
-                     dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256), lds, s, a,
-                     lanes);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256),
+                     lds, s, a, lanes);
+}
+
+template <typename T, typename S>
+void DistillTile(const LGBM_DistillArgs& a, bool across, hipStream_t s) {
+  if (!across) LaunchDistillTile<T, S, 4, false>(a, s);
+  else if (a.classes <= 8) LaunchDistillTile<T, S, 8, true>(a, s);
+  else if (a.classes <= 256) LaunchDistillTile<T, S, 16, true>(a, s);
+  else LaunchDistillTile<T, S, 32, true>(a, s);
 }
 
 /*! whether the rows of a class stand closer together than the classes of a row */
@@ -1781,10 +1865,15 @@ void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
   if (a.classes <= (across ? 512 : 256)) {
     ByType(a.scores.type, [&](auto t) {
       using T = decltype(t);
-      if (!across) LaunchDistillTile<T, 4, false>(a, s);
-      else if (a.classes <= 8) LaunchDistillTile<T, 8, true>(a, s);
-      else if (a.classes <= 256) LaunchDistillTile<T, 16, true>(a, s);
-      else LaunchDistillTile<T, 32, true>(a, s);
+      LGBM_DistillArgs part = a;
+      if constexpr (std::is_same_v<T, double>) {
+        part.gradient.data = part.hessian.data = nullptr;
+        if (a.loss.data) DistillTile<double, double>(part, across, s);
+        part = a;
+        part.loss.data = nullptr;
+      }
+      if (part.loss.data || part.gradient.data || part.hessian.data)
+        DistillTile<T, float>(part, across, s);
     });
     OPS_HIP_OK(hipGetLastError());
     return;
