@@ -570,14 +570,21 @@ template <typename T> struct Chunk {
   T v[kSize];
 };
 
+/*! a row's workgroup: its threads, the chunks each holds in registers, and whether a row may
+ *  have more than these */
+template <int kBlock, int kCached, bool kMore = false> struct RowShape {
+  static constexpr int block = kBlock, cached = kCached;
+  static constexpr bool more = kMore;
+};
+
 /*!
  * A row whose classes stand next to each other, as its workgroup holds it: the first
  * kBlock * kCached chunks in registers, one chunk a thread in turn, further chunks read again
  * in each pass, and the classes after the last whole chunk one a thread. Chunks are read at
  * their elements' alignment: the hardware splits what crosses a line.
  */
-template <typename T, int kBlock, int kCached> struct RowOf {
-  static constexpr int kSize = Chunk<T>::kSize;
+template <typename T, typename Shape> struct RowOf {
+  static constexpr int kSize = Chunk<T>::kSize, kBlock = Shape::block, kCached = Shape::cached;
   using A = Acc<T>;
   const T* x;
   int chunks, tail;  // whole chunks, and the class of this thread after them (-1: none)
@@ -621,9 +628,11 @@ template <typename T, int kBlock, int kCached> struct RowOf {
       const int chunk = n * kBlock + threadIdx.x;
       if (chunk < chunks) Give(raw[n], chunk, f);
     }
+    if constexpr (Shape::more) {
 #pragma unroll 4
-    for (int chunk = kCached * kBlock + threadIdx.x; chunk < chunks; chunk += kBlock)
-      Give(Read(chunk), chunk, f);
+      for (int chunk = kCached * kBlock + threadIdx.x; chunk < chunks; chunk += kBlock)
+        Give(Read(chunk), chunk, f);
+    }
     if (tail >= 0) {
       const A v[1] = {tail_value};
       f(tail, v);
@@ -653,15 +662,15 @@ __device__ __forceinline__ void BlockSums(A (&v)[kCount], A* lds) {
 
 /*!
  * One workgroup a row of many classes: read once, as far as its registers reach, then the
- * maximum, the sums and the gradients from there. A thread looks at the bits of its chunk's
- * slots together, and leaves the fast path only where one is set.
+ * maximum, the sums and the gradients from there. Every thread writes its classes as if they
+ * had no slot; after a barrier the slots' threads write theirs over that.
  */
-template <typename T, int kBlock, int kCached>
-__global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
+template <typename T, typename Shape, bool kHessian>
+__global__ void __launch_bounds__(Shape::block) k_distill_row(LGBM_DistillArgs a) {
   using A = Acc<T>;
   using O = Out<T>;
-  using Row = RowOf<T, kBlock, kCached>;
-  constexpr int kWaves = kBlock / kWave;
+  using Row = RowOf<T, Shape>;
+  constexpr int kBlock = Shape::block, kWaves = kBlock / kWave;
   extern __shared__ uint32_t mark[];
   __shared__ int s_cls[kMaxTop];
   __shared__ A s_max[2][kWaves], s_sum[4 * kWaves], s_more[3][kWaves];
@@ -670,14 +679,13 @@ __global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
   const int tid = threadIdx.x, c = a.classes, k = a.k;
   O* grad = a.gradient.data ? static_cast<O*>(a.gradient.data) + row * a.gradient.stride[0]
                             : nullptr;
-  O* hess = a.hessian.data ? static_cast<O*>(a.hessian.data) + row * a.hessian.stride[0]
-                           : nullptr;
+  O* hess = kHessian ? static_cast<O*>(a.hessian.data) + row * a.hessian.stride[0] : nullptr;
   const A w = a.weight.data ? LoadFloat<A>(a.weight, row * a.weight.stride[0]) : A(1);
   auto put_zeros = [&] {
     if (a.loss.data && tid == 0) StoreFloat(a.loss, row * a.loss.stride[0], A(0));
     for (int i = tid; i < c; i += kBlock) {
       if (grad) grad[i] = static_cast<O>(0.0f);
-      if (hess) hess[i] = static_cast<O>(0.0f);
+      if (kHessian) hess[i] = static_cast<O>(0.0f);
     }
   };
   if (w == A(0)) {
@@ -692,7 +700,8 @@ __global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
   // the slots, one a thread
   const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
   const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
-  const bool rest = a.teacher_rest.data != nullptr, two = alpha < A(1);
+  const bool rest = a.teacher_rest.data != nullptr, hard_term = alpha < A(1);
+  const bool two = hard_term && scale != scale1;  // a softmax at another temperature
   int cls = -1;
   A logit = NegInf<A>(), z_slot = NegInf<A>();
   if (tid < k) {
@@ -707,7 +716,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
   }
   const A r = rest ? scale1 * LoadFloat<A>(a.teacher_rest, row * a.teacher_rest.stride[0])
                    : NegInf<A>();
-  const int label = two ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
+  const int label = hard_term ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
   const A z_label = label >= 0 ? static_cast<A>(z.x[label]) : A(0);
   __syncthreads();
   if (cls >= 0 && (atomicOr(&mark[cls >> 5], 1u << (cls & 31)) >> (cls & 31) & 1u)) s_dup = 1;
@@ -750,13 +759,12 @@ __global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
     A e[kSize], sum = 0;
 #pragma unroll
     for (int i = 0; i < kSize; ++i) e[i] = Exp2(Fma(v[i], scale, off));
-    if (bits == 0) {
+    if (bits != 0) {
 #pragma unroll
-      for (int i = 0; i < kSize; ++i) sum += e[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < kSize; ++i) sum += bits >> i & 1u ? A(0) : e[i];
+      for (int i = 0; i < kSize; ++i) e[i] = bits >> i & 1u ? A(0) : e[i];
     }
+#pragma unroll
+    for (int i = 0; i < kSize; ++i) sum += e[i];
     left += sum;
     if (two) {
       sum = 0;
@@ -771,8 +779,8 @@ __global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
   const A u = sums[2];
   BlockSums<kBlock>(sums, s_sum);
   left = sums[0];
-  total1 = sums[3];
   const A total = left + sums[1];
+  total1 = two ? sums[3] : total;
   if (total == A(0)) {  // every class is masked
     put_zeros();
     return;
@@ -825,62 +833,68 @@ __global__ void __launch_bounds__(kBlock) k_distill_row(LGBM_DistillArgs a) {
   const A inv = A(1) / total, inv1 = hard > A(0) ? A(1) / total1 : A(0);
   const A spread = rest && left > A(0) ? share / left : A(0);
   const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
-  const bool moved = rest_off != off;
   // a class without a slot: its gradient is one factor of each exponential
-  const A coef = soft > A(0) ? w * soft * temp * (moved ? inv : inv - spread) : A(0);
-  const A coef_rest = moved && soft > A(0) ? -w * soft * temp * spread : A(0);
+  const bool moved = rest_off != off;
+  const A each = w * soft * temp;  // 0 where there is no teacher, whose inv may be anything
+  A coef = soft > A(0) ? each * (moved ? inv : inv - spread) : A(0);
   const A coef1 = hard > A(0) ? w * hard * inv1 : A(0);
-  auto gradient_of = [&](A v) {
-    A g = coef * Exp2(Fma(v, scale, off));
-    if (hard > A(0)) g = Fma(coef1, Exp2(Fma(v, scale1, off1)), g);
-    if (moved) g = Fma(coef_rest, Exp2(Fma(v, scale, rest_off)), g);
-    return g;
-  };
-  auto hessian_of = [&](A v) {
-    const A q = Exp2(Fma(v, scale, off)) * inv;
-    A h = soft > A(0) ? soft * q * (A(1) - q) : A(0);
-    if (hard > A(0)) {
-      const A q1 = Exp2(Fma(v, scale1, off1)) * inv1;
-      h += hard * q1 * (A(1) - q1);
-    }
-    return h * factor * w;
-  };
-  z.Each([&](int base, const auto& v) {
-    constexpr int kSize = kSizeOf<decltype(v)>;
-    const uint32_t bits = bits_of(base, kSize);
-    O g[kSize], h[kSize];
-    if (grad) {
+  if (!two) coef += coef1;
+  if (grad) {
+    if (moved) {
+      const A coef_rest = soft > A(0) ? -each * spread : A(0);
+      z.Each([&](int base, const auto& v) {
 #pragma unroll
-      for (int i = 0; i < kSize; ++i) g[i] = static_cast<O>(gradient_of(v[i]));
-    }
-    if (hess) {
+        for (int i = 0; i < kSizeOf<decltype(v)>; ++i) {
+          A g = coef * Exp2(Fma(v[i], scale, off));
+          if (two) g = Fma(coef1, Exp2(Fma(v[i], scale1, off1)), g);
+          grad[base + i] = static_cast<O>(Fma(coef_rest, Exp2(Fma(v[i], scale, rest_off)), g));
+        }
+      });
+    } else {
+      z.Each([&](int base, const auto& v) {
+        constexpr int kSize = kSizeOf<decltype(v)>;
+        O g[kSize];
+        if (two) {
 #pragma unroll
-      for (int i = 0; i < kSize; ++i) h[i] = static_cast<O>(hessian_of(v[i]));
-    }
-    if (bits == 0 &&
-        static_cast<unsigned>(label - base) >= static_cast<unsigned>(kSize)) {
-      if (grad) __builtin_memcpy(grad + base, &g, sizeof(O) * kSize);
-      if (hess) __builtin_memcpy(hess + base, &h, sizeof(O) * kSize);
-    } else {  // a slot's class is its thread's, below
+          for (int i = 0; i < kSize; ++i)
+            g[i] = static_cast<O>(Fma(coef1, Exp2(Fma(v[i], scale1, off1)),
+                                      coef * Exp2(Fma(v[i], scale, off))));
+        } else {
 #pragma unroll
-      for (int i = 0; i < kSize; ++i) {
-        if (bits >> i & 1u) continue;
-        if (grad)
-          grad[base + i] = base + i == label
-                               ? static_cast<O>(gradient_of(v[i]) - w * hard)
-                               : g[i];
-        if (hess) hess[base + i] = h[i];
+          for (int i = 0; i < kSize; ++i)
+            g[i] = static_cast<O>(coef * Exp2(Fma(v[i], scale, off)));
+        }
+        __builtin_memcpy(grad + base, &g, sizeof(g));
+      });
+    }
+  }
+  if (kHessian) {
+    z.Each([&](int base, const auto& v) {
+#pragma unroll
+      for (int i = 0; i < kSizeOf<decltype(v)>; ++i) {
+        const A q = Exp2(Fma(v[i], scale, off)) * inv;
+        A h = soft > A(0) ? soft * q * (A(1) - q) : A(0);
+        if (hard > A(0)) {
+          const A q1 = Exp2(Fma(v[i], scale1, off1)) * inv1;
+          h += hard * q1 * (A(1) - q1);
+        }
+        hess[base + i] = static_cast<O>(h * factor * w);
       }
-    }
-  });
-  if (cls >= 0) {
-    const A q = Exp2(log_e) * inv;
+    });
+  }
+  if (!grad) return;
+  __syncthreads();
+  auto put = [&](int at, A v, A p, A from, bool spread_it) {
+    const A q = Exp2(Fma(v, scale, off)) * inv;
+    if (spread_it) p = spread > A(0) ? spread * Exp2(Fma(v, scale, from)) : A(0);
     A g = soft > A(0) ? soft * temp * (q - p) : A(0);
     if (hard > A(0))
-      g += hard * (Exp2(Fma(z_slot, scale1, off1)) * inv1 - (cls == label ? A(1) : A(0)));
-    if (grad) grad[cls] = static_cast<O>(g * w);
-    if (hess) hess[cls] = static_cast<O>(hessian_of(z_slot));
-  }
+      g += hard * (Exp2(Fma(v, scale1, off1)) * inv1 - (at == label ? A(1) : A(0)));
+    grad[at] = static_cast<O>(g * w);
+  };
+  if (cls >= 0) put(cls, z_slot, p, off, false);
+  // the label's class, where it has no slot
+  if (tid == 0 && label >= 0 && !bits_of(label, 1)) put(label, z_label, A(0), rest_off, true);
 }
 
 // ------------------------------------------------------------------ top logits, any strides
@@ -1141,10 +1155,10 @@ constexpr int kTopCandidates = 1024;  // of a row at most, or it goes the slow w
  * exponentials of the others; the candidates are put in order by counting. Rows with more
  * candidates than fit, of many equal scores for instance, are done digit by digit (TopAny).
  */
-template <typename T, int kBlock, int kCached>
-__global__ void __launch_bounds__(kBlock) k_top_row(LGBM_TopLogitsArgs a) {
+template <typename T, typename Shape>
+__global__ void __launch_bounds__(Shape::block) k_top_row(LGBM_TopLogitsArgs a) {
   using A = Acc<T>;
-  constexpr int kWaves = kBlock / kWave;
+  constexpr int kBlock = Shape::block, kWaves = kBlock / kWave;
   static_assert(std::is_same_v<A, float>, "keys of 32 bits");
   __shared__ int hist[kTopBins];
   __shared__ A s_low[kWaves], s_high[kWaves], s_sum[kWaves];
@@ -1155,7 +1169,7 @@ __global__ void __launch_bounds__(kBlock) k_top_row(LGBM_TopLogitsArgs a) {
   __shared__ A s_rest[kTopCandidates];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, k = a.k;
-  RowOf<T, kBlock, kCached> z(
+  RowOf<T, Shape> z(
       static_cast<const T*>(a.scores.data) + row * a.scores.stride[0], a.classes);
   z.Load();
   for (int i = tid; i < kTopBins; i += kBlock) hist[i] = 0;
@@ -1168,6 +1182,11 @@ __global__ void __launch_bounds__(kBlock) k_top_row(LGBM_TopLogitsArgs a) {
 #pragma unroll
     for (int i = 0; i < kSizeOf<decltype(v)>; ++i) part[i & 3] = Max(part[i & 3], v[i]);
   });
+  // a quarter of them is enough where it still is four times k
+  if (kBlock >= 4 * k) {
+    part[0] = Max(Max(part[0], part[1]), Max(part[2], part[3]));
+    part[1] = part[2] = part[3] = NegInf<A>();
+  }
   A high = NegInf<A>(), low = -NegInf<A>();
   int valid = 0;
 #pragma unroll
@@ -1250,7 +1269,8 @@ __global__ void __launch_bounds__(kBlock) k_top_row(LGBM_TopLogitsArgs a) {
     A top = v[0];
 #pragma unroll
     for (int i = 1; i < kSize; ++i) top = Max(top, v[i]);
-    if (top >= edge) {
+    const bool some = top >= edge;
+    if (some) {
 #pragma unroll
       for (int i = 0; i < kSize; ++i) {
         if (!(v[i] >= edge)) continue;
@@ -1262,9 +1282,16 @@ __global__ void __launch_bounds__(kBlock) k_top_row(LGBM_TopLogitsArgs a) {
       }
     }
     if (rest) {
-      A own = 0;
+      A e[kSize], own = 0;
+      // at most one below the edge; the bounds turn NaN to zero, and cost nothing
 #pragma unroll
-      for (int i = 0; i < kSize; ++i) own += v[i] < edge ? Exp2(Fma(v[i], scale, off)) : A(0);
+      for (int i = 0; i < kSize; ++i) e[i] = fminf(fmaxf(Exp2(Fma(v[i], scale, off)), 0.0f), 1.0f);
+      if (some) {
+#pragma unroll
+        for (int i = 0; i < kSize; ++i) e[i] = v[i] < edge ? e[i] : A(0);
+      }
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) own += e[i];
       sum += own;
     }
   });
@@ -1276,14 +1303,19 @@ __global__ void __launch_bounds__(kBlock) k_top_row(LGBM_TopLogitsArgs a) {
   }
   int32_t* out_class = static_cast<int32_t*>(a.top_class.data) + row * a.top_class.stride[0];
   T* out_logit = static_cast<T*>(a.top_logit.data) + row * a.top_logit.stride[0];
-  for (int i = tid; i < n; i += kBlock) {
+  // eight lanes compare one candidate with the others
+  for (int i = tid / 8; i < n; i += kBlock / 8) {
     const A v = s_value[i];
     const int cls = s_cls[i];
     int rank = 0;
-    for (int o = 0; o < n; ++o) {
+    for (int o = tid % 8; o < n; o += 8) {
       const A u = s_value[o];
       rank += u > v || (u == v && s_cls[o] < cls);
     }
+    rank += __shfl_xor(rank, 1);
+    rank += __shfl_xor(rank, 2);
+    rank += __shfl_xor(rank, 4);
+    if (tid % 8 != 0) continue;
     if (rank < k) {
       out_class[rank * a.top_class.stride[1]] = cls;
       out_logit[rank * a.top_logit.stride[1]] = static_cast<T>(v);
@@ -1815,10 +1847,26 @@ void LaunchTopTile(const LGBM_TopLogitsArgs& a, hipStream_t s) {
                      lanes);
 }
 
-template <typename T, int kBlock, int kCached>
+template <typename T, typename Shape>
 void LaunchTopRow(const LGBM_TopLogitsArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_top_row<T, kBlock, kCached>), dim3(static_cast<uint32_t>(a.rows)),
-                     dim3(kBlock), 0, s, a);
+  hipLaunchKernelGGL((k_top_row<T, Shape>), dim3(static_cast<uint32_t>(a.rows)),
+                     dim3(Shape::block), 0, s, a);
+}
+
+/*!
+ * The workgroup of a row of `chunks` whole chunks, f(threads, chunks a thread in registers).
+ * Many rows: few threads with much of the row each, so that four rows or more share a compute
+ * unit and one computes while another waits for its scores. Rows that leave compute units
+ * idle: as many threads as there are, so that the one row is done sooner.
+ */
+template <typename F> void ByRow(int64_t rows, int chunks, F&& f) {
+  if (chunks <= 256) f(RowShape<256, 1>{});
+  else if (rows < 512 && chunks <= 4096) f(RowShape<1024, 4>{});
+  else if (chunks <= 1024) f(RowShape<256, 4>{});
+  else if (chunks <= 2048) f(RowShape<256, 8>{});
+  else if (chunks <= 4096) f(RowShape<256, 16>{});
+  else if (rows >= 512 && chunks <= 8192) f(RowShape<512, 16>{});
+  else f(RowShape<1024, 12, true>{});
 }
 
 void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
@@ -1836,11 +1884,9 @@ void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
     }
     if constexpr (!std::is_same_v<T, double>) {
       if (a.scores.stride[1] == 1) {
-        const int chunks = a.classes / Chunk<T>::kSize;
-        if (chunks <= 256) LaunchTopRow<T, 256, 1>(a, s);
-        else if (chunks <= 1024) LaunchTopRow<T, 256, 4>(a, s);
-        else if (chunks <= 4096) LaunchTopRow<T, 512, 8>(a, s);
-        else LaunchTopRow<T, 1024, 8>(a, s);
+        ByRow(a.rows, a.classes / Chunk<T>::kSize, [&](auto shape) {
+          LaunchTopRow<T, decltype(shape)>(a, s);
+        });
         return;
       }
     }
@@ -1850,12 +1896,15 @@ void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
   OPS_HIP_OK(hipGetLastError());
 }
 
-template <typename T, int kBlock, int kCached>
+template <typename T, typename Shape>
 void LaunchDistillRow(const LGBM_DistillArgs& a, hipStream_t s) {
-  auto kernel = k_distill_row<T, kBlock, kCached>;
   const size_t lds = sizeof(uint32_t) * ((a.classes + 31) / 32);
-  AllowLds(kernel, lds);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(kBlock), lds, s, a);
+  auto launch = [&](auto kernel) {
+    AllowLds(kernel, lds);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(Shape::block), lds, s, a);
+  };
+  if (a.hessian.data) launch(k_distill_row<T, Shape, true>);
+  else launch(k_distill_row<T, Shape, false>);
 }
 
 void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
@@ -1884,13 +1933,9 @@ void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
     ByType(a.scores.type, [&](auto t) {
       using T = decltype(t);
       if constexpr (!std::is_same_v<T, double>) {
-        constexpr int kSize = Chunk<T>::kSize;
-        const int chunks = (a.classes + kSize - 1) / kSize;
-        if (chunks <= 256) LaunchDistillRow<T, 256, 1>(a, s);
-        else if (chunks <= 1024) LaunchDistillRow<T, 256, 4>(a, s);
-        else if (chunks <= 4096) LaunchDistillRow<T, 512, 8>(a, s);
-        else if (chunks <= 8192) LaunchDistillRow<T, 1024, 8>(a, s);
-        else LaunchDistillRow<T, 1024, 12>(a, s);
+        ByRow(a.rows, a.classes / Chunk<T>::kSize, [&](auto shape) {
+          LaunchDistillRow<T, decltype(shape)>(a, s);
+        });
       }
     });
     OPS_HIP_OK(hipGetLastError());
