@@ -290,21 +290,27 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
  * The threads that share a row. kAcross: a class's rows stand next to each other in memory
  * (a booster's scores), so neighbouring threads are neighbouring rows, and a row's L threads
  * are R apart; otherwise a row's threads are L neighbours. Thread l of a row holds the
- * classes e * L + l. R * L = 256.
+ * classes e * L + l. R * L = 256. kAcross of one thread a row (kAlone) shares nothing, and its
+ * classes are the same for all threads, so that their addresses are scalar arithmetic.
  */
-template <bool kAcross> struct Team {
+enum TeamKind { kNeighbours, kAcross, kAlone };
+template <TeamKind kKind> struct Team {
   int L, R, l, r;
-  __device__ explicit Team(int lanes) : L(lanes), R(256 / lanes) {
-    l = kAcross ? threadIdx.x / R : threadIdx.x % L;
-    r = kAcross ? threadIdx.x % R : threadIdx.x / L;
+  __device__ explicit Team(int lanes) {
+    L = kKind == kAlone ? 1 : lanes;
+    R = 256 / L;
+    l = kKind == kAlone ? 0 : kKind == kAcross ? threadIdx.x / R : threadIdx.x % L;
+    r = kKind == kNeighbours ? threadIdx.x / L : threadIdx.x % R;
   }
   /*! of one thread a row nothing is shared */
   __device__ void Sync() const {
-    if (!(kAcross && L == 1)) __syncthreads();
+    if (kKind != kAlone) __syncthreads();
   }
+  /*! whether v holds for a thread that this one has to keep step with */
+  __device__ bool Any(bool v) const { return kKind == kAlone ? v : __syncthreads_or(v); }
   template <typename A, typename F> __device__ A Reduce(A v, A* lds, const F& f) const {
-    if (kAcross) {
-      if (L == 1) return v;
+    if (kKind == kAlone) return v;
+    if (kKind == kAcross) {
       __syncthreads();
       lds[threadIdx.x] = v;
       __syncthreads();
@@ -347,7 +353,7 @@ template <typename F> void AllowLds(F* kernel, size_t bytes) {
  * gradient by about its own rounding and takes a third off a booster's (185 -> 125 us for two
  * million rows of seven classes with hessians, where 64-bit exponentials are the bound).
  */
-template <typename T, typename S, int E, bool kAcross>
+template <typename T, typename S, int E, TeamKind kKind>
 __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int lanes) {
   using A = Acc<T>;
   using O = Out<T>;
@@ -355,17 +361,28 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   constexpr W kNone = ~W{0}, kSlot = W{1} << (sizeof(W) * 8 - 1);
   extern __shared__ unsigned long long tile_lds[];
   W* want = reinterpret_cast<W*>(tile_lds);  // R * classes
-  __shared__ A red_high[kAcross ? 256 : 1];
-  __shared__ S red[kAcross ? 256 : 1];
-  const Team<kAcross> team(lanes);
+  __shared__ A red_high[kKind == kAcross ? 256 : 1];
+  __shared__ S red[kKind == kAcross ? 256 : 1];
+  const Team<kKind> team(lanes);
   const int c = a.classes, k = a.k, L = team.L, R = team.R;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * R + team.r;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * R;
+  const int64_t row = first + team.r;
   const bool there = row < a.rows;
-  auto place = [&](int cls) { return kAcross ? cls * R + team.r : team.r * c + cls; };
+  // of a strided array, the place of this row: the workgroup's by scalar arithmetic
+  auto at_row = [&](const LGBM_Array& v) {
+    const int64_t step = v.stride[0];
+    const int64_t more = step == static_cast<int>(step)
+                             ? static_cast<int64_t>(team.r) * static_cast<int>(step)
+                             : team.r * step;
+    return first * step + more;
+  };
+  auto place = [&](int cls) {
+    return kKind == kNeighbours ? team.r * c + cls : cls * R + team.r;
+  };
 
-  const S w = !there ? S(0) : a.weight.data ? LoadFloat<S>(a.weight, row * a.weight.stride[0])
+  const S w = !there ? S(0) : a.weight.data ? LoadFloat<S>(a.weight, at_row(a.weight))
                                             : S(1);
-  const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+  const T* x = static_cast<const T*>(a.scores.data) + at_row(a.scores);
   auto score = [&](int cls) { return static_cast<A>(x[cls * a.scores.stride[1]]); };
   A z[E];  // not kept beyond the exponentials: the few that need a score later read it again
 #pragma unroll
@@ -380,18 +397,17 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   // exponents are formed as the scores are held, and taken as the statistics are
   auto exponent = [](A v, A by, A from) { return static_cast<S>(Fma(v, by, from)); };
   const bool teach = w != S(0) && alpha > S(0);
-  // the slots of this thread: the first few stay in registers
+  // the slots of this thread: the first few stay in registers, read before any is looked at
   constexpr int kHeld = 4;
   int held_cls[kHeld];
   S held_logit[kHeld];
+  const int64_t class_row = at_row(a.teacher_class), logit_row = at_row(a.teacher_logit);
   auto load_class = [&](int j) {
-    return LoadClass(a.teacher_class,
-                     row * a.teacher_class.stride[0] + j * a.teacher_class.stride[1], c);
+    return LoadClass(a.teacher_class, class_row + j * a.teacher_class.stride[1], c);
   };
   auto load_logit = [&](int j) {
-    return static_cast<S>(scale *
-                          LoadFloat<A>(a.teacher_logit, row * a.teacher_logit.stride[0] +
-                                                            j * a.teacher_logit.stride[1]));
+    return static_cast<S>(scale) *
+           LoadFloat<S>(a.teacher_logit, logit_row + j * a.teacher_logit.stride[1]);
   };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
@@ -422,8 +438,8 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
 
   // the teacher's distribution, in logarithms to base two
   const bool rest = a.teacher_rest.data != nullptr;
-  const S r = rest && teach ? static_cast<S>(scale1 * LoadFloat<A>(a.teacher_rest,
-                                                                   row * a.teacher_rest.stride[0]))
+  const S r = rest && teach ? static_cast<S>(scale1) * LoadFloat<S>(a.teacher_rest,
+                                                                     at_row(a.teacher_rest))
                             : NegInf<S>();
   S t_high = r;
   S t_nan = r != r ? S(1) : S(0);
@@ -468,7 +484,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   S log_left = Log2(left);
   A rest_off = off;
   const bool again = rest && left < SmallRest<S>();
-  if (__syncthreads_or(again)) {
+  if (team.Any(again)) {
     A own = NegInf<A>();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -493,7 +509,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
     }
   }
   const bool live = w != S(0) && !(total == S(0));  // otherwise every class is masked
-  const int y = hard_term && live ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
+  const int y = hard_term && live ? LoadClass(a.label, at_row(a.label), c) : -1;
 
   // the table's slots give way to their probabilities; every class has one such slot
   S kl = 0;
@@ -518,7 +534,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
                (Log2(total1) - exponent(score(y), scale1, off1));
         v *= w;
       }
-      StoreFloat(a.loss, row * a.loss.stride[0], v);
+      StoreFloat(a.loss, at_row(a.loss), v);
     }
   }
   if (!a.gradient.data && !a.hessian.data) return;
@@ -528,6 +544,8 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   const S spread = rest && left > S(0) ? share / left : S(0);
   const S factor = c > 1 ? static_cast<S>(c) / static_cast<S>(c - 1) : S(1);
   const bool moved = rest_off != off;
+  O* grad = static_cast<O*>(a.gradient.data) + (a.gradient.data ? at_row(a.gradient) : 0);
+  O* hess = static_cast<O*>(a.hessian.data) + (a.hessian.data ? at_row(a.hessian) : 0);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int cls = e * L + team.l;
@@ -552,12 +570,8 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
         h += hard * q1 * (S(1) - q1);
       }
     }
-    if (a.gradient.data)
-      static_cast<O*>(a.gradient.data)[row * a.gradient.stride[0] + cls * a.gradient.stride[1]] =
-          static_cast<O>(g * w);
-    if (a.hessian.data)
-      static_cast<O*>(a.hessian.data)[row * a.hessian.stride[0] + cls * a.hessian.stride[1]] =
-          static_cast<O>(h * factor * w);
+    if (a.gradient.data) grad[cls * a.gradient.stride[1]] = static_cast<O>(g * w);
+    if (a.hessian.data) hess[cls * a.hessian.stride[1]] = static_cast<O>(h * factor * w);
   }
 }
 
@@ -570,29 +584,34 @@ template <typename T> struct Chunk {
   T v[kSize];
 };
 
-/*! a row's workgroup: its threads, the chunks each holds in registers, and whether a row may
- *  have more than these */
+/*!
+ * A row's workgroup: its threads, and the chunks that each holds in registers. kMore: a row
+ * may have more than these; then up to kLdsChunks more a thread stand in LDS, as far as it
+ * reaches, and what is left is read from memory in each pass.
+ */
 template <int kBlock, int kCached, bool kMore = false> struct RowShape {
   static constexpr int block = kBlock, cached = kCached;
   static constexpr bool more = kMore;
 };
+constexpr int kLdsChunks = 8;
 
 /*!
- * A row whose classes stand next to each other, as its workgroup holds it: the first
- * kBlock * kCached chunks in registers, one chunk a thread in turn, further chunks read again
- * in each pass, and the classes after the last whole chunk one a thread. Chunks are read at
- * their elements' alignment: the hardware splits what crosses a line.
+ * A row whose classes stand next to each other, as its workgroup holds it: one chunk a thread
+ * in turn, and the classes after the last whole chunk one a thread. Chunks are read at their
+ * elements' alignment: the hardware splits what crosses a line.
  */
 template <typename T, typename Shape> struct RowOf {
   static constexpr int kSize = Chunk<T>::kSize, kBlock = Shape::block, kCached = Shape::cached;
   using A = Acc<T>;
   const T* x;
   int chunks, tail;  // whole chunks, and the class of this thread after them (-1: none)
+  int in_lds;        // chunks a thread in LDS
+  Words* lds;
   A tail_value;
   Words raw[kCached];
 
-  __device__ __forceinline__ RowOf(const T* row, int classes)
-      : x(row), chunks(classes / kSize) {
+  __device__ __forceinline__ RowOf(const T* row, int classes, Words* lds_space, int lds_chunks)
+      : x(row), chunks(classes / kSize), in_lds(lds_chunks), lds(lds_space) {
     tail = chunks * kSize + static_cast<int>(threadIdx.x);
     if (tail >= classes) tail = -1;
   }
@@ -608,6 +627,13 @@ template <typename T, typename Shape> struct RowOf {
       raw[n] = chunk < chunks ? Read(chunk) : Words{};
     }
     tail_value = tail >= 0 ? static_cast<A>(x[tail]) : A(0);
+    if constexpr (Shape::more) {  // every thread reads back what it wrote itself
+#pragma unroll 4
+      for (int n = 0; n < in_lds; ++n) {
+        const int chunk = (kCached + n) * kBlock + threadIdx.x;
+        if (chunk < chunks) lds[n * kBlock + threadIdx.x] = Read(chunk);
+      }
+    }
   }
   template <typename F>
   static __device__ __forceinline__ void Give(const Words& words, int chunk, const F& f) {
@@ -618,8 +644,8 @@ template <typename T, typename Shape> struct RowOf {
     for (int i = 0; i < kSize; ++i) v[i] = static_cast<A>(got.v[i]);
     f(chunk * kSize, v);
   }
-  /*! f(first class, values) of all that this thread holds, kSize or one at a time */
-  template <typename F> __device__ __forceinline__ void Each(const F& f) {
+  /*! f(first class, values) of what this thread holds, kSize or one at a time */
+  template <typename F> __device__ __forceinline__ void EachHeld(const F& f) {
 #pragma unroll
     for (int n = 0; n < kCached; ++n) {
       // what a pass makes of the row is not kept for the next: the compiler would hold its
@@ -629,14 +655,27 @@ template <typename T, typename Shape> struct RowOf {
       if (chunk < chunks) Give(raw[n], chunk, f);
     }
     if constexpr (Shape::more) {
-#pragma unroll 4
-      for (int chunk = kCached * kBlock + threadIdx.x; chunk < chunks; chunk += kBlock)
-        Give(Read(chunk), chunk, f);
+      for (int n = 0; n < in_lds; ++n) {
+        const int chunk = (kCached + n) * kBlock + threadIdx.x;
+        if (chunk < chunks) Give(lds[n * kBlock + threadIdx.x], chunk, f);
+      }
     }
     if (tail >= 0) {
       const A v[1] = {tail_value};
       f(tail, v);
     }
+  }
+  /*! f(first class, values) of what this thread reads each time */
+  template <typename F> __device__ __forceinline__ void EachMore(const F& f) const {
+    if constexpr (Shape::more) {
+#pragma unroll 4
+      for (int chunk = (kCached + in_lds) * kBlock + threadIdx.x; chunk < chunks; chunk += kBlock)
+        Give(Read(chunk), chunk, f);
+    }
+  }
+  template <typename F> __device__ __forceinline__ void Each(const F& f) {
+    EachHeld(f);
+    EachMore(f);
   }
 };
 
@@ -666,12 +705,14 @@ __device__ __forceinline__ void BlockSums(A (&v)[kCount], A* lds) {
  * had no slot; after a barrier the slots' threads write theirs over that.
  */
 template <typename T, typename Shape, bool kHessian>
-__global__ void __launch_bounds__(Shape::block) k_distill_row(LGBM_DistillArgs a) {
+__global__ void __launch_bounds__(Shape::block, Shape::cached >= 12 ? 4 : 1)
+k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   using A = Acc<T>;
   using O = Out<T>;
   using Row = RowOf<T, Shape>;
   constexpr int kBlock = Shape::block, kWaves = kBlock / kWave;
-  extern __shared__ uint32_t mark[];
+  extern __shared__ Words row_lds[];  // the chunks, then the marks
+  uint32_t* mark = reinterpret_cast<uint32_t*>(row_lds + lds_chunks * Shape::block);
   __shared__ int s_cls[kMaxTop];
   __shared__ A s_max[2][kWaves], s_sum[4 * kWaves], s_more[3][kWaves];
   __shared__ int s_dup;
@@ -692,7 +733,7 @@ __global__ void __launch_bounds__(Shape::block) k_distill_row(LGBM_DistillArgs a
     put_zeros();
     return;
   }
-  Row z(static_cast<const T*>(a.scores.data) + row * a.scores.stride[0], c);
+  Row z(static_cast<const T*>(a.scores.data) + row * a.scores.stride[0], c, row_lds, lds_chunks);
   z.Load();
   for (int i = tid; i < (c + 31) / 32; i += kBlock) mark[i] = 0;
   if (tid == 0) s_dup = 0;
@@ -721,11 +762,54 @@ __global__ void __launch_bounds__(Shape::block) k_distill_row(LGBM_DistillArgs a
   __syncthreads();
   if (cls >= 0 && (atomicOr(&mark[cls >> 5], 1u << (cls & 31)) >> (cls & 31) & 1u)) s_dup = 1;
 
+  auto bits_of = [&](int base, int size) {  // those of a chunk stand in one word
+    return mark[base >> 5] >> (base & 31) & ((1u << size) - 1u);
+  };
+  // the sums of a chunk's exponentials of the classes without a slot, and of all at T = 1
+  auto add_chunk = [&](int base, const auto& v, A from, A from1, A& rest_sum, A& all_sum) {
+    constexpr int kSize = kSizeOf<decltype(v)>;
+    const uint32_t bits = bits_of(base, kSize);
+    A e[kSize], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kSize; ++i) e[i] = Exp2(Fma(v[i], scale, from));
+    if (bits != 0) {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) e[i] = bits >> i & 1u ? A(0) : e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kSize; ++i) sum += e[i];
+    rest_sum += sum;
+    if (two) {
+      sum = 0;
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) sum += Exp2(Fma(v[i], scale1, from1));
+      all_sum += sum;
+    }
+  };
   A high = NegInf<A>();
-  z.Each([&](int, const auto& v) {
+  z.EachHeld([&](int, const auto& v) {
 #pragma unroll
     for (int i = 0; i < kSizeOf<decltype(v)>; ++i) high = Max(high, v[i]);
   });
+  // what is not held is read once for both, its sums against this thread's maximum so far
+  A more_high = NegInf<A>(), more_left = 0, more_total1 = 0;
+  if constexpr (Shape::more) {
+    __syncthreads();  // the marks
+    z.EachMore([&](int base, const auto& v) {
+      A top = v[0];
+#pragma unroll
+      for (int i = 1; i < kSizeOf<decltype(v)>; ++i) top = Max(top, v[i]);
+      if (top > more_high) {
+        more_left *= Exp2((more_high - top) * scale);
+        if (two) more_total1 *= Exp2((more_high - top) * scale1);
+        more_high = top;
+      }
+      const A from = more_high > NegInf<A>() ? -more_high : A(0);
+      add_chunk(base, v, from * scale, from * scale1, more_left, more_total1);
+    });
+    high = Max(high, more_high);
+  }
+  const A own_high = more_high;
   high = WaveMax(high);
   A t_high = WaveMax(Max(logit, r));
   if (tid % kWave == 0) {
@@ -749,30 +833,15 @@ __global__ void __launch_bounds__(Shape::block) k_distill_row(LGBM_DistillArgs a
   if (!t_some) t_high = A(0);
 
   const A off = -high * scale, off1 = -high * scale1;
-  auto bits_of = [&](int base, int size) {  // those of a chunk stand in one word
-    return mark[base >> 5] >> (base & 31) & ((1u << size) - 1u);
-  };
   A left = 0, total1 = 0;
-  z.Each([&](int base, const auto& v) {
-    constexpr int kSize = kSizeOf<decltype(v)>;
-    const uint32_t bits = bits_of(base, kSize);
-    A e[kSize], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kSize; ++i) e[i] = Exp2(Fma(v[i], scale, off));
-    if (bits != 0) {
-#pragma unroll
-      for (int i = 0; i < kSize; ++i) e[i] = bits >> i & 1u ? A(0) : e[i];
+  z.EachHeld([&](int base, const auto& v) { add_chunk(base, v, off, off1, left, total1); });
+  if constexpr (Shape::more) {
+    if (own_high > NegInf<A>() || more_left != A(0)) {
+      left += more_left * Exp2((own_high > NegInf<A>() ? own_high - high : A(0)) * scale);
+      if (two)
+        total1 += more_total1 * Exp2((own_high > NegInf<A>() ? own_high - high : A(0)) * scale1);
     }
-#pragma unroll
-    for (int i = 0; i < kSize; ++i) sum += e[i];
-    left += sum;
-    if (two) {
-      sum = 0;
-#pragma unroll
-      for (int i = 0; i < kSize; ++i) sum += Exp2(Fma(v[i], scale1, off1));
-      total1 += sum;
-    }
-  });
+  }
   const A log_e = Fma(z_slot, scale, off);
   A sums[4] = {left, cls >= 0 ? Exp2(log_e) : A(0),
                cls >= 0 && !(logit == NegInf<A>()) ? Exp2(logit - t_high) : A(0), total1};
@@ -1068,12 +1137,12 @@ __global__ void __launch_bounds__(kBlock) k_top_any(LGBM_TopLogitsArgs a) {
  * Up to E * L classes, in the registers of their row's threads (Team): k times the largest
  * that is left, by comparison with all others. Of equals the lowest class is met first.
  */
-template <typename T, int E, bool kAcross>
+template <typename T, int E, TeamKind kKind>
 __global__ void __launch_bounds__(256) k_top_tile(LGBM_TopLogitsArgs a, int lanes) {
   using A = Acc<T>;
   __shared__ A red[256];
   __shared__ int red_cls[256];
-  const Team<kAcross> team(lanes);
+  const Team<kKind> team(lanes);
   const int c = a.classes, L = team.L, R = team.R;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * R + team.r;
   const bool there = row < a.rows;
@@ -1103,15 +1172,13 @@ __global__ void __launch_bounds__(256) k_top_tile(LGBM_TopLogitsArgs a, int lane
         cls = o;
       }
     };
-    if (kAcross) {
-      if (L > 1) {
-        __syncthreads();
-        red[threadIdx.x] = best;
-        red_cls[threadIdx.x] = cls;
-        __syncthreads();
-        for (int i = 0; i < L; ++i) other(red[i * R + team.r], red_cls[i * R + team.r]);
-      }
-    } else {
+    if (kKind == kAcross) {
+      __syncthreads();
+      red[threadIdx.x] = best;
+      red_cls[threadIdx.x] = cls;
+      __syncthreads();
+      for (int i = 0; i < L; ++i) other(red[i * R + team.r], red_cls[i * R + team.r]);
+    } else if (kKind == kNeighbours) {
       for (int d = L / 2; d > 0; d >>= 1) {
         const A v = __shfl_xor(best, d);
         const int o = __shfl_xor(cls, d);
@@ -1156,7 +1223,8 @@ constexpr int kTopCandidates = 1024;  // of a row at most, or it goes the slow w
  * candidates than fit, of many equal scores for instance, are done digit by digit (TopAny).
  */
 template <typename T, typename Shape>
-__global__ void __launch_bounds__(Shape::block) k_top_row(LGBM_TopLogitsArgs a) {
+__global__ void __launch_bounds__(Shape::block, Shape::cached >= 12 ? 4 : 1)
+k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
   using A = Acc<T>;
   constexpr int kBlock = Shape::block, kWaves = kBlock / kWave;
   static_assert(std::is_same_v<A, float>, "keys of 32 bits");
@@ -1169,8 +1237,9 @@ __global__ void __launch_bounds__(Shape::block) k_top_row(LGBM_TopLogitsArgs a) 
   __shared__ A s_rest[kTopCandidates];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, k = a.k;
-  RowOf<T, Shape> z(
-      static_cast<const T*>(a.scores.data) + row * a.scores.stride[0], a.classes);
+  extern __shared__ Words row_lds[];
+  RowOf<T, Shape> z(static_cast<const T*>(a.scores.data) + row * a.scores.stride[0], a.classes,
+                    row_lds, lds_chunks);
   z.Load();
   for (int i = tid; i < kTopBins; i += kBlock) hist[i] = 0;
   if (tid == 0) {
@@ -1264,37 +1333,52 @@ __global__ void __launch_bounds__(Shape::block) k_top_row(LGBM_TopLogitsArgs a) 
   A off = bounded ? -edge * scale : A(0);  // unbounded, nothing but -inf is below the edge
   const bool rest = a.log_rest.data != nullptr;
   A sum = 0;
-  z.Each([&](int base, const auto& v) {
+  // a chunk with candidates is only noted (as the how-manieth of this thread) and looked at
+  // afterwards: most turns of a wave have one, in one lane of it
+  uint64_t noted = 0;
+  int turn = 0;
+  auto pick = [&](int base, const auto& v) {
     constexpr int kSize = kSizeOf<decltype(v)>;
-    A top = v[0];
 #pragma unroll
-    for (int i = 1; i < kSize; ++i) top = Max(top, v[i]);
-    const bool some = top >= edge;
-    if (some) {
-#pragma unroll
-      for (int i = 0; i < kSize; ++i) {
-        if (!(v[i] >= edge)) continue;
+    for (int i = 0; i < kSize; ++i) {
+      if (v[i] >= edge) {
         const int at = atomicAdd(&s_count, 1);
         if (at < kTopCandidates) {
           s_value[at] = v[i];
           s_cls[at] = base + i;
         }
+      } else if (rest && v[i] < edge) {  // not NaN
+        sum += Exp2(Fma(v[i], scale, off));
       }
     }
-    if (rest) {
-      A e[kSize], own = 0;
-      // at most one below the edge; the bounds turn NaN to zero, and cost nothing
+  };
+  z.Each([&](int base, const auto& v) {
+    constexpr int kSize = kSizeOf<decltype(v)>;
+    if constexpr (kSize == 1) {
+      pick(base, v);
+    } else {
+      A top = v[0];
 #pragma unroll
-      for (int i = 0; i < kSize; ++i) e[i] = fminf(fmaxf(Exp2(Fma(v[i], scale, off)), 0.0f), 1.0f);
-      if (some) {
+      for (int i = 1; i < kSize; ++i) top = Max(top, v[i]);
+      const bool some = top >= edge;
+      if (turn < 64) noted |= static_cast<uint64_t>(some) << turn;
+      else if (some) pick(base, v);
+      ++turn;
+      if (rest) {
+        // at most one, and NaN as zero: the bounds are the exponential's own modifier
+        A own = 0;
 #pragma unroll
-        for (int i = 0; i < kSize; ++i) e[i] = v[i] < edge ? e[i] : A(0);
+        for (int i = 0; i < kSize; ++i)
+          own += fminf(fmaxf(Exp2(Fma(v[i], scale, off)), 0.0f), 1.0f);
+        sum += some ? A(0) : own;
       }
-#pragma unroll
-      for (int i = 0; i < kSize; ++i) own += e[i];
-      sum += own;
     }
   });
+  while (noted != 0) {
+    const int chunk = (__ffsll(static_cast<unsigned long long>(noted)) - 1) * kBlock + tid;
+    noted &= noted - 1;
+    RowOf<T, Shape>::Give(z.Read(chunk), chunk, pick);
+  }
   __syncthreads();
   const int n = s_count;
   if (n > kTopCandidates) {
@@ -1815,11 +1899,11 @@ int LanesFor(int classes, int each) {
   return lanes;
 }
 
-template <typename T, typename S, int E, bool kAcross>
+template <typename T, typename S, int E, TeamKind kKind>
 void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
   const int lanes = LanesFor(a.classes, E), rows = 256 / lanes;
   const size_t lds = sizeof(Word<S>) * rows * a.classes;  // at most 2048 * E bytes
-  auto kernel = k_distill_tile<T, S, E, kAcross>;
+  auto kernel = k_distill_tile<T, S, E, kKind>;
   AllowLds(kernel, lds);
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256),
                      lds, s, a, lanes);
@@ -1827,10 +1911,12 @@ void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
 
 template <typename T, typename S>
 void DistillTile(const LGBM_DistillArgs& a, bool across, hipStream_t s) {
-  if (!across) LaunchDistillTile<T, S, 4, false>(a, s);
-  else if (a.classes <= 8) LaunchDistillTile<T, S, 8, true>(a, s);
-  else if (a.classes <= 256) LaunchDistillTile<T, S, 16, true>(a, s);
-  else LaunchDistillTile<T, S, 32, true>(a, s);
+  if (!across) LaunchDistillTile<T, S, 4, kNeighbours>(a, s);
+  else if (a.classes <= 4) LaunchDistillTile<T, S, 4, kAlone>(a, s);
+  else if (a.classes <= 8) LaunchDistillTile<T, S, 8, kAlone>(a, s);
+  else if (a.classes <= 16) LaunchDistillTile<T, S, 16, kAlone>(a, s);
+  else if (a.classes <= 256) LaunchDistillTile<T, S, 16, kAcross>(a, s);
+  else LaunchDistillTile<T, S, 32, kAcross>(a, s);
 }
 
 /*! whether the rows of a class stand closer together than the classes of a row */
@@ -1839,18 +1925,31 @@ bool ClassMajor(const LGBM_Array& scores) {
   return row_step != 0 && row_step < std::abs(scores.stride[1]);
 }
 
-template <typename T, int E, bool kAcross>
+template <typename T, int E, TeamKind kKind>
 void LaunchTopTile(const LGBM_TopLogitsArgs& a, hipStream_t s) {
   const int lanes = LanesFor(a.classes, E), rows = 256 / lanes;
-  hipLaunchKernelGGL((k_top_tile<T, E, kAcross>),
+  hipLaunchKernelGGL((k_top_tile<T, E, kKind>),
                      dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256), 0, s, a,
                      lanes);
 }
 
+/*! chunks a thread that stand in LDS, where `other` bytes of its 160 KiB have another use */
+template <typename Shape> int LdsChunksOf(int chunks, size_t other) {
+  if (!Shape::more) return 0;
+  const int wanted = (chunks - Shape::cached * Shape::block + Shape::block - 1) / Shape::block;
+  const int room = static_cast<int>((160 * 1024 - std::min<size_t>(other, 160 * 1024)) /
+                                    (sizeof(Words) * Shape::block));
+  return std::max(0, std::min({wanted, room, kLdsChunks}));
+}
+
 template <typename T, typename Shape>
 void LaunchTopRow(const LGBM_TopLogitsArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_top_row<T, Shape>), dim3(static_cast<uint32_t>(a.rows)),
-                     dim3(Shape::block), 0, s, a);
+  const int held = LdsChunksOf<Shape>(a.classes / Chunk<T>::kSize, 24576);
+  const size_t lds = sizeof(Words) * held * Shape::block;
+  auto kernel = k_top_row<T, Shape>;
+  AllowLds(kernel, lds);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(Shape::block), lds, s, a,
+                     held);
 }
 
 /*!
@@ -1876,10 +1975,12 @@ void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
   ByType(a.scores.type, [&](auto t) {
     using T = decltype(t);
     if (a.classes <= (across ? 512 : 256)) {
-      if (!across) LaunchTopTile<T, 4, false>(a, s);
-      else if (a.classes <= 8) LaunchTopTile<T, 8, true>(a, s);
-      else if (a.classes <= 256) LaunchTopTile<T, 16, true>(a, s);
-      else LaunchTopTile<T, 32, true>(a, s);
+      if (!across) LaunchTopTile<T, 4, kNeighbours>(a, s);
+      else if (a.classes <= 4) LaunchTopTile<T, 4, kAlone>(a, s);
+      else if (a.classes <= 8) LaunchTopTile<T, 8, kAlone>(a, s);
+      else if (a.classes <= 16) LaunchTopTile<T, 16, kAlone>(a, s);
+      else if (a.classes <= 256) LaunchTopTile<T, 16, kAcross>(a, s);
+      else LaunchTopTile<T, 32, kAcross>(a, s);
       return;
     }
     if constexpr (!std::is_same_v<T, double>) {
@@ -1898,10 +1999,13 @@ void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
 
 template <typename T, typename Shape>
 void LaunchDistillRow(const LGBM_DistillArgs& a, hipStream_t s) {
-  const size_t lds = sizeof(uint32_t) * ((a.classes + 31) / 32);
+  const size_t marks = sizeof(uint32_t) * ((a.classes + 31) / 32);
+  const int held = LdsChunksOf<Shape>(a.classes / Chunk<T>::kSize, marks + 4096);
+  const size_t lds = marks + sizeof(Words) * held * Shape::block;
   auto launch = [&](auto kernel) {
     AllowLds(kernel, lds);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(Shape::block), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(Shape::block), lds, s, a,
+                       held);
   };
   if (a.hessian.data) launch(k_distill_row<T, Shape, true>);
   else launch(k_distill_row<T, Shape, false>);
