@@ -642,7 +642,7 @@ template <typename T, typename Shape> struct RowOf {
     A v[kSize];
 #pragma unroll
     for (int i = 0; i < kSize; ++i) v[i] = static_cast<A>(got.v[i]);
-    f(chunk * kSize, v);
+    f(chunk * kSize, v, words);
   }
   /*! f(first class, values) of what this thread holds, kSize or one at a time */
   template <typename F> __device__ __forceinline__ void EachHeld(const F& f) {
@@ -787,7 +787,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     }
   };
   A high = NegInf<A>();
-  z.EachHeld([&](int, const auto& v) {
+  z.EachHeld([&](int, const auto& v, auto...) {
 #pragma unroll
     for (int i = 0; i < kSizeOf<decltype(v)>; ++i) high = Max(high, v[i]);
   });
@@ -795,7 +795,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   A more_high = NegInf<A>(), more_left = 0, more_total1 = 0;
   if constexpr (Shape::more) {
     __syncthreads();  // the marks
-    z.EachMore([&](int base, const auto& v) {
+    z.EachMore([&](int base, const auto& v, auto...) {
       A top = v[0];
 #pragma unroll
       for (int i = 1; i < kSizeOf<decltype(v)>; ++i) top = Max(top, v[i]);
@@ -834,7 +834,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
 
   const A off = -high * scale, off1 = -high * scale1;
   A left = 0, total1 = 0;
-  z.EachHeld([&](int base, const auto& v) { add_chunk(base, v, off, off1, left, total1); });
+  z.EachHeld([&](int base, const auto& v, auto...) { add_chunk(base, v, off, off1, left, total1); });
   if constexpr (Shape::more) {
     if (own_high > NegInf<A>() || more_left != A(0)) {
       left += more_left * Exp2((own_high > NegInf<A>() ? own_high - high : A(0)) * scale);
@@ -862,7 +862,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   A log_left = Log2(left), rest_off = off;
   if (rest && left < SmallRest<A>()) {
     A own = NegInf<A>();
-    z.Each([&](int base, const auto& v) {
+    z.Each([&](int base, const auto& v, auto...) {
     constexpr int kSize = kSizeOf<decltype(v)>;
       const uint32_t bits = bits_of(base, kSize);
 #pragma unroll
@@ -873,7 +873,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     if (own > NegInf<A>()) {
       rest_off = -own * scale;
       left = 0;
-      z.Each([&](int base, const auto& v) {
+      z.Each([&](int base, const auto& v, auto...) {
     constexpr int kSize = kSizeOf<decltype(v)>;
         const uint32_t bits = bits_of(base, kSize);
 #pragma unroll
@@ -911,7 +911,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   if (grad) {
     if (moved) {
       const A coef_rest = soft > A(0) ? -each * spread : A(0);
-      z.Each([&](int base, const auto& v) {
+      z.Each([&](int base, const auto& v, auto...) {
 #pragma unroll
         for (int i = 0; i < kSizeOf<decltype(v)>; ++i) {
           A g = coef * Exp2(Fma(v[i], scale, off));
@@ -920,7 +920,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
         }
       });
     } else {
-      z.Each([&](int base, const auto& v) {
+      z.Each([&](int base, const auto& v, auto...) {
         constexpr int kSize = kSizeOf<decltype(v)>;
         O g[kSize];
         if (two) {
@@ -938,7 +938,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     }
   }
   if (kHessian) {
-    z.Each([&](int base, const auto& v) {
+    z.Each([&](int base, const auto& v, auto...) {
 #pragma unroll
       for (int i = 0; i < kSizeOf<decltype(v)>; ++i) {
         const A q = Exp2(Fma(v[i], scale, off)) * inv;
@@ -1213,6 +1213,16 @@ __global__ void __launch_bounds__(256) k_top_tile(LGBM_TopLogitsArgs a, int lane
 // ------------------------------------------------------------------ top logits, many classes
 constexpr int kTopBins = 512;         // of the threads' maxima
 constexpr int kTopCandidates = 1024;  // of a row at most, or it goes the slow way
+constexpr int kTopChunks = 512;       // that hold them
+
+/*! a candidate as one number: the larger comes first, and of equal values the lower class */
+__device__ __forceinline__ uint64_t Candidate(float v, int cls) {
+  return static_cast<uint64_t>(KeyOf(v)) << 32 | ~static_cast<uint32_t>(cls);
+}
+/*! the value of a key that is not zero */
+__device__ __forceinline__ float ValueOf(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 
 /*!
  * One workgroup a row. Every thread takes the maxima of four parts of what it holds: the k-th
@@ -1232,8 +1242,9 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
   __shared__ A s_low[kWaves], s_high[kWaves], s_sum[kWaves];
   __shared__ int s_bin, s_count, s_valid;
   __shared__ uint32_t s_edge;
-  __shared__ A s_value[kTopCandidates];
-  __shared__ int s_cls[kTopCandidates];
+  __shared__ uint64_t s_list[kTopCandidates];
+  __shared__ Words s_aside[kTopChunks];
+  __shared__ int s_base[kTopChunks], s_chunks;
   __shared__ A s_rest[kTopCandidates];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, k = a.k;
@@ -1243,11 +1254,11 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
   z.Load();
   for (int i = tid; i < kTopBins; i += kBlock) hist[i] = 0;
   if (tid == 0) {
-    s_count = s_valid = s_bin = 0;
+    s_count = s_valid = s_bin = s_chunks = 0;
     s_edge = ~0u;
   }
   A part[4] = {NegInf<A>(), NegInf<A>(), NegInf<A>(), NegInf<A>()};
-  z.Each([&](int, const auto& v) {
+  z.Each([&](int, const auto& v, auto...) {
 #pragma unroll
     for (int i = 0; i < kSizeOf<decltype(v)>; ++i) part[i & 3] = Max(part[i & 3], v[i]);
   });
@@ -1327,57 +1338,62 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
     __syncthreads();
   }
   // the smallest of the maxima in the bins down to the k-th
-  A edge = bounded ? __uint_as_float(s_edge & 0x80000000u ? s_edge & 0x7fffffffu : ~s_edge)
-                   : -FLT_MAX;
+  const A edge = bounded ? ValueOf(s_edge) : -FLT_MAX;
   const A scale = static_cast<A>(kLog2e / a.temperature);
   A off = bounded ? -edge * scale : A(0);  // unbounded, nothing but -inf is below the edge
   const bool rest = a.log_rest.data != nullptr;
   A sum = 0;
-  // a chunk with candidates is only noted (as the how-manieth of this thread) and looked at
-  // afterwards: most turns of a wave have one, in one lane of it
-  uint64_t noted = 0;
-  int turn = 0;
-  auto pick = [&](int base, const auto& v) {
-    constexpr int kSize = kSizeOf<decltype(v)>;
-#pragma unroll
-    for (int i = 0; i < kSize; ++i) {
-      if (v[i] >= edge) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < kTopCandidates) {
-          s_value[at] = v[i];
-          s_cls[at] = base + i;
-        }
-      } else if (rest && v[i] < edge) {  // not NaN
-        sum += Exp2(Fma(v[i], scale, off));
-      }
-    }
+  // a chunk with candidates is only put aside and looked at afterwards, an element a thread:
+  // most turns of a wave meet one, in one of its lanes
+  auto pick = [&](int cls, A v) {
+    if (!(v >= edge)) return;
+    const int at = atomicAdd(&s_count, 1);
+    if (at < kTopCandidates) s_list[at] = Candidate(v, cls);
   };
-  z.Each([&](int base, const auto& v) {
+  z.Each([&](int base, const auto& v, auto... words) {
     constexpr int kSize = kSizeOf<decltype(v)>;
-    if constexpr (kSize == 1) {
-      pick(base, v);
+    if constexpr (sizeof...(words) == 0) {
+      pick(base, v[0]);
+      if (rest && v[0] < edge) sum += Exp2(Fma(v[0], scale, off));
     } else {
       A top = v[0];
 #pragma unroll
       for (int i = 1; i < kSize; ++i) top = Max(top, v[i]);
-      const bool some = top >= edge;
-      if (turn < 64) noted |= static_cast<uint64_t>(some) << turn;
-      else if (some) pick(base, v);
-      ++turn;
+      A e[kSize];
       if (rest) {
         // at most one, and NaN as zero: the bounds are the exponential's own modifier
-        A own = 0;
 #pragma unroll
         for (int i = 0; i < kSize; ++i)
-          own += fminf(fmaxf(Exp2(Fma(v[i], scale, off)), 0.0f), 1.0f);
-        sum += some ? A(0) : own;
+          e[i] = fminf(fmaxf(Exp2(Fma(v[i], scale, off)), 0.0f), 1.0f);
+      }
+      if (top >= edge) {
+        const int at = atomicAdd(&s_chunks, 1);
+        if (at < kTopChunks) {
+          s_aside[at] = (words, ...);
+          s_base[at] = base;
+        }
+#pragma unroll
+        for (int i = 0; i < kSize; ++i) e[i] = v[i] < edge ? e[i] : A(0);
+      }
+      if (rest) {
+        A own = 0;
+#pragma unroll
+        for (int i = 0; i < kSize; ++i) own += e[i];
+        sum += own;
       }
     }
   });
-  while (noted != 0) {
-    const int chunk = (__ffsll(static_cast<unsigned long long>(noted)) - 1) * kBlock + tid;
-    noted &= noted - 1;
-    RowOf<T, Shape>::Give(z.Read(chunk), chunk, pick);
+  __syncthreads();
+  if (s_chunks > kTopChunks) {
+    TopAny<T, kBlock>(a, row);
+    return;
+  }
+  {
+    constexpr int kSize = Chunk<T>::kSize;
+    const T* aside = reinterpret_cast<const T*>(s_aside);
+    const int many = s_chunks * kSize;
+    for (int i = tid; i < many; i += kBlock)
+      pick(s_base[i / kSize] + i % kSize, static_cast<A>(aside[i]));
   }
   __syncthreads();
   const int n = s_count;
@@ -1389,20 +1405,19 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
   T* out_logit = static_cast<T*>(a.top_logit.data) + row * a.top_logit.stride[0];
   // eight lanes compare one candidate with the others
   for (int i = tid / 8; i < n; i += kBlock / 8) {
-    const A v = s_value[i];
-    const int cls = s_cls[i];
+    const uint64_t own = s_list[i];
     int rank = 0;
-    for (int o = tid % 8; o < n; o += 8) {
-      const A u = s_value[o];
-      rank += u > v || (u == v && s_cls[o] < cls);
-    }
+#pragma unroll 4
+    for (int o = tid % 8; o < n; o += 8) rank += s_list[o] > own;
     rank += __shfl_xor(rank, 1);
     rank += __shfl_xor(rank, 2);
     rank += __shfl_xor(rank, 4);
     if (tid % 8 != 0) continue;
+    const int cls = static_cast<int>(~static_cast<uint32_t>(own));
+    const A v = ValueOf(static_cast<uint32_t>(own >> 32));
     if (rank < k) {
       out_class[rank * a.top_class.stride[1]] = cls;
-      out_logit[rank * a.top_logit.stride[1]] = static_cast<T>(v);
+      out_logit[rank * a.top_logit.stride[1]] = z.x[cls];  // as it is, signed zeros too
     } else {
       s_rest[rank - k] = v;  // in order, so that their sum is the same every time
     }
@@ -1417,7 +1432,7 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
   sum = BlockSum<kBlock>(sum, s_sum);
   if (n <= k && sum < SmallRest<A>()) {  // far below the edge: against its own maximum
     A own = NegInf<A>();
-    z.Each([&](int, const auto& v) {
+    z.Each([&](int, const auto& v, auto...) {
 #pragma unroll
       for (int i = 0; i < kSizeOf<decltype(v)>; ++i) own = Max(own, v[i] < edge ? v[i] : own);
     });
@@ -1425,7 +1440,7 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
     sum = 0;
     if (own > NegInf<A>()) {
       off = -own * scale;
-      z.Each([&](int, const auto& v) {
+      z.Each([&](int, const auto& v, auto...) {
 #pragma unroll
         for (int i = 0; i < kSizeOf<decltype(v)>; ++i)
           sum += v[i] < edge ? Exp2(Fma(v[i], scale, off)) : A(0);
@@ -1944,7 +1959,7 @@ template <typename Shape> int LdsChunksOf(int chunks, size_t other) {
 
 template <typename T, typename Shape>
 void LaunchTopRow(const LGBM_TopLogitsArgs& a, hipStream_t s) {
-  const int held = LdsChunksOf<Shape>(a.classes / Chunk<T>::kSize, 24576);
+  const int held = LdsChunksOf<Shape>(a.classes / Chunk<T>::kSize, 32768);
   const size_t lds = sizeof(Words) * held * Shape::block;
   auto kernel = k_top_row<T, Shape>;
   AllowLds(kernel, lds);
