@@ -1417,7 +1417,8 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
     const A v = ValueOf(static_cast<uint32_t>(own >> 32));
     if (rank < k) {
       out_class[rank * a.top_class.stride[1]] = cls;
-      out_logit[rank * a.top_logit.stride[1]] = z.x[cls];  // as it is, signed zeros too
+      // as it is: of the zeros the key does not know the sign
+      out_logit[rank * a.top_logit.stride[1]] = v == A(0) ? z.x[cls] : static_cast<T>(v);
     } else {
       s_rest[rank - k] = v;  // in order, so that their sum is the same every time
     }

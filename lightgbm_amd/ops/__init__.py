@@ -69,13 +69,16 @@ for _f in (_LIB.LGBM_TopLogits, _LIB.LGBM_Distill, _LIB.LGBM_VerifyDrafts):
     _f.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
 _LIB.LGBM_VerifyDraftsWorkspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]
 
+_WORKSPACE = {}  # bytes, by a call's sizes
+
 # torch is looked up when the first array that may be its is seen: the package works without
 _torch = None
 _Tensor = ()
+_raw_stream = None
 
 
 def _is_tensor(x):
-    global _torch, _Tensor
+    global _torch, _Tensor, _raw_stream
     if _torch is None:
         _torch = sys.modules.get("torch")
         if _torch is None:
@@ -85,12 +88,10 @@ def _is_tensor(x):
                            (_I64, "int64"), (_F16, "float16"), (_BF16, "bfloat16")):
             _TORCH_TYPES[getattr(_torch, name)] = code
             _TORCH_OF[code] = getattr(_torch, name)
+        # the current stream of a device as a pointer, where torch has it without an object
+        _raw_stream = getattr(_torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: _torch.cuda.current_stream(index).cuda_stream)
     return isinstance(x, _Tensor)
-
-
-def _stream_of(device):
-    """The current stream of a device, as a pointer."""
-    return _torch.cuda.current_stream(device).cuda_stream
 
 
 class _Place:
@@ -105,33 +106,45 @@ class _Place:
         if self.tensor:
             self.on = x.device
             if x.is_cuda:
-                self.device = self.on.index
+                self.device = x.get_device()
             elif self.on.type != "cpu":
                 raise LightGBMError(f"tensors on {self.on} are not supported")
 
     def stream(self):
-        return _stream_of(self.on) if self.device >= 0 else None
+        return _raw_stream(self.device) if self.device >= 0 else None
 
-    def empty(self, shape, code, class_major=False):
+    def empty(self, shape, code):
+        """A new array in row order, and the six fields of its LGBM_Array."""
+        step = shape[1] if len(shape) == 2 else 1
         if self.tensor:
-            if class_major:
-                return _torch.empty(shape[::-1], dtype=_TORCH_OF[code], device=self.on).t()
-            return _torch.empty(shape, dtype=_TORCH_OF[code], device=self.on)
-        return np.empty(shape, dtype=_NUMPY_OF[code], order="F" if class_major else "C")
+            made = _torch.empty(shape, dtype=_TORCH_OF[code], device=self.on)
+            at = made.data_ptr()
+        else:
+            made = np.empty(shape, dtype=_NUMPY_OF[code])
+            at = made.__array_interface__["data"][0]
+        return made, (at, step, 1, 0, code, 0)
+
+    def scores(self, rows, classes, code, class_major):
+        """The same, in the order of scores [rows, classes]."""
+        if not class_major:
+            return self.empty((rows, classes), code)
+        made, (at, *_) = self.empty((classes, rows), code)
+        return made.T, (at, 1, rows, 0, code, 0)
 
     def array(self, x, name, shape):
         """The six fields of an LGBM_Array of x, which has to be of this place and shape."""
         if x is None:
             return _NONE
         if _is_tensor(x):
-            if (x.device != self.on) if self.tensor else x.is_cuda:
+            # -1: the host
+            if x.get_device() != self.device or x.is_cuda != (self.device >= 0):
                 raise LightGBMError(f"{name} is on {x.device}, the first array on "
                                     f"{self.on or 'the host'}")
         elif self.device >= 0:
             raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
         elif not isinstance(x, np.ndarray):
             x = np.asarray(x)
-        if tuple(x.shape) != shape:
+        if x.shape != shape:
             raise LightGBMError(f"{name} must have the shape {list(shape)}, got {list(x.shape)}")
         return _fields(x, name)
 
@@ -187,12 +200,12 @@ def top_logits(scores, k, temperature=1.0, rest=True):
     x = _fields(scores, "scores")
     code = x[4]
     k = int(k)
-    out_class = where.empty((rows, max(k, 0)), _I32)
-    out_logit = where.empty((rows, max(k, 0)), code)
-    log_rest = where.empty((rows,), _F64 if code == _F64 else _F32) if rest else None
+    out_class, to_class = where.empty((rows, max(k, 0)), _I32)
+    out_logit, to_logit = where.empty((rows, max(k, 0)), code)
+    log_rest, to_rest = (where.empty((rows,), _F64 if code == _F64 else _F32) if rest
+                         else (None, _NONE))
     _safe_call(_LIB.LGBM_TopLogits(
-        _TOP.pack(rows, classes, k, temperature, *x, *_fields(out_class, ""),
-                  *_fields(out_logit, ""), *(_fields(log_rest, "") if rest else _NONE)),
+        _TOP.pack(rows, classes, k, temperature, *x, *to_class, *to_logit, *to_rest),
         where.device, where.stream()))
     return TopLogits(out_class, out_logit, log_rest)
 
@@ -215,14 +228,12 @@ def _distill(scores, teacher, labels, weight, temperature, alpha, loss, gradient
               *where.array(teacher[2] if len(teacher) == 3 else None, "teacher log_rest", row),
               *where.array(None if alpha == 1.0 else labels, "labels", row),
               *where.array(weight, "weight", row))
-    made_loss = where.empty(row, _F64 if code == _F64 else _F32) if loss else None
-    made_grad = where.empty((rows, classes), out, class_major) if gradient else None
-    made_hess = where.empty((rows, classes), out, class_major) if hessian else None
-    _safe_call(_LIB.LGBM_Distill(
-        _DISTILL.pack(*fields, *(_fields(made_loss, "") if loss else _NONE),
-                      *(_fields(made_grad, "") if gradient else _NONE),
-                      *(_fields(made_hess, "") if hessian else _NONE)),
-        where.device, where.stream()))
+    absent = (None, _NONE)
+    made_loss, to_loss = where.empty(row, _F64 if code == _F64 else _F32) if loss else absent
+    made_grad, to_grad = where.scores(rows, classes, out, class_major) if gradient else absent
+    made_hess, to_hess = where.scores(rows, classes, out, class_major) if hessian else absent
+    _safe_call(_LIB.LGBM_Distill(_DISTILL.pack(*fields, *to_loss, *to_grad, *to_hess),
+                                 where.device, where.stream()))
     return made_loss, made_grad, made_hess
 
 
@@ -285,16 +296,21 @@ def verify_drafts(target_prob, drafts, draft_prob, accept_uniform, sample_unifor
               *where.array(accept_uniform, "accept_uniform", (rows, t)),
               *where.array(sample_uniform, "sample_uniform", (rows,)),
               *where.array(lengths, "lengths", (rows,)))
-    out_class = where.empty((rows, places), _I32)
-    out_accepted = where.empty((rows,), _I32)
-    fields += (*_fields(out_class, ""), *_fields(out_accepted, ""))
-    scratch = 0
-    size = 0
+    out_class, to_class = where.empty((rows, places), _I32)
+    out_accepted, to_accepted = where.empty((rows,), _I32)
+    fields += (*to_class, *to_accepted)
+    scratch = size = 0
     if where.device >= 0:
-        need = ctypes.c_int64(0)
-        _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_VERIFY.pack(*fields, 0, 0),
-                                                   ctypes.byref(need)))
-        size = need.value
+        # what the call needs goes by its sizes, types and strides alone
+        plan = (rows, classes, t, fields[3 + 4], fields[3 + 3], draft_prob is None or fields[9 + 3])
+        size = _WORKSPACE.get(plan)
+        if size is None:
+            need = ctypes.c_int64(0)
+            _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_VERIFY.pack(*fields, 0, 0),
+                                                       ctypes.byref(need)))
+            if len(_WORKSPACE) >= 1024:
+                _WORKSPACE.clear()
+            size = _WORKSPACE[plan] = need.value
         if size:
             # freed to the caching allocator, which gives it out again in the stream's order
             space = _torch.empty((size,), dtype=_torch.uint8, device=where.on)
