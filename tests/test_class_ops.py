@@ -12,6 +12,9 @@ compared. The 32-bit gradients of float64 scores are allowed the 32-bit terms: t
 their exponents in 64 bits and takes the exponentials in 32.
 """
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -666,6 +669,212 @@ def test_refuses_mixed_places():
         ops.distill_loss(_put("gpu", z), (ids, t))
     with pytest.raises(LightGBMError):
         ops.distill_loss(_put("torch", z), (_put("gpu", ids), _put("torch", t)))
+
+
+# ------------------------------------------------------------------ on the device
+def _set(rows, classes, dtype, seed, order="C", drafts=2):
+    """Inputs of one call of each operator, on the GPU."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    z = 3 * torch.randn((rows, classes), generator=g, device="cuda", dtype=torch.float64)
+    z = z.to(TORCH[dtype])
+    if order == "F":
+        z = z.t().contiguous().t()
+    p = torch.softmax(torch.randn((rows, drafts + 1, classes), generator=g, device="cuda"), 2)
+    q = torch.softmax(torch.randn((rows, drafts, classes), generator=g, device="cuda"), 2)
+    return {"z": z, "labels": torch.randint(0, classes, (rows,), generator=g, device="cuda"),
+            "p": p, "q": q,
+            "drafts": torch.randint(0, classes, (rows, drafts), generator=g, device="cuda"),
+            "u": torch.rand((rows, drafts), generator=g, device="cuda"),
+            "v": torch.rand((rows,), generator=g, device="cuda")}
+
+
+def _run_set(s, k):
+    """The operators one after the other, as a training and serving program calls them."""
+    top = ops.top_logits(s["z"], k, temperature=2.0)
+    got = ops.distill_gradients(s["z"] * 0.5, top, labels=s["labels"], temperature=2.0, alpha=0.5,
+                                hessian=True, loss=True)
+    loss = ops.distill_loss(s["z"] * 0.5, top, temperature=2.0)
+    drawn = ops.verify_drafts(s["p"], s["drafts"], s["q"], s["u"], s["v"])
+    return [*top, *got, loss, *drawn]
+
+
+def _same(a, b):
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+DEVICE_SETS = [(5, 9, "f64", "F", 3), (70, 200, "f32", "F", 40), (6, 40, "bf16", "C", 7),
+               (4, 3001, "f16", "C", 33), (2, 70001, "f32", "C", 20), (3, 3000, "f64", "C", 9),
+               (600, 20011, "bf16", "C", 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,dtype,order,k", DEVICE_SETS)
+def test_repeats_bit_for_bit(rows, classes, dtype, order, k):
+    s = _set(rows, classes, dtype, 0, order)
+    want = _run_set(s, k)
+    for _ in range(5):
+        _same(_run_set(s, k), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,dtype,order,k", DEVICE_SETS)
+def test_graphs(rows, classes, dtype, order, k):
+    """Two graphs of the same calls, replayed in turn on new inputs with the program's own eager
+    work between: every replay is the eager result."""
+    graphs = []
+    for seed in (1, 2):
+        s = _set(rows, classes, dtype, seed, order)
+        _run_set(s, k)  # the kernels are loaded before the capture
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _run_set(s, k)
+        graphs.append((g, s, out))
+    for turn in range(4):
+        for g, s, out in graphs:
+            new = _set(rows, classes, dtype, 10 + turn, order)
+            for name, x in new.items():
+                s[name].copy_(x)
+            want = _run_set(new, k)
+            g.replay()
+            torch.cuda.synchronize()
+            _same(out, want)
+    for g, s, out in graphs:  # both on their way at once
+        g.replay()
+    torch.cuda.synchronize()
+    _same(graphs[0][2], graphs[1][2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,dtype,order,k", DEVICE_SETS)
+def test_streams(rows, classes, dtype, order, k):
+    """Calls on two streams at once, inputs made and results used on the call's own stream."""
+    want = [_run_set(_set(rows, classes, dtype, seed, order), k) for seed in (1, 2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for turn in range(3):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                s = _set(rows, classes, dtype, i + 1, order)
+                got[i] = [x.clone() for x in _run_set(s, k)]
+    torch.cuda.synchronize()
+    for i in range(2):
+        _same(got[i], want[i])
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """The last rows of an array of more than 2^31 elements are what they are alone."""
+    rows, classes = 66000, 32768
+    z = torch.empty((rows, classes), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(0)
+    z.normal_(generator=g)
+    last = z[-3:].clone()
+    top = ops.top_logits(z, 9)
+    alone = ops.top_logits(last, 9)
+    _same([x[-3:] for x in top[:2]], alone[:2])
+    # few rows are shared among more threads than many, so sums have another order
+    rel = _rel(classes, "f32")
+    rest = _get(alone.log_rest)
+    assert np.all(np.abs(_get(top.log_rest[-3:]) - rest) <= 2 * rel * (1 + np.abs(rest)))
+    got = ops.distill_gradients(z, top, loss=True)
+    loss, grad, _, size_l, size_g = _plain_distill(
+        _get(last), _get(alone.classes), _get(alone.logits), _get(top.log_rest[-3:]), None, None,
+        1.0, 1.0)
+    assert np.all(np.abs(_get(got.loss[-3:]) - loss) <= 3 * rel * size_l +
+                  HALF_STEP["f32"] * np.abs(loss))
+    assert np.all(np.abs(_get(got.gradient[-3:]) - grad) <= 3 * rel * size_g +
+                  (1 + rel) * HALF_STEP["bf16"] * np.abs(grad) + TINY["bf16"])
+    del got, top
+    turned = torch.empty((300, 7200000), dtype=torch.float32, device="cuda")
+    turned.normal_(generator=g)
+    end = turned.t()[-2:].contiguous().t().contiguous().t()  # class-major too
+    _same([x[-2:] for x in ops.top_logits(turned.t(), 5)], ops.top_logits(end, 5))
+    p = torch.softmax(z[-4:].float(), 1).view(2, 2, classes)
+    wide = torch.zeros((33000, 2, classes), dtype=torch.float32, device="cuda")
+    wide[-2:] = p
+    wide[:-2, :, 3] = 1.0
+    drafts = torch.zeros((33000, 1), dtype=torch.int64, device="cuda")
+    u = torch.full((33000, 1), 0.5, device="cuda")
+    v = torch.rand(33000, generator=g, device="cuda")
+    got = ops.verify_drafts(wide, drafts, None, u, v)
+    want = ops.verify_drafts(p, drafts[-2:], None, u[-2:], v[-2:])
+    _same([x[-2:] for x in got], want)
+    assert bool((got.classes[:-2, 0] == 3).all())
+
+
+def _padded(shape, dtype, value):
+    """A tensor inside a larger one of a single value, and the larger one."""
+    big = torch.full([n + 6 for n in shape], value, dtype=dtype, device="cuda")
+    return big[tuple(slice(3, 3 + n) for n in shape)], big
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,dtype,order,k", DEVICE_SETS)
+def test_nothing_else_is_written(rows, classes, dtype, order, k):
+    """Through the C ABI, results into views of larger tensors: what is around them stays."""
+    s = _set(rows, classes, dtype, 3, order)
+    want = _run_set(s, k)
+    wide = TORCH["f64" if dtype == "f64" else "f32"]
+    out = TORCH["f32" if dtype == "f64" else dtype]
+    made = [_padded((rows, k), torch.int32, -9), _padded((rows, k), TORCH[dtype], 7.0),
+            _padded((rows,), wide, 7.0), _padded((rows, classes), out, 7.0),
+            _padded((rows, classes), out, 7.0), _padded((rows,), wide, 7.0),
+            _padded((rows, 3), torch.int32, -9), _padded((rows,), torch.int32, -9)]
+    f = lambda x: ops._fields(x, "")  # noqa: E731
+    view = [m[0] for m in made]
+    stream = torch.cuda.current_stream().cuda_stream
+    lib = ops._LIB
+    ops._safe_call(lib.LGBM_TopLogits(ops._TOP.pack(
+        rows, classes, k, 2.0, *f(s["z"]), *f(view[0]), *f(view[1]), *f(view[2])), 0, stream))
+    student = s["z"] * 0.5
+    ops._safe_call(lib.LGBM_Distill(ops._DISTILL.pack(
+        rows, classes, k, 2.0, 0.5, *f(student), *f(view[0]), *f(view[1]), *f(view[2]),
+        *f(s["labels"]), *ops._NONE, *f(view[5]), *f(view[3]), *f(view[4])), 0, stream))
+    verify = (rows, classes, 2, *f(s["p"]), *f(s["q"]), *f(s["drafts"]), *f(s["u"]), *f(s["v"]),
+              *ops._NONE, *f(view[6]), *f(view[7]))
+    need = ops.ctypes.c_int64(0)
+    ops._safe_call(lib.LGBM_VerifyDraftsWorkspace(ops._VERIFY.pack(*verify, 0, 0),
+                                                  ops.ctypes.byref(need)))
+    space = torch.full((need.value + 64,), 77, dtype=torch.uint8, device="cuda")
+    if need.value:
+        with pytest.raises(LightGBMError):
+            ops._safe_call(lib.LGBM_VerifyDrafts(ops._VERIFY.pack(
+                *verify, space.data_ptr(), need.value - 1), 0, stream))
+        with pytest.raises(LightGBMError):
+            ops._safe_call(lib.LGBM_VerifyDrafts(ops._VERIFY.pack(*verify, 0, need.value), 0,
+                                                 stream))
+    ops._safe_call(lib.LGBM_VerifyDrafts(ops._VERIFY.pack(*verify, space.data_ptr(), need.value),
+                                         0, stream))
+    torch.cuda.synchronize()
+    assert bool((space[need.value:] == 77).all())
+    order_of = [0, 1, 2, 3, 4, 5, 7, 8]
+    for (got, big), w in zip(made, [want[i] for i in order_of]):
+        # the C ABI's gradients are in row order here, whatever the scores' order is
+        assert torch.equal(got, w)
+        keep = big.flatten()[0].item()
+        big[tuple(slice(3, 3 + n) for n in got.shape)] = keep
+        assert bool((big == keep).all())
+
+
+@pytest.mark.gpu
+def test_torch_first():
+    """This process has loaded lightgbm_amd first; the other order of import serves too."""
+    code = ("import torch, numpy as np; x = torch.randn(4, 300, device='cuda')\n"
+            "import lightgbm_amd as lgb\n"
+            "t = lgb.ops.top_logits(x, 3); assert torch.equal(t.logits, x.topk(3)[0])\n"
+            "X = np.random.RandomState(0).randn(500, 4)\n"
+            "b = lgb.train({'objective': 'regression', 'device_type': 'gpu', 'verbosity': -1},"
+            " lgb.Dataset(X, label=X[:, 0]), 2)\n"
+            "assert b.num_trees() == 2; print('both')")
+    root = Path(__file__).resolve().parent.parent
+    got = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=100)
+    assert got.returncode == 0 and "both" in got.stdout, got.stderr[-2000:]
 
 
 def test_lgb_exports_ops():

@@ -222,3 +222,16 @@ def test_teacher_student_drafts(place):
     np.testing.assert_array_equal(got.classes, want.classes)
     assert np.all((got.accepted >= 0) & (got.accepted <= 2))
     assert np.all(np.take_along_axis(got.classes, got.accepted[:, None], 1) >= 0)
+
+
+@pytest.mark.gpu
+def test_shards_have_their_rows_of_the_teacher():
+    """num_gpu=2 on one card: the same gradients, summed in another order."""
+    X, raw, y = _data(2000)
+    top = ops.top_logits(raw, 3, temperature=2.0)
+    preds = []
+    for num_gpu in (1, 2):
+        bst = lgb.train(_params("gpu", distill_temperature=2.0, num_gpu=num_gpu),
+                        lgb.Dataset(X, label=y, teacher=top), 5)
+        preds.append(bst.predict(X, raw_score=True))
+    assert np.quantile(np.abs(preds[0] - preds[1]), 0.99) < 1e-4
