@@ -1210,11 +1210,7 @@ __global__ void __launch_bounds__(256) k_top_tile(LGBM_TopLogitsArgs a, int lane
                           : high);
 }
 
-// ------------------------------------------------------------------ top logits, many classes
-constexpr int kTopBins = 512;         // of the threads' maxima
-constexpr int kTopCandidates = 1024;  // of a row at most, or it goes the slow way
-constexpr int kTopChunks = 512;       // that hold them
-
+// ------------------------------------------------------------------ top logits, some classes
 /*! a candidate as one number: the larger comes first, and of equal values the lower class */
 __device__ __forceinline__ uint64_t Candidate(float v, int cls) {
   return static_cast<uint64_t>(KeyOf(v)) << 32 | ~static_cast<uint32_t>(cls);
@@ -1223,6 +1219,190 @@ __device__ __forceinline__ uint64_t Candidate(float v, int cls) {
 __device__ __forceinline__ float ValueOf(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+__device__ __forceinline__ double ValueOf(uint64_t key) {
+  return __longlong_as_double(static_cast<long long>(key >> 63 ? key & ~(1ull << 63) : ~key));
+}
+/*! the same number in every lane, as a scalar */
+__device__ __forceinline__ uint32_t Scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t Scalar(uint64_t v) {
+  return static_cast<uint64_t>(Scalar(static_cast<uint32_t>(v >> 32))) << 32 |
+         Scalar(static_cast<uint32_t>(v));
+}
+/*! LDS that this wave's lanes wrote is there for its other lanes */
+__device__ __forceinline__ void WaveSync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kTurnedRows = 16;
+
+/*!
+ * One wave a row of up to E * 64 classes, which its lanes hold: the k-th largest by bisection
+ * over the keys between the row's smallest and largest. A step compares what each lane holds
+ * with the middle and counts the lanes' answers, without a word between lanes; it ends as
+ * soon as the count is k. No wave waits for another. kTurned: the rows of a class stand next
+ * to each other, so a workgroup turns sixteen rows in LDS first.
+ */
+template <typename T, int E, bool kTurned>
+__global__ void __launch_bounds__(256) k_top_wave(LGBM_TopLogitsArgs a) {
+  using A = Acc<T>;
+  using K = Key<T>;
+  constexpr bool kWide = std::is_same_v<T, double>;
+  constexpr int kRows = kTurned ? kTurnedRows : 4;
+  extern __shared__ unsigned long long turned_lds[];
+  __shared__ uint64_t s_list[4][kMaxTop];
+  __shared__ int s_cls[kWide ? 4 : 1][kMaxTop];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, c = a.classes;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), a.rows - first));
+  T* turned = reinterpret_cast<T*>(turned_lds);
+  const int step = c | 1;  // of the turned rows: odd, so that they begin in different banks
+  if constexpr (kTurned) {
+    const int r = threadIdx.x % kRows;
+    const T* x = static_cast<const T*>(a.scores.data) + (first + r) * a.scores.stride[0];
+    if (r < rows)
+#pragma unroll 4
+      for (int cls = threadIdx.x / kRows; cls < c; cls += 256 / kRows)
+        turned[r * step + cls] = x[cls * a.scores.stride[1]];
+    __syncthreads();
+  }
+  const unsigned long long below = (1ull << lane) - 1;
+  const A scale = static_cast<A>(kLog2e / a.temperature);
+  for (int i = wave; i < rows; i += 4) {
+    const int64_t row = first + i;
+    const T* x = static_cast<const T*>(a.scores.data) + row * a.scores.stride[0];
+    A z[E], high = NegInf<A>(), low = -NegInf<A>();
+    int valid = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int cls = e * kWave + lane;
+      z[e] = NegInf<A>();
+      if (e * kWave < c) {
+        if (cls < c)
+          z[e] = kTurned ? static_cast<A>(turned[i * step + cls])
+                         : static_cast<A>(x[cls * a.scores.stride[1]]);
+        const bool able = z[e] > NegInf<A>();
+        if (!able) z[e] = NegInf<A>();  // NaN
+        valid += able;  // (a ballot of x > -inf is compiled to one that counts NaN)
+        high = Max(high, z[e]);
+        if (able) low = -Max(-low, -z[e]);
+      }
+    }
+    valid = WaveSum(valid);
+    const int take = min(a.k, valid);
+    // the largest key that `take` scores reach
+    K from = 0, to = 0;
+    int reached = valid;
+    if (take > 0) {
+      from = Scalar(KeyOf(-WaveMax(-low)));
+      to = Scalar(KeyOf(WaveMax(high)));
+    }
+    while (from < to && reached != take) {
+      const K middle = from + (to - from + 1) / 2;
+      const A at = ValueOf(middle);
+      int count = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e * kWave < c) count += __popcll(__ballot(z[e] >= at));
+      if (count >= take) {
+        from = middle;
+        reached = count;
+      } else {
+        to = middle - 1;
+      }
+    }
+    const A edge = take > 0 ? ValueOf(from) : -NegInf<A>();
+    int spare = reached - take;  // of the scores equal to the edge, the highest classes
+    if (take == 0) spare = 0;
+    uint32_t chosen = 0;
+    if (spare == 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e * kWave < c && z[e] >= edge && take > 0) chosen |= 1u << e;
+    } else {
+      int above = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e * kWave < c) above += __popcll(__ballot(z[e] > edge));
+      int need = take - above;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (e * kWave >= c) continue;
+        const unsigned long long equal = __ballot(z[e] == edge);
+        if (z[e] > edge || (z[e] == edge && __popcll(equal & below) < need)) chosen |= 1u << e;
+        need = max(0, need - static_cast<int>(__popcll(equal)));
+      }
+    }
+    int put = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (e * kWave >= c) continue;
+      const unsigned long long who = __ballot(chosen >> e & 1u);
+      if (chosen >> e & 1u) {
+        const int at = put + __popcll(who & below), cls = e * kWave + lane;
+        if constexpr (kWide) {
+          s_list[wave][at] = KeyOf(z[e]);
+          s_cls[wave][at] = cls;
+        } else {
+          s_list[wave][at] = Candidate(z[e], cls);
+        }
+      }
+      put += __popcll(who);
+    }
+    WaveSync();
+    int32_t* out_class = static_cast<int32_t*>(a.top_class.data) + row * a.top_class.stride[0];
+    T* out_logit = static_cast<T*>(a.top_logit.data) + row * a.top_logit.stride[0];
+    for (int j = lane; j < a.k; j += kWave) {
+      int rank = j, cls = -1;
+      T value = static_cast<T>(-INFINITY);
+      if (j < take) {
+        const uint64_t own = s_list[wave][j];
+        rank = 0;
+        if constexpr (kWide) {
+          cls = s_cls[wave][j];
+#pragma unroll 4
+          for (int o = 0; o < take; ++o) {
+            const uint64_t other = s_list[wave][o];
+            rank += other > own || (other == own && s_cls[wave][o] < cls);
+          }
+          value = ValueOf(own);
+        } else {
+          cls = static_cast<int>(~static_cast<uint32_t>(own));
+#pragma unroll 4
+          for (int o = 0; o < take; ++o) rank += s_list[wave][o] > own;
+          value = static_cast<T>(ValueOf(static_cast<uint32_t>(own >> 32)));
+        }
+        // as it is: of the zeros the key does not know the sign
+        if (static_cast<A>(value) == A(0)) value = x[cls * a.scores.stride[1]];
+      }
+      out_class[rank * a.top_class.stride[1]] = cls;
+      out_logit[rank * a.top_logit.stride[1]] = value;
+    }
+    WaveSync();  // the list is the next row's
+    if (a.log_rest.data == nullptr) continue;
+    A next = NegInf<A>(), sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (!(chosen >> e & 1u)) next = Max(next, z[e]);
+    next = WaveMax(next);
+    if (next > NegInf<A>() && next < static_cast<A>(INFINITY)) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e * kWave < c && !(chosen >> e & 1u)) sum += Exp2((z[e] - next) * scale);
+      sum = WaveSum(sum);
+    }
+    if (lane == 0)
+      StoreFloat(a.log_rest, row * a.log_rest.stride[0],
+                 sum > A(0)
+                     ? next / static_cast<A>(a.temperature) + Log2(sum) * static_cast<A>(kLn2)
+                     : next);
+  }
+}
+
+// ------------------------------------------------------------------ top logits, many classes
+constexpr int kTopBins = 512;         // of the threads' maxima
+constexpr int kTopCandidates = 1024;  // of a row at most, or it goes the slow way
+constexpr int kTopChunks = 512;       // that hold them
 
 /*!
  * One workgroup a row. Every thread takes the maxima of four parts of what it holds: the k-th
@@ -1927,7 +2107,8 @@ void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
 
 template <typename T, typename S>
 void DistillTile(const LGBM_DistillArgs& a, bool across, hipStream_t s) {
-  if (!across) LaunchDistillTile<T, S, 4, kNeighbours>(a, s);
+  if (!across && a.classes <= 64) LaunchDistillTile<T, S, 4, kNeighbours>(a, s);
+  else if (!across) LaunchDistillTile<T, S, 16, kNeighbours>(a, s);
   else if (a.classes <= 4) LaunchDistillTile<T, S, 4, kAlone>(a, s);
   else if (a.classes <= 8) LaunchDistillTile<T, S, 8, kAlone>(a, s);
   else if (a.classes <= 16) LaunchDistillTile<T, S, 16, kAlone>(a, s);
@@ -1947,6 +2128,16 @@ void LaunchTopTile(const LGBM_TopLogitsArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_top_tile<T, E, kKind>),
                      dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256), 0, s, a,
                      lanes);
+}
+
+template <typename T, int E, bool kTurned>
+void LaunchTopWave(const LGBM_TopLogitsArgs& a, hipStream_t s) {
+  const int64_t rows = kTurned ? kTurnedRows : 4;
+  const size_t lds = kTurned ? sizeof(T) * rows * (a.classes | 1) : 0;
+  auto kernel = k_top_wave<T, E, kTurned>;
+  AllowLds(kernel, lds);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256),
+                     lds, s, a);
 }
 
 /*! chunks a thread that stand in LDS, where `other` bytes of its 160 KiB have another use */
@@ -1990,13 +2181,23 @@ void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
   const bool across = ClassMajor(a.scores);
   ByType(a.scores.type, [&](auto t) {
     using T = decltype(t);
-    if (a.classes <= (across ? 512 : 256)) {
-      if (!across) LaunchTopTile<T, 4, kNeighbours>(a, s);
+    if (a.classes <= 512) {
+      // With k times the largest of what is left, a row's time grows with k; by bisection
+      // hardly. Class-major float64, 100 classes: k = 10 of float32 97 us against 173, k = 40
+      // 253 against 237, k = 140 of 300 3569 against 1510. Row-major: 250 classes of bfloat16,
+      // k = 50, 3024 against 423; up to 64 classes four or more rows share a wave instead.
+      // A wave of 1000 classes has no registers left for a second one beside it: 964 us
+      // against 761 of a workgroup a row.
+      if (!across && a.classes <= 64) LaunchTopTile<T, 4, kNeighbours>(a, s);
+      else if (!across && a.classes <= 256) LaunchTopWave<T, 4, false>(a, s);
+      else if (!across) LaunchTopWave<T, 8, false>(a, s);
       else if (a.classes <= 4) LaunchTopTile<T, 4, kAlone>(a, s);
       else if (a.classes <= 8) LaunchTopTile<T, 8, kAlone>(a, s);
       else if (a.classes <= 16) LaunchTopTile<T, 16, kAlone>(a, s);
-      else if (a.classes <= 256) LaunchTopTile<T, 16, kAcross>(a, s);
-      else LaunchTopTile<T, 32, kAcross>(a, s);
+      else if (a.k <= 32 && a.classes <= 256) LaunchTopTile<T, 16, kAcross>(a, s);
+      else if (a.k <= 32) LaunchTopTile<T, 32, kAcross>(a, s);
+      else if (a.classes <= 256) LaunchTopWave<T, 4, true>(a, s);
+      else LaunchTopWave<T, 8, true>(a, s);
       return;
     }
     if constexpr (!std::is_same_v<T, double>) {
@@ -2031,7 +2232,7 @@ void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
   OnDevice on(device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool across = ClassMajor(a.scores);
-  if (a.classes <= (across ? 512 : 256)) {
+  if (a.classes <= 512) {
     ByType(a.scores.type, [&](auto t) {
       using T = decltype(t);
       LGBM_DistillArgs part = a;
