@@ -388,9 +388,13 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int cls = e * L + team.l;
-    z[e] = w != S(0) && cls < c ? score(cls) : NegInf<A>();
+    z[e] = there && cls < c ? score(cls) : NegInf<A>();
     if (cls < c) want[place(cls)] = kNone;
   }
+  // whatever the row's weight is, all that is read of it is asked for here at once
+  const bool rest = a.teacher_rest.data != nullptr, hard_term = static_cast<S>(a.alpha) < S(1);
+  const int label = hard_term && there ? LoadClass(a.label, at_row(a.label), c) : -1;
+  const S rest_read = rest && there ? LoadFloat<S>(a.teacher_rest, at_row(a.teacher_rest)) : S(0);
   team.Sync();
   const S temp = static_cast<S>(a.temperature), alpha = static_cast<S>(a.alpha);
   const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
@@ -412,8 +416,17 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int j = team.l + i * L;
-    held_cls[i] = teach && j < k ? load_class(j) : -1;
-    held_logit[i] = held_cls[i] >= 0 ? load_logit(j) : S(0);
+    const bool read = there && j < k;
+    held_cls[i] = read ? load_class(j) : -1;
+    held_logit[i] = read ? load_logit(j) : S(0);
+  }
+  if (!teach) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held_cls[i] = -1;
+  }
+  if (w == S(0)) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] = NegInf<A>();
   }
   // f(slot, class, logit) of all of them
   auto all_slots = [&](auto&& f) {
@@ -437,10 +450,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   team.Sync();
 
   // the teacher's distribution, in logarithms to base two
-  const bool rest = a.teacher_rest.data != nullptr;
-  const S r = rest && teach ? static_cast<S>(scale1) * LoadFloat<S>(a.teacher_rest,
-                                                                     at_row(a.teacher_rest))
-                            : NegInf<S>();
+  const S r = rest && teach ? static_cast<S>(scale1) * rest_read : NegInf<S>();
   S t_high = r;
   S t_nan = r != r ? S(1) : S(0);
   auto for_slots = [&](auto&& f) {  // the slots that count, with their place in the table
@@ -466,7 +476,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
 
   // the student's: the classes without a slot are summed on their own
   const A off = -high * scale, off1 = -high * scale1;
-  const bool hard_term = alpha < S(1), two = hard_term && scale != scale1;
+  const bool two = hard_term && scale != scale1;
   S ez[E], e1[E], left = 0, named = 0, total1 = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -509,7 +519,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
     }
   }
   const bool live = w != S(0) && !(total == S(0));  // otherwise every class is masked
-  const int y = hard_term && live ? LoadClass(a.label, at_row(a.label), c) : -1;
+  const int y = live ? label : -1;
 
   // the table's slots give way to their probabilities; every class has one such slot
   S kl = 0;
