@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   const S log_total = Log2(total);
   S log_left = Log2(left);
   A rest_off = off;
-  const bool again = rest && left < SmallRest<S>();
+  const bool again = rest && w != S(0) && left < SmallRest<S>();
   if (team.Any(again)) {
     A own = NegInf<A>();
 #pragma unroll
