@@ -14,6 +14,8 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <cstdlib>
+#include <initializer_list>
 #include <type_traits>
 
 namespace migbm {
@@ -2089,6 +2091,26 @@ class OnDevice {
   bool moved_ = false;
 };
 
+// A launch has fewer than 2^32 threads, and a workgroup of 1024 may have a row for itself.
+constexpr int64_t kRowsAtOnce = int64_t{1} << 21;
+
+/*! an array from row `start` on */
+void Advance(LGBM_Array* a, int64_t start) {
+  if (a->data != nullptr)
+    a->data = static_cast<char*>(a->data) + start * a->stride[0] * ElementSize(a->type);
+}
+
+/*! f(arguments of some rows) until all rows have had their turn; `arrays` are all of a call's */
+template <typename Args, typename F>
+void InParts(const Args& a, int64_t most, std::initializer_list<LGBM_Array Args::*> arrays, F&& f) {
+  for (int64_t start = 0; start < a.rows; start += most) {
+    Args part = a;
+    part.rows = std::min(most, a.rows - start);
+    for (auto array : arrays) Advance(&(part.*array), start);
+    f(part);
+  }
+}
+
 template <typename F> void ByType(int type, F&& f) {
   switch (type) {
     case C_API_DTYPE_FLOAT64: f(double{}); break;
@@ -2185,9 +2207,7 @@ template <typename F> void ByRow(int64_t rows, int chunks, F&& f) {
   else f(RowShape<1024, 12, true>{});
 }
 
-void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
-  OnDevice on(device);
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+void TopLogitsPart(const LGBM_TopLogitsArgs& a, hipStream_t s) {
   const bool across = ClassMajor(a.scores);
   ByType(a.scores.type, [&](auto t) {
     using T = decltype(t);
@@ -2238,9 +2258,14 @@ void LaunchDistillRow(const LGBM_DistillArgs& a, hipStream_t s) {
   else launch(k_distill_row<T, Shape, false>);
 }
 
-void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
+void TopLogitsDevice(const LGBM_TopLogitsArgs& a, int device, void* stream) {
   OnDevice on(device);
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  using Args = LGBM_TopLogitsArgs;
+  InParts(a, kRowsAtOnce, {&Args::scores, &Args::top_class, &Args::top_logit, &Args::log_rest},
+          [&](const Args& part) { TopLogitsPart(part, static_cast<hipStream_t>(stream)); });
+}
+
+void DistillPart(const LGBM_DistillArgs& a, hipStream_t s) {
   const bool across = ClassMajor(a.scores);
   if (a.classes <= 512) {
     ByType(a.scores.type, [&](auto t) {
@@ -2282,17 +2307,31 @@ void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
   OPS_HIP_OK(hipGetLastError());
 }
 
+void DistillDevice(const LGBM_DistillArgs& a, int device, void* stream) {
+  OnDevice on(device);
+  using Args = LGBM_DistillArgs;
+  InParts(a, kRowsAtOnce,
+          {&Args::scores, &Args::teacher_class, &Args::teacher_logit, &Args::teacher_rest,
+           &Args::label, &Args::weight, &Args::loss, &Args::gradient, &Args::hessian},
+          [&](const Args& part) { DistillPart(part, static_cast<hipStream_t>(stream)); });
+}
+
+constexpr int64_t kSplitRows = 32768;  // sequences of the split kernels at once
+
 /*! workgroups a sequence, 0 where the split kernels do not apply */
 int SplitsOf(const LGBM_VerifyArgs& a) {
-  if (a.classes <= kFewClasses || a.rows > 65535) return 0;  // a grid's second dimension
+  if (a.classes <= kFewClasses) return 0;
   if (a.target.stride[2] != 1 || (a.draft_prob.data && a.draft_prob.stride[2] != 1)) return 0;
   const int64_t wanted = (1024 + a.rows - 1) / a.rows, fitting = (a.classes + 2047) / 2048;
   return static_cast<int>(std::min<int64_t>({wanted, fitting, kMostSplits}));
 }
 
 int64_t VerifyWorkspaceDevice(const LGBM_VerifyArgs& a) {
-  return a.rows * SplitsOf(a) * kSplitWaves * static_cast<int64_t>(sizeof(double));
+  return std::min(a.rows, kSplitRows) * SplitsOf(a) * kSplitWaves *
+         static_cast<int64_t>(sizeof(double));
 }
+
+void VerifyPart(const LGBM_VerifyArgs& a, int splits, hipStream_t s);
 
 void VerifyDevice(const LGBM_VerifyArgs& a, int device, void* stream) {
   const int splits = SplitsOf(a);
@@ -2301,7 +2340,15 @@ void VerifyDevice(const LGBM_VerifyArgs& a, int device, void* stream) {
                static_cast<long long>(VerifyWorkspaceDevice(a)),
                static_cast<long long>(a.workspace ? a.workspace_bytes : 0));
   OnDevice on(device);
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  using Args = LGBM_VerifyArgs;
+  // parts follow each other on the stream, and use the same workspace
+  InParts(a, splits > 0 ? kSplitRows : kRowsAtOnce,
+          {&Args::target, &Args::draft_prob, &Args::draft_class, &Args::accept, &Args::sample,
+           &Args::length, &Args::out_class, &Args::out_accepted},
+          [&](const Args& part) { VerifyPart(part, splits, static_cast<hipStream_t>(stream)); });
+}
+
+void VerifyPart(const LGBM_VerifyArgs& a, int splits, hipStream_t s) {
   const uint32_t rows = static_cast<uint32_t>(a.rows);
   ByType(a.target.type, [&](auto t) {
     using T = decltype(t);

@@ -458,6 +458,7 @@ class Distill : public ObjectiveFunction {
         alpha_(cfg.distill_alpha) {}
   void Init(const Metadata& meta, data_size_t num_data) override {
     num_data_ = num_data;
+    if (num_class_ < 2) Log::Fatal("The distill objective needs num_class > 1");
     meta_ = &meta;  // its arrays are looked up anew in each iteration, as they may be set again
     LGBM_DistillArgs a = Args(nullptr);
     a.scores.data = a.loss.data = &a;  // checked for presence alone

@@ -545,6 +545,8 @@ class Dataset:
         if rest is not None and rest.shape != (rows,):
             raise LightGBMError(f"teacher log_rest must have the shape [{rows}], "
                                 f"got {list(rest.shape)}")
+        if classes.size > np.iinfo(np.int32).max:
+            raise LightGBMError(f"a teacher of {classes.size} logits is too large for a Dataset")
         # ids that 32 bits do not hold are no classes
         big = np.iinfo(np.int32).max
         classes = np.where((classes >= 0) & (classes <= big), classes, -1)

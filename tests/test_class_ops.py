@@ -214,7 +214,8 @@ def _top_case(place, x, dtype, k, t=1.0, order="C", pad=0):
 @pytest.mark.parametrize("place", PLACES)
 @pytest.mark.parametrize("rows,classes,k", [
     (1, 1, 1), (3, 2, 1), (5, 7, 3), (70, 10, 10), (130, 33, 4), (3, 64, 64), (2, 65, 20),
-    (4, 257, 256), (9, 1000, 17), (2, 1025, 100), (3, 4099, 64), (2, 20011, 256), (1, 70001, 33)])
+    (4, 257, 256), (20, 512, 100), (9, 1000, 17), (2, 1025, 100), (3, 4099, 64), (2, 20011, 256), (1, 70001, 33),
+    (1, 200003, 40)])
 def test_top_logits_sizes(place, rows, classes, k):
     rng = np.random.default_rng(rows * classes + k)
     for dtype in _types(place):
@@ -323,7 +324,7 @@ def _distill_case(place, z, teacher, dtype, labels=None, weight=None, t=1.0, alp
 
 SIZES = [(1, 1, 1), (2, 2, 1), (5, 3, 2), (70, 7, 3), (200, 10, 10), (65, 33, 9), (3, 64, 20),
          (66, 65, 64), (3, 300, 150), (4, 1000, 8), (2, 1025, 256), (3, 4099, 50), (2, 20011, 17),
-         (1, 70001, 64)]
+         (20, 512, 30), (1, 70001, 64), (1, 200003, 40)]
 
 
 @pytest.mark.parametrize("place", PLACES)
@@ -805,6 +806,36 @@ def test_offsets_beyond_32_bits():
     want = ops.verify_drafts(p, drafts[-2:], None, u[-2:], v[-2:])
     _same([x[-2:] for x in got], want)
     assert bool((got.classes[:-2, 0] == 3).all())
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_has():
+    """Rows past a part's end are what they are alone, and so are the last of the part before."""
+    rows = (1 << 21) + 5
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    for order, classes in (("C", 3), ("F", 2)):
+        z = torch.randn((rows, classes), generator=g, device="cuda")
+        z = z if order == "C" else z.t().contiguous().t()
+        end = slice(rows - 9, rows)
+        few = z[end].clone() if order == "C" else z[end].t().contiguous().t()
+        top, alone = ops.top_logits(z, 1), ops.top_logits(few, 1)
+        _same([x[end] for x in top], alone)
+        labels = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+        got = ops.distill_gradients(z, top, labels=labels, alpha=0.5, hessian=True, loss=True)
+        want = ops.distill_gradients(few, alone, labels=labels[end], alpha=0.5, hessian=True,
+                                     loss=True)
+        _same([x[end] for x in got], want)
+    for rows, classes in (((1 << 21) + 5, 2), (32768 + 5, 300)):
+        end = slice(rows - 9, rows)
+        p = torch.rand((rows, 2, classes), generator=g, device="cuda")
+        q = torch.rand((rows, 1, classes), generator=g, device="cuda")
+        x = torch.randint(0, classes, (rows, 1), generator=g, device="cuda")
+        u = torch.rand((rows, 1), generator=g, device="cuda")
+        v = torch.rand((rows,), generator=g, device="cuda")
+        got = ops.verify_drafts(p, x, q, u, v)
+        want = ops.verify_drafts(p[end], x[end], q[end], u[end], v[end])
+        _same([r[end] for r in got], want)
 
 
 def _padded(shape, dtype, value):

@@ -170,6 +170,9 @@ def test_cv_refit_and_a_new_teacher():
 def test_objective_refusals():
     X, raw, y = _data(60)
     top = ops.top_logits(raw, 3)
+    with pytest.raises(LightGBMError):
+        lgb.train({"objective": "distill", "verbosity": -1},
+                  lgb.Dataset(X, label=y, teacher=top), 1)  # of one class
     for teacher, more in ((None, {}), (top, {"distill_temperature": 0.0}),
                           (top, {"distill_alpha": 1.5}), (top, {"distill_alpha": -0.1})):
         with pytest.raises(LightGBMError):
