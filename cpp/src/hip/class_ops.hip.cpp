@@ -574,7 +574,8 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
         S p = FromBits(bits);
         if (bits == kNone) {
           p = S(0);
-          if (spread > S(0)) p = spread * (moved ? Exp2(exponent(score(cls), scale, rest_off)) : ez[e]);
+          const S e_rest = moved ? Exp2(exponent(score(cls), scale, rest_off)) : ez[e];
+          if (spread > S(0)) p = spread * e_rest;
           else if (spread != spread) p = spread;
         }
         g = soft * temp * (q - p);
@@ -855,7 +856,9 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
 
   const A off = -high * scale, off1 = -high * scale1;
   A left = 0, total1 = 0;
-  z.EachHeld([&](int base, const auto& v, auto...) { add_chunk(base, v, off, off1, left, total1); });
+  z.EachHeld([&](int base, const auto& v, auto...) {
+    add_chunk(base, v, off, off1, left, total1);
+  });
   if constexpr (Shape::more) {
     if (own_high > NegInf<A>() || more_left != A(0)) {
       left += more_left * Exp2((own_high > NegInf<A>() ? own_high - high : A(0)) * scale);
@@ -1072,7 +1075,8 @@ __device__ __forceinline__ void TopAny(const LGBM_TopLogitsArgs& a, int64_t row)
       for (int i = tid; i < c; i += kBlock) {
         const K key = KeyOf(value(i));
         // the digits above are the edge's; the last shift is all of the key
-        const bool same = shift == sizeof(K) * 8 - 8 || (key >> (shift + 8)) == (edge >> (shift + 8));
+        const bool same = shift == sizeof(K) * 8 - 8 ||
+                          (key >> (shift + 8)) == (edge >> (shift + 8));
         if (key != 0 && same) atomicAdd(&hist[static_cast<int>(key >> shift) & 255], 1);
       }
       __syncthreads();
@@ -1089,7 +1093,8 @@ __device__ __forceinline__ void TopAny(const LGBM_TopLogitsArgs& a, int64_t row)
       __syncthreads();
       for (int i = tid; i < c; i += kBlock) {
         const int turned = 0xffffff - i;
-        if (KeyOf(value(i)) == edge && (shift == 16 || (turned >> (shift + 8)) == (high >> (shift + 8))))
+        if (KeyOf(value(i)) == edge &&
+            (shift == 16 || (turned >> (shift + 8)) == (high >> (shift + 8))))
           atomicAdd(&hist[(turned >> shift) & 255], 1);
       }
       __syncthreads();
@@ -2202,7 +2207,8 @@ void LaunchTopWave(const LGBM_TopLogitsArgs& a, hipStream_t s) {
 template <typename Shape> int LdsChunksOf(int chunks, size_t other) {
   if (!Shape::more) return 0;
   const int wanted = (chunks - Shape::cached * Shape::block + Shape::block - 1) / Shape::block;
-  const int room = static_cast<int>((160 * 1024 - std::min<size_t>(other, 160 * 1024)) /
+  const size_t all = Shape::block <= 512 ? 80 * 1024 : 160 * 1024;  // two, or one a compute unit
+  const int room = static_cast<int>((all - std::min<size_t>(other, all)) /
                                     (sizeof(Words) * Shape::block));
   return std::max(0, std::min({wanted, room, kLdsChunks}));
 }
@@ -2221,15 +2227,20 @@ void LaunchTopRow(const LGBM_TopLogitsArgs& a, hipStream_t s) {
  * The workgroup of a row of `chunks` whole chunks, f(threads, chunks a thread in registers).
  * Many rows: few threads with much of the row each, so that four rows or more share a compute
  * unit and one computes while another waits for its scores. Rows that leave compute units
- * idle: as many threads as there are, so that the one row is done sooner.
+ * idle: as many threads as there are, so that the one row is done sooner. Rows that do not
+ * fit: two share a compute unit if they are only read (1000 x 150000 bfloat16: top 64 92 us
+ * against 107 of one, loss 88 against 104), but where as much is written again the part that
+ * is read twice costs more than the other row hides (1500 x 131077 float32: 445 us against
+ * 399).
  */
-template <typename F> void ByRow(int64_t rows, int chunks, F&& f) {
+template <typename F> void ByRow(int64_t rows, int chunks, bool writes, F&& f) {
   if (chunks <= 256) f(RowShape<256, 1>{});
   else if (rows < 512 && chunks <= 4096) f(RowShape<1024, 4>{});
   else if (chunks <= 1024) f(RowShape<256, 4>{});
   else if (chunks <= 2048) f(RowShape<256, 8>{});
   else if (chunks <= 4096) f(RowShape<256, 16>{});
   else if (rows >= 512 && chunks <= 8192) f(RowShape<512, 16>{});
+  else if (rows >= 512 && !writes) f(RowShape<512, 16, true>{});
   else f(RowShape<1024, 12, true>{});
 }
 
@@ -2258,7 +2269,7 @@ void TopLogitsPart(const LGBM_TopLogitsArgs& a, hipStream_t s) {
     }
     if constexpr (!std::is_same_v<T, double>) {
       if (a.scores.stride[1] == 1) {
-        ByRow(a.rows, a.classes / Chunk<T>::kSize, [&](auto shape) {
+        ByRow(a.rows, a.classes / Chunk<T>::kSize, false, [&](auto shape) {
           LaunchTopRow<T, decltype(shape)>(a, s);
         });
         return;
@@ -2315,7 +2326,8 @@ void DistillPart(const LGBM_DistillArgs& a, hipStream_t s) {
     ByType(a.scores.type, [&](auto t) {
       using T = decltype(t);
       if constexpr (!std::is_same_v<T, double>) {
-        ByRow(a.rows, a.classes / Chunk<T>::kSize, [&](auto shape) {
+        const bool writes = a.gradient.data || a.hessian.data;
+        ByRow(a.rows, a.classes / Chunk<T>::kSize, writes, [&](auto shape) {
           LaunchDistillRow<T, decltype(shape)>(a, s);
         });
       }

@@ -214,8 +214,8 @@ def _top_case(place, x, dtype, k, t=1.0, order="C", pad=0):
 @pytest.mark.parametrize("place", PLACES)
 @pytest.mark.parametrize("rows,classes,k", [
     (1, 1, 1), (3, 2, 1), (5, 7, 3), (70, 10, 10), (130, 33, 4), (3, 64, 64), (2, 65, 20),
-    (4, 257, 256), (20, 512, 100), (9, 1000, 17), (2, 1025, 100), (3, 4099, 64), (2, 20011, 256), (1, 70001, 33),
-    (1, 200003, 40)])
+    (4, 257, 256), (20, 512, 100), (9, 1000, 17), (2, 1025, 100), (3, 4099, 64), (2, 20011, 256),
+    (1, 70001, 33), (1, 200003, 40)])
 def test_top_logits_sizes(place, rows, classes, k):
     rng = np.random.default_rng(rows * classes + k)
     for dtype in _types(place):
@@ -447,7 +447,10 @@ def test_distill_gradient_is_the_slope(place, order, classes):
     mix = {"labels": _put(place, labels, "i32"), "weight": _put(place, weight, "f32"),
            "temperature": 2.0, "alpha": 0.6}
     grad = _get(ops.distill_gradients(_put(place, z, "f64", order), teacher, **mix).gradient)
-    loss = lambda x: _get(ops.distill_loss(_put(place, x, "f64", order), teacher, **mix))  # noqa: E731
+
+    def loss(x):
+        return _get(ops.distill_loss(_put(place, x, "f64", order), teacher, **mix))
+
     top = np.abs(loss(z)).max()
     size_g = _plain_distill(z, ids, logits.astype(float), rest.astype(float), labels,
                             weight.astype(float), 2.0, 0.6)[4]
@@ -707,7 +710,7 @@ def _same(a, b):
 
 DEVICE_SETS = [(5, 9, "f64", "F", 3), (70, 200, "f32", "F", 40), (6, 40, "bf16", "C", 7),
                (4, 3001, "f16", "C", 33), (2, 70001, "f32", "C", 20), (3, 3000, "f64", "C", 9),
-               (600, 20011, "bf16", "C", 64)]
+               (600, 20011, "bf16", "C", 64), (600, 40001, "f32", "C", 9)]
 
 
 @pytest.mark.gpu
@@ -806,6 +809,43 @@ def test_offsets_beyond_32_bits():
     want = ops.verify_drafts(p, drafts[-2:], None, u[-2:], v[-2:])
     _same([x[-2:] for x in got], want)
     assert bool((got.classes[:-2, 0] == 3).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,dtype,k", [
+    (1100, 2500, "f32", 30), (600, 9001, "bf16", 64), (520, 24001, "f32", 100),
+    (520, 60001, "f32", 64), (520, 110003, "f16", 33)])
+def test_many_rows_of_many_classes(rows, classes, dtype, k):
+    """Shapes that only many rows take, some of whose rows are held against the plain forms."""
+    rng = np.random.default_rng(classes)
+    some = [0, 1, 255, 256, rows - 1]
+    s = _set(rows, classes, dtype, 5)
+    top = ops.top_logits(s["z"], k, temperature=2.0)
+    z = _get(s["z"])[some]
+    ids, logits, rest = _plain_top(z, k, 2.0)
+    np.testing.assert_array_equal(_get(top.classes)[some], ids)
+    np.testing.assert_array_equal(_get(top.logits)[some], logits)
+    rel = _rel(classes, dtype)
+    assert np.all(np.abs(_get(top.log_rest)[some] - rest) <= 2 * rel * (1 + np.abs(rest)))
+    student = _put("gpu", _round(rng.permutation(z.T).T, dtype), dtype)
+    student = student[torch.arange(rows, device="cuda") % len(some)]
+    teacher = ops.TopLogits(*[x[some][torch.arange(rows) % len(some)] for x in top])
+    labels = torch.arange(rows, device="cuda") % classes
+    mix = {"labels": labels, "temperature": 2.0, "alpha": 0.5}
+    here = list(range(len(some)))
+    loss, grad, _, size_l, size_g = _plain_distill(
+        _get(student)[here], _get(teacher.classes)[here], _get(teacher.logits)[here],
+        _get(teacher.log_rest)[here].astype(float), _get(labels)[here], None, 2.0, 0.5)
+    got = ops.distill_gradients(student, teacher, **mix)
+    for x in (ops.distill_loss(student, teacher, **mix),
+              ops.distill_gradients(student, teacher, loss=True, **mix).loss):
+        assert np.all(np.abs(_get(x)[here] - loss) <= 3 * rel * size_l +
+                      HALF_STEP["f32"] * np.abs(loss))
+    assert np.all(np.abs(_get(got.gradient)[here] - grad) <= 3 * rel * size_g +
+                  (1 + rel) * HALF_STEP[dtype] * np.abs(grad) + TINY[dtype])
+    # the same row again and again has the same results
+    again = _get(got.gradient)[len(some):2 * len(some)] - _get(got.gradient)[here]
+    assert np.count_nonzero(again) <= 2 * len(some)  # but for the classes of the labels
 
 
 @pytest.mark.gpu
