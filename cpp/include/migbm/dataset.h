@@ -63,6 +63,8 @@ class Metadata {
   const float* teacher_rest() const {
     return teacher_rest_.empty() ? nullptr : teacher_rest_.data();
   }
+  /*! changes whenever any of the teacher's arrays is set or taken away */
+  int teacher_version() const { return teacher_version_; }
   int64_t num_teacher_logit() const { return static_cast<int64_t>(teacher_logit_.size()); }
   /*! throws unless there are as many classes as logits, in whole rows */
   void CheckTeacher() const;
@@ -107,6 +109,7 @@ class Metadata {
   std::vector<int32_t> teacher_class_;
   std::vector<float> teacher_logit_;
   std::vector<float> teacher_rest_;
+  int teacher_version_ = 0;
   std::vector<int32_t> streamed_query_ids_;
 };
 

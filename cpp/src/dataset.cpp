@@ -65,18 +65,21 @@ static void CheckTeacherLength(const char* what, int64_t n, data_size_t rows) {
 }
 
 void Metadata::SetTeacherClass(const int32_t* p, int64_t n) {
+  ++teacher_version_;
   if (p == nullptr || n == 0) { teacher_class_.clear(); return; }
   CheckTeacherLength("teacher_class", n, num_data_);
   teacher_class_.assign(p, p + n);
 }
 
 void Metadata::SetTeacherLogit(const float* p, int64_t n) {
+  ++teacher_version_;
   if (p == nullptr || n == 0) { teacher_logit_.clear(); return; }
   CheckTeacherLength("teacher_logit", n, num_data_);
   teacher_logit_.assign(p, p + n);
 }
 
 void Metadata::SetTeacherRest(const float* p, int64_t n) {
+  ++teacher_version_;
   if (p == nullptr || n == 0) { teacher_rest_.clear(); return; }
   MIGBM_CHECK_EQ(n, num_data_);
   teacher_rest_.assign(p, p + n);

@@ -2579,6 +2579,7 @@ class HIPTreeLearner : public TreeLearner {
 
  private:
   void UploadGradients(const score_t* g, const score_t* h);
+  void UploadTeacher(const Metadata& meta);
   void LaunchHist(const int* leafA_ptr, int leafB_from_counters, int blocks, bool zero_spare = true);
   void ReduceSpareHist(int spare_slot);
   void LaunchBestSplit(const int* leafA_ptr, int leafB_from_counters);
@@ -2642,11 +2643,10 @@ class HIPTreeLearner : public TreeLearner {
   int num_queries_ = 0;
   DevBuf<double> d_score_;
   DevBuf<float> d_label_, d_weight_;
-  // the distill objective's teacher, as it was when the training data was uploaded
+  // the distill objective's teacher, and the version of the dataset's that it is
   DevBuf<int32_t> d_teacher_class_;
   DevBuf<float> d_teacher_logit_, d_teacher_rest_;
-  int teacher_slots_ = 0;
-  bool teacher_rest_ = false;
+  int teacher_version_ = 0;
   DevBuf<uint32_t> d_idx_, d_idx_tmp_;
   DevBuf<uint8_t> d_marks_;
   DevBuf<int> d_block_cnt_, d_block_loff_, d_block_roff_;
@@ -2991,24 +2991,7 @@ void HIPTreeLearner::Init(const Dataset* train_data, bool is_constant_hessian) {
   d_label_.Alloc(num_data_);
   HIP_OK(hipMemcpy(d_label_.ptr, train_data->metadata().label(), sizeof(float) * num_data_,
                    hipMemcpyHostToDevice));
-  const Metadata& meta = train_data->metadata();
-  teacher_slots_ = meta.teacher_slots();
-  teacher_rest_ = meta.teacher_rest() != nullptr;
-  if (teacher_slots_ > 0) {
-    meta.CheckTeacher();
-    const size_t count = static_cast<size_t>(num_data_) * teacher_slots_;
-    d_teacher_class_.Alloc(count);
-    d_teacher_logit_.Alloc(count);
-    HIP_OK(hipMemcpy(d_teacher_class_.ptr, meta.teacher_class(), sizeof(int32_t) * count,
-                     hipMemcpyHostToDevice));
-    HIP_OK(hipMemcpy(d_teacher_logit_.ptr, meta.teacher_logit(), sizeof(float) * count,
-                     hipMemcpyHostToDevice));
-    if (teacher_rest_) {
-      d_teacher_rest_.Alloc(num_data_);
-      HIP_OK(hipMemcpy(d_teacher_rest_.ptr, meta.teacher_rest(), sizeof(float) * num_data_,
-                       hipMemcpyHostToDevice));
-    }
-  }
+  UploadTeacher(train_data->metadata());
   weights_present_ = train_data->metadata().weights() != nullptr;
   if (weights_present_) {
     d_weight_.Alloc(num_data_);
@@ -3169,6 +3152,25 @@ void HIPTreeLearner::UploadGradients(const score_t* g, const score_t* h) {
                         stream_));
 }
 
+void HIPTreeLearner::UploadTeacher(const Metadata& meta) {
+  teacher_version_ = meta.teacher_version();
+  if (meta.teacher_slots() == 0) return;
+  meta.CheckTeacher();
+  const size_t count = static_cast<size_t>(num_data_) * meta.teacher_slots();
+  HIP_OK(hipStreamSynchronize(stream_));  // an iteration may still read the one before
+  d_teacher_class_.Alloc(count);
+  d_teacher_logit_.Alloc(count);
+  HIP_OK(hipMemcpy(d_teacher_class_.ptr, meta.teacher_class(), sizeof(int32_t) * count,
+                   hipMemcpyHostToDevice));
+  HIP_OK(hipMemcpy(d_teacher_logit_.ptr, meta.teacher_logit(), sizeof(float) * count,
+                   hipMemcpyHostToDevice));
+  if (meta.teacher_rest() != nullptr) {
+    d_teacher_rest_.Alloc(num_data_);
+    HIP_OK(hipMemcpy(d_teacher_rest_.ptr, meta.teacher_rest(), sizeof(float) * num_data_,
+                     hipMemcpyHostToDevice));
+  }
+}
+
 void HIPTreeLearner::DeviceBoosting(const ObjectiveFunction* obj) {
   const std::string name = obj->GetName();
   const int n = num_data_;
@@ -3199,11 +3201,10 @@ void HIPTreeLearner::DeviceBoosting(const ObjectiveFunction* obj) {
     LGBM_DistillArgs a = class_ops::DistillArgsOf(meta, n, num_class_score_,
                                                   config_->distill_temperature,
                                                   config_->distill_alpha, d_score_.ptr);
-    if (a.k != teacher_slots_ || (a.teacher_rest.data != nullptr) != teacher_rest_)
-      Log::Fatal("The teacher was changed after the training data was uploaded");
+    if (meta.teacher_version() != teacher_version_) UploadTeacher(meta);
     a.teacher_class.data = d_teacher_class_.ptr;
     a.teacher_logit.data = d_teacher_logit_.ptr;
-    if (teacher_rest_) a.teacher_rest.data = d_teacher_rest_.ptr;
+    if (a.teacher_rest.data != nullptr) a.teacher_rest.data = d_teacher_rest_.ptr;
     a.label.data = d_label_.ptr;
     a.weight.data = weights_present_ ? d_weight_.ptr : nullptr;
     a.gradient = class_ops::ArrayOf(d_grad_.ptr, C_API_DTYPE_FLOAT32, 1, n);
@@ -4289,6 +4290,7 @@ class MultiGpuTreeLearner : public TreeLearner {
     train_data_ = train_data;
     is_constant_hessian_ = is_constant_hessian;
     num_data_ = train_data->num_data();
+    teacher_version_ = train_data->metadata().teacher_version();
     if (train_data->metadata().query_boundaries() != nullptr)
       Log::Fatal("ranking objectives with num_gpu>1 in one process are not supported; "
                  "use one process per GPU (tree_learner=data)");
@@ -4425,6 +4427,8 @@ class MultiGpuTreeLearner : public TreeLearner {
   }
 
   void DeviceBoosting(const ObjectiveFunction* obj) override {
+    if (train_data_->metadata().teacher_version() != teacher_version_)
+      Log::Fatal("A teacher cannot be set while a booster trains with num_gpu > 1");
     workers_->RunAll([&](int r) { learners_[r]->DeviceBoosting(obj); });
   }
   void DeviceAddInitScore(double v) override {
@@ -4480,6 +4484,7 @@ class MultiGpuTreeLearner : public TreeLearner {
   }
 
  private:
+  int teacher_version_ = 0;  // of the dataset that the shards were cut from
   const Config* config_;
   const Dataset* train_data_ = nullptr;
   bool is_constant_hessian_ = false;

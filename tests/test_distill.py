@@ -158,13 +158,26 @@ def test_cv_refit_and_a_new_teacher():
     bst = lgb.train(_params("cpu"), lgb.Dataset(X, label=y, teacher=top), 3)
     new = bst.refit(X, y, teacher=top)
     assert np.all(np.isfinite(new.predict(X)))
-    # a teacher that is set while a booster trains is the next iteration's
-    ds = lgb.Dataset(X, label=y, teacher=top)
-    live = lgb.Booster(_params("cpu"), ds)
-    live.update()
-    ds.set_teacher((np.tile(np.arange(5), (600, 1)), raw.astype(np.float32)))
-    live.update()
-    assert live.num_trees() == 10 and np.all(np.isfinite(live.predict(X)))
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_a_new_teacher_is_the_next_iterations(place):
+    """Of other slots or of the same, while a booster trains: as if the scores of the first
+    iteration had been given to a booster of the new teacher as its start."""
+    X, raw, y = _data()
+    top = ops.top_logits(raw, 3)
+    for new in ((np.tile(np.arange(5), (600, 1)), -2 * raw.astype(np.float32)),
+                ops.top_logits(-raw, 3)):
+        ds = lgb.Dataset(X, label=y, teacher=top)
+        live = lgb.Booster(_params(place, boost_from_average=False), ds)
+        live.update()
+        start = live.predict(X, raw_score=True)
+        ds.set_teacher(new)
+        live.update()
+        other = lgb.train(_params(place, boost_from_average=False),
+                          lgb.Dataset(X, label=y, teacher=new, init_score=start), 1)
+        d = live.predict(X, raw_score=True) - start - other.predict(X, raw_score=True)
+        assert np.quantile(np.abs(d), 0.99) < 1e-4
 
 
 def test_objective_refusals():
