@@ -2249,13 +2249,18 @@ void TopLogitsPart(const LGBM_TopLogitsArgs& a, hipStream_t s) {
   ByType(a.scores.type, [&](auto t) {
     using T = decltype(t);
     if (a.classes <= 512) {
-      // With k times the largest of what is left, a row's time grows with k; by bisection
-      // hardly. Class-major float64, 100 classes: k = 10 of float32 97 us against 173, k = 40
-      // 253 against 237, k = 140 of 300 3569 against 1510. Row-major: 250 classes of bfloat16,
-      // k = 50, 3024 against 423; up to 64 classes four or more rows share a wave instead.
-      // A wave of 1000 classes has no registers left for a second one beside it: 964 us
-      // against 761 of a workgroup a row.
+      // With k times the largest of what is left, a row's time grows with k and with the lanes
+      // it takes; by bisection hardly. Row-major, the two meet where k times the lanes is about
+      // 300: 400000 x 100 float32 (8 lanes) k = 10 146 us against 362, k = 50 514 against 401;
+      // 300000 x 250 bfloat16 (16 lanes) k = 5 168 against 338, k = 20 402 against 381; 200000
+      // x 300 float32 (32 lanes) k = 5 179 against 336, k = 20 526 against 369. Class-major,
+      // where bisection has to turn the rows first: 200000 x 100 float32 k = 10 97 against 173,
+      // 100000 x 100 float64 k = 40 253 against 237, 100000 x 300 k = 140 3569 against 1510. A
+      // wave of 1000 classes has no registers left for others beside it: 100000 x 1000
+      // bfloat16, k = 100, 964 against 761 of a workgroup a row.
       if (!across && a.classes <= 64) LaunchTopTile<T, 4, kNeighbours>(a, s);
+      else if (!across && a.k * LanesFor(a.classes, 16) <= 300)
+        LaunchTopTile<T, 16, kNeighbours>(a, s);
       else if (!across && a.classes <= 256) LaunchTopWave<T, 4, false>(a, s);
       else if (!across) LaunchTopWave<T, 8, false>(a, s);
       else if (a.classes <= 4) LaunchTopTile<T, 4, kAlone>(a, s);

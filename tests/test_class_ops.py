@@ -214,8 +214,8 @@ def _top_case(place, x, dtype, k, t=1.0, order="C", pad=0):
 @pytest.mark.parametrize("place", PLACES)
 @pytest.mark.parametrize("rows,classes,k", [
     (1, 1, 1), (3, 2, 1), (5, 7, 3), (70, 10, 10), (130, 33, 4), (3, 64, 64), (2, 65, 20),
-    (4, 257, 256), (20, 512, 100), (9, 1000, 17), (2, 1025, 100), (3, 4099, 64), (2, 20011, 256),
-    (1, 70001, 33), (1, 200003, 40)])
+    (37, 100, 10), (9, 300, 9), (4, 257, 256), (20, 512, 100), (9, 1000, 17), (2, 1025, 100),
+    (3, 4099, 64), (2, 20011, 256), (1, 70001, 33), (1, 200003, 40)])
 def test_top_logits_sizes(place, rows, classes, k):
     rng = np.random.default_rng(rows * classes + k)
     for dtype in _types(place):

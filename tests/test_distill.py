@@ -251,3 +251,14 @@ def test_shards_have_their_rows_of_the_teacher():
                         lgb.Dataset(X, label=y, teacher=top), 5)
         preds.append(bst.predict(X, raw_score=True))
     assert np.quantile(np.abs(preds[0] - preds[1]), 0.99) < 1e-4
+
+
+@pytest.mark.gpu
+def test_shards_refuse_a_new_teacher():
+    X, raw, y = _data()
+    ds = lgb.Dataset(X, label=y, teacher=ops.top_logits(raw, 3))
+    live = lgb.Booster(_params("gpu", num_gpu=2), ds)
+    live.update()
+    ds.set_teacher(ops.top_logits(-raw, 3))
+    with pytest.raises(LightGBMError):
+        live.update()
