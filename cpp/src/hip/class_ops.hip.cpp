@@ -884,26 +884,16 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   const A t_log = t_high + Log2(t_sum), log_total = Log2(total);
   const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
   A log_left = Log2(left), rest_off = off;
-  if (rest && left < SmallRest<A>()) {
+  if (rest && left < SmallRest<A>()) {  // seldom, so from memory in a plain loop
     A own = NegInf<A>();
-    z.Each([&](int base, const auto& v, auto...) {
-    constexpr int kSize = kSizeOf<decltype(v)>;
-      const uint32_t bits = bits_of(base, kSize);
-#pragma unroll
-      for (int i = 0; i < kSize; ++i)
-        if (!(bits >> i & 1u)) own = Max(own, v[i]);
-    });
+    for (int i = tid; i < c; i += kBlock)
+      if (!bits_of(i, 1)) own = Max(own, static_cast<A>(z.x[i]));
     own = BlockMax<kBlock>(own, s_more[1]);
     if (own > NegInf<A>()) {
       rest_off = -own * scale;
       left = 0;
-      z.Each([&](int base, const auto& v, auto...) {
-    constexpr int kSize = kSizeOf<decltype(v)>;
-        const uint32_t bits = bits_of(base, kSize);
-#pragma unroll
-        for (int i = 0; i < kSize; ++i)
-          if (!(bits >> i & 1u)) left += Exp2(Fma(v[i], scale, rest_off));
-      });
+      for (int i = tid; i < c; i += kBlock)
+        if (!bits_of(i, 1)) left += Exp2(Fma(static_cast<A>(z.x[i]), scale, rest_off));
       left = BlockSum<kBlock>(left, s_more[2]);
       log_left = Log2(left) - rest_off + off;
     }
@@ -1646,21 +1636,21 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
   // two sums, each against a value near its own: of what is below the edge, and of the
   // candidates that were not chosen
   sum = BlockSum<kBlock>(sum, s_sum);
-  if (n <= k && sum < SmallRest<A>()) {  // far below the edge: against its own maximum
+  if (n <= k && sum < SmallRest<A>()) {
+    // far below the edge: against its own maximum; seldom, so from memory in a plain loop
     A own = NegInf<A>();
-    z.Each([&](int, const auto& v, auto...) {
-#pragma unroll
-      for (int i = 0; i < kSizeOf<decltype(v)>; ++i) own = Max(own, v[i] < edge ? v[i] : own);
-    });
+    for (int i = tid; i < a.classes; i += kBlock) {
+      const A v = static_cast<A>(z.x[i]);
+      if (v < edge) own = Max(own, v);
+    }
     own = BlockMax<kBlock>(own, s_low);
     sum = 0;
     if (own > NegInf<A>()) {
       off = -own * scale;
-      z.Each([&](int, const auto& v, auto...) {
-#pragma unroll
-        for (int i = 0; i < kSizeOf<decltype(v)>; ++i)
-          sum += v[i] < edge ? Exp2(Fma(v[i], scale, off)) : A(0);
-      });
+      for (int i = tid; i < a.classes; i += kBlock) {
+        const A v = static_cast<A>(z.x[i]);
+        if (v < edge) sum += Exp2(Fma(v, scale, off));
+      }
       sum = BlockSum<kBlock>(sum, s_high);
     }
   }
