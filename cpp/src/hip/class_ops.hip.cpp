@@ -2244,20 +2244,22 @@ void TopLogitsPart(const LGBM_TopLogitsArgs& a, hipStream_t s) {
       // 300: 400000 x 100 float32 (8 lanes) k = 10 146 us against 362, k = 50 514 against 401;
       // 300000 x 250 bfloat16 (16 lanes) k = 5 168 against 338, k = 20 402 against 381; 200000
       // x 300 float32 (32 lanes) k = 5 179 against 336, k = 20 526 against 369. Class-major,
-      // where bisection has to turn the rows first: 200000 x 100 float32 k = 10 97 against 173,
-      // 100000 x 100 float64 k = 40 253 against 237, 100000 x 300 k = 140 3569 against 1510. A
+      // where a round is two barriers and bisection has to turn the rows first, about 256, and
+      // 25 rounds: float64, 8000 x 100 k = 8 20 against 29, k = 30 55 against 39; 8000 x 300
+      // k = 8 36 against 43, k = 30 100 against 54; 40000 x 100 k = 8 32 against 76. A
       // wave of 1000 classes has no registers left for others beside it: 100000 x 1000
       // bfloat16, k = 100, 964 against 761 of a workgroup a row.
+      const int rounds = a.k * LanesFor(a.classes, 16);
+      const bool few = across ? a.k <= 25 && rounds <= 256 : rounds <= 300;
       if (!across && a.classes <= 64) LaunchTopTile<T, 4, kNeighbours>(a, s);
-      else if (!across && a.k * LanesFor(a.classes, 16) <= 300)
-        LaunchTopTile<T, 16, kNeighbours>(a, s);
+      else if (!across && few) LaunchTopTile<T, 16, kNeighbours>(a, s);
       else if (!across && a.classes <= 256) LaunchTopWave<T, 4, false>(a, s);
       else if (!across) LaunchTopWave<T, 8, false>(a, s);
       else if (a.classes <= 4) LaunchTopTile<T, 4, kAlone>(a, s);
       else if (a.classes <= 8) LaunchTopTile<T, 8, kAlone>(a, s);
       else if (a.classes <= 16) LaunchTopTile<T, 16, kAlone>(a, s);
-      else if (a.k <= 32 && a.classes <= 256) LaunchTopTile<T, 16, kAcross>(a, s);
-      else if (a.k <= 32) LaunchTopTile<T, 32, kAcross>(a, s);
+      else if (few && a.classes <= 256) LaunchTopTile<T, 16, kAcross>(a, s);
+      else if (few) LaunchTopTile<T, 32, kAcross>(a, s);
       else if (a.classes <= 256) LaunchTopWave<T, 4, true>(a, s);
       else LaunchTopWave<T, 8, true>(a, s);
       return;
