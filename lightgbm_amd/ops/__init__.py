@@ -97,9 +97,10 @@ def _is_tensor(x):
 class _Place:
     """Where a call runs, and how its results are made: as its first array is."""
 
-    __slots__ = ("tensor", "device", "on")
+    __slots__ = ("tensor", "device", "on", "made")
 
     def __init__(self, x):
+        self.made = []  # arrays that stand for other objects, alive as long as the call
         self.device = -1
         self.on = None
         self.tensor = _is_tensor(x)
@@ -144,6 +145,7 @@ class _Place:
             raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
         elif not isinstance(x, np.ndarray):
             x = np.asarray(x)
+            self.made.append(x)
         if x.shape != shape:
             raise LightGBMError(f"{name} must have the shape {list(shape)}, got {list(x.shape)}")
         return _fields(x, name)

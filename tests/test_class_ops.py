@@ -950,3 +950,31 @@ def test_torch_first():
 
 def test_lgb_exports_ops():
     assert lgb.ops is ops
+
+
+# ------------------------------------------------------------------ lists
+def test_lists_are_their_arrays():
+    """Every argument may be a list; the array made of it lives until the call has returned.
+    Large enough that memory freed before would be used again."""
+    rng = np.random.default_rng(21)
+    rows, classes, k = 5000, 10, 3
+    z = rng.standard_normal((rows, classes))
+    ids, logits, rest = _teacher(rng, rows, classes, k, True)
+    args = [ids, logits.astype(float), rest.astype(float), rng.integers(0, classes, rows),
+            0.5 + rng.random(rows)]
+
+    def distill(turn):
+        c, t, r, y, w = map(turn, args)
+        got = ops.distill_gradients(turn(z), (c, t, r), labels=y, weight=w, alpha=0.5, loss=True,
+                                    hessian=True)
+        return [*got, ops.distill_loss(turn(z), (c, t, r), labels=y, weight=w, alpha=0.5)]
+
+    p = _softmax(rng.standard_normal((rows, 3, classes)))
+    q = _softmax(rng.standard_normal((rows, 2, classes)))
+    drafts = rng.integers(0, classes, (rows, 2))
+    u, v, lengths = rng.random((rows, 2)), rng.random(rows), rng.integers(0, 3, rows)
+    for call in (distill, lambda turn: ops.top_logits(turn(z), k),
+                 lambda turn: ops.verify_drafts(*map(turn, (p, drafts, q, u, v)),
+                                                lengths=turn(lengths))):
+        for got, want in zip(call(lambda x: x.tolist()), call(lambda x: x)):
+            np.testing.assert_array_equal(got, want)
