@@ -526,7 +526,7 @@ class Dataset:
             for name in ("teacher_class", "teacher_logit", "teacher_log_rest"):
                 self.set_field(name, None)
             return self
-        parts = [p.detach().cpu().float().numpy() if hasattr(p, "detach") and
+        parts = [p.detach().resolve_neg().cpu().float().numpy() if hasattr(p, "detach") and
                  p.dtype.is_floating_point else p.cpu().numpy() if hasattr(p, "detach") else
                  None if p is None else np.asarray(p) for p in teacher]
         if not 2 <= len(parts) <= 3:

@@ -141,6 +141,8 @@ class _Place:
             if x.get_device() != self.device or x.is_cuda != (self.device >= 0):
                 raise LightGBMError(f"{name} is on {x.device}, the first array on "
                                     f"{self.on or 'the host'}")
+            if x.is_neg():
+                self.made.append(x := _written_out(x))
         elif self.device >= 0:
             raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
         elif not isinstance(x, np.ndarray):
@@ -149,6 +151,12 @@ class _Place:
         if x.shape != shape:
             raise LightGBMError(f"{name} must have the shape {list(shape)}, got {list(x.shape)}")
         return _fields(x, name)
+
+
+def _written_out(x):
+    """A tensor whose memory holds its own values: a view that negates (the imaginary part of a
+    conjugate) is written out, on its device's current stream."""
+    return x.resolve_neg() if x.is_neg() else x
 
 
 def _fields(x, name):
@@ -178,7 +186,9 @@ def _fields(x, name):
 
 def _shaped(x, name, dims=2):
     """x as an array, with its shape, which has to have so many dimensions."""
-    if not isinstance(x, np.ndarray) and not _is_tensor(x):
+    if _is_tensor(x):
+        x = _written_out(x)
+    elif not isinstance(x, np.ndarray):
         x = np.asarray(x)
     shape = x.shape
     if len(shape) != dims:

@@ -978,3 +978,34 @@ def test_lists_are_their_arrays():
                                                 lengths=turn(lengths))):
         for got, want in zip(call(lambda x: x.tolist()), call(lambda x: x)):
             np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("place", PLACES[1:])
+def test_views_that_negate(place):
+    """The imaginary part of a conjugate is a real tensor whose memory holds the other sign."""
+    rng = np.random.default_rng(22)
+
+    def turned(x):
+        x = _put(place, -np.asarray(x), "f32")
+        x = torch.complex(torch.zeros_like(x), x).conj().imag
+        assert x.is_neg()
+        return x
+
+    z = rng.standard_normal((6, 9)).astype(np.float32)
+    ids, logits, rest = _teacher(rng, 6, 9, 3, True)
+    weight = np.float32(0.5 + rng.random(6))
+    results = []
+    for f in (turned, lambda x: _put(place, x, "f32")):
+        teacher = (_put(place, ids, "i32"), f(logits), f(rest))
+        results.append([*ops.top_logits(f(z), 3),
+                        *ops.distill_gradients(f(z), teacher, weight=f(weight), loss=True,
+                                               hessian=True),
+                        ops.distill_loss(f(z), teacher, weight=f(weight))])
+        p = np.float32(_softmax(rng.standard_normal((6, 3, 9)))) if not results[1:] else p
+        u, v = (np.full((6, 2), 0.5), np.full(6, 0.5))
+        results[-1] += [*ops.verify_drafts(f(p), _put(place, ids[:, :2], "i32"),
+                                           f(p[:, ::-1][:, :2]), f(u), f(v))]
+        ds = lgb.Dataset(np.zeros((6, 1)), params={"min_data_in_bin": 1, "verbosity": -1},
+                         teacher=teacher).construct().get_teacher()
+        results[-1] += [torch.from_numpy(x) for x in ds]
+    _same(*results)
