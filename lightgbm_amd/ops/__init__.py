@@ -12,6 +12,7 @@ do. The functions record nothing for automatic differentiation: `distill_gradien
 backward pass of `distill_loss`.
 """
 import ctypes
+import operator
 import struct
 import sys
 from typing import Any, NamedTuple, Optional
@@ -64,6 +65,15 @@ _TOP = struct.Struct("@qiid" + "Pqqqii" * 4)
 _DISTILL = struct.Struct("@qiidd" + "Pqqqii" * 9)
 _VERIFY = struct.Struct("@qii" + "Pqqqii" * 8 + "Pq")
 _NONE = (0, 0, 0, 0, 0, 0)
+
+
+def _packed(form, *values):
+    """A call's arguments as the C ABI has them."""
+    try:
+        return form.pack(*values)
+    except struct.error as e:
+        raise LightGBMError(f"an argument is not of its kind, or out of range: {e}") from None
+
 
 for _f in (_LIB.LGBM_TopLogits, _LIB.LGBM_Distill, _LIB.LGBM_VerifyDrafts):
     _f.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
@@ -211,13 +221,18 @@ def top_logits(scores, k, temperature=1.0, rest=True):
     where = _Place(scores)
     x = _fields(scores, "scores")
     code = x[4]
-    k = int(k)
-    out_class, to_class = where.empty((rows, max(k, 0)), _I32)
-    out_logit, to_logit = where.empty((rows, max(k, 0)), code)
+    try:
+        k = operator.index(k)
+    except TypeError:
+        raise LightGBMError(f"k must be a whole number, got {k!r}") from None
+    if not 1 <= k <= min(classes, 256):
+        raise LightGBMError(f"k must be 1..{min(classes, 256)} for {classes} classes, got {k}")
+    out_class, to_class = where.empty((rows, k), _I32)
+    out_logit, to_logit = where.empty((rows, k), code)
     log_rest, to_rest = (where.empty((rows,), _F64 if code == _F64 else _F32) if rest
                          else (None, _NONE))
     _safe_call(_LIB.LGBM_TopLogits(
-        _TOP.pack(rows, classes, k, temperature, *x, *to_class, *to_logit, *to_rest),
+        _packed(_TOP, rows, classes, k, temperature, *x, *to_class, *to_logit, *to_rest),
         where.device, where.stream()))
     return TopLogits(out_class, out_logit, log_rest)
 
@@ -244,7 +259,7 @@ def _distill(scores, teacher, labels, weight, temperature, alpha, loss, gradient
     made_loss, to_loss = where.empty(row, _F64 if code == _F64 else _F32) if loss else absent
     made_grad, to_grad = where.scores(rows, classes, out, class_major) if gradient else absent
     made_hess, to_hess = where.scores(rows, classes, out, class_major) if hessian else absent
-    _safe_call(_LIB.LGBM_Distill(_DISTILL.pack(*fields, *to_loss, *to_grad, *to_hess),
+    _safe_call(_LIB.LGBM_Distill(_packed(_DISTILL, *fields, *to_loss, *to_grad, *to_hess),
                                  where.device, where.stream()))
     return made_loss, made_grad, made_hess
 
@@ -318,7 +333,7 @@ def verify_drafts(target_prob, drafts, draft_prob, accept_uniform, sample_unifor
         size = _WORKSPACE.get(plan)
         if size is None:
             need = ctypes.c_int64(0)
-            _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_VERIFY.pack(*fields, 0, 0),
+            _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_packed(_VERIFY, *fields, 0, 0),
                                                        ctypes.byref(need)))
             if len(_WORKSPACE) >= 1024:
                 _WORKSPACE.clear()
@@ -327,6 +342,6 @@ def verify_drafts(target_prob, drafts, draft_prob, accept_uniform, sample_unifor
             # freed to the caching allocator, which gives it out again in the stream's order
             space = _torch.empty((size,), dtype=_torch.uint8, device=where.on)
             scratch = space.data_ptr()
-    _safe_call(_LIB.LGBM_VerifyDrafts(_VERIFY.pack(*fields, scratch, size), where.device,
+    _safe_call(_LIB.LGBM_VerifyDrafts(_packed(_VERIFY, *fields, scratch, size), where.device,
                                       where.stream()))
     return VerifiedDrafts(out_class, out_accepted)

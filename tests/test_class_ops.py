@@ -1009,3 +1009,22 @@ def test_views_that_negate(place):
                          teacher=teacher).construct().get_teacher()
         results[-1] += [torch.from_numpy(x) for x in ds]
     _same(*results)
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_refuses_what_is_no_number(place):
+    """Whole numbers and numbers of other kinds than an argument's, and ones of no size."""
+    f = lambda *shape: _put(place, np.ones(shape, np.float32))  # noqa: E731
+    teacher = (_put(place, np.ones((3, 2), np.int32)), f(3, 2))
+    for k in (2.9, 2.0, "2", None, 10 ** 12, -1):
+        with pytest.raises(LightGBMError):
+            ops.top_logits(f(3, 4), k)
+    for bad in (None, "1", 1j, [1.0]):
+        with pytest.raises(LightGBMError):
+            ops.top_logits(f(3, 4), 1, temperature=bad)
+        with pytest.raises(LightGBMError):
+            ops.distill_loss(f(3, 4), teacher, temperature=bad)
+        with pytest.raises(LightGBMError):
+            ops.distill_gradients(f(3, 4), teacher, labels=teacher[0][:, 0], alpha=bad)
+    got = ops.top_logits(f(3, 4), np.int64(2), temperature=np.float32(1.5))
+    assert tuple(got.classes.shape) == (3, 2)
