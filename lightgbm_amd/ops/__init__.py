@@ -9,7 +9,8 @@ Arrays are numpy arrays or torch tensors. Tensors on a HIP device are used where
 work goes to the current stream of their device, nothing is copied and nothing waits, and the
 results are tensors of that device. Everything else is computed on the host. Any strides will
 do. The functions record nothing for automatic differentiation: `distill_gradients` is the
-backward pass of `distill_loss`.
+backward pass of `distill_loss`. A tensor that requires a gradient is refused where gradients are
+recorded (detach it, or call under `torch.no_grad()`), and so is one that carries a tangent.
 """
 import ctypes
 import operator
@@ -146,26 +147,34 @@ class _Place:
         """The six fields of an LGBM_Array of x, which has to be of this place and shape."""
         if x is None:
             return _NONE
+        given = x
         if _is_tensor(x):
             # -1: the host
             if x.get_device() != self.device or x.is_cuda != (self.device >= 0):
                 raise LightGBMError(f"{name} is on {x.device}, the first array on "
                                     f"{self.on or 'the host'}")
-            if x.is_neg():
-                self.made.append(x := _written_out(x))
+            x = _plain_tensor(x, name)
         elif self.device >= 0:
             raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
         elif not isinstance(x, np.ndarray):
             x = np.asarray(x)
+        if x is not given:
             self.made.append(x)
         if x.shape != shape:
             raise LightGBMError(f"{name} must have the shape {list(shape)}, got {list(x.shape)}")
         return _fields(x, name)
 
 
-def _written_out(x):
-    """A tensor whose memory holds its own values: a view that negates (the imaginary part of a
-    conjugate) is written out, on its device's current stream."""
+def _plain_tensor(x, name):
+    """A tensor that is no more than its memory's values: a view that negates (the imaginary part
+    of a conjugate) is written out, on its device's current stream; one whose gradient or tangent
+    would be lost is refused."""
+    if x.requires_grad and _torch.is_grad_enabled():
+        raise LightGBMError(f"{name} requires a gradient, and this function records none: detach "
+                            "it, or call under torch.no_grad()")
+    forward = _torch.autograd.forward_ad
+    if getattr(forward, "_current_level", 0) >= 0 and forward.unpack_dual(x).tangent is not None:
+        raise LightGBMError(f"{name} carries a tangent, which this function would lose")
     return x.resolve_neg() if x.is_neg() else x
 
 
@@ -197,7 +206,7 @@ def _fields(x, name):
 def _shaped(x, name, dims=2):
     """x as an array, with its shape, which has to have so many dimensions."""
     if _is_tensor(x):
-        x = _written_out(x)
+        x = _plain_tensor(x, name)
     elif not isinstance(x, np.ndarray):
         x = np.asarray(x)
     shape = x.shape

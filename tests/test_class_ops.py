@@ -1028,3 +1028,37 @@ def test_refuses_what_is_no_number(place):
             ops.distill_gradients(f(3, 4), teacher, labels=teacher[0][:, 0], alpha=bad)
     got = ops.top_logits(f(3, 4), np.int64(2), temperature=np.float32(1.5))
     assert tuple(got.classes.shape) == (3, 2)
+
+
+@pytest.mark.parametrize("place", PLACES[1:])
+def test_refuses_to_lose_gradients(place):
+    """Of each argument in turn, where gradients are recorded, and nowhere else."""
+    rng = np.random.default_rng(23)
+    p = np.float32(_softmax(rng.standard_normal((6, 3, 9))))
+    f32 = lambda x: _put(place, x, "f32")  # noqa: E731
+    ids = _put(place, rng.integers(0, 9, (6, 2)), "i32")
+    top = (f32(p[:, 0]),)
+    distill = (f32(p[:, 0]), f32(p[:, 0, :2]), f32(p[:, 0, 0]), f32(p[:, 0, 0]))
+    verify = (f32(p), f32(p[:, :2]), f32(p[:, 0, :2]), f32(p[:, 0, 0]))
+    calls = [(lambda z: ops.top_logits(z, 3), top),
+             (lambda z, t, r, w: ops.distill_loss(z, (ids, t, r), weight=w), distill),
+             (lambda z, t, r, w: ops.distill_gradients(z, (ids, t, r), weight=w, hessian=True),
+              distill),
+             (lambda p, q, u, v: ops.verify_drafts(p, ids, q, u, v), verify)]
+    forward = torch.autograd.forward_ad
+    for call, args in calls:
+        want = call(*args)
+        want = [want] if torch.is_tensor(want) else [x for x in want if x is not None]
+        for i in range(len(args)):
+            asking = [x.clone().requires_grad_(i == j) for j, x in enumerate(args)]
+            with pytest.raises(LightGBMError):
+                call(*asking)
+            for quiet in (torch.no_grad, torch.inference_mode):
+                with quiet():
+                    got = call(*asking)
+                _same([got] if torch.is_tensor(got) else [x for x in got if x is not None], want)
+            with forward.dual_level():
+                dual = [forward.make_dual(x, x) if i == j else x for j, x in enumerate(args)]
+                with pytest.raises(LightGBMError):
+                    call(*dual)
+                call(*args)
