@@ -38,6 +38,8 @@ class ObjectiveFunction {
   }
   virtual bool IsRenewTreeOutput() const { return NeedRenewTreeOutput(); }
   virtual data_size_t NumPositiveData() const { return 0; }
+  /*! the temperature and alpha that a distillation objective was made with */
+  virtual void DistillTerms(double* /*temperature*/, double* /*alpha*/) const {}
   /*! average output flag (RF / some objectives) */
   virtual bool average_output() const { return false; }
 

@@ -3198,9 +3198,12 @@ void HIPTreeLearner::DeviceBoosting(const ObjectiveFunction* obj) {
                        num_class_score_, d_grad_.ptr, d_hess_.ptr);
   } else if (name == "distill") {
     const Metadata& meta = train_data_->metadata();
-    LGBM_DistillArgs a = class_ops::DistillArgsOf(meta, n, num_class_score_,
-                                                  config_->distill_temperature,
-                                                  config_->distill_alpha, d_score_.ptr);
+    // the objective's own, as its start, the metric and the model text have them: the
+    // configuration's may have been reset since
+    double temperature = 1.0, alpha = 1.0;
+    obj->DistillTerms(&temperature, &alpha);
+    LGBM_DistillArgs a = class_ops::DistillArgsOf(meta, n, num_class_score_, temperature, alpha,
+                                                  d_score_.ptr);
     if (meta.teacher_version() != teacher_version_) UploadTeacher(meta);
     a.teacher_class.data = d_teacher_class_.ptr;
     a.teacher_logit.data = d_teacher_logit_.ptr;

@@ -521,6 +521,10 @@ class Distill : public ObjectiveFunction {
     for (int c = 0; c < num_class_; ++c) sum += out[c] = std::exp(in[c] - mx);
     for (int c = 0; c < num_class_; ++c) out[c] /= sum;
   }
+  void DistillTerms(double* temperature, double* alpha) const override {
+    *temperature = temperature_;
+    *alpha = alpha_;
+  }
   const char* GetName() const override { return "distill"; }
   std::string ToString() const override {
     std::stringstream ss;

@@ -262,3 +262,26 @@ def test_shards_refuse_a_new_teacher():
     ds.set_teacher(ops.top_logits(-raw, 3))
     with pytest.raises(LightGBMError):
         live.update()
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_a_booster_keeps_the_loss_it_was_made_with(place):
+    """Resetting the objective's parameters while it trains changes neither the gradients nor
+    what the model text says of them."""
+    X, raw, y = _data()
+    top = ops.top_logits(raw, 3, temperature=2.0)
+    preds = []
+    for new in ({}, {"distill_alpha": 0.1, "distill_temperature": 5.0}):
+        live = lgb.Booster(_params(place, distill_temperature=2.0, distill_alpha=0.9),
+                           lgb.Dataset(X, label=y, teacher=top))
+        live.update()
+        if new:
+            live.reset_parameter(new)
+        for _ in range(3):
+            live.update()
+        preds.append(live.predict(X, raw_score=True))
+        assert "distill_temperature:2 distill_alpha:0.9" in live.model_to_string().replace(
+            "0.90000000000000002", "0.9")
+    d = np.abs(preds[0] - preds[1])
+    # on the device histograms of atomics move a leaf by some 1e-6 of it unless a split is a tie
+    assert np.quantile(d, 0.99) <= (0 if place == "cpu" else 1e-4)
