@@ -2643,10 +2643,10 @@ class HIPTreeLearner : public TreeLearner {
   int num_queries_ = 0;
   DevBuf<double> d_score_;
   DevBuf<float> d_label_, d_weight_;
-  // the distill objective's teacher, and the version of the dataset's that it is
+  // the distill objective's teacher, and the version of the dataset's that it is (-1: none yet)
   DevBuf<int32_t> d_teacher_class_;
   DevBuf<float> d_teacher_logit_, d_teacher_rest_;
-  int teacher_version_ = 0;
+  int teacher_version_ = -1;
   DevBuf<uint32_t> d_idx_, d_idx_tmp_;
   DevBuf<uint8_t> d_marks_;
   DevBuf<int> d_block_cnt_, d_block_loff_, d_block_roff_;
@@ -2991,7 +2991,7 @@ void HIPTreeLearner::Init(const Dataset* train_data, bool is_constant_hessian) {
   d_label_.Alloc(num_data_);
   HIP_OK(hipMemcpy(d_label_.ptr, train_data->metadata().label(), sizeof(float) * num_data_,
                    hipMemcpyHostToDevice));
-  UploadTeacher(train_data->metadata());
+  teacher_version_ = -1;
   weights_present_ = train_data->metadata().weights() != nullptr;
   if (weights_present_) {
     d_weight_.Alloc(num_data_);
@@ -3154,8 +3154,6 @@ void HIPTreeLearner::UploadGradients(const score_t* g, const score_t* h) {
 
 void HIPTreeLearner::UploadTeacher(const Metadata& meta) {
   teacher_version_ = meta.teacher_version();
-  if (meta.teacher_slots() == 0) return;
-  meta.CheckTeacher();
   const size_t count = static_cast<size_t>(num_data_) * meta.teacher_slots();
   HIP_OK(hipStreamSynchronize(stream_));  // an iteration may still read the one before
   d_teacher_class_.Alloc(count);

@@ -285,3 +285,28 @@ def test_a_booster_keeps_the_loss_it_was_made_with(place):
     d = np.abs(preds[0] - preds[1])
     # on the device histograms of atomics move a leaf by some 1e-6 of it unless a split is a tie
     assert np.quantile(d, 0.99) <= (0 if place == "cpu" else 1e-4)
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_other_objectives_do_not_look_at_the_teacher(place):
+    """Not at one whose logits are missing either."""
+    X, raw, y = _data()
+    ds = lgb.Dataset(X, label=y).construct()
+    ds.set_field("teacher_class", np.zeros((600, 2), np.int32))
+    bst = lgb.train(_params(place, objective="multiclass"), ds, 2)
+    plain = lgb.train(_params(place, objective="multiclass"), lgb.Dataset(X, label=y), 2)
+    d = np.abs(bst.predict(X, raw_score=True) - plain.predict(X, raw_score=True))
+    assert np.quantile(d, 0.99) <= (0 if place == "cpu" else 1e-4)
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_other_training_data_bring_their_teacher(place):
+    """Two data sets of as many changes to their teachers, one given in the other's place."""
+    X, raw, y = _data()
+    top, new = ops.top_logits(raw, 3), ops.top_logits(-raw, 3)
+    params = _params(place, boost_from_average=False)
+    live = lgb.Booster(params, lgb.Dataset(X, label=y, teacher=top))
+    live.update(train_set=lgb.Dataset(X, label=y, teacher=new))
+    other = lgb.train(params, lgb.Dataset(X, label=y, teacher=new), 1)
+    d = live.predict(X, raw_score=True) - other.predict(X, raw_score=True)
+    assert np.quantile(np.abs(d), 0.99) < 1e-4
