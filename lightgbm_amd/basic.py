@@ -556,14 +556,14 @@ class Dataset:
         return self
 
     def get_teacher(self):
-        """The teacher as ops.TopLogits of numpy arrays, or None."""
+        """The teacher as ops.TopLogits of numpy arrays, or None: also where of its fields only
+        one of classes and logits is set, or they have not the same number of slots."""
         from .ops import TopLogits
-        classes = self.get_field("teacher_class")
-        if classes is None:
+        classes, logits = self.get_field("teacher_class"), self.get_field("teacher_logit")
+        if classes is None or logits is None or classes.size != logits.size:
             return None
         rows = self.num_data()
-        return TopLogits(classes.reshape(rows, -1),
-                         self.get_field("teacher_logit").reshape(rows, -1),
+        return TopLogits(classes.reshape(rows, -1), logits.reshape(rows, -1),
                          self.get_field("teacher_log_rest"))
 
     def set_init_score(self, init_score):

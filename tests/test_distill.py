@@ -310,3 +310,18 @@ def test_other_training_data_bring_their_teacher(place):
     other = lgb.train(params, lgb.Dataset(X, label=y, teacher=new), 1)
     d = live.predict(X, raw_score=True) - other.predict(X, raw_score=True)
     assert np.quantile(np.abs(d), 0.99) < 1e-4
+
+
+def test_half_a_teacher_is_none():
+    X, raw, y = _data(60)
+    top = ops.top_logits(raw, 3)
+    for fields in (("teacher_class",), ("teacher_logit",), ("teacher_log_rest",)):
+        ds = lgb.Dataset(X, label=y).construct()
+        for name, part in zip(("teacher_class", "teacher_logit", "teacher_log_rest"), top):
+            if name in fields:
+                ds.set_field(name, part)
+        assert ds.get_teacher() is None
+    ds.set_teacher(top)
+    assert ds.get_teacher() is not None
+    ds.set_field("teacher_logit", top.logits[:, :2])
+    assert ds.get_teacher() is None
