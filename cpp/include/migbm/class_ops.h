@@ -15,7 +15,7 @@
 namespace migbm {
 namespace class_ops {
 
-constexpr int kMaxTop = 256;            //!< largest number of top logits a row may have
+constexpr int kMaxTop = kMaxTeacherSlots;  //!< largest number of top logits a row may have
 constexpr int kMaxClasses = 1 << 20;    //!< largest number of classes
 constexpr int kMaxDrafts = 1024;        //!< largest number of drafted classes a sequence may have
 

@@ -20,6 +20,8 @@
 namespace migbm {
 
 /*! Per-row ancillary data. Parity: reference Metadata (dataset.h:48-400). */
+constexpr int kMaxTeacherSlots = 256;  //!< largest number of top logits a row's teacher may have
+
 class Metadata {
  public:
   void Init(data_size_t num_data, bool has_weight, bool has_query);

@@ -62,6 +62,9 @@ static void CheckTeacherLength(const char* what, int64_t n, data_size_t rows) {
   if (rows <= 0 || n % rows != 0)
     Log::Fatal("Length of %s (%lld) is no multiple of the number of rows (%d)", what,
                static_cast<long long>(n), rows);
+  if (n / rows > kMaxTeacherSlots)
+    Log::Fatal("A teacher has 1..%d slots a row, got %lld of %s", kMaxTeacherSlots,
+               static_cast<long long>(n / rows), what);
 }
 
 void Metadata::SetTeacherClass(const int32_t* p, int64_t n) {
@@ -1406,7 +1409,7 @@ std::unique_ptr<Dataset> Dataset::LoadFromBinFile(const char* filename) {
   }
   int32_t slots = 0;
   if (fread(&slots, sizeof(slots), 1, fp) == 1) {
-    MIGBM_CHECK(slots > 0 && slots <= 256);
+    MIGBM_CHECK(slots > 0 && slots <= kMaxTeacherSlots);
     uint8_t has_rest;
     MIGBM_CHECK_EQ(fread(&has_rest, 1, 1, fp), 1u);
     const size_t n = static_cast<size_t>(slots) * d->num_data_;

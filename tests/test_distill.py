@@ -325,3 +325,16 @@ def test_half_a_teacher_is_none():
     assert ds.get_teacher() is not None
     ds.set_field("teacher_logit", top.logits[:, :2])
     assert ds.get_teacher() is None
+
+
+def test_too_many_slots_are_refused_at_once(tmp_path):
+    """Not only when the objective looks at them, or a binary file with them is read."""
+    X, raw, y = _data(60)
+    ds = lgb.Dataset(X, label=y).construct()
+    for name, kind in (("teacher_class", np.int32), ("teacher_logit", np.float32)):
+        with pytest.raises(LightGBMError):
+            ds.set_field(name, np.zeros((60, 257), kind))
+        ds.set_field(name, np.zeros((60, 256), kind))
+    ds.save_binary(str(tmp_path / "t.bin"))
+    back = lgb.Dataset(str(tmp_path / "t.bin")).construct().get_teacher()
+    assert back.classes.shape == (60, 256)
