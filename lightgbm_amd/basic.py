@@ -437,7 +437,11 @@ class Dataset:
         elif field_name in ("teacher_class", "teacher_logit", "teacher_log_rest"):
             self.construct()
             kind = np.int32 if field_name == "teacher_class" else np.float32
-            arr = np.ascontiguousarray(np.asarray(data).ravel(), dtype=kind)
+            arr = np.asarray(data).ravel()
+            if kind is np.int32:
+                # ids that 32 bits do not hold are no classes
+                arr = np.where((arr >= 0) & (arr <= np.iinfo(kind).max), arr, -1)
+            arr = np.ascontiguousarray(arr, dtype=kind)
             _safe_call(_LIB.LGBM_DatasetSetField(
                 self._handle, _c_str(field_name), arr.ctypes.data_as(ctypes.c_void_p),
                 ctypes.c_int(len(arr)),
@@ -547,9 +551,6 @@ class Dataset:
                                 f"got {list(rest.shape)}")
         if classes.size > np.iinfo(np.int32).max:
             raise LightGBMError(f"a teacher of {classes.size} logits is too large for a Dataset")
-        # ids that 32 bits do not hold are no classes
-        big = np.iinfo(np.int32).max
-        classes = np.where((classes >= 0) & (classes <= big), classes, -1)
         self.set_field("teacher_class", classes)
         self.set_field("teacher_logit", logits)
         self.set_field("teacher_log_rest", rest)

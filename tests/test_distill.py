@@ -338,3 +338,14 @@ def test_too_many_slots_are_refused_at_once(tmp_path):
     ds.save_binary(str(tmp_path / "t.bin"))
     back = lgb.Dataset(str(tmp_path / "t.bin")).construct().get_teacher()
     assert back.classes.shape == (60, 256)
+
+
+def test_ids_beyond_32_bits_are_no_classes():
+    X, raw, y = _data(60)
+    wide = np.tile([2 ** 32 + 1, 3, -2 ** 32], (60, 1))
+    for give in (lambda ds: ds.set_field("teacher_class", wide),
+                 lambda ds: ds.set_teacher((wide, np.zeros((60, 3))))):
+        ds = lgb.Dataset(X, label=y).construct()
+        give(ds)
+        got = ds.get_field("teacher_class").reshape(60, 3)
+        np.testing.assert_array_equal(got, np.tile([-1, 3, -1], (60, 1)))
