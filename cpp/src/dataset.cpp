@@ -1077,22 +1077,26 @@ std::unique_ptr<Dataset> Dataset::Subset(const data_size_t* indices, data_size_t
     for (data_size_t i = 0; i < n; ++i) pos[i] = metadata_.positions()[indices[i]];
     d->metadata_.SetPosition(pos.data(), n);
   }
-  if (const int k = metadata_.teacher_slots(); k > 0) {
-    metadata_.CheckTeacher();
-    std::vector<int32_t> cls(static_cast<size_t>(n) * k);
-    std::vector<float> logit(cls.size());
-    for (data_size_t i = 0; i < n; ++i) {
-      const size_t from = static_cast<size_t>(indices[i]) * k, to = static_cast<size_t>(i) * k;
-      std::copy_n(metadata_.teacher_class() + from, k, cls.begin() + to);
-      std::copy_n(metadata_.teacher_logit() + from, k, logit.begin() + to);
-    }
+  // a teacher's arrays, each as far as it is set
+  auto rows_of = [&](const auto* from, int64_t width) {
+    std::vector<std::remove_const_t<std::remove_pointer_t<decltype(from)>>> to;
+    to.reserve(static_cast<size_t>(n) * width);
+    for (data_size_t i = 0; i < n; ++i)
+      to.insert(to.end(), from + indices[i] * width, from + (indices[i] + 1) * width);
+    return to;
+  };
+  const Metadata& from = metadata_;
+  if (from.teacher_class() != nullptr) {
+    const auto cls = rows_of(from.teacher_class(), from.teacher_slots());
     d->metadata_.SetTeacherClass(cls.data(), static_cast<int64_t>(cls.size()));
+  }
+  if (from.teacher_logit() != nullptr) {
+    const auto logit = rows_of(from.teacher_logit(), from.num_teacher_logit() / num_data_);
     d->metadata_.SetTeacherLogit(logit.data(), static_cast<int64_t>(logit.size()));
-    if (metadata_.teacher_rest() != nullptr) {
-      std::vector<float> rest(n);
-      for (data_size_t i = 0; i < n; ++i) rest[i] = metadata_.teacher_rest()[indices[i]];
-      d->metadata_.SetTeacherRest(rest.data(), n);
-    }
+  }
+  if (from.teacher_rest() != nullptr) {
+    const auto rest = rows_of(from.teacher_rest(), 1);
+    d->metadata_.SetTeacherRest(rest.data(), n);
   }
   return d;
 }
@@ -1256,6 +1260,10 @@ void Dataset::PushRawRow(data_size_t row, const double* values, int ncol) {
 static const char kBinMagic[] = "migbm.dataset.v1";
 
 void Dataset::SaveBinaryFile(const char* filename) const {
+  // a file holds a whole teacher or none
+  if (metadata_.teacher_class() != nullptr || metadata_.teacher_logit() != nullptr ||
+      metadata_.teacher_rest() != nullptr)
+    metadata_.CheckTeacher();
   FILE* fp = fopen(filename, "wb");
   if (!fp) Log::Fatal("Cannot open %s for writing", filename);
   fwrite(kBinMagic, 1, sizeof(kBinMagic), fp);
@@ -1311,7 +1319,6 @@ void Dataset::SaveBinaryFile(const char* filename) const {
   }
   // a teacher follows where there is one: slots a row, whether the rest is known, the arrays
   if (const int32_t slots = metadata_.teacher_slots(); slots > 0) {
-    metadata_.CheckTeacher();
     const uint8_t has_rest = metadata_.teacher_rest() != nullptr;
     const size_t n = static_cast<size_t>(slots) * num_data_;
     fwrite(&slots, sizeof(slots), 1, fp);

@@ -349,3 +349,26 @@ def test_ids_beyond_32_bits_are_no_classes():
         give(ds)
         got = ds.get_field("teacher_class").reshape(60, 3)
         np.testing.assert_array_equal(got, np.tile([-1, 3, -1], (60, 1)))
+
+
+def test_half_a_teacher_travels_as_far_as_it_can(tmp_path):
+    """A subset has what is set; a binary file, which has whole teachers only, is refused before
+    anything is written."""
+    X, raw, y = _data(60)
+    top = ops.top_logits(raw, 3)
+    names = ("teacher_class", "teacher_logit", "teacher_log_rest")
+    for name, part in zip(names, top):
+        ds = lgb.Dataset(X, label=y, free_raw_data=False).construct()
+        ds.set_field(name, part)
+        sub = ds.subset(np.arange(0, 60, 7))
+        for other in names:
+            got = sub.get_field(other)
+            if other == name:
+                np.testing.assert_array_equal(
+                    got, np.asarray(part[::7], got.dtype).ravel())
+            else:
+                assert got is None
+        path = tmp_path / f"{name}.bin"
+        with pytest.raises(LightGBMError):
+            ds.save_binary(str(path))
+        assert not path.exists()
