@@ -464,9 +464,10 @@ class Distill : public ObjectiveFunction {
     a.scores.data = a.loss.data = &a;  // checked for presence alone
     a.loss.type = C_API_DTYPE_FLOAT64;
     class_ops::Check(a);
-    // where the boosting starts: the mean over the rows of what the scores are to reach. What
-    // the teacher leaves unnamed is shared evenly, a row without a teacher counts evenly too.
-    start_.assign(num_class_, 0.0);
+    // where the boosting starts: the scores that suit the mean over the rows of what the teacher
+    // and the labels want. What the teacher leaves unnamed is shared evenly, a row without a
+    // teacher counts evenly too.
+    std::vector<double> soft(num_class_, 0.0), hard(num_class_, 0.0);
     std::vector<double> p(a.k);
     std::vector<char> named(num_class_);
     double sum_w = 0;
@@ -495,16 +496,19 @@ class Distill : public ObjectiveFunction {
       if (!(sum > 0) || !std::isfinite(sum)) continue;
       sum_w += w;
       for (int j = 0; j < a.k; ++j)
-        if (p[j] > 0) start_[cls[j]] += w * alpha_ * p[j] / sum;
+        if (p[j] > 0) soft[cls[j]] += w * p[j] / sum;
       const int others = num_class_ - n;
       if (others > 0)
         for (int c = 0; c < num_class_; ++c)
-          if (!named[c]) start_[c] += w * alpha_ * rest / sum / others;
+          if (!named[c]) soft[c] += w * rest / sum / others;
       const int y = alpha_ < 1.0 ? static_cast<int>(meta.label()[i]) : -1;
-      if (y >= 0 && y < num_class_) start_[y] += w * (1.0 - alpha_);
+      if (y >= 0 && y < num_class_) hard[y] += w;
     }
-    for (double& s : start_)
-      s = std::log(std::max(kEpsilon, sum_w > 0 ? s / sum_w : 1.0 / num_class_));
+    for (int c = 0; c < num_class_; ++c) {
+      soft[c] = sum_w > 0 ? soft[c] / sum_w : 1.0 / num_class_;
+      hard[c] = sum_w > 0 ? hard[c] / sum_w : 0.0;
+    }
+    SetStart(soft, hard);
   }
   void GetGradients(const double* score, score_t* grad, score_t* hess) const override {
     LGBM_DistillArgs a = Args(score);
@@ -537,6 +541,58 @@ class Distill : public ObjectiveFunction {
  private:
   LGBM_DistillArgs Args(const double* score) const {
     return class_ops::DistillArgsOf(*meta_, num_data_, num_class_, temperature_, alpha_, score);
+  }
+
+  /*!
+   * The constant scores b that minimise the loss against mean targets: with Q = softmax(b / T)
+   * and p = softmax(b), for every class
+   *   alpha T Q_c + (1 - alpha) L p_c = m_c = alpha T soft_c + (1 - alpha) hard_c,
+   * L being the sum of hard. At T = 1, or with one of the terms alone, that is a logarithm.
+   * Otherwise b is shifted until Q_c = exp(b_c / T), so that
+   *   alpha T exp(b_c / T) + B exp(b_c) = m_c
+   * has one unknown for all classes, B. It is bisected for the sum of Q to be one; the logarithm
+   * of the left side is convex in b_c, so that Newton's steps come down to the root from where
+   * one of the two terms alone is m_c.
+   */
+  void SetStart(const std::vector<double>& soft, const std::vector<double>& hard) {
+    const int n = num_class_;
+    const double t = temperature_, labelled = std::accumulate(hard.begin(), hard.end(), 0.0);
+    start_.resize(n);
+    if (t == 1.0 || alpha_ == 0.0) {
+      for (int c = 0; c < n; ++c)
+        start_[c] = std::log(std::max(kEpsilon, alpha_ * soft[c] + (1.0 - alpha_) * hard[c]));
+      return;
+    }
+    if (alpha_ == 1.0 || !(labelled > 0)) {
+      for (int c = 0; c < n; ++c) start_[c] = t * std::log(std::max(kEpsilon, soft[c]));
+      return;
+    }
+    const double log_a = std::log(alpha_ * t), hard_term = (1.0 - alpha_) * labelled;
+    std::vector<double> log_m(n);
+    for (int c = 0; c < n; ++c)
+      log_m[c] = std::log(std::max(kEpsilon * (alpha_ * t + hard_term),
+                                   alpha_ * t * soft[c] + (1.0 - alpha_) * hard[c]));
+    // p's own sum of exponentials is between that of the largest class alone, at least
+    // exp(-T log n), and n
+    double low = std::log(hard_term) - std::log(n), high = std::log(hard_term) + t * std::log(n);
+    for (int turn = 0; turn < 200 && high - low > 1e-14 * (1.0 + std::fabs(low)); ++turn) {
+      const double log_b = 0.5 * (low + high);
+      double sum = 0;
+      for (int c = 0; c < n; ++c) {
+        double x = std::min(t * (log_m[c] - log_a), log_m[c] - log_b);
+        for (int step = 0; step < 50; ++step) {
+          const double u = log_a + x / t, v = log_b + x, top = std::max(u, v);
+          const double eu = std::exp(u - top), ev = std::exp(v - top);
+          const double move = (top + std::log(eu + ev) - log_m[c]) * (eu + ev) / (eu / t + ev);
+          x -= move;
+          if (!(move > 1e-14 * (1.0 + std::fabs(x)))) break;
+        }
+        start_[c] = x;
+        sum += std::exp(x / t);
+      }
+      if (sum > 1.0) low = log_b;
+      else high = log_b;
+    }
   }
 
   data_size_t num_data_ = 0;

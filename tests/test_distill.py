@@ -372,3 +372,37 @@ def test_half_a_teacher_travels_as_far_as_it_can(tmp_path):
         with pytest.raises(LightGBMError):
             ds.save_binary(str(path))
         assert not path.exists()
+
+
+def _start(teacher, y, classes, t, alpha):
+    """A new booster's constant scores, its trees shrunk to nothing; and the dataset's teacher."""
+    X = np.random.RandomState(9).randn(len(y), 3)
+    ds = lgb.Dataset(X, label=y, teacher=teacher)
+    bst = lgb.train(_params("cpu", classes, learning_rate=1e-12, distill_temperature=t,
+                            distill_alpha=alpha), ds, 1)
+    return bst.predict(X[:1], raw_score=True)[0], ds.get_teacher()
+
+
+@pytest.mark.parametrize("t", [0.25, 1.0, 4.0, 100.0])
+@pytest.mark.parametrize("alpha", [1.0, 0.9, 0.3, 1e-6, 0.0])
+def test_starts_where_the_mean_gradient_is_zero(t, alpha):
+    """The gradients are of size T and rounded to 32 bits; the trees move a score by 1e-12 times a
+    leaf of at most some units times T, and a gradient by no more than that."""
+    _, raw, y = _data(400, 7, seed=4)
+    b, teacher = _start(ops.top_logits(raw, 4, temperature=t)[:2], y, 7, t, alpha)
+    grad = ops.distill_gradients(np.tile(b, (400, 1)), teacher, labels=y.astype(np.int32),
+                                 temperature=t, alpha=alpha).gradient
+    mean = grad.astype(np.float64).mean(0)
+    assert np.all(np.abs(mean) <= 2 * max(t, 1.0) * 2.0 ** -24 + 1e-10 * max(t, 1.0))
+
+
+def test_starts_at_the_mean_of_the_teacher_at_its_temperature():
+    """With the teacher alone the start's softmax at T is the mean of its probabilities."""
+    _, raw, y = _data(50)
+    b, top = _start(ops.top_logits(raw, 2, temperature=4.0), y, 5, 4.0, 1.0)
+    want = np.zeros((50, 5))
+    for i in range(50):
+        norm = np.logaddexp(np.logaddexp.reduce(top.logits[i] / 4.0), top.log_rest[i])
+        want[i] = np.exp(top.log_rest[i] - norm) / 3
+        want[i, top.classes[i]] = np.exp(top.logits[i] / 4.0 - norm)
+    np.testing.assert_allclose(np.exp(b / 4) / np.exp(b / 4).sum(), want.mean(0), rtol=1e-6)
