@@ -233,7 +233,7 @@ void DistillHost(const LGBM_DistillArgs& a) {
       const double r = rest ? LoadFloat(a.teacher_rest, i * a.teacher_rest.stride[0]) : -kInf;
       log_p[n] = r;
       const double norm = LogSumExp(log_p.data(), n + 1);
-      bool nan = std::isnan(r);
+      bool nan = std::isnan(r) || norm == kInf;  // of infinite weights none is a share
       for (int j = 0; j < n; ++j) nan |= std::isnan(log_p[j]);
       const double lse = nan ? std::nan("") : norm;
       const bool taught = nan || norm > -kInf;
@@ -276,7 +276,7 @@ void DistillHost(const LGBM_DistillArgs& a) {
           if (taught && alpha > 0) {
             const double q = e[j] / total;
             const double other = own == high ? e[j] : std::exp((z[j] - own) / t);
-            g = alpha * t * (q - (slot[j] >= 0 ? p[slot[j]] : ratio > 0 ? ratio * other : 0.0));
+            g = alpha * t * (q - (slot[j] >= 0 ? p[slot[j]] : ratio == 0 ? 0.0 : ratio * other));
             h = alpha * q * (1 - q);
           }
           if (labelled) {

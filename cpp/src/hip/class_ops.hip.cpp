@@ -969,7 +969,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   __syncthreads();
   auto put = [&](int at, A v, A p, A from, bool spread_it) {
     const A q = Exp2(Fma(v, scale, off)) * inv;
-    if (spread_it) p = spread > A(0) ? spread * Exp2(Fma(v, scale, from)) : A(0);
+    if (spread_it) p = spread == A(0) ? A(0) : spread * Exp2(Fma(v, scale, from));
     A g = soft > A(0) ? soft * temp * (q - p) : A(0);
     if (hard > A(0))
       g += hard * (Exp2(Fma(v, scale1, off1)) * inv1 - (at == label ? A(1) : A(0)));

@@ -1062,3 +1062,39 @@ def test_refuses_to_lose_gradients(place):
                 with pytest.raises(LightGBMError):
                     call(*dual)
                 call(*args)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 150, 5000])
+def test_distill_teacher_of_no_number(place, classes):
+    """NaN or +inf among a teacher's logits, or as its rest, makes NaN of all that its row wants:
+    of the slots, and of the other classes where it speaks of them. Other rows keep theirs."""
+    rng = np.random.default_rng(24)
+    z = rng.standard_normal((5, classes))
+    ids = np.tile([1, 0, 2], (5, 1))
+    logits = np.tile(np.float32([3, 2, 1]), (5, 1))
+    rest = np.full(5, 0.5, np.float32)
+    clean = logits.copy(), rest.copy()
+    logits[0, 1], logits[1, 0], rest[2], rest[3] = np.nan, INF, np.nan, INF
+    labels = np.full(5, 4)
+    for dtype in _types(place):
+        for order in "CF":
+            for alpha in (1.0, 0.5):
+                for with_rest in (True, False):
+                    def call(t, r):
+                        got = ops.distill_gradients(
+                            _put(place, z, dtype, order),
+                            (_put(place, ids, "i32"), _put(place, t, "f32"),
+                             _put(place, r, "f32") if with_rest else None),
+                            labels=_put(place, labels, "i32"), alpha=alpha, loss=True)
+                        return _get(got.gradient), _get(got.loss)
+                    grad, loss = call(logits, rest)
+                    want, want_loss = call(*clean)
+                    bad = 4 if with_rest else 2
+                    assert np.all(np.isnan(loss[:bad])) and np.all(np.isnan(grad[:bad, :3]))
+                    if with_rest:
+                        assert np.all(np.isnan(grad[:bad]))
+                    else:
+                        np.testing.assert_array_equal(grad[:bad, 3:], want[:bad, 3:])
+                    np.testing.assert_array_equal(grad[bad:], want[bad:])
+                    np.testing.assert_array_equal(loss[bad:], want_loss[bad:])
