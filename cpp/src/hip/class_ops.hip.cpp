@@ -4,9 +4,11 @@
  *
  * A row (or a sequence) belongs to a few lanes, a wave or a workgroup, by its number of classes
  * and by which of its strides is the smaller. Everything is held in 32 bits (64 for float64
- * scores); exponentials are taken to base two of one fused multiply-add,
- *   exp((z - high) / T) = 2^(z * s - high * s),  s = log2(e) / T,
- * whose rounding of high * s is a factor common to the row and cancels in every quotient.
+ * scores); exponentials are taken to base two,
+ *   exp((z - high) / T) = 2^((z - high) * s),  s = log2(e) / T,
+ * of a difference that is formed first: z * s - high * s would be one operation, but high * s may
+ * not be a number (masks of the type's lowest value) or be off by more than the exponent's range
+ * (large scores at a small T), and is another factor wherever another maximum stands for high.
  */
 #include <hip/hip_runtime.h>
 
@@ -43,7 +45,6 @@ __device__ __forceinline__ double Exp2(double x) { return exp2(x); }
 __device__ __forceinline__ float Log2(float x) { return log2f(x); }
 __device__ __forceinline__ double Log2(double x) { return log2(x); }
 __device__ __forceinline__ float Fma(float a, float b, float c) { return fmaf(a, b, c); }
-__device__ __forceinline__ double Fma(double a, double b, double c) { return fma(a, b, c); }
 __device__ __forceinline__ float Max(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double Max(double a, double b) { return fmax(a, b); }
 
@@ -211,15 +212,14 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
   const A t_high = t_high_or > NegInf<A>() ? t_high_or : A(0);
 
   // sums
-  const A off = -high * scale, off1 = -high * scale1;
   const A z_slot = cls >= 0 ? static_cast<A>(z[cls * zs]) : NegInf<A>();
-  const A log_e = Fma(z_slot, scale, off);
+  const A log_e = (z_slot - high) * scale;
   const A e_slot = cls >= 0 ? Exp2(log_e) : A(0);
   A left = 0, total1 = 0;
   for (int i = tid; i < c; i += kBlock) {
     const A v = static_cast<A>(z[i * zs]);
-    if (!(mark[i >> 5] >> (i & 31) & 1u)) left += Exp2(Fma(v, scale, off));
-    if (alpha < A(1)) total1 += Exp2(Fma(v, scale1, off1));
+    if (!(mark[i >> 5] >> (i & 31) & 1u)) left += Exp2((v - high) * scale);
+    if (alpha < A(1)) total1 += Exp2((v - high) * scale1);
   }
   left = BlockSum<kBlock>(left, s_red[0]);
   const A total = left + BlockSum<kBlock>(e_slot, s_red[2]);
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
   const A t_sum = BlockSum<kBlock>(u, s_red[4]) + u_rest;
   const A log_total = Log2(total);
   const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
-  A log_left = Log2(left), rest_off = off;
+  A log_left = Log2(left), rest_high = high;
   bool again = rest && left < SmallRest<A>();
   if (again) {
     A own = NegInf<A>();
@@ -238,13 +238,13 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
     own = BlockMax<kBlock>(own, s_red[1]);
     again = own > NegInf<A>();
     if (again) {
-      rest_off = -own * scale;
+      rest_high = own;
       left = 0;
       for (int i = tid; i < c; i += kBlock)
         if (!(mark[i >> 5] >> (i & 31) & 1u))
-          left += Exp2(Fma(static_cast<A>(z[i * zs]), scale, rest_off));
+          left += Exp2((static_cast<A>(z[i * zs]) - own) * scale);
       left = BlockSum<kBlock>(left, s_red[5]);
-      log_left = Log2(left) - rest_off + off;
+      log_left = Log2(left) + (own - high) * scale;
     }
   }
   const int y = alpha < A(1) ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
       A v = taught ? alpha * temp * temp * (kl * static_cast<A>(kLn2)) : A(0);
       if (y >= 0)
         v += (A(1) - alpha) * static_cast<A>(kLn2) *
-             (Log2(total1) - Fma(static_cast<A>(z[y * zs]), scale1, off1));
+             (Log2(total1) - (static_cast<A>(z[y * zs]) - high) * scale1);
       StoreFloat(a.loss, row * a.loss.stride[0], v * w);
     }
   }
@@ -272,13 +272,13 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
   const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
   // P_c of the classes without a slot is written with the row, that of a slot by its thread
   auto put = [&](int i, A v, A want, bool spread_it) {
-    const A e = Exp2(Fma(v, scale, off));
+    const A e = Exp2((v - high) * scale);
     const A q = e * inv;
-    if (spread_it) want = spread * (again ? Exp2(Fma(v, scale, rest_off)) : e);
+    if (spread_it) want = spread * (again ? Exp2((v - rest_high) * scale) : e);
     A g = soft > A(0) ? soft * temp * (q - want) : A(0);
     A h = soft > A(0) ? soft * q * (A(1) - q) : A(0);
     if (hard > A(0)) {
-      const A q1 = Exp2(Fma(v, scale1, off1)) * inv1;
+      const A q1 = Exp2((v - high) * scale1) * inv1;
       g += hard * (q1 - (i == y ? A(1) : A(0)));
       h += hard * q1 * (A(1) - q1);
     }
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   const S temp = static_cast<S>(a.temperature), alpha = static_cast<S>(a.alpha);
   const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
   // exponents are formed as the scores are held, and taken as the statistics are
-  auto exponent = [](A v, A by, A from) { return static_cast<S>(Fma(v, by, from)); };
+  auto exponent = [](A v, A from, A by) { return static_cast<S>((v - from) * by); };
   const bool teach = w != S(0) && alpha > S(0);
   // the slots of this thread: the first few stay in registers, read before any is looked at
   constexpr int kHeld = 4;
@@ -481,16 +481,15 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   const S share = taught ? u_rest / t_sum : S(0);
 
   // the student's: the classes without a slot are summed on their own
-  const A off = -high * scale, off1 = -high * scale1;
   const bool two = hard_term && scale != scale1;
   S ez[E], e1[E], left = 0, named = 0, total1 = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int cls = e * L + team.l;
-    ez[e] = Exp2(exponent(z[e], scale, off));
+    ez[e] = Exp2(exponent(z[e], high, scale));
     if (cls < c && want[place(cls)] != kNone) named += ez[e];
     else left += ez[e];
-    e1[e] = two ? Exp2(exponent(z[e], scale1, off1)) : ez[e];
+    e1[e] = two ? Exp2(exponent(z[e], high, scale1)) : ez[e];
     total1 += e1[e];
   }
   left = team.Sum(left, red);
@@ -498,7 +497,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   total1 = two ? team.Sum(total1, red) : total;
   const S log_total = Log2(total);
   S log_left = Log2(left);
-  A rest_off = off;
+  A rest_high = high;
   const bool again = rest && w != S(0) && left < SmallRest<S>();
   if (team.Any(again)) {
     A own = NegInf<A>();
@@ -509,19 +508,18 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
     }
     own = team.Max(own, red_high);
     const bool able = again && own > NegInf<A>();
-    const A own_off = -own * scale;
     S sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int cls = e * L + team.l;
       if (able && cls < c && want[place(cls)] == kNone)
-        sum += Exp2(exponent(score(cls), scale, own_off));
+        sum += Exp2(exponent(score(cls), own, scale));
     }
     sum = team.Sum(sum, red);
     if (able) {
       left = sum;
-      rest_off = own_off;
-      log_left = Log2(left) + static_cast<S>(off - rest_off);
+      rest_high = own;
+      log_left = Log2(left) + exponent(own, high, scale);
     }
   }
   const bool live = w != S(0) && !(total == S(0));  // otherwise every class is masked
@@ -534,7 +532,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
     const S lp = t - t_log;
     const S p = taught ? Exp2(lp) : S(0);
     if (a.loss.data && !(p == S(0))) {
-      kl += p * (lp - (exponent(score(cls), scale, off) - log_total));
+      kl += p * (lp - (exponent(score(cls), high, scale) - log_total));
     }
     *at = ToBits(p) & ~kSlot;
   });
@@ -547,7 +545,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
         if (taught) v = alpha * temp * temp * (kl * static_cast<S>(kLn2));
         if (y >= 0)
           v += (S(1) - alpha) * static_cast<S>(kLn2) *
-               (Log2(total1) - exponent(score(y), scale1, off1));
+               (Log2(total1) - exponent(score(y), high, scale1));
         v *= w;
       }
       StoreFloat(a.loss, at_row(a.loss), v);
@@ -559,7 +557,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   const S inv = S(1) / total, inv1 = hard > S(0) ? S(1) / total1 : S(0);
   const S spread = rest && left > S(0) ? share / left : S(0);
   const S factor = c > 1 ? static_cast<S>(c) / static_cast<S>(c - 1) : S(1);
-  const bool moved = rest_off != off;
+  const bool moved = rest_high != high;
   O* grad = static_cast<O*>(a.gradient.data) + (a.gradient.data ? at_row(a.gradient) : 0);
   O* hess = static_cast<O*>(a.hessian.data) + (a.hessian.data ? at_row(a.hessian) : 0);
 #pragma unroll
@@ -574,7 +572,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
         S p = FromBits(bits);
         if (bits == kNone) {
           p = S(0);
-          const S e_rest = moved ? Exp2(exponent(score(cls), scale, rest_off)) : ez[e];
+          const S e_rest = moved ? Exp2(exponent(score(cls), rest_high, scale)) : ez[e];
           if (spread > S(0)) p = spread * e_rest;
           else if (spread != spread) p = spread;
         }
@@ -788,12 +786,12 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     return mark[base >> 5] >> (base & 31) & ((1u << size) - 1u);
   };
   // the sums of a chunk's exponentials of the classes without a slot, and of all at T = 1
-  auto add_chunk = [&](int base, const auto& v, A from, A from1, A& rest_sum, A& all_sum) {
+  auto add_chunk = [&](int base, const auto& v, A from, A& rest_sum, A& all_sum) {
     constexpr int kSize = kSizeOf<decltype(v)>;
     const uint32_t bits = bits_of(base, kSize);
     A e[kSize], sum = 0;
 #pragma unroll
-    for (int i = 0; i < kSize; ++i) e[i] = Exp2(Fma(v[i], scale, from));
+    for (int i = 0; i < kSize; ++i) e[i] = Exp2((v[i] - from) * scale);
     if (bits != 0) {
 #pragma unroll
       for (int i = 0; i < kSize; ++i) e[i] = bits >> i & 1u ? A(0) : e[i];
@@ -804,7 +802,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     if (two) {
       sum = 0;
 #pragma unroll
-      for (int i = 0; i < kSize; ++i) sum += Exp2(Fma(v[i], scale1, from1));
+      for (int i = 0; i < kSize; ++i) sum += Exp2((v[i] - from) * scale1);
       all_sum += sum;
     }
   };
@@ -826,8 +824,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
         if (two) more_total1 *= Exp2((more_high - top) * scale1);
         more_high = top;
       }
-      const A from = more_high > NegInf<A>() ? -more_high : A(0);
-      add_chunk(base, v, from * scale, from * scale1, more_left, more_total1);
+      add_chunk(base, v, more_high > NegInf<A>() ? more_high : A(0), more_left, more_total1);
     });
     high = Max(high, more_high);
   }
@@ -854,10 +851,9 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   const bool t_some = t_high > NegInf<A>();
   if (!t_some) t_high = A(0);
 
-  const A off = -high * scale, off1 = -high * scale1;
   A left = 0, total1 = 0;
   z.EachHeld([&](int base, const auto& v, auto...) {
-    add_chunk(base, v, off, off1, left, total1);
+    add_chunk(base, v, high, left, total1);
   });
   if constexpr (Shape::more) {
     if (own_high > NegInf<A>() || more_left != A(0)) {
@@ -866,7 +862,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
         total1 += more_total1 * Exp2((own_high > NegInf<A>() ? own_high - high : A(0)) * scale1);
     }
   }
-  const A log_e = Fma(z_slot, scale, off);
+  const A log_e = (z_slot - high) * scale;
   A sums[4] = {left, cls >= 0 ? Exp2(log_e) : A(0),
                cls >= 0 && !(logit == NegInf<A>()) ? Exp2(logit - t_high) : A(0), total1};
   const A u = sums[2];
@@ -883,19 +879,19 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   const bool taught = alpha > A(0) && (t_some || t_sum != t_sum);
   const A t_log = t_high + Log2(t_sum), log_total = Log2(total);
   const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
-  A log_left = Log2(left), rest_off = off;
+  A log_left = Log2(left), rest_high = high;
   if (rest && left < SmallRest<A>()) {  // seldom, so from memory in a plain loop
     A own = NegInf<A>();
     for (int i = tid; i < c; i += kBlock)
       if (!bits_of(i, 1)) own = Max(own, static_cast<A>(z.x[i]));
     own = BlockMax<kBlock>(own, s_more[1]);
     if (own > NegInf<A>()) {
-      rest_off = -own * scale;
+      rest_high = own;
       left = 0;
       for (int i = tid; i < c; i += kBlock)
-        if (!bits_of(i, 1)) left += Exp2(Fma(static_cast<A>(z.x[i]), scale, rest_off));
+        if (!bits_of(i, 1)) left += Exp2((static_cast<A>(z.x[i]) - own) * scale);
       left = BlockSum<kBlock>(left, s_more[2]);
-      log_left = Log2(left) - rest_off + off;
+      log_left = Log2(left) + (own - high) * scale;
     }
   }
 
@@ -907,7 +903,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
       if (rest && !(share == A(0))) kl[0] += share * (r - t_log - (log_left - log_total));
       A v = taught ? alpha * temp * temp * (kl[0] * static_cast<A>(kLn2)) : A(0);
       if (label >= 0)
-        v += (A(1) - alpha) * static_cast<A>(kLn2) * (Log2(total1) - Fma(z_label, scale1, off1));
+        v += (A(1) - alpha) * static_cast<A>(kLn2) * (Log2(total1) - (z_label - high) * scale1);
       StoreFloat(a.loss, row * a.loss.stride[0], v * w);
     }
   }
@@ -917,7 +913,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   const A spread = rest && left > A(0) ? share / left : A(0);
   const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
   // a class without a slot: its gradient is one factor of each exponential
-  const bool moved = rest_off != off;
+  const bool moved = rest_high != high;
   const A each = w * soft * temp;  // 0 where there is no teacher, whose inv may be anything
   A coef = soft > A(0) ? each * (moved ? inv : inv - spread) : A(0);
   const A coef1 = hard > A(0) ? w * hard * inv1 : A(0);
@@ -928,9 +924,9 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
       z.Each([&](int base, const auto& v, auto...) {
 #pragma unroll
         for (int i = 0; i < kSizeOf<decltype(v)>; ++i) {
-          A g = coef * Exp2(Fma(v[i], scale, off));
-          if (two) g = Fma(coef1, Exp2(Fma(v[i], scale1, off1)), g);
-          grad[base + i] = static_cast<O>(Fma(coef_rest, Exp2(Fma(v[i], scale, rest_off)), g));
+          A g = coef * Exp2((v[i] - high) * scale);
+          if (two) g = Fma(coef1, Exp2((v[i] - high) * scale1), g);
+          grad[base + i] = static_cast<O>(Fma(coef_rest, Exp2((v[i] - rest_high) * scale), g));
         }
       });
     } else {
@@ -940,12 +936,12 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
         if (two) {
 #pragma unroll
           for (int i = 0; i < kSize; ++i)
-            g[i] = static_cast<O>(Fma(coef1, Exp2(Fma(v[i], scale1, off1)),
-                                      coef * Exp2(Fma(v[i], scale, off))));
+            g[i] = static_cast<O>(Fma(coef1, Exp2((v[i] - high) * scale1),
+                                      coef * Exp2((v[i] - high) * scale)));
         } else {
 #pragma unroll
           for (int i = 0; i < kSize; ++i)
-            g[i] = static_cast<O>(coef * Exp2(Fma(v[i], scale, off)));
+            g[i] = static_cast<O>(coef * Exp2((v[i] - high) * scale));
         }
         __builtin_memcpy(grad + base, &g, sizeof(g));
       });
@@ -955,10 +951,10 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     z.Each([&](int base, const auto& v, auto...) {
 #pragma unroll
       for (int i = 0; i < kSizeOf<decltype(v)>; ++i) {
-        const A q = Exp2(Fma(v[i], scale, off)) * inv;
+        const A q = Exp2((v[i] - high) * scale) * inv;
         A h = soft > A(0) ? soft * q * (A(1) - q) : A(0);
         if (hard > A(0)) {
-          const A q1 = Exp2(Fma(v[i], scale1, off1)) * inv1;
+          const A q1 = Exp2((v[i] - high) * scale1) * inv1;
           h += hard * q1 * (A(1) - q1);
         }
         hess[base + i] = static_cast<O>(h * factor * w);
@@ -968,16 +964,16 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   if (!grad) return;
   __syncthreads();
   auto put = [&](int at, A v, A p, A from, bool spread_it) {
-    const A q = Exp2(Fma(v, scale, off)) * inv;
-    if (spread_it) p = spread == A(0) ? A(0) : spread * Exp2(Fma(v, scale, from));
+    const A q = Exp2((v - high) * scale) * inv;
+    if (spread_it) p = spread == A(0) ? A(0) : spread * Exp2((v - from) * scale);
     A g = soft > A(0) ? soft * temp * (q - p) : A(0);
     if (hard > A(0))
-      g += hard * (Exp2(Fma(v, scale1, off1)) * inv1 - (at == label ? A(1) : A(0)));
+      g += hard * (Exp2((v - high) * scale1) * inv1 - (at == label ? A(1) : A(0)));
     grad[at] = static_cast<O>(g * w);
   };
-  if (cls >= 0) put(cls, z_slot, p, off, false);
+  if (cls >= 0) put(cls, z_slot, p, high, false);
   // the label's class, where it has no slot
-  if (tid == 0 && label >= 0 && !bits_of(label, 1)) put(label, z_label, A(0), rest_off, true);
+  if (tid == 0 && label >= 0 && !bits_of(label, 1)) put(label, z_label, A(0), rest_high, true);
 }
 
 // ------------------------------------------------------------------ top logits, any strides

@@ -1098,3 +1098,143 @@ def test_distill_teacher_of_no_number(place, classes):
                         np.testing.assert_array_equal(grad[:bad, 3:], want[:bad, 3:])
                     np.testing.assert_array_equal(grad[bad:], want[bad:])
                     np.testing.assert_array_equal(loss[bad:], want_loss[bad:])
+
+
+# ------------------------------------------------------------------ scores of any size
+# The device's exponents are (z - high) * s: the difference, s and the product are rounded, so a
+# term 2^-x is off by (3 x + 4) eps of itself, and by less than 8 eps of the row's largest: `_rel`
+# covers that, being applied three times over. How large z itself is does not come in.
+def _plain_gradient(z, classes, logits, rest, labels, t, alpha):
+    """Gradient, hessian and their scale in 64 bits, for scores so far apart that even there a
+    logarithm of a sum keeps nothing of the sum: every softmax is taken against a maximum of its
+    own, of differences."""
+    def softmax(x):
+        e = np.exp(x - x.max())
+        return e / e.sum()
+
+    n, c = z.shape
+    grad, hess, size = np.zeros((n, c)), np.zeros((n, c)), np.zeros((n, c))
+    for i in range(n):
+        with np.errstate(over="ignore"):
+            q, q1 = softmax((z[i] - z[i].max()) / t), softmax(z[i] - z[i].max())
+        slot = {}
+        for j, x in enumerate(classes[i]):
+            if 0 <= x < c:
+                slot.setdefault(int(x), logits[i, j] / t)
+        p = softmax(np.array([*slot.values(), -INF if rest is None else rest[i]]))
+        want = np.zeros(c)
+        others = np.ones(c, bool)
+        others[list(slot)] = False
+        if p[-1] > 0:
+            own = z[i][others]
+            with np.errstate(over="ignore"):
+                want[others] = p[-1] * softmax((own - own.max()) / t)
+        want[list(slot)] = p[:-1]
+        grad[i] = alpha * t * (q - want)
+        hess[i] = alpha * q * (1 - q)
+        size[i] = alpha * t * (q + want)
+        if alpha < 1:
+            hit = np.arange(c) == labels[i]
+            grad[i] += (1 - alpha) * (q1 - hit)
+            hess[i] += (1 - alpha) * q1 * (1 - q1)
+            size[i] += (1 - alpha) * (q1 + hit)
+    return grad, hess * (c / (c - 1)), size
+
+
+def _gradient_case(place, z, teacher, dtype, labels=None, t=1.0, alpha=1.0, order="C", rel=None,
+                   rows=None):
+    """Gradient and hessian of the rows (all of them, or the first few)."""
+    z = _round(z, dtype)
+    ids, logits, rest = teacher
+    many = slice(None) if rows is None else np.arange(rows) % len(z)
+    pick = lambda x: None if x is None else x[many]  # noqa: E731
+    got = ops.distill_gradients(
+        _put(place, pick(z), dtype, order),
+        (_put(place, pick(ids), "i32"), _put(place, pick(logits), "f32"),
+         _put(place, pick(rest), "f32")),
+        labels=_put(place, pick(labels), "i32"), temperature=t, alpha=alpha, hessian=True)
+    grad, hess, size = _plain_gradient(z, ids, logits.astype(np.float64),
+                                       None if rest is None else rest.astype(np.float64),
+                                       labels, t, alpha)
+    out = "f32" if dtype == "f64" else dtype
+    rel = rel or 3 * _rel(z.shape[1], "f32")
+    for a, b, far in ((got.gradient, grad, rel * size),
+                      (got.hessian, hess, 2 * rel * size / min(t, 1.0))):
+        a = _get(a[:len(z)])
+        far = far + (1 + rel) * HALF_STEP[out] * np.abs(b) + TINY[out] * max(t, 1.0)
+        assert np.all(np.abs(a - b) <= far), np.nanmax(np.abs(a - b) - far)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 40, 150, 600, 5000, 90001, 200003])
+def test_distill_masked_by_the_lowest(place, classes):
+    """Masks of the type's lowest value: whole rows, which are uniform, all unnamed classes, with a
+    rest that wants something of them and without, and half of a row; rows of the highest value."""
+    rng = np.random.default_rng(classes)
+    ids = np.tile([1, 0, 2], (7, 1))
+    logits = np.tile(np.float32([3, 2, 1]), (7, 1))
+    rest = np.full(7, 0.5, np.float32)
+    rest[3] = -INF
+    labels = np.array([4, 4, 1, 4, 0, 4, 4])
+    for dtype in _types(place):
+        low = torch.finfo(TORCH[dtype]).min
+        z = rng.standard_normal((7, classes))
+        z[0] = low
+        z[1, 3:] = z[2, 3:] = z[3, 3:] = low
+        z[4, 1::2] = low
+        z[5] = -low
+        z[6] = low
+        z[6, 0] = 1.0
+        for order in "CF" if classes < 20000 else "C":
+            for t in (1.0, 0.5):
+                _gradient_case(place, z, (ids, logits, rest), dtype, t=t, order=order)
+                _gradient_case(place, z, (ids, logits, rest), dtype, labels=labels, t=t, alpha=0.5,
+                               order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 150, 600, 5000, 90001])
+def test_distill_of_small_temperature(place, classes):
+    """Large scores over a small temperature: every row has a largest score, so all are live."""
+    rng = np.random.default_rng(classes)
+    ids = np.tile([1, 0, 2], (4, 1))
+    logits = np.tile(np.float32([3e-6, 2e-6, 1e-6]), (4, 1))
+    rest = np.full(4, 2.5, np.float32)
+    labels = np.array([4, 1, 0, 4])
+    for dtype in _types(place):
+        z = rng.standard_normal((4, classes))
+        z[0] += 60000.0
+        z[1] -= 60000.0
+        z[2] = 50000.0
+        for order in "CF" if classes < 20000 else "C":
+            for alpha in (1.0, 0.5):
+                _gradient_case(place, z, (ids, logits, rest), dtype, labels=labels, t=1e-6,
+                               alpha=alpha, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes,dtype", [(131077, "f32"), (200003, "f32"), (200003, "f16"),
+                                           (200003, "bf16")])
+@pytest.mark.parametrize("offset", [0.0, -1000.0, 50000.0])
+def test_distill_large_rows_with_an_offset(place, classes, dtype, offset):
+    """Rows of which a part is read again: what is held and what is not have sums of their own. A
+    term that matters, 2^-x with x below 64, is off by (3 * 64 + 4) eps, a sum of a thread's 200
+    terms in chunks and the tree by 64 more; a quotient has two of them."""
+    if place == "numpy" and dtype == "bf16":
+        pytest.skip("numpy has no bfloat16")
+    rng = np.random.default_rng(classes)
+    teacher = _teacher(rng, 3, classes, 20, True)
+    z = 3 * rng.standard_normal((3, classes)) + offset
+    labels = rng.integers(0, classes, 3)
+    for t, alpha in ((1.0, 1.0), (2.0, 0.5)):
+        _gradient_case(place, z, teacher, dtype, labels=labels, t=t, alpha=alpha,
+                       rel=2 * 260 * HALF_STEP["f32"])
+    if place == "gpu":  # as many rows as share a compute unit, where they are only read
+        z = _round(z, dtype)
+        loss, _, _, size, _ = _plain_distill(z, teacher[0], teacher[1].astype(float),
+                                             teacher[2].astype(float), None, None, 1.0, 1.0)
+        many = torch.arange(600) % 3
+        got = ops.distill_loss(_put("gpu", z, dtype)[many], ops.TopLogits(
+            *[_put("gpu", x)[many] for x in (teacher[0].astype(np.int32), *teacher[1:])]))
+        far = 2 * 260 * HALF_STEP["f32"] * size + HALF_STEP["f32"] * np.abs(loss)
+        assert np.all(np.abs(_get(got)[:3] - loss) <= far)
