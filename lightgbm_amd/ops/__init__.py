@@ -68,12 +68,8 @@ _VERIFY = struct.Struct("@qii" + "Pqqqii" * 8 + "Pq")
 _NONE = (0, 0, 0, 0, 0, 0)
 
 
-def _packed(form, *values):
-    """A call's arguments as the C ABI has them."""
-    try:
-        return form.pack(*values)
-    except struct.error as e:
-        raise LightGBMError(f"an argument is not of its kind, or out of range: {e}") from None
+def _unpackable(e):
+    return LightGBMError(f"an argument is not of its kind, or out of range: {e}")
 
 
 for _f in (_LIB.LGBM_TopLogits, _LIB.LGBM_Distill, _LIB.LGBM_VerifyDrafts):
@@ -86,15 +82,17 @@ _WORKSPACE = {}  # bytes, by a call's sizes
 _torch = None
 _Tensor = ()
 _raw_stream = None
+_forward = None  # torch.autograd.forward_ad; its level is -1 where no tangents are about
 
 
 def _is_tensor(x):
-    global _torch, _Tensor, _raw_stream
+    global _torch, _Tensor, _raw_stream, _forward
     if _torch is None:
         _torch = sys.modules.get("torch")
         if _torch is None:
             return False
         _Tensor = _torch.Tensor
+        _forward = _torch.autograd.forward_ad
         for code, name in ((_F32, "float32"), (_F64, "float64"), (_I32, "int32"),
                            (_I64, "int64"), (_F16, "float16"), (_BF16, "bfloat16")):
             _TORCH_TYPES[getattr(_torch, name)] = code
@@ -149,11 +147,11 @@ class _Place:
             return _NONE
         given = x
         if _is_tensor(x):
-            # -1: the host
-            if x.get_device() != self.device or x.is_cuda != (self.device >= 0):
+            if x.get_device() != self.device if self.device >= 0 else not x.is_cpu:
                 raise LightGBMError(f"{name} is on {x.device}, the first array on "
                                     f"{self.on or 'the host'}")
-            x = _plain_tensor(x, name)
+            if x.requires_grad or x.is_neg() or _forward._current_level >= 0:
+                x = _plain_tensor(x, name)
         elif self.device >= 0:
             raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
         elif not isinstance(x, np.ndarray):
@@ -172,8 +170,7 @@ def _plain_tensor(x, name):
     if x.requires_grad and _torch.is_grad_enabled():
         raise LightGBMError(f"{name} requires a gradient, and this function records none: detach "
                             "it, or call under torch.no_grad()")
-    forward = _torch.autograd.forward_ad
-    if getattr(forward, "_current_level", 0) >= 0 and forward.unpack_dual(x).tangent is not None:
+    if _forward.unpack_dual(x).tangent is not None:
         raise LightGBMError(f"{name} carries a tangent, which this function would lose")
     return x.resolve_neg() if x.is_neg() else x
 
@@ -206,7 +203,8 @@ def _fields(x, name):
 def _shaped(x, name, dims=2):
     """x as an array, with its shape, which has to have so many dimensions."""
     if _is_tensor(x):
-        x = _plain_tensor(x, name)
+        if x.requires_grad or x.is_neg() or _forward._current_level >= 0:
+            x = _plain_tensor(x, name)
     elif not isinstance(x, np.ndarray):
         x = np.asarray(x)
     shape = x.shape
@@ -240,9 +238,11 @@ def top_logits(scores, k, temperature=1.0, rest=True):
     out_logit, to_logit = where.empty((rows, k), code)
     log_rest, to_rest = (where.empty((rows,), _F64 if code == _F64 else _F32) if rest
                          else (None, _NONE))
-    _safe_call(_LIB.LGBM_TopLogits(
-        _packed(_TOP, rows, classes, k, temperature, *x, *to_class, *to_logit, *to_rest),
-        where.device, where.stream()))
+    try:
+        args = _TOP.pack(rows, classes, k, temperature, *x, *to_class, *to_logit, *to_rest)
+    except struct.error as e:
+        raise _unpackable(e) from None
+    _safe_call(_LIB.LGBM_TopLogits(args, where.device, where.stream()))
     return TopLogits(out_class, out_logit, log_rest)
 
 
@@ -268,8 +268,11 @@ def _distill(scores, teacher, labels, weight, temperature, alpha, loss, gradient
     made_loss, to_loss = where.empty(row, _F64 if code == _F64 else _F32) if loss else absent
     made_grad, to_grad = where.scores(rows, classes, out, class_major) if gradient else absent
     made_hess, to_hess = where.scores(rows, classes, out, class_major) if hessian else absent
-    _safe_call(_LIB.LGBM_Distill(_packed(_DISTILL, *fields, *to_loss, *to_grad, *to_hess),
-                                 where.device, where.stream()))
+    try:
+        args = _DISTILL.pack(*fields, *to_loss, *to_grad, *to_hess)
+    except struct.error as e:
+        raise _unpackable(e) from None
+    _safe_call(_LIB.LGBM_Distill(args, where.device, where.stream()))
     return made_loss, made_grad, made_hess
 
 
@@ -342,7 +345,7 @@ def verify_drafts(target_prob, drafts, draft_prob, accept_uniform, sample_unifor
         size = _WORKSPACE.get(plan)
         if size is None:
             need = ctypes.c_int64(0)
-            _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_packed(_VERIFY, *fields, 0, 0),
+            _safe_call(_LIB.LGBM_VerifyDraftsWorkspace(_VERIFY.pack(*fields, 0, 0),
                                                        ctypes.byref(need)))
             if len(_WORKSPACE) >= 1024:
                 _WORKSPACE.clear()
@@ -351,6 +354,6 @@ def verify_drafts(target_prob, drafts, draft_prob, accept_uniform, sample_unifor
             # freed to the caching allocator, which gives it out again in the stream's order
             space = _torch.empty((size,), dtype=_torch.uint8, device=where.on)
             scratch = space.data_ptr()
-    _safe_call(_LIB.LGBM_VerifyDrafts(_packed(_VERIFY, *fields, scratch, size), where.device,
+    _safe_call(_LIB.LGBM_VerifyDrafts(_VERIFY.pack(*fields, scratch, size), where.device,
                                       where.stream()))
     return VerifiedDrafts(out_class, out_accepted)

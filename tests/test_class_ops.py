@@ -1100,6 +1100,15 @@ def test_distill_teacher_of_no_number(place, classes):
                     np.testing.assert_array_equal(loss[bad:], want_loss[bad:])
 
 
+def test_refuses_tensors_without_memory():
+    """A weight that holds no values is not a weight that is absent."""
+    z, ids, t = torch.ones(3, 4), torch.ones((3, 2), dtype=torch.int32), torch.ones(3, 2)
+    with pytest.raises(LightGBMError):
+        ops.distill_loss(z, (ids, t), weight=torch.ones(3, device="meta"))
+    with pytest.raises(LightGBMError):
+        ops.top_logits(z.to("meta"), 1)
+
+
 # ------------------------------------------------------------------ scores of any size
 # The device's exponents are (z - high) * s: the difference, s and the product are rounded, so a
 # term 2^-x is off by (3 x + 4) eps of itself, and by less than 8 eps of the row's largest: `_rel`
