@@ -112,7 +112,7 @@ class _Place:
         self.made = []  # arrays that stand for other objects, alive as long as the call
         self.device = -1
         self.on = None
-        self.tensor = _is_tensor(x)
+        self.tensor = isinstance(x, _Tensor)  # _shaped has seen it
         if self.tensor:
             self.on = x.device
             if x.is_cuda:
@@ -145,22 +145,29 @@ class _Place:
         """The six fields of an LGBM_Array of x, which has to be of this place and shape."""
         if x is None:
             return _NONE
-        given = x
-        if _is_tensor(x):
+        if isinstance(x, _Tensor) or _is_tensor(x):
+            # -1: the host
             if x.get_device() != self.device if self.device >= 0 else not x.is_cpu:
                 raise LightGBMError(f"{name} is on {x.device}, the first array on "
                                     f"{self.on or 'the host'}")
             if x.requires_grad or x.is_neg() or _forward._current_level >= 0:
                 x = _plain_tensor(x, name)
-        elif self.device >= 0:
+                self.made.append(x)
+            if x.shape != shape:
+                raise _shape_error(x, name, shape)
+            return _tensor_fields(x, name)
+        if self.device >= 0:
             raise LightGBMError(f"{name} must be a tensor on {self.on}, as the first array is")
-        elif not isinstance(x, np.ndarray):
+        if not isinstance(x, np.ndarray):
             x = np.asarray(x)
-        if x is not given:
             self.made.append(x)
         if x.shape != shape:
-            raise LightGBMError(f"{name} must have the shape {list(shape)}, got {list(x.shape)}")
-        return _fields(x, name)
+            raise _shape_error(x, name, shape)
+        return _array_fields(x, name)
+
+
+def _shape_error(x, name, shape):
+    return LightGBMError(f"{name} must have the shape {list(shape)}, got {list(x.shape)}")
 
 
 def _plain_tensor(x, name):
@@ -176,33 +183,41 @@ def _plain_tensor(x, name):
 
 
 def _fields(x, name):
-    if isinstance(x, np.ndarray):
-        dtype = x.dtype
-        code = _NUMPY_TYPES.get(dtype.kind + str(dtype.itemsize)) if dtype.isnative else None
-        steps = x.strides
-        if code is not None:
-            size = dtype.itemsize
-            if any(s % size for s in steps):
-                raise LightGBMError(f"{name} has strides that are no multiple of its elements")
-            steps = [s // size for s in steps]
-            at = x.__array_interface__["data"][0]
-    else:
-        code = _TORCH_TYPES.get(x.dtype)
-        steps = x.stride()
-        at = x.data_ptr()
+    return _array_fields(x, name) if isinstance(x, np.ndarray) else _tensor_fields(x, name)
+
+
+def _array_fields(x, name):
+    dtype = x.dtype
+    code = _NUMPY_TYPES.get(dtype.kind + str(dtype.itemsize)) if dtype.isnative else None
     if code is None:
-        raise LightGBMError(f"{name} has the type {x.dtype}, which is not supported")
+        raise _type_error(x, name)
+    size = dtype.itemsize
+    if any(s % size for s in x.strides):
+        raise LightGBMError(f"{name} has strides that are no multiple of its elements")
+    steps = [s // size for s in x.strides] + [0, 0]
+    return (x.__array_interface__["data"][0], *steps[:3], code, 0)
+
+
+def _tensor_fields(x, name):
+    code = _TORCH_TYPES.get(x.dtype)
+    if code is None:
+        raise _type_error(x, name)
+    steps = x.stride()
     n = len(steps)
     if n == 2:
-        return (at, steps[0], steps[1], 0, code, 0)
+        return (x.data_ptr(), steps[0], steps[1], 0, code, 0)
     if n == 1:
-        return (at, steps[0], 0, 0, code, 0)
-    return (at, steps[0], steps[1], steps[2], code, 0)
+        return (x.data_ptr(), steps[0], 0, 0, code, 0)
+    return (x.data_ptr(), *steps, code, 0)
+
+
+def _type_error(x, name):
+    return LightGBMError(f"{name} has the type {x.dtype}, which is not supported")
 
 
 def _shaped(x, name, dims=2):
     """x as an array, with its shape, which has to have so many dimensions."""
-    if _is_tensor(x):
+    if isinstance(x, _Tensor) or _is_tensor(x):
         if x.requires_grad or x.is_neg() or _forward._current_level >= 0:
             x = _plain_tensor(x, name)
     elif not isinstance(x, np.ndarray):
