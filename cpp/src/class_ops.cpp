@@ -228,9 +228,16 @@ void DistillHost(const LGBM_DistillArgs& a) {
         if (cls[j] < 0) continue;
         slot[y] = j;
         log_p[n++] = LoadFloat(a.teacher_logit, i * a.teacher_logit.stride[0] +
-                                                    j * a.teacher_logit.stride[1]) / t;
+                                                    j * a.teacher_logit.stride[1]);
       }
-      const double r = rest ? LoadFloat(a.teacher_rest, i * a.teacher_rest.stride[0]) : -kInf;
+      // against the largest logit first: over a small T a logit may be beyond 64 bits
+      double top = -kInf;
+      for (int j = 0; j < n; ++j) top = std::max(top, log_p[j]);
+      const bool some = top > -kInf;
+      if (!some) top = 0.0;
+      for (int j = 0; j < n; ++j) log_p[j] = (log_p[j] - top) / t;
+      const double r_read = rest ? LoadFloat(a.teacher_rest, i * a.teacher_rest.stride[0]) : -kInf;
+      const double r = r_read == -kInf || !some ? r_read : r_read - top / t;
       log_p[n] = r;
       const double norm = LogSumExp(log_p.data(), n + 1);
       bool nan = std::isnan(r) || norm == kInf;  // of infinite weights none is a share

@@ -82,6 +82,26 @@ __device__ __forceinline__ void StoreFloat(const LGBM_Array& a, int64_t at, A v)
   else static_cast<float*>(a.data)[at] = static_cast<float>(v);
 }
 
+// ------------------------------------------------------------------ keys
+/*! keys order as the values do, zeros of both signs alike; 0: never chosen (NaN, -inf) */
+__device__ __forceinline__ uint32_t KeyOf(float v) {
+  if (!(v > -INFINITY)) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t KeyOf(double v) {
+  if (!(v > -INFINITY)) return 0ull;
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+  return b >> 63 ? ~b : b | (1ull << 63);
+}
+/*! the value of a key that is not zero */
+__device__ __forceinline__ float ValueOf(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ double ValueOf(uint64_t key) {
+  return __longlong_as_double(static_cast<long long>(key >> 63 ? key & ~(1ull << 63) : ~key));
+}
+
 // ------------------------------------------------------------------ reductions
 constexpr int kWave = 64;
 
@@ -126,6 +146,34 @@ constexpr double kLn2 = 0.69314718055994530942;
 template <typename A> __device__ __forceinline__ A SmallRest() { return static_cast<A>(0x1p-100); }
 
 /*!
+ * A row's teacher: the weights of its slots and of its rest, as exponents to base two against
+ * the largest of them. Logits may have any common offset, and a rounding at their size is
+ * another factor for each slot, so they are subtracted as they are, and in 64 bits: 32 would move
+ * the probabilities by 9e-5 at logits near 1000. `largest` is the slots' largest logit,
+ * `log_rest` the rest's logarithm at the temperature, -inf where there is none; `by` is
+ * log2(e) / T.
+ */
+struct TeacherScale {
+  double scale, top, shift, rest;
+  __device__ __forceinline__ TeacherScale(double largest, double log_rest, double by)
+      : scale(by), top(0.0), shift(0.0) {
+    const bool some = largest > -INFINITY;
+    if (some) top = largest;
+    rest = some ? fma(-top, scale, log_rest * kLog2e) : 0.0;
+    if (log_rest == -INFINITY) rest = -INFINITY;  // whatever the slots are
+    else if (!(log_rest < INFINITY)) rest = NAN;  // of infinite weights none is a share
+    if (rest > 0.0) {
+      shift = -rest;
+      rest = 0.0;
+    }
+  }
+  template <typename S> __device__ __forceinline__ S Slot(double logit) const {
+    return static_cast<S>(fma(logit - top, scale, shift));
+  }
+  template <typename S> __device__ __forceinline__ S Rest() const { return static_cast<S>(rest); }
+};
+
+/*!
  * One workgroup a row, the row read from memory in each of its passes: maximum, sums,
  * gradients. With the teacher's slots (class c_j, logit t_j) and, where given, the
  * logarithm r of what it gives to all other classes,
@@ -142,11 +190,12 @@ template <typename A> __device__ __forceinline__ A SmallRest() { return static_c
  * bfloat16 gradients 785 us, where the rows' kernel takes 224).
  */
 template <typename T, int kBlock>
-__global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
+__global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, double by) {
   using A = Acc<T>;
   extern __shared__ uint32_t mark[];
   __shared__ int s_cls[kMaxTop];
   __shared__ A s_red[6][kBlock / kWave];
+  __shared__ double s_top[kBlock / kWave];
   __shared__ int s_dup;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, c = a.classes, k = a.k;
@@ -160,7 +209,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
   const int64_t gs = a.gradient.stride[1], hs = a.hessian.stride[1];
   const A w = a.weight.data ? LoadFloat<A>(a.weight, row * a.weight.stride[0]) : A(1);
   const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
-  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
+  const A scale = static_cast<A>(by), scale1 = static_cast<A>(kLog2e);
 
   for (int i = tid; i < (c + 31) / 32; i += kBlock) mark[i] = 0;
   if (tid == 0) s_dup = 0;
@@ -199,17 +248,14 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
     for (int i = 0; i < tid; ++i)
       if (s_cls[i] == cls) cls = -1;
   }
-  const A logit = cls >= 0 ? scale * LoadFloat<A>(a.teacher_logit,
-                                                  row * a.teacher_logit.stride[0] +
-                                                      tid * a.teacher_logit.stride[1])
-                           : NegInf<A>();
+  const double logit = cls >= 0 ? LoadFloat<double>(a.teacher_logit,
+                                                    row * a.teacher_logit.stride[0] +
+                                                        tid * a.teacher_logit.stride[1])
+                                : NegInf<double>();
   const bool rest = a.teacher_rest.data != nullptr;
-  const A r = rest ? scale1 * LoadFloat<A>(a.teacher_rest, row * a.teacher_rest.stride[0])
-                   : NegInf<A>();
-  const A t_high_or = BlockMax<kBlock>(Max(logit, r), s_red[1]);
-  const bool t_nan = __syncthreads_or(logit != logit || r != r);
-  const bool taught = alpha > A(0) && (t_high_or > NegInf<A>() || t_nan);
-  const A t_high = t_high_or > NegInf<A>() ? t_high_or : A(0);
+  const TeacherScale teacher(
+      BlockMax<kBlock>(logit, s_top),
+      rest ? LoadFloat<double>(a.teacher_rest, row * a.teacher_rest.stride[0]) : NegInf<double>(), by);
 
   // sums
   const A z_slot = cls >= 0 ? static_cast<A>(z[cls * zs]) : NegInf<A>();
@@ -224,9 +270,12 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
   left = BlockSum<kBlock>(left, s_red[0]);
   const A total = left + BlockSum<kBlock>(e_slot, s_red[2]);
   if (alpha < A(1)) total1 = BlockSum<kBlock>(total1, s_red[3]);
-  const A u = logit > NegInf<A>() || logit != logit ? Exp2(logit - t_high) : A(0);
-  const A u_rest = rest ? Exp2(r - t_high) : A(0);
+  const A log_u = cls >= 0 ? teacher.template Slot<A>(logit) : NegInf<A>();
+  const A log_u_rest = teacher.template Rest<A>();
+  const A u = Exp2(log_u), u_rest = Exp2(log_u_rest);
   const A t_sum = BlockSum<kBlock>(u, s_red[4]) + u_rest;
+  // the largest weight is one, so a sum of zero is a row without a teacher
+  const bool taught = alpha > A(0) && !(t_sum == A(0));
   const A log_total = Log2(total);
   const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
   A log_left = Log2(left), rest_high = high;
@@ -252,12 +301,12 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a) {
   if (a.loss.data) {
     A kl = 0;
     if (cls >= 0 && !(p == A(0)))
-      kl = p * (logit - t_high - Log2(t_sum) - (log_e - log_total));
+      kl = p * (log_u - Log2(t_sum) - (log_e - log_total));
     __syncthreads();
     kl = BlockSum<kBlock>(kl, s_red[0]);
     if (tid == 0) {
       if (rest && !(share == A(0)))
-        kl += share * (r - t_high - Log2(t_sum) - (log_left - log_total));
+        kl += share * (log_u_rest - Log2(t_sum) - (log_left - log_total));
       A v = taught ? alpha * temp * temp * (kl * static_cast<A>(kLn2)) : A(0);
       if (y >= 0)
         v += (A(1) - alpha) * static_cast<A>(kLn2) *
@@ -360,7 +409,7 @@ template <typename F> void AllowLds(F* kernel, size_t bytes) {
  * labels, weights and hessians 79 us, 3.8 TB/s of what has to move.
  */
 template <typename T, typename S, int E, TeamKind kKind>
-__global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int lanes) {
+__global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double by, int lanes) {
   using A = Acc<T>;
   using O = Out<T>;
   using W = Word<S>;
@@ -369,6 +418,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   W* want = reinterpret_cast<W*>(tile_lds);  // R * classes
   __shared__ A red_high[kKind == kAcross ? 256 : 1];
   __shared__ S red[kKind == kAcross ? 256 : 1];
+  __shared__ double red_top[kKind == kAcross ? 256 : 1];
   const Team<kKind> team(lanes);
   const int c = a.classes, k = a.k, L = team.L, R = team.R;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * R;
@@ -400,31 +450,31 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   // whatever the row's weight is, all that is read of it is asked for here at once
   const bool rest = a.teacher_rest.data != nullptr, hard_term = static_cast<S>(a.alpha) < S(1);
   const int label = hard_term && there ? LoadClass(a.label, at_row(a.label), c) : -1;
-  const S rest_read = rest && there ? LoadFloat<S>(a.teacher_rest, at_row(a.teacher_rest)) : S(0);
+  const double rest_read = rest && there ? LoadFloat<double>(a.teacher_rest, at_row(a.teacher_rest))
+                                         : 0.0;
   team.Sync();
   const S temp = static_cast<S>(a.temperature), alpha = static_cast<S>(a.alpha);
-  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
+  const A scale = static_cast<A>(by), scale1 = static_cast<A>(kLog2e);
   // exponents are formed as the scores are held, and taken as the statistics are
   auto exponent = [](A v, A from, A by) { return static_cast<S>((v - from) * by); };
   const bool teach = w != S(0) && alpha > S(0);
   // the slots of this thread: the first few stay in registers, read before any is looked at
   constexpr int kHeld = 4;
   int held_cls[kHeld];
-  S held_logit[kHeld];
+  double held_logit[kHeld];
   const int64_t class_row = at_row(a.teacher_class), logit_row = at_row(a.teacher_logit);
   auto load_class = [&](int j) {
     return LoadClass(a.teacher_class, class_row + j * a.teacher_class.stride[1], c);
   };
   auto load_logit = [&](int j) {
-    return static_cast<S>(scale) *
-           LoadFloat<S>(a.teacher_logit, logit_row + j * a.teacher_logit.stride[1]);
+    return LoadFloat<double>(a.teacher_logit, logit_row + j * a.teacher_logit.stride[1]);
   };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int j = team.l + i * L;
     const bool read = there && j < k;
     held_cls[i] = read ? load_class(j) : -1;
-    held_logit[i] = read ? load_logit(j) : S(0);
+    held_logit[i] = read ? load_logit(j) : 0.0;
   }
   if (!teach) {
 #pragma unroll
@@ -445,7 +495,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
       if (cls >= 0) f(j, cls, load_logit(j));
     }
   };
-  all_slots([&](int j, int cls, S) {
+  all_slots([&](int j, int cls, double) {
     atomicMin(&want[place(cls)], kSlot | static_cast<W>(j));
   });
   A high = NegInf<A>();
@@ -456,28 +506,22 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   team.Sync();
 
   // the teacher's distribution, in logarithms to base two
-  const S r = rest && teach ? static_cast<S>(scale1) * rest_read : NegInf<S>();
-  S t_high = r;
-  S t_nan = r != r ? S(1) : S(0);
   auto for_slots = [&](auto&& f) {  // the slots that count, with their place in the table
-    all_slots([&](int j, int cls, S t) {
+    all_slots([&](int j, int cls, double t) {
       W* at = &want[place(cls)];
       if (*at == (kSlot | static_cast<W>(j))) f(cls, t, at);
     });
   };
-  for_slots([&](int, S t, W*) {
-    t_high = Max(t_high, t);
-    if (t != t) t_nan = S(1);
-  });
-  t_high = team.Max(t_high, red);
-  t_nan = team.Max(t_nan, red);
-  const bool taught = teach && (t_high > NegInf<S>() || t_nan > S(0));
-  if (!(t_high > NegInf<S>())) t_high = S(0);
+  double t_top = NegInf<double>();
+  for_slots([&](int, double t, W*) { t_top = Max(t_top, t); });
+  const TeacherScale teacher(team.Max(t_top, red_top), rest && teach ? rest_read : NegInf<double>(), by);
   S t_sum = 0;
-  for_slots([&](int, S t, W*) { t_sum += Exp2(t - t_high); });
-  const S u_rest = rest ? Exp2(r - t_high) : S(0);
+  for_slots([&](int, double t, W*) { t_sum += Exp2(teacher.template Slot<S>(t)); });
+  const S log_u_rest = teacher.template Rest<S>(), u_rest = Exp2(log_u_rest);
   t_sum = team.Sum(t_sum, red) + u_rest;
-  const S t_log = t_high + Log2(t_sum);
+  // the largest weight is one, so a sum of zero is a row without a teacher
+  const bool taught = teach && !(t_sum == S(0));
+  const S t_log = Log2(t_sum);
   const S share = taught ? u_rest / t_sum : S(0);
 
   // the student's: the classes without a slot are summed on their own
@@ -528,8 +572,8 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
   // the table's slots give way to their probabilities; every class has one such slot
   S kl = 0;
   team.Sync();
-  for_slots([&](int cls, S t, W* at) {
-    const S lp = t - t_log;
+  for_slots([&](int cls, double t, W* at) {
+    const S lp = teacher.template Slot<S>(t) - t_log;
     const S p = taught ? Exp2(lp) : S(0);
     if (a.loss.data && !(p == S(0))) {
       kl += p * (lp - (exponent(score(cls), high, scale) - log_total));
@@ -541,7 +585,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, int la
     if (there && team.l == 0) {
       S v = 0;
       if (live) {
-        if (rest && !(share == S(0))) kl += share * (r - t_log - (log_left - log_total));
+        if (rest && !(share == S(0))) kl += share * (log_u_rest - t_log - (log_left - log_total));
         if (taught) v = alpha * temp * temp * (kl * static_cast<S>(kLn2));
         if (y >= 0)
           v += (S(1) - alpha) * static_cast<S>(kLn2) *
@@ -613,9 +657,10 @@ constexpr int kLdsChunks = 8;
 /*!
  * A row whose classes stand next to each other, as its workgroup holds it: one chunk a thread
  * in turn, and the classes after the last whole chunk one a thread. Chunks are read at their
- * elements' alignment: the hardware splits what crosses a line.
+ * elements' alignment: the hardware splits what crosses a line. kAnew: each pass counts its chunks
+ * anew, where their numbers, kept from one pass to the next, are the registers too many.
  */
-template <typename T, typename Shape> struct RowOf {
+template <typename T, typename Shape, bool kAnew = false> struct RowOf {
   static constexpr int kSize = Chunk<T>::kSize, kBlock = Shape::block, kCached = Shape::cached;
   using A = Acc<T>;
   const T* x;
@@ -661,18 +706,20 @@ template <typename T, typename Shape> struct RowOf {
   }
   /*! f(first class, values) of what this thread holds, kSize or one at a time */
   template <typename F> __device__ __forceinline__ void EachHeld(const F& f) {
+    int own = threadIdx.x;
+    if (kAnew) asm volatile("" : "+v"(own));
 #pragma unroll
     for (int n = 0; n < kCached; ++n) {
       // what a pass makes of the row is not kept for the next: the compiler would hold its
       // conversions and exponentials in registers that are not there
       asm volatile("" : "+v"(raw[n]));
-      const int chunk = n * kBlock + threadIdx.x;
+      const int chunk = n * kBlock + own;
       if (chunk < chunks) Give(raw[n], chunk, f);
     }
     if constexpr (Shape::more) {
       for (int n = 0; n < in_lds; ++n) {
-        const int chunk = (kCached + n) * kBlock + threadIdx.x;
-        if (chunk < chunks) Give(lds[n * kBlock + threadIdx.x], chunk, f);
+        const int chunk = (kCached + n) * kBlock + own;
+        if (chunk < chunks) Give(lds[n * kBlock + own], chunk, f);
       }
     }
     if (tail >= 0) {
@@ -726,15 +773,16 @@ __device__ __forceinline__ void BlockSums(A (&v)[kCount], A* lds) {
  */
 template <typename T, typename Shape, bool kHessian>
 __global__ void __launch_bounds__(Shape::block, Shape::cached >= 12 ? 4 : 1)
-k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
+k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
   using A = Acc<T>;
   using O = Out<T>;
-  using Row = RowOf<T, Shape>;
+  using Row = RowOf<T, Shape, (Shape::block > 256)>;
   constexpr int kBlock = Shape::block, kWaves = kBlock / kWave;
   extern __shared__ Words row_lds[];  // the chunks, then the marks
   uint32_t* mark = reinterpret_cast<uint32_t*>(row_lds + lds_chunks * Shape::block);
   __shared__ int s_cls[kMaxTop];
-  __shared__ A s_max[2][kWaves], s_sum[4 * kWaves], s_more[3][kWaves];
+  __shared__ A s_max[2][kWaves], s_sum[4 * kWaves], s_more[2][kWaves];
+  __shared__ double s_top[kWaves];
   __shared__ int s_dup;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, c = a.classes, k = a.k;
@@ -760,23 +808,23 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
 
   // the slots, one a thread
   const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
-  const A scale = static_cast<A>(kLog2e / a.temperature), scale1 = static_cast<A>(kLog2e);
+  const A scale = static_cast<A>(by), scale1 = static_cast<A>(kLog2e);
   const bool rest = a.teacher_rest.data != nullptr, hard_term = alpha < A(1);
   const bool two = hard_term && scale != scale1;  // a softmax at another temperature
   int cls = -1;
   A logit = NegInf<A>(), z_slot = NegInf<A>();
+  const int64_t logit_at = row * a.teacher_logit.stride[0] + tid * a.teacher_logit.stride[1];
   if (tid < k) {
     cls = LoadClass(a.teacher_class,
                     row * a.teacher_class.stride[0] + tid * a.teacher_class.stride[1], c);
     if (cls >= 0) {
-      logit = scale * LoadFloat<A>(a.teacher_logit, row * a.teacher_logit.stride[0] +
-                                                        tid * a.teacher_logit.stride[1]);
+      logit = LoadFloat<A>(a.teacher_logit, logit_at);
       z_slot = static_cast<A>(z.x[cls]);
     }
     s_cls[tid] = cls;
   }
-  const A r = rest ? scale1 * LoadFloat<A>(a.teacher_rest, row * a.teacher_rest.stride[0])
-                   : NegInf<A>();
+  const int64_t rest_at = row * a.teacher_rest.stride[0];
+  A r = rest ? LoadFloat<A>(a.teacher_rest, rest_at) : NegInf<A>();
   const int label = hard_term ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
   const A z_label = label >= 0 ? static_cast<A>(z.x[label]) : A(0);
   __syncthreads();
@@ -830,7 +878,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   }
   const A own_high = more_high;
   high = WaveMax(high);
-  A t_high = WaveMax(Max(logit, r));
+  A t_high = WaveMax(logit);
   if (tid % kWave == 0) {
     s_max[0][tid / kWave] = high;
     s_max[1][tid / kWave] = t_high;
@@ -845,11 +893,18 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     for (int i = 0; i < tid && tid < k; ++i)
       if (s_cls[i] == cls) cls = -1;
     if (cls < 0) logit = z_slot = NegInf<A>();
-    t_high = BlockMax<kBlock>(Max(logit, r), s_more[0]);
+    t_high = BlockMax<kBlock>(logit, s_more[0]);
   }
   if (!(high > NegInf<A>())) high = A(0);
-  const bool t_some = t_high > NegInf<A>();
-  if (!t_some) t_high = A(0);
+  // what 32 bits hold is exact in them; what they do not is read again
+  double t_top = t_high, t_own = logit, t_rest = r;
+  if (a.teacher_logit.type == C_API_DTYPE_FLOAT64) {
+    t_own = cls >= 0 ? At<double>(a.teacher_logit, logit_at) : NegInf<double>();
+    t_top = BlockMax<kBlock>(t_own, s_top);
+  }
+  if (rest && a.teacher_rest.type == C_API_DTYPE_FLOAT64) t_rest = At<double>(a.teacher_rest, rest_at);
+  const TeacherScale teacher(t_top, t_rest, by);
+  const A log_u = teacher.template Slot<A>(t_own), log_u_rest = teacher.template Rest<A>();
 
   A left = 0, total1 = 0;
   z.EachHeld([&](int base, const auto& v, auto...) {
@@ -864,7 +919,7 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
   }
   const A log_e = (z_slot - high) * scale;
   A sums[4] = {left, cls >= 0 ? Exp2(log_e) : A(0),
-               cls >= 0 && !(logit == NegInf<A>()) ? Exp2(logit - t_high) : A(0), total1};
+               Exp2(log_u), total1};
   const A u = sums[2];
   BlockSums<kBlock>(sums, s_sum);
   left = sums[0];
@@ -874,33 +929,34 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
     put_zeros();
     return;
   }
-  const A u_rest = rest ? Exp2(r - t_high) : A(0);
+  const A u_rest = Exp2(log_u_rest);
   const A t_sum = sums[2] + u_rest;
-  const bool taught = alpha > A(0) && (t_some || t_sum != t_sum);
-  const A t_log = t_high + Log2(t_sum), log_total = Log2(total);
+  // the largest weight is one, so a sum of zero is a row without a teacher
+  const bool taught = alpha > A(0) && !(t_sum == A(0));
+  const A t_log = Log2(t_sum), log_total = Log2(total);
   const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
   A log_left = Log2(left), rest_high = high;
   if (rest && left < SmallRest<A>()) {  // seldom, so from memory in a plain loop
     A own = NegInf<A>();
     for (int i = tid; i < c; i += kBlock)
       if (!bits_of(i, 1)) own = Max(own, static_cast<A>(z.x[i]));
-    own = BlockMax<kBlock>(own, s_more[1]);
+    own = BlockMax<kBlock>(own, s_more[0]);
     if (own > NegInf<A>()) {
       rest_high = own;
       left = 0;
       for (int i = tid; i < c; i += kBlock)
         if (!bits_of(i, 1)) left += Exp2((static_cast<A>(z.x[i]) - own) * scale);
-      left = BlockSum<kBlock>(left, s_more[2]);
+      left = BlockSum<kBlock>(left, s_more[1]);
       log_left = Log2(left) + (own - high) * scale;
     }
   }
 
   if (a.loss.data) {
-    A kl[1] = {cls >= 0 && !(p == A(0)) ? p * (logit - t_log - (log_e - log_total)) : A(0)};
+    A kl[1] = {cls >= 0 && !(p == A(0)) ? p * (log_u - t_log - (log_e - log_total)) : A(0)};
     __syncthreads();
     BlockSums<kBlock>(kl, s_sum);
     if (tid == 0) {
-      if (rest && !(share == A(0))) kl[0] += share * (r - t_log - (log_left - log_total));
+      if (rest && !(share == A(0))) kl[0] += share * (log_u_rest - t_log - (log_left - log_total));
       A v = taught ? alpha * temp * temp * (kl[0] * static_cast<A>(kLn2)) : A(0);
       if (label >= 0)
         v += (A(1) - alpha) * static_cast<A>(kLn2) * (Log2(total1) - (z_label - high) * scale1);
@@ -977,17 +1033,6 @@ k_distill_row(LGBM_DistillArgs a, int lds_chunks) {
 }
 
 // ------------------------------------------------------------------ top logits, any strides
-/*! keys order as the values do, zeros of both signs alike; 0: never chosen (NaN, -inf) */
-__device__ __forceinline__ uint32_t KeyOf(float v) {
-  if (!(v > -INFINITY)) return 0u;
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ uint64_t KeyOf(double v) {
-  if (!(v > -INFINITY)) return 0ull;
-  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
-  return b >> 63 ? ~b : b | (1ull << 63);
-}
 template <typename T> using Key = std::conditional_t<std::is_same_v<T, double>, uint64_t, uint32_t>;
 
 /*!
@@ -1230,13 +1275,6 @@ __global__ void __launch_bounds__(256) k_top_tile(LGBM_TopLogitsArgs a, int lane
 /*! a candidate as one number: the larger comes first, and of equal values the lower class */
 __device__ __forceinline__ uint64_t Candidate(float v, int cls) {
   return static_cast<uint64_t>(KeyOf(v)) << 32 | ~static_cast<uint32_t>(cls);
-}
-/*! the value of a key that is not zero */
-__device__ __forceinline__ float ValueOf(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
-__device__ __forceinline__ double ValueOf(uint64_t key) {
-  return __longlong_as_double(static_cast<long long>(key >> 63 ? key & ~(1ull << 63) : ~key));
 }
 /*! the same number in every lane, as a scalar */
 __device__ __forceinline__ uint32_t Scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -2151,7 +2189,7 @@ void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
   auto kernel = k_distill_tile<T, S, E, kKind>;
   AllowLds(kernel, lds);
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256),
-                     lds, s, a, lanes);
+                     lds, s, a, kLog2e / a.temperature, lanes);
 }
 
 template <typename T, typename S>
@@ -2282,7 +2320,7 @@ void LaunchDistillRow(const LGBM_DistillArgs& a, hipStream_t s) {
   auto launch = [&](auto kernel) {
     AllowLds(kernel, lds);
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(Shape::block), lds, s, a,
-                       held);
+                       kLog2e / a.temperature, held);
   };
   if (a.hessian.data) launch(k_distill_row<T, Shape, true>);
   else launch(k_distill_row<T, Shape, false>);
@@ -2333,7 +2371,7 @@ void DistillPart(const LGBM_DistillArgs& a, hipStream_t s) {
   ByType(a.scores.type, [&](auto t) {
     auto kernel = k_distill_any<decltype(t), 256>;
     AllowLds(kernel, lds);
-    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, a, kLog2e / a.temperature);
   });
   OPS_HIP_OK(hipGetLastError());
 }

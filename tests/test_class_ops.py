@@ -1247,3 +1247,63 @@ def test_distill_large_rows_with_an_offset(place, classes, dtype, offset):
             *[_put("gpu", x)[many] for x in (teacher[0].astype(np.int32), *teacher[1:])]))
         far = 2 * 260 * HALF_STEP["f32"] * size + HALF_STEP["f32"] * np.abs(loss)
         assert np.all(np.abs(_get(got)[:3] - loss) <= far)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 40, 150, 600, 5000])
+@pytest.mark.parametrize("offset", [-1e3, 1e4, -1e5])
+def test_distill_teacher_with_an_offset(place, classes, offset):
+    """What all logits and the rest have in common changes nothing, and neither does its size. The
+    exponents are formed in 64 bits, where an offset of 1e5 over T leaves 1e-10."""
+    rng = np.random.default_rng(classes)
+    ids, logits, rest = _teacher(rng, 4, classes, 5, True)
+    logits = (logits + offset).astype(np.float32)
+    labels = rng.integers(0, classes, 4)
+    for t in (1.0, 0.75):
+        r = (rest + offset / t).astype(np.float32)
+        for dtype in _types(place):
+            z = 3 * rng.standard_normal((4, classes))
+            for order in "CF":
+                for far in (r, None):
+                    _gradient_case(place, z, (ids, logits, far), dtype, labels=labels, t=t,
+                                   alpha=0.5, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 150, 5000])
+def test_distill_teacher_of_the_lowest_value(place, classes):
+    """Slots of the type's lowest logit are alike, and nothing beside a rest or a better slot."""
+    rng = np.random.default_rng(classes)
+    ids = np.tile([1, 0, 2], (3, 1))
+    low = torch.finfo(torch.float32).min
+    logits = np.tile(np.float32([low, low, low]), (3, 1))
+    logits[1, 2] = 5.0
+    z = rng.standard_normal((3, classes))
+    labels = np.full(3, 3)
+    for t in (1.0, 0.5):
+        for rest in (None, np.float32([0.5, 0.5, -INF])):
+            for order in "CF":
+                for dtype in _types(place):
+                    _gradient_case(place, z, (ids, logits, rest), dtype, labels=labels, t=t,
+                                   alpha=0.5, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 150, 5000])
+def test_distill_teacher_in_64_bits(place, classes):
+    """Logits that 32 bits would round: what a float64 teacher says is read as it is, beside scores
+    of any type."""
+    rng = np.random.default_rng(classes)
+    ids, logits, rest = _teacher(rng, 4, classes, 5, True)
+    logits = logits.astype(np.float64) / 3 + 1e6
+    rest = rest.astype(np.float64) / 3 + 1e6
+    for dtype in _types(place):
+        z = _round(rng.standard_normal((4, classes)), dtype)
+        for order in "CF":
+            got = _get(ops.distill_gradients(_put(place, z, dtype, order),
+                                             (_put(place, ids, "i32"), _put(place, logits, "f64"),
+                                              _put(place, rest, "f64"))).gradient)
+            want, _, size = _plain_gradient(z, ids, logits, rest, None, 1.0, 1.0)
+            out = HALF_STEP["f32" if dtype == "f64" else dtype]
+            far = 3 * _rel(classes, "f32") * size + 2 * out * np.abs(want)
+            assert np.all(np.abs(got - want) <= far + TINY["f32" if dtype == "f64" else dtype])
