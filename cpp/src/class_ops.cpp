@@ -274,7 +274,7 @@ void DistillHost(const LGBM_DistillArgs& a) {
       const bool labelled = y >= 0 && y < c;
       if (a.loss.data) {
         double v = taught && alpha > 0 ? alpha * t * t * kl : 0.0;
-        if (labelled) v += (1 - alpha) * (std::log(total1) + high - z[y]);
+        if (labelled) v += (1 - alpha) * (std::log(total1) - (z[y] - high));
         StoreFloat(a.loss, i * a.loss.stride[0], v * w);
       }
       if (a.gradient.data || a.hessian.data) {

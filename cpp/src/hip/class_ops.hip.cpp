@@ -174,6 +174,16 @@ struct TeacherScale {
 };
 
 /*!
+ * p log(p / q) of a class or of the rest, whose logarithm of q is that of a score `far` below the
+ * row's largest: log_pq is the logarithm of p over q without it, to base two. In 64 bits, as a
+ * score of the type's lowest value is farther than 32 hold, and the loss it makes is not.
+ */
+__device__ __forceinline__ double Divergence(double p, double log_pq, double far,
+                                             double temperature) {
+  return p * (log_pq * kLn2 - far / temperature);
+}
+
+/*!
  * One workgroup a row, the row read from memory in each of its passes: maximum, sums,
  * gradients. With the teacher's slots (class c_j, logit t_j) and, where given, the
  * logarithm r of what it gives to all other classes,
@@ -259,8 +269,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, doub
 
   // sums
   const A z_slot = cls >= 0 ? static_cast<A>(z[cls * zs]) : NegInf<A>();
-  const A log_e = (z_slot - high) * scale;
-  const A e_slot = cls >= 0 ? Exp2(log_e) : A(0);
+  const A e_slot = cls >= 0 ? Exp2((z_slot - high) * scale) : A(0);
   A left = 0, total1 = 0;
   for (int i = tid; i < c; i += kBlock) {
     const A v = static_cast<A>(z[i * zs]);
@@ -278,7 +287,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, doub
   const bool taught = alpha > A(0) && !(t_sum == A(0));
   const A log_total = Log2(total);
   const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
-  A log_left = Log2(left), rest_high = high;
+  A rest_high = high;
   bool again = rest && left < SmallRest<A>();
   if (again) {
     A own = NegInf<A>();
@@ -293,24 +302,25 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, doub
         if (!(mark[i >> 5] >> (i & 31) & 1u))
           left += Exp2((static_cast<A>(z[i * zs]) - own) * scale);
       left = BlockSum<kBlock>(left, s_red[5]);
-      log_left = Log2(left) + (own - high) * scale;
     }
   }
   const int y = alpha < A(1) ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
 
   if (a.loss.data) {
-    A kl = 0;
+    double kl = 0;
     if (cls >= 0 && !(p == A(0)))
-      kl = p * (log_u - Log2(t_sum) - (log_e - log_total));
+      kl = Divergence(p, log_u - Log2(t_sum) + log_total, static_cast<double>(z_slot) - high,
+                      a.temperature);
     __syncthreads();
-    kl = BlockSum<kBlock>(kl, s_red[0]);
+    kl = BlockSum<kBlock>(kl, s_top);
     if (tid == 0) {
       if (rest && !(share == A(0)))
-        kl += share * (log_u_rest - Log2(t_sum) - (log_left - log_total));
-      A v = taught ? alpha * temp * temp * (kl * static_cast<A>(kLn2)) : A(0);
+        kl += Divergence(share, log_u_rest - Log2(t_sum) - Log2(left) + log_total,
+                         static_cast<double>(rest_high) - high, a.temperature);
+      double v = taught ? a.alpha * a.temperature * a.temperature * kl : 0.0;
       if (y >= 0)
-        v += (A(1) - alpha) * static_cast<A>(kLn2) *
-             (Log2(total1) - (static_cast<A>(z[y * zs]) - high) * scale1);
+        v += (1.0 - a.alpha) *
+             (Log2(total1) * kLn2 - (static_cast<double>(static_cast<A>(z[y * zs])) - high));
       StoreFloat(a.loss, row * a.loss.stride[0], v * w);
     }
   }
@@ -540,7 +550,6 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
   const S total = left + team.Sum(named, red);
   total1 = two ? team.Sum(total1, red) : total;
   const S log_total = Log2(total);
-  S log_left = Log2(left);
   A rest_high = high;
   const bool again = rest && w != S(0) && left < SmallRest<S>();
   if (team.Any(again)) {
@@ -563,33 +572,33 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
     if (able) {
       left = sum;
       rest_high = own;
-      log_left = Log2(left) + exponent(own, high, scale);
     }
   }
   const bool live = w != S(0) && !(total == S(0));  // otherwise every class is masked
   const int y = live ? label : -1;
 
   // the table's slots give way to their probabilities; every class has one such slot
-  S kl = 0;
+  double kl = 0;
   team.Sync();
   for_slots([&](int cls, double t, W* at) {
     const S lp = teacher.template Slot<S>(t) - t_log;
     const S p = taught ? Exp2(lp) : S(0);
     if (a.loss.data && !(p == S(0))) {
-      kl += p * (lp - (exponent(score(cls), high, scale) - log_total));
+      kl += Divergence(p, lp + log_total, static_cast<double>(score(cls)) - high, a.temperature);
     }
     *at = ToBits(p) & ~kSlot;
   });
   if (a.loss.data) {
-    kl = team.Sum(kl, red);
+    kl = team.Sum(kl, red_top);
     if (there && team.l == 0) {
-      S v = 0;
+      double v = 0;
       if (live) {
-        if (rest && !(share == S(0))) kl += share * (log_u_rest - t_log - (log_left - log_total));
-        if (taught) v = alpha * temp * temp * (kl * static_cast<S>(kLn2));
+        if (rest && !(share == S(0)))
+          kl += Divergence(share, log_u_rest - t_log - Log2(left) + log_total,
+                           static_cast<double>(rest_high) - high, a.temperature);
+        if (taught) v = a.alpha * a.temperature * a.temperature * kl;
         if (y >= 0)
-          v += (S(1) - alpha) * static_cast<S>(kLn2) *
-               (Log2(total1) - exponent(score(y), high, scale1));
+          v += (1.0 - a.alpha) * (Log2(total1) * kLn2 - (static_cast<double>(score(y)) - high));
         v *= w;
       }
       StoreFloat(a.loss, at_row(a.loss), v);
@@ -917,8 +926,7 @@ k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
         total1 += more_total1 * Exp2((own_high > NegInf<A>() ? own_high - high : A(0)) * scale1);
     }
   }
-  const A log_e = (z_slot - high) * scale;
-  A sums[4] = {left, cls >= 0 ? Exp2(log_e) : A(0),
+  A sums[4] = {left, cls >= 0 ? Exp2((z_slot - high) * scale) : A(0),
                Exp2(log_u), total1};
   const A u = sums[2];
   BlockSums<kBlock>(sums, s_sum);
@@ -935,7 +943,7 @@ k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
   const bool taught = alpha > A(0) && !(t_sum == A(0));
   const A t_log = Log2(t_sum), log_total = Log2(total);
   const A p = taught ? u / t_sum : A(0), share = taught ? u_rest / t_sum : A(0);
-  A log_left = Log2(left), rest_high = high;
+  A rest_high = high;
   if (rest && left < SmallRest<A>()) {  // seldom, so from memory in a plain loop
     A own = NegInf<A>();
     for (int i = tid; i < c; i += kBlock)
@@ -947,19 +955,23 @@ k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
       for (int i = tid; i < c; i += kBlock)
         if (!bits_of(i, 1)) left += Exp2((static_cast<A>(z.x[i]) - own) * scale);
       left = BlockSum<kBlock>(left, s_more[1]);
-      log_left = Log2(left) + (own - high) * scale;
     }
   }
 
   if (a.loss.data) {
-    A kl[1] = {cls >= 0 && !(p == A(0)) ? p * (log_u - t_log - (log_e - log_total)) : A(0)};
+    double kl[1] = {0.0};
+    if (cls >= 0 && !(p == A(0)))
+      kl[0] = Divergence(p, log_u - t_log + log_total, static_cast<double>(z_slot) - high,
+                         a.temperature);
     __syncthreads();
-    BlockSums<kBlock>(kl, s_sum);
+    BlockSums<kBlock>(kl, s_top);
     if (tid == 0) {
-      if (rest && !(share == A(0))) kl[0] += share * (log_u_rest - t_log - (log_left - log_total));
-      A v = taught ? alpha * temp * temp * (kl[0] * static_cast<A>(kLn2)) : A(0);
+      if (rest && !(share == A(0)))
+        kl[0] += Divergence(share, log_u_rest - t_log - Log2(left) + log_total,
+                            static_cast<double>(rest_high) - high, a.temperature);
+      double v = taught ? a.alpha * a.temperature * a.temperature * kl[0] : 0.0;
       if (label >= 0)
-        v += (A(1) - alpha) * static_cast<A>(kLn2) * (Log2(total1) - (z_label - high) * scale1);
+        v += (1.0 - a.alpha) * (Log2(total1) * kLn2 - (static_cast<double>(z_label) - high));
       StoreFloat(a.loss, row * a.loss.stride[0], v * w);
     }
   }

@@ -1307,3 +1307,57 @@ def test_distill_teacher_in_64_bits(place, classes):
             out = HALF_STEP["f32" if dtype == "f64" else dtype]
             far = 3 * _rel(classes, "f32") * size + 2 * out * np.abs(want)
             assert np.all(np.abs(got - want) <= far + TINY["f32" if dtype == "f64" else dtype])
+
+
+def _plain_loss(z, classes, logits, rest, labels, t, alpha):
+    """The loss in 64 bits from differences, for scores of any size."""
+    loss = np.zeros(len(z))
+    for i, x in enumerate(z):
+        with np.errstate(over="ignore"):
+            d = (x - x.max()) / t
+        log_all = math.log(np.exp(d).sum())
+        names = [int(j) for j in classes[i]]
+        p = np.array([*(logits[i] / t), rest[i]])
+        log_p = p - _lse(p)
+        others = np.ones(len(x), bool)
+        others[names] = False
+        own = x[others].max()
+        with np.errstate(over="ignore"):
+            left = math.log(np.exp((x[others] - own) / t).sum()) + (own - x.max()) / t
+        log_q = np.array([*d[names], left]) - log_all
+        loss[i] = alpha * t * t * (np.exp(log_p) * (log_p - log_q)).sum()
+        if alpha < 1:
+            loss[i] += (1 - alpha) * (math.log(np.exp(x - x.max()).sum()) - (
+                x[labels[i]] - x.max()))
+    return loss
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 40, 150, 600, 5000, 90001])
+def test_distill_loss_of_the_lowest(place, classes):
+    """Where the student masks with the type's lowest value what the teacher or the label wants, the
+    loss is large and finite. It has one term of that size, off by what the probability and the
+    logarithms beside it are."""
+    rng = np.random.default_rng(classes)
+    ids = np.tile([1, 0, 2], (4, 1))
+    logits = np.tile(np.float32([3, 2, 1]), (4, 1))
+    rest = np.full(4, 0.5, np.float32)
+    labels = np.array([4, 4, 4, 0])
+    for dtype in _types(place):
+        z = rng.standard_normal((4, classes))
+        low = torch.finfo(TORCH[dtype]).min
+        z[0] = low
+        z[1, 3:] = low     # the rest
+        z[2, 2] = low      # a slot
+        z[3, 4] = z[3, 0] = low
+        z = _round(z, dtype)
+        for order in "CF" if classes < 20000 else "C":
+            for t, alpha in ((1.0, 1.0), (1.0, 0.5), (2.0, 0.75)):
+                got = _get(ops.distill_loss(
+                    _put(place, z, dtype, order),
+                    (_put(place, ids, "i32"), _put(place, logits, "f32"), _put(place, rest, "f32")),
+                    labels=_put(place, labels, "i32"), temperature=t, alpha=alpha))
+                want = _plain_loss(z, ids, logits.astype(float), rest.astype(float), labels, t,
+                                   alpha)
+                far = 3 * _rel(classes, dtype) * (20 * t * t + np.abs(want))
+                assert np.all(np.abs(got - want) <= far), (got, want)
