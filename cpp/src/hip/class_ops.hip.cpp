@@ -1485,7 +1485,7 @@ constexpr int kTopChunks = 512;       // that hold them
  */
 template <typename T, typename Shape>
 __global__ void __launch_bounds__(Shape::block, Shape::cached >= 12 ? 4 : 1)
-k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
+k_top_row(LGBM_TopLogitsArgs a, double by, int lds_chunks) {
   using A = Acc<T>;
   constexpr int kBlock = Shape::block, kWaves = kBlock / kWave;
   static_assert(std::is_same_v<A, float>, "keys of 32 bits");
@@ -1590,8 +1590,8 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
   }
   // the smallest of the maxima in the bins down to the k-th
   const A edge = bounded ? ValueOf(s_edge) : -FLT_MAX;
-  const A scale = static_cast<A>(kLog2e / a.temperature);
-  A off = bounded ? -edge * scale : A(0);  // unbounded, nothing but -inf is below the edge
+  const A scale = static_cast<A>(by);
+  A from = bounded ? edge : A(0);  // unbounded, nothing but -inf is below the edge
   const bool rest = a.log_rest.data != nullptr;
   A sum = 0;
   // a chunk with candidates is only put aside and looked at afterwards, an element a thread:
@@ -1605,7 +1605,7 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
     constexpr int kSize = kSizeOf<decltype(v)>;
     if constexpr (sizeof...(words) == 0) {
       pick(base, v[0]);
-      if (rest && v[0] < edge) sum += Exp2(Fma(v[0], scale, off));
+      if (rest && v[0] < edge) sum += Exp2((v[0] - from) * scale);
     } else {
       A top = v[0];
 #pragma unroll
@@ -1615,7 +1615,7 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
         // at most one, and NaN as zero: the bounds are the exponential's own modifier
 #pragma unroll
         for (int i = 0; i < kSize; ++i)
-          e[i] = fminf(fmaxf(Exp2(Fma(v[i], scale, off)), 0.0f), 1.0f);
+          e[i] = fminf(fmaxf(Exp2((v[i] - from) * scale), 0.0f), 1.0f);
       }
       if (top >= edge) {
         const int at = atomicAdd(&s_chunks, 1);
@@ -1692,25 +1692,27 @@ k_top_row(LGBM_TopLogitsArgs a, int lds_chunks) {
     own = BlockMax<kBlock>(own, s_low);
     sum = 0;
     if (own > NegInf<A>()) {
-      off = -own * scale;
+      from = own;
       for (int i = tid; i < a.classes; i += kBlock) {
         const A v = static_cast<A>(z.x[i]);
-        if (v < edge) sum += Exp2(Fma(v, scale, off));
+        if (v < edge) sum += Exp2((v - from) * scale);
       }
       sum = BlockSum<kBlock>(sum, s_high);
     }
   }
-  A log_rest = sum > A(0) ? Log2(sum) - off : NegInf<A>();
   if (n > k) {
     const A next = s_rest[0];
     A more = 0;
     for (int i = tid; i < n - k; i += kBlock) more += Exp2((s_rest[i] - next) * scale);
     more = BlockSum<kBlock>(more, s_high);
-    const A log_more = Fma(next, scale, Log2(more)), top = Max(log_rest, log_more);
-    log_rest = top + Log2(Exp2(log_rest - top) + Exp2(log_more - top));
+    // the next candidate is not below the edge, and has a term of one in its own sum
+    sum = more + (sum > A(0) ? sum * Exp2((from - next) * scale) : A(0));
+    from = next;
   }
   if (tid == 0)
-    StoreFloat(a.log_rest, row * a.log_rest.stride[0], log_rest * static_cast<A>(kLn2));
+    StoreFloat(a.log_rest, row * a.log_rest.stride[0],
+               sum > A(0) ? fma(from, by, static_cast<double>(Log2(sum))) * kLn2
+                          : -static_cast<double>(INFINITY));
 }
 
 // ------------------------------------------------------------------ verification
@@ -2256,7 +2258,7 @@ void LaunchTopRow(const LGBM_TopLogitsArgs& a, hipStream_t s) {
   auto kernel = k_top_row<T, Shape>;
   AllowLds(kernel, lds);
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.rows)), dim3(Shape::block), lds, s, a,
-                     held);
+                     kLog2e / a.temperature, held);
 }
 
 /*!

@@ -1361,3 +1361,35 @@ def test_distill_loss_of_the_lowest(place, classes):
                                    alpha)
                 far = 3 * _rel(classes, dtype) * (20 * t * t + np.abs(want))
                 assert np.all(np.abs(got - want) <= far), (got, want)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [8, 100, 400, 600, 1000, 5000, 90001, 200003])
+def test_top_logits_masked_by_the_lowest(place, classes):
+    """Masks of the type's lowest value are scores: they are chosen after all others, and what is
+    not chosen of them has a logarithm of their size. Exactly k others, fewer, none, one more."""
+    rng = np.random.default_rng(classes)
+    k = 5
+    for dtype in _types(place):
+        low = torch.finfo(TORCH[dtype]).min
+        x = np.full((5, classes), low)
+        for i, many in enumerate((k, k - 2, 0, k + 1, classes // 2)):
+            x[i, rng.permutation(classes)[:many]] = rng.standard_normal(many)
+        for order in "CF" if classes < 20000 else "C":
+            _top_case(place, x, dtype, k, order=order)
+            _top_case(place, x, dtype, k, t=2.0, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [8, 100, 400, 600, 5000, 90001])
+def test_top_logits_of_small_temperature(place, classes):
+    """Large scores over a small temperature, and scores with a large offset: the rest's logarithm
+    is that of a size, with the same few roundings."""
+    rng = np.random.default_rng(classes)
+    for dtype in _types(place):
+        x = rng.standard_normal((3, classes))
+        x[0] += 60000.0
+        x[1] -= 60000.0
+        for order in "CF" if classes < 20000 else "C":
+            for t in (1e-6, 0.01, 1.0):
+                _top_case(place, x, dtype, 3, t=t, order=order)
