@@ -274,11 +274,11 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, doub
   for (int i = tid; i < c; i += kBlock) {
     const A v = static_cast<A>(z[i * zs]);
     if (!(mark[i >> 5] >> (i & 31) & 1u)) left += Exp2((v - high) * scale);
-    if (alpha < A(1)) total1 += Exp2((v - high) * scale1);
+    if (a.alpha < 1.0) total1 += Exp2((v - high) * scale1);
   }
   left = BlockSum<kBlock>(left, s_red[0]);
   const A total = left + BlockSum<kBlock>(e_slot, s_red[2]);
-  if (alpha < A(1)) total1 = BlockSum<kBlock>(total1, s_red[3]);
+  if (a.alpha < 1.0) total1 = BlockSum<kBlock>(total1, s_red[3]);
   const A log_u = cls >= 0 ? teacher.template Slot<A>(logit) : NegInf<A>();
   const A log_u_rest = teacher.template Rest<A>();
   const A u = Exp2(log_u), u_rest = Exp2(log_u_rest);
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, doub
       left = BlockSum<kBlock>(left, s_red[5]);
     }
   }
-  const int y = alpha < A(1) ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
+  const int y = a.alpha < 1.0 ? LoadClass(a.label, row * a.label.stride[0], c) : -1;
 
   if (a.loss.data) {
     double kl = 0;
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, doub
     }
   }
   if (!grad && !hess) return;
-  const A soft = taught ? alpha : A(0), hard = y >= 0 ? A(1) - alpha : A(0);
+  const A soft = taught ? alpha : A(0), hard = y >= 0 ? static_cast<A>(1.0 - a.alpha) : A(0);
   const A inv = A(1) / total, inv1 = hard > A(0) ? A(1) / total1 : A(0);
   const A spread = rest && left > A(0) ? share / left : A(0);
   const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
     if (cls < c) want[place(cls)] = kNone;
   }
   // whatever the row's weight is, all that is read of it is asked for here at once
-  const bool rest = a.teacher_rest.data != nullptr, hard_term = static_cast<S>(a.alpha) < S(1);
+  const bool rest = a.teacher_rest.data != nullptr, hard_term = a.alpha < 1.0;
   const int label = hard_term && there ? LoadClass(a.label, at_row(a.label), c) : -1;
   const double rest_read = rest && there ? LoadFloat<double>(a.teacher_rest, at_row(a.teacher_rest))
                                          : 0.0;
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
   }
   if (!a.gradient.data && !a.hessian.data) return;
   team.Sync();
-  const S soft = taught ? alpha : S(0), hard = y >= 0 ? S(1) - alpha : S(0);
+  const S soft = taught ? alpha : S(0), hard = y >= 0 ? static_cast<S>(1.0 - a.alpha) : S(0);
   const S inv = S(1) / total, inv1 = hard > S(0) ? S(1) / total1 : S(0);
   const S spread = rest && left > S(0) ? share / left : S(0);
   const S factor = c > 1 ? static_cast<S>(c) / static_cast<S>(c - 1) : S(1);
@@ -818,7 +818,7 @@ k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
   // the slots, one a thread
   const A temp = static_cast<A>(a.temperature), alpha = static_cast<A>(a.alpha);
   const A scale = static_cast<A>(by), scale1 = static_cast<A>(kLog2e);
-  const bool rest = a.teacher_rest.data != nullptr, hard_term = alpha < A(1);
+  const bool rest = a.teacher_rest.data != nullptr, hard_term = a.alpha < 1.0;
   const bool two = hard_term && scale != scale1;  // a softmax at another temperature
   int cls = -1;
   A logit = NegInf<A>(), z_slot = NegInf<A>();
@@ -976,7 +976,7 @@ k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
     }
   }
   if (!grad && !hess) return;
-  const A soft = taught ? alpha : A(0), hard = label >= 0 ? A(1) - alpha : A(0);
+  const A soft = taught ? alpha : A(0), hard = label >= 0 ? static_cast<A>(1.0 - a.alpha) : A(0);
   const A inv = A(1) / total, inv1 = hard > A(0) ? A(1) / total1 : A(0);
   const A spread = rest && left > A(0) ? share / left : A(0);
   const A factor = c > 1 ? static_cast<A>(c) / static_cast<A>(c - 1) : A(1);

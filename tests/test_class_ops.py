@@ -1393,3 +1393,31 @@ def test_top_logits_of_small_temperature(place, classes):
         for order in "CF" if classes < 20000 else "C":
             for t in (1e-6, 0.01, 1.0):
                 _top_case(place, x, dtype, 3, t=t, order=order)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [6, 40, 150, 600, 5000])
+@pytest.mark.parametrize("less", [1e-3, 1e-6, 1e-12])
+def test_distill_alpha_next_to_one(place, classes, less):
+    """The labels' weight is what alpha leaves, however little: of rows without a teacher it is all
+    there is, and relative to it the errors are those of any softmax."""
+    rng = np.random.default_rng(classes)
+    alpha = 1.0 - less
+    ids = np.full((4, 2), -1)
+    logits = np.zeros((4, 2), np.float32)
+    labels = rng.integers(0, classes, 4)
+    for dtype in _types(place):
+        z = _round(rng.standard_normal((4, classes)), dtype)
+        for order in "CF":
+            got = ops.distill_gradients(
+                _put(place, z, dtype, order), (_put(place, ids, "i32"), _put(place, logits, "f32")),
+                labels=_put(place, labels, "i32"), alpha=alpha, loss=True)
+            q = _softmax(z)
+            hit = np.arange(classes) == labels[:, None]
+            want, size = (1.0 - alpha) * (q - hit), (1.0 - alpha) * (q + hit)
+            out = "f32" if dtype == "f64" else dtype
+            far = 3 * _rel(classes, "f32") * size + 2 * HALF_STEP[out] * np.abs(want) + TINY[out]
+            assert np.all(np.abs(_get(got.gradient) - want) <= far)
+            loss = (1.0 - alpha) * -np.log(q[hit])
+            assert np.all(np.abs(_get(got.loss) - loss) <= 3 * _rel(classes, dtype) * (
+                (1.0 - alpha) * (2 + np.abs(np.log(q[hit])))) + HALF_STEP["f32"] * loss)
