@@ -42,6 +42,24 @@ template <typename T> using Out = std::conditional_t<std::is_same_v<T, double>, 
 template <typename A> __device__ __forceinline__ A NegInf() { return -static_cast<A>(INFINITY); }
 __device__ __forceinline__ float Exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ double Exp2(double x) { return exp2(x); }
+/*!
+ * 2^x to 2e-10 of itself, for sums and quotients that end in 32 bits: the exponential's series in
+ * f ln 2, |f| <= 1/2, whose ninth term is at most (ln 2 / 2)^9 / 9!. 0 for -inf, NaN for NaN.
+ */
+__device__ __forceinline__ double ShortExp2(double x) {
+  constexpr double kLn2 = 0.69314718055994530942;
+  const double n = rint(x), f = (x - n) * kLn2;
+  double p = 1.0 / 40320;
+  p = fma(p, f, 1.0 / 5040);
+  p = fma(p, f, 1.0 / 720);
+  p = fma(p, f, 1.0 / 120);
+  p = fma(p, f, 1.0 / 24);
+  p = fma(p, f, 1.0 / 6);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return x < -1000.0 ? 0.0 : ldexp(p, static_cast<int>(n));
+}
 __device__ __forceinline__ float Log2(float x) { return log2f(x); }
 __device__ __forceinline__ double Log2(double x) { return log2(x); }
 __device__ __forceinline__ float Fma(float a, float b, float c) { return fmaf(a, b, c); }
@@ -412,15 +430,18 @@ template <typename F> void AllowLds(F* kernel, size_t bytes) {
  * Up to E * L classes: a row is read once and stays in its threads' registers. What the
  * teacher wants of each class is a table in LDS, one word a class: first the lowest slot that
  * names the class (with the sign bit set, kNone: none), then that slot's probability.
- * The statistics are held in S: float64 scores have their loss in 64 bits, and their 32-bit
- * gradients from exponents that are formed in 64 bits and rounded to 32, which moves a
- * gradient by about its own rounding; in 64-bit exponentials alone a booster's gradients took
- * 185 us where they took 125. Bound by memory: two million rows of seven float64 classes with
- * labels, weights and hessians 79 us, 3.8 TB/s of what has to move.
+ * Everything is held as wide as the scores' statistics, 64 bits for float64 scores, whose 32-bit
+ * gradients are then off by hardly more than their own rounding; in 32 bits they were off by five
+ * times as much (1.3e-7 of the largest), in 82 us where this takes 101. kLoss: whether the loss is
+ * among what may be asked for. Of float64 scores it has a launch of its own, as it needs the
+ * exponentials in all of 64 bits, which cost a gradient 123 us. Bound by the arithmetic of 64 bits
+ * beside memory: two million rows of seven float64 classes with labels, weights and hessians 101
+ * us, 3.0 TB/s of what has to move.
  */
-template <typename T, typename S, int E, TeamKind kKind>
+template <typename T, bool kLoss, int E, TeamKind kKind>
 __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double by, int lanes) {
   using A = Acc<T>;
+  using S = A;
   using O = Out<T>;
   using W = Word<S>;
   constexpr W kNone = ~W{0}, kSlot = W{1} << (sizeof(W) * 8 - 1);
@@ -465,8 +486,10 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
   team.Sync();
   const S temp = static_cast<S>(a.temperature), alpha = static_cast<S>(a.alpha);
   const A scale = static_cast<A>(by), scale1 = static_cast<A>(kLog2e);
-  // exponents are formed as the scores are held, and taken as the statistics are
-  auto exponent = [](A v, A from, A by) { return static_cast<S>((v - from) * by); };
+  auto exp2_of = [](S v) {
+    if constexpr (std::is_same_v<S, double> && !kLoss) return ShortExp2(v);
+    else return Exp2(v);
+  };
   const bool teach = w != S(0) && alpha > S(0);
   // the slots of this thread: the first few stay in registers, read before any is looked at
   constexpr int kHeld = 4;
@@ -526,13 +549,13 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
   for_slots([&](int, double t, W*) { t_top = Max(t_top, t); });
   const TeacherScale teacher(team.Max(t_top, red_top), rest && teach ? rest_read : NegInf<double>(), by);
   S t_sum = 0;
-  for_slots([&](int, double t, W*) { t_sum += Exp2(teacher.template Slot<S>(t)); });
-  const S log_u_rest = teacher.template Rest<S>(), u_rest = Exp2(log_u_rest);
+  for_slots([&](int, double t, W*) { t_sum += exp2_of(teacher.template Slot<S>(t)); });
+  const S log_u_rest = teacher.template Rest<S>(), u_rest = exp2_of(log_u_rest);
   t_sum = team.Sum(t_sum, red) + u_rest;
   // the largest weight is one, so a sum of zero is a row without a teacher
   const bool taught = teach && !(t_sum == S(0));
-  const S t_log = Log2(t_sum);
-  const S share = taught ? u_rest / t_sum : S(0);
+  const S t_inv = taught ? S(1) / t_sum : S(0);
+  const S share = u_rest * t_inv;
 
   // the student's: the classes without a slot are summed on their own
   const bool two = hard_term && scale != scale1;
@@ -540,16 +563,15 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int cls = e * L + team.l;
-    ez[e] = Exp2(exponent(z[e], high, scale));
+    ez[e] = exp2_of((z[e] - high) * scale);
     if (cls < c && want[place(cls)] != kNone) named += ez[e];
     else left += ez[e];
-    e1[e] = two ? Exp2(exponent(z[e], high, scale1)) : ez[e];
+    e1[e] = two ? exp2_of((z[e] - high) * scale1) : ez[e];
     total1 += e1[e];
   }
   left = team.Sum(left, red);
   const S total = left + team.Sum(named, red);
   total1 = two ? team.Sum(total1, red) : total;
-  const S log_total = Log2(total);
   A rest_high = high;
   const bool again = rest && w != S(0) && left < SmallRest<S>();
   if (team.Any(again)) {
@@ -566,7 +588,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
     for (int e = 0; e < E; ++e) {
       const int cls = e * L + team.l;
       if (able && cls < c && want[place(cls)] == kNone)
-        sum += Exp2(exponent(score(cls), own, scale));
+        sum += exp2_of((score(cls) - own) * scale);
     }
     sum = team.Sum(sum, red);
     if (able) {
@@ -579,22 +601,22 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
 
   // the table's slots give way to their probabilities; every class has one such slot
   double kl = 0;
+  const S log_both = kLoss ? Log2(total) - Log2(t_sum) : S(0);
   team.Sync();
   for_slots([&](int cls, double t, W* at) {
-    const S lp = teacher.template Slot<S>(t) - t_log;
-    const S p = taught ? Exp2(lp) : S(0);
-    if (a.loss.data && !(p == S(0))) {
-      kl += Divergence(p, lp + log_total, static_cast<double>(score(cls)) - high, a.temperature);
-    }
+    const S log_u = teacher.template Slot<S>(t);
+    const S p = taught ? exp2_of(log_u) * t_inv : S(0);
+    if (kLoss && a.loss.data && !(p == S(0)))
+      kl += Divergence(p, log_u + log_both, static_cast<double>(score(cls)) - high, a.temperature);
     *at = ToBits(p) & ~kSlot;
   });
-  if (a.loss.data) {
+  if (kLoss && a.loss.data) {
     kl = team.Sum(kl, red_top);
     if (there && team.l == 0) {
       double v = 0;
       if (live) {
         if (rest && !(share == S(0)))
-          kl += Divergence(share, log_u_rest - t_log - Log2(left) + log_total,
+          kl += Divergence(share, log_u_rest - Log2(left) + log_both,
                            static_cast<double>(rest_high) - high, a.temperature);
         if (taught) v = a.alpha * a.temperature * a.temperature * kl;
         if (y >= 0)
@@ -625,7 +647,7 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
         S p = FromBits(bits);
         if (bits == kNone) {
           p = S(0);
-          const S e_rest = moved ? Exp2(exponent(score(cls), rest_high, scale)) : ez[e];
+          const S e_rest = moved ? exp2_of((score(cls) - rest_high) * scale) : ez[e];
           if (spread > S(0)) p = spread * e_rest;
           else if (spread != spread) p = spread;
         }
@@ -2196,25 +2218,25 @@ int LanesFor(int classes, int each) {
   return lanes;
 }
 
-template <typename T, typename S, int E, TeamKind kKind>
+template <typename T, bool kLoss, int E, TeamKind kKind>
 void LaunchDistillTile(const LGBM_DistillArgs& a, hipStream_t s) {
   const int lanes = LanesFor(a.classes, E), rows = 256 / lanes;
-  const size_t lds = sizeof(Word<S>) * rows * a.classes;  // at most 2048 * E bytes
-  auto kernel = k_distill_tile<T, S, E, kKind>;
+  const size_t lds = sizeof(Word<Acc<T>>) * rows * a.classes;  // at most 2048 * E bytes
+  auto kernel = k_distill_tile<T, kLoss, E, kKind>;
   AllowLds(kernel, lds);
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>((a.rows + rows - 1) / rows)), dim3(256),
                      lds, s, a, kLog2e / a.temperature, lanes);
 }
 
-template <typename T, typename S>
+template <typename T, bool kLoss>
 void DistillTile(const LGBM_DistillArgs& a, bool across, hipStream_t s) {
-  if (!across && a.classes <= 64) LaunchDistillTile<T, S, 4, kNeighbours>(a, s);
-  else if (!across) LaunchDistillTile<T, S, 16, kNeighbours>(a, s);
-  else if (a.classes <= 4) LaunchDistillTile<T, S, 4, kAlone>(a, s);
-  else if (a.classes <= 8) LaunchDistillTile<T, S, 8, kAlone>(a, s);
-  else if (a.classes <= 16) LaunchDistillTile<T, S, 16, kAlone>(a, s);
-  else if (a.classes <= 256) LaunchDistillTile<T, S, 16, kAcross>(a, s);
-  else LaunchDistillTile<T, S, 32, kAcross>(a, s);
+  if (!across && a.classes <= 64) LaunchDistillTile<T, kLoss, 4, kNeighbours>(a, s);
+  else if (!across) LaunchDistillTile<T, kLoss, 16, kNeighbours>(a, s);
+  else if (a.classes <= 4) LaunchDistillTile<T, kLoss, 4, kAlone>(a, s);
+  else if (a.classes <= 8) LaunchDistillTile<T, kLoss, 8, kAlone>(a, s);
+  else if (a.classes <= 16) LaunchDistillTile<T, kLoss, 16, kAlone>(a, s);
+  else if (a.classes <= 256) LaunchDistillTile<T, kLoss, 16, kAcross>(a, s);
+  else LaunchDistillTile<T, kLoss, 32, kAcross>(a, s);
 }
 
 /*! whether the rows of a class stand closer together than the classes of a row */
@@ -2355,12 +2377,12 @@ void DistillPart(const LGBM_DistillArgs& a, hipStream_t s) {
       LGBM_DistillArgs part = a;
       if constexpr (std::is_same_v<T, double>) {
         part.gradient.data = part.hessian.data = nullptr;
-        if (a.loss.data) DistillTile<double, double>(part, across, s);
+        if (a.loss.data) DistillTile<double, true>(part, across, s);
         part = a;
         part.loss.data = nullptr;
       }
       if (part.loss.data || part.gradient.data || part.hessian.data)
-        DistillTile<T, float>(part, across, s);
+        DistillTile<T, !std::is_same_v<T, double>>(part, across, s);
     });
     OPS_HIP_OK(hipGetLastError());
     return;
