@@ -48,13 +48,19 @@ __device__ __forceinline__ double Exp2(double x) { return exp2(x); }
  */
 __device__ __forceinline__ double ShortExp2(double x) {
   constexpr double kLn2 = 0.69314718055994530942;
+  // a multiply-add whose addend is a scalar: the compiler's own form copies it to registers
+  auto step = [](double p, double f, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(p), "v"(f), "s"(c));
+    return r;
+  };
   const double n = rint(x), f = (x - n) * kLn2;
   double p = 1.0 / 40320;
-  p = fma(p, f, 1.0 / 5040);
-  p = fma(p, f, 1.0 / 720);
-  p = fma(p, f, 1.0 / 120);
-  p = fma(p, f, 1.0 / 24);
-  p = fma(p, f, 1.0 / 6);
+  p = step(p, f, 1.0 / 5040);
+  p = step(p, f, 1.0 / 720);
+  p = step(p, f, 1.0 / 120);
+  p = step(p, f, 1.0 / 24);
+  p = step(p, f, 1.0 / 6);
   p = fma(p, f, 0.5);
   p = fma(p, f, 1.0);
   p = fma(p, f, 1.0);
@@ -432,11 +438,11 @@ template <typename F> void AllowLds(F* kernel, size_t bytes) {
  * names the class (with the sign bit set, kNone: none), then that slot's probability.
  * Everything is held as wide as the scores' statistics, 64 bits for float64 scores, whose 32-bit
  * gradients are then off by hardly more than their own rounding; in 32 bits they were off by five
- * times as much (1.3e-7 of the largest), in 82 us where this takes 101. kLoss: whether the loss is
+ * times as much (2.8e-7 of the largest), in 82 us where this takes 96. kLoss: whether the loss is
  * among what may be asked for. Of float64 scores it has a launch of its own, as it needs the
  * exponentials in all of 64 bits, which cost a gradient 123 us. Bound by the arithmetic of 64 bits
- * beside memory: two million rows of seven float64 classes with labels, weights and hessians 101
- * us, 3.0 TB/s of what has to move.
+ * beside memory: two million rows of seven float64 classes with labels, weights and hessians 96
+ * us, 3.2 TB/s of what has to move.
  */
 template <typename T, bool kLoss, int E, TeamKind kKind>
 __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double by, int lanes) {
@@ -556,6 +562,21 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
   const bool taught = teach && !(t_sum == S(0));
   const S t_inv = taught ? S(1) / t_sum : S(0);
   const S share = u_rest * t_inv;
+  // the table's slots give way to their probabilities; every class has one such slot. Where the
+  // loss is taken from them too, that is where the student's sums are known.
+  auto put_slots = [&](auto&& f) {
+    team.Sync();
+    for_slots([&](int cls, double t, W* at) {
+      const S log_u = teacher.template Slot<S>(t);
+      const S p = taught ? exp2_of(log_u) * t_inv : S(0);
+      f(cls, p, log_u);
+      *at = ToBits(p) & ~kSlot;
+    });
+  };
+  if constexpr (!kLoss) {
+    put_slots([](int, S, S) {});
+    team.Sync();
+  }
 
   // the student's: the classes without a slot are summed on their own
   const bool two = hard_term && scale != scale1;
@@ -599,35 +620,33 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
   const bool live = w != S(0) && !(total == S(0));  // otherwise every class is masked
   const int y = live ? label : -1;
 
-  // the table's slots give way to their probabilities; every class has one such slot
-  double kl = 0;
-  const S log_both = kLoss ? Log2(total) - Log2(t_sum) : S(0);
-  team.Sync();
-  for_slots([&](int cls, double t, W* at) {
-    const S log_u = teacher.template Slot<S>(t);
-    const S p = taught ? exp2_of(log_u) * t_inv : S(0);
-    if (kLoss && a.loss.data && !(p == S(0)))
-      kl += Divergence(p, log_u + log_both, static_cast<double>(score(cls)) - high, a.temperature);
-    *at = ToBits(p) & ~kSlot;
-  });
-  if (kLoss && a.loss.data) {
-    kl = team.Sum(kl, red_top);
-    if (there && team.l == 0) {
-      double v = 0;
-      if (live) {
-        if (rest && !(share == S(0)))
-          kl += Divergence(share, log_u_rest - Log2(left) + log_both,
-                           static_cast<double>(rest_high) - high, a.temperature);
-        if (taught) v = a.alpha * a.temperature * a.temperature * kl;
-        if (y >= 0)
-          v += (1.0 - a.alpha) * (Log2(total1) * kLn2 - (static_cast<double>(score(y)) - high));
-        v *= w;
+  if constexpr (kLoss) {
+    double kl = 0;
+    const S log_both = Log2(total) - Log2(t_sum);
+    put_slots([&](int cls, S p, S log_u) {
+      if (a.loss.data && !(p == S(0)))
+        kl += Divergence(p, log_u + log_both, static_cast<double>(score(cls)) - high,
+                         a.temperature);
+    });
+    if (a.loss.data) {
+      kl = team.Sum(kl, red_top);
+      if (there && team.l == 0) {
+        double v = 0;
+        if (live) {
+          if (rest && !(share == S(0)))
+            kl += Divergence(share, log_u_rest - Log2(left) + log_both,
+                             static_cast<double>(rest_high) - high, a.temperature);
+          if (taught) v = a.alpha * a.temperature * a.temperature * kl;
+          if (y >= 0)
+            v += (1.0 - a.alpha) * (Log2(total1) * kLn2 - (static_cast<double>(score(y)) - high));
+          v *= w;
+        }
+        StoreFloat(a.loss, at_row(a.loss), v);
       }
-      StoreFloat(a.loss, at_row(a.loss), v);
     }
+    team.Sync();
   }
   if (!a.gradient.data && !a.hessian.data) return;
-  team.Sync();
   const S soft = taught ? alpha : S(0), hard = y >= 0 ? static_cast<S>(1.0 - a.alpha) : S(0);
   const S inv = S(1) / total, inv1 = hard > S(0) ? S(1) / total1 : S(0);
   const S spread = rest && left > S(0) ? share / left : S(0);
