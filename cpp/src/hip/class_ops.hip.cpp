@@ -1000,17 +1000,22 @@ k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
   }
 
   if (a.loss.data) {
-    double kl[1] = {0.0};
-    if (cls >= 0 && !(p == A(0)))
-      kl[0] = Divergence(p, log_u - t_log + log_total, static_cast<double>(z_slot) - high,
-                         a.temperature);
+    double kl = 0;
+    if (tid - tid % kWave < k) {  // the waves with slots
+      if (cls >= 0 && !(p == A(0)))
+        kl = Divergence(p, log_u - t_log + log_total, static_cast<double>(z_slot) - high,
+                        a.temperature);
+      kl = WaveSum(kl);
+    }
+    if (tid % kWave == 0) s_top[tid / kWave] = kl;
     __syncthreads();
-    BlockSums<kBlock>(kl, s_top);
     if (tid == 0) {
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) kl += s_top[i];
       if (rest && !(share == A(0)))
-        kl[0] += Divergence(share, log_u_rest - t_log - Log2(left) + log_total,
-                            static_cast<double>(rest_high) - high, a.temperature);
-      double v = taught ? a.alpha * a.temperature * a.temperature * kl[0] : 0.0;
+        kl += Divergence(share, log_u_rest - t_log - Log2(left) + log_total,
+                         static_cast<double>(rest_high) - high, a.temperature);
+      double v = taught ? a.alpha * a.temperature * a.temperature * kl : 0.0;
       if (label >= 0)
         v += (1.0 - a.alpha) * (Log2(total1) * kLn2 - (static_cast<double>(z_label) - high));
       StoreFloat(a.loss, row * a.loss.stride[0], v * w);

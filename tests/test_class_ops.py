@@ -1421,3 +1421,84 @@ def test_distill_alpha_next_to_one(place, classes, less):
             loss = (1.0 - alpha) * -np.log(q[hit])
             assert np.all(np.abs(_get(got.loss) - loss) <= 3 * _rel(classes, dtype) * (
                 (1.0 - alpha) * (2 + np.abs(np.log(q[hit])))) + HALF_STEP["f32"] * loss)
+
+
+# ------------------------------------------------------------------ rows that registers do not hold
+# 81920 float32 or 163840 16-bit classes stand in a workgroup of 1024 threads, half of them in one
+# of 512; what is beyond is read again in each pass.
+LARGE = [(90001, "f32"), (200003, "f32"), (200003, "f16"), (200003, "bf16")]
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes,dtype", LARGE)
+def test_distill_large_rows_masked(place, classes, dtype):
+    """Masks, NaN and infinities, a rest that underflows, in what is held and in what is read again."""
+    if place == "numpy" and dtype == "bf16":
+        pytest.skip("numpy has no bfloat16")
+    rng = np.random.default_rng(classes)
+    rows = 10
+    ids, logits, rest = _teacher(rng, rows, classes, 9, True)
+    labels = rng.integers(0, classes, rows)
+    z = 2 * rng.standard_normal((rows, classes))
+    z[0, rng.random(classes) < 0.3] = -INF
+    z[1, :classes - 100] = -INF            # only the end is there
+    z[2, 100:] = -INF                      # only the beginning
+    z[3] = -INF
+    z[4, classes // 2:] = -INF
+    np.put_along_axis(z, ids, 1.0, axis=1)
+    z[3] = -INF
+    z[np.arange(rows), labels] = np.where(np.arange(rows) == 3, -INF, 1.0)
+    z[5], z[6] = z[5] - 300.0, z[6] - 300.0
+    z[5, ids[5, 0]] = 0.0                  # the others underflow
+    z[6, ids[6, 0]] = 100.0
+    z[7, classes - 1] = np.nan
+    z[8, classes - 2] = INF
+    z[9, 3] = np.nan
+    labels[7:] = -1
+    clean = np.arange(rows) < 7
+    for t, alpha in ((1.0, 1.0), (2.0, 0.5)):
+        teacher = ids, logits, rest
+        _distill_case(place, z[clean], tuple(x[clean] for x in teacher), dtype,
+                      labels=labels[clean], t=t, alpha=alpha)
+        got = ops.distill_gradients(_put(place, z, dtype), (
+            _put(place, ids, "i32"), _put(place, logits, "f32"), _put(place, rest, "f32")),
+            labels=_put(place, labels, "i32"), temperature=t, alpha=alpha, loss=True, hessian=True)
+        bad = np.isnan(_get(got.loss))
+        np.testing.assert_array_equal(bad, ~clean)
+        for x in (_get(got.gradient), _get(got.hessian)):
+            assert np.all(np.isnan(x[7:])) and np.all(np.isfinite(x[:7]))
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes,dtype", LARGE)
+def test_top_logits_large_rows(place, classes, dtype):
+    """Ties, masks and NaN, scores that stand out at the row's ends, and a rest that underflows."""
+    if place == "numpy" and dtype == "bf16":
+        pytest.skip("numpy has no bfloat16")
+    rng = np.random.default_rng(classes)
+    x = rng.standard_normal((9, classes))
+    x[0] = 1.5
+    x[1] = rng.integers(0, 3, classes)
+    x[2, :classes - 30] = -INF
+    x[3, 30:] = np.nan
+    x[4, rng.random(classes) < 0.5] = -INF
+    x[5] = np.arange(classes) // 4096
+    x[6, -3:], x[6, :3] = 200.0, 200.0
+    x[7, classes - 5] = INF
+    x[8] = np.where(np.arange(classes) % 2, 0.0, -0.0)
+    for k in (1, 40, 256):
+        _top_case(place, x, dtype, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,dtype", [
+    (1100, 2500, "f32"), (1100, 7001, "f32"), (600, 9001, "bf16"), (600, 20011, "f16"),
+    (520, 24001, "f32"), (520, 60001, "f16"), (600, 3000, "bf16")])
+def test_hessians_of_many_rows(rows, classes, dtype):
+    """The shapes that only many rows take, against the plain form."""
+    rng = np.random.default_rng(classes)
+    teacher = _teacher(rng, 3, classes, 20, True)
+    z = 3 * rng.standard_normal((3, classes))
+    labels = rng.integers(0, classes, 3)
+    for t, alpha in ((2.0, 0.5), (1.0, 1.0)):
+        _gradient_case("gpu", z, teacher, dtype, labels=labels, t=t, alpha=alpha, rows=rows)
