@@ -302,10 +302,13 @@ class DistillLossMetric : public Metric {
   }
   const std::vector<std::string>& GetName() const override { return names_; }
   double factor_to_bigger_better() const override { return 1.0; }
-  std::vector<double> Eval(const double* score, const ObjectiveFunction*) const override {
+  std::vector<double> Eval(const double* score, const ObjectiveFunction* objective) const override {
     std::vector<double> loss(num_data_);
+    // beside the distill objective its loss, whatever has been set since
+    double temperature = temperature_, alpha = alpha_;
+    if (objective != nullptr) objective->DistillTerms(&temperature, &alpha);
     LGBM_DistillArgs a =
-        class_ops::DistillArgsOf(*meta_, num_data_, nc_, temperature_, alpha_, score);
+        class_ops::DistillArgsOf(*meta_, num_data_, nc_, temperature, alpha, score);
     a.loss = class_ops::ArrayOf(loss.data(), C_API_DTYPE_FLOAT64, 1);
     class_ops::Distill(a, -1, nullptr);
     double sum = 0;

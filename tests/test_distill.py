@@ -406,3 +406,19 @@ def test_starts_at_the_mean_of_the_teacher_at_its_temperature():
         want[i] = np.exp(top.log_rest[i] - norm) / 3
         want[i, top.classes[i]] = np.exp(top.logits[i] / 4.0 - norm)
     np.testing.assert_allclose(np.exp(b / 4) / np.exp(b / 4).sum(), want.mean(0), rtol=1e-6)
+
+
+def test_a_later_metric_is_of_the_same_loss():
+    """A validation set added after the parameters have been reset is evaluated as the others."""
+    X, raw, y = _data()
+    top = ops.top_logits(raw, 3, temperature=2.0)
+    train = lgb.Dataset(X, label=y, teacher=top)
+    live = lgb.Booster(_params("cpu", distill_temperature=2.0, distill_alpha=0.9), train)
+    first = train.create_valid(X, label=y, teacher=top)
+    live.add_valid(first, "first")
+    live.update()
+    live.reset_parameter({"distill_alpha": 0.1, "distill_temperature": 5.0})
+    live.add_valid(train.create_valid(X, label=y, teacher=top), "second")
+    live.update()
+    found = {name: value for name, _, value, _ in live.eval_valid()}
+    assert found["first"] == found["second"]
