@@ -220,8 +220,8 @@ __device__ __forceinline__ double Divergence(double p, double log_pq, double far
  * The slots' classes are bits in LDS, so that the sum over the others is taken directly and
  * not as a difference, which a confident student would cancel to nothing. The first slot of
  * a class counts. It serves what the kernels below do not: more than 512 classes of float64 or
- * in strides. Bound by its three passes over memory, one element a thread (8192 x 32768
- * bfloat16 gradients 785 us, where the rows' kernel takes 224).
+ * in strides. Bound by its three passes over memory, one element a thread (8192 x 32768 bfloat16
+ * gradients and loss of every second column 1039 us; of neighbours, by the rows' kernel, 233).
  */
 template <typename T, int kBlock>
 __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, double by) {
@@ -816,10 +816,10 @@ __device__ __forceinline__ void BlockSums(A (&v)[kCount], A* lds) {
  * maximum, the sums and the gradients from there. Every thread writes its classes as if they
  * had no slot; after a barrier the slots' threads write theirs over that, which leaves the
  * write pass without a test. Bound by memory where the row fits (8192 x 32768 bfloat16 with
- * the loss 224 us, 4.8 TB/s; the loss alone of 2048 x 32768 float32 49 us, 5.5 TB/s), by two
- * exponentials a score where labels have a temperature of their own (3001 x 20011 float16 40
- * us, 3.0 TB/s), by reading a third of the row twice where it does not fit (501 x 131077
- * float32 146 us, 3.6 TB/s).
+ * the loss 227 us, 4.7 TB/s; the loss alone of 2048 x 32768 float32 49 us, 5.5 TB/s), by
+ * arithmetic that does not overlap the loads where labels have a temperature of their own (3001 x
+ * 20011 float16 42 us, 2.9 TB/s, the vector units busy for 61% of it), by reading a third of the
+ * row twice where it does not fit (501 x 131077 float32 142 us, 3.7 TB/s).
  */
 template <typename T, typename Shape, bool kHessian>
 __global__ void __launch_bounds__(Shape::block, Shape::cached >= 12 ? 4 : 1)
@@ -1126,8 +1126,8 @@ __device__ __forceinline__ void PickDigit(const int* hist, int take, int* digit,
  * One workgroup a row, in any strides and with any ties: the k-th largest key is found
  * digit by digit (eight bits a pass, counted in LDS), its equals are cut by class the same
  * way, and what is chosen is put in order by counting how many precede it. Eight to fourteen
- * passes over memory: 4096 x 50021 bfloat16, k = 64, 1727 us, where the rows' kernel takes
- * 131; rows of many equal scores and float64 rows of more than 512 classes come here.
+ * passes over memory: 4096 x 50021 bfloat16, k = 64, of every second column 2507 us; of
+ * neighbours, by the rows' kernel, 129. Rows of many equal scores and float64 rows of more than 512 classes come here.
  */
 template <typename T, int kBlock>
 __device__ __forceinline__ void TopAny(const LGBM_TopLogitsArgs& a, int64_t row) {
@@ -1253,8 +1253,8 @@ __global__ void __launch_bounds__(kBlock) k_top_any(LGBM_TopLogitsArgs a) {
 /*!
  * Up to E * L classes, in the registers of their row's threads (Team): k times the largest
  * that is left, by comparison with all others. Of equals the lowest class is met first. Bound
- * by memory for small k (1000000 x 10 float64, k = 4, 35 us, 3.8 TB/s), by the comparisons
- * for larger (200000 x 100 float32, k = 10, 100 us).
+ * by memory for small k (1000000 x 10 float64, k = 4, 34 us, 3.9 TB/s), by the comparisons
+ * for larger (400000 x 100 float32, k = 10, 144 us, the vector units busy throughout).
  */
 template <typename T, int E, TeamKind kKind>
 __global__ void __launch_bounds__(256) k_top_tile(LGBM_TopLogitsArgs a, int lanes) {
@@ -1353,9 +1353,9 @@ constexpr int kTurnedRows = 16;
  * over the keys between the row's smallest and largest. A step compares what each lane holds
  * with the middle and counts the lanes' answers, without a word between lanes; it ends as
  * soon as the count is k. No wave waits for another. kTurned: the rows of a class stand next
- * to each other, so a workgroup turns sixteen rows in LDS first. Bound by the scalar work of
- * some twenty steps and the ranking (300000 x 250 bfloat16, k = 50, 422 us; k rounds of the
- * largest that is left took 3024).
+ * to each other, so a workgroup turns sixteen rows in LDS first. Bound by the vector work of
+ * some twenty steps and the ranking (300000 x 250 bfloat16, k = 50, 405 us, the vector units busy
+ * throughout; k rounds of the largest that is left took 3024).
  */
 template <typename T, int E, bool kTurned>
 __global__ void __launch_bounds__(256) k_top_wave(LGBM_TopLogitsArgs a) {
@@ -1525,7 +1525,7 @@ constexpr int kTopChunks = 512;       // that hold them
  * pass over the registers picks the scores that reach it (candidates) and sums the
  * exponentials of the others; the candidates are put in order by counting. Rows with more
  * candidates than fit, of many equal scores for instance, are done digit by digit (TopAny).
- * 4096 x 50021 bfloat16, k = 64: 131 us, of which reading and the maxima alone are 84 (4.9
+ * 4096 x 50021 bfloat16, k = 64: 126 us, of which reading and the maxima alone are 84 (4.9
  * TB/s), the second pass 17 and the ranking the rest, as the two rows that a compute unit
  * holds do not hide it.
  */
@@ -2053,7 +2053,7 @@ __device__ __forceinline__ double WaveMass(const Residual<T>& f, int begin, int 
  * Each wave of `splits` workgroups a sequence sums one segment of the row that the class is
  * drawn from. Which row that is, every workgroup finds for itself: a few gathers, instead of
  * a launch before this one. The first of them writes what is known already. Bound by memory
- * for a batch (256 x 50021 bfloat16, both sides, 14 us, 3.6 TB/s), by latency for one sequence
+ * for a batch (256 x 50021 bfloat16, both sides, 15 us, 3.4 TB/s), by latency for one sequence
  * (131072 float32 classes over 64 workgroups 4.4 us; one workgroup for all 230).
  */
 template <typename T>

@@ -1,15 +1,15 @@
 """Operators over class scores against plain 64-bit numpy, on the host and on the GPU.
 
-Tolerances. The device takes exponentials of z * s - high * s with s = log2(e) / T in 32 bits
+Tolerances. The device takes exponentials of (z - high) * s with s = log2(e) / T in 32 bits
 (64 for float64 scores), eps = 2^-24 (2^-53) being half a step. One term of a softmax with
-exponent x (base two) is off by at most eps * (2 |x| + 4) of itself: the rounding of s, that of
-the fused product, and one step of the exponential; as 2^-x (2 |x| + 4) <= 4.2, that is below
-8 eps of the row's largest term, and below (2 * 64 + 4) eps of the term for every term above
-2^-64. The rounding of high * s is common to the row. A sum of n terms adds at most one
-rounding for each addition along its longest chain: n / 64 + 32 (a lane's own terms, then the
-tree). `_rel` is the sum of these; a result's own rounding to its type is added where it is
-compared. The 32-bit gradients of float64 scores are allowed the 32-bit terms: the device forms
-their exponents in 64 bits and takes the exponentials in 32.
+exponent x (base two) is off by at most eps * (3 |x| + 4) of itself: the roundings of s, of the
+difference and of the product, and one step of the exponential; as 2^-x (3 |x| + 4) <= 5.7, that
+is below 8 eps of the row's largest term, and below (2 * 64 + 4) eps of the term for every term
+above 2^-42; of up to 2^20 classes, what is smaller adds up to 2^-22. A sum of n terms adds at
+most one rounding for each addition along its longest chain: n / 64 + 32 (a lane's own terms,
+then the tree). `_rel` is the sum of these; a result's own rounding to
+its type is added where it is compared. The 32-bit gradients of float64 scores are allowed the
+32-bit terms: the device computes them in 64 and needs less.
 """
 import math
 import subprocess
