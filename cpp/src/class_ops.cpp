@@ -143,14 +143,31 @@ void CheckTemperature(double t) {
   if (!(t >= 1e-6 && t <= 1e6)) Log::Fatal("temperature must be in 1e-6..1e6, got %g", t);
 }
 
+/*! the threads of a call, and what each of them works in: made before they start, as memory that
+ *  is not there ends a process that asks for it among them. kApart more elements than are used
+ *  keep two threads' arrays, which stand next to each other, out of one line. */
+constexpr int kApart = 32;
+template <typename Scratch> std::vector<Scratch> ScratchOf(int64_t rows, const Scratch& one) {
+  return std::vector<Scratch>(
+      static_cast<size_t>(std::min<int64_t>(rows, omp_get_max_threads())), one);
+}
+
 // ------------------------------------------------------------------ host: top logits
+struct TopScratch {
+  std::vector<double> x, left;
+  std::vector<int> order;
+};
+
 void TopLogitsHost(const LGBM_TopLogitsArgs& a) {
   const int c = a.classes, k = a.k;
-#pragma omp parallel
+  auto scratch = ScratchOf(a.rows, TopScratch{std::vector<double>(c + kApart),
+                                              std::vector<double>(c + kApart),
+                                              std::vector<int>(c + kApart)});
+#pragma omp parallel num_threads(static_cast<int>(scratch.size()))
   {
-    std::vector<double> x(c);
-    std::vector<int> order(c);
-    std::vector<double> left;
+    TopScratch& own = scratch[omp_get_thread_num()];
+    double *const x = own.x.data(), *const left = own.left.data();
+    int* const order = own.order.data();
 #pragma omp for schedule(static)
     for (int64_t i = 0; i < a.rows; ++i) {
       const int64_t row = i * a.scores.stride[0];
@@ -160,7 +177,7 @@ void TopLogitsHost(const LGBM_TopLogitsArgs& a) {
         if (x[j] > -kInf) order[n++] = j;  // neither -inf nor NaN
       }
       const int got = std::min(n, k);
-      std::partial_sort(order.begin(), order.begin() + got, order.begin() + n,
+      std::partial_sort(order, order + got, order + n,
                         [&](int p, int q) { return x[p] > x[q] || (x[p] == x[q] && p < q); });
       for (int j = 0; j < k; ++j) {
         const int64_t at = i * a.top_class.stride[0] + j * a.top_class.stride[1];
@@ -170,24 +187,34 @@ void TopLogitsHost(const LGBM_TopLogitsArgs& a) {
         else StoreFloat(a.top_logit, al, -kInf);
       }
       if (a.log_rest.data != nullptr) {
-        left.clear();
-        for (int j = got; j < n; ++j) left.push_back(x[order[j]] / a.temperature);
-        StoreFloat(a.log_rest, i * a.log_rest.stride[0], LogSumExp(left.data(), left.size()));
+        for (int j = got; j < n; ++j) left[j - got] = x[order[j]] / a.temperature;
+        StoreFloat(a.log_rest, i * a.log_rest.stride[0], LogSumExp(left, n - got));
       }
     }
   }
 }
 
 // ------------------------------------------------------------------ host: distillation
+struct DistillScratch {
+  std::vector<double> z, e, e1, log_p, p;
+  std::vector<int> slot, cls;
+};
+
 void DistillHost(const LGBM_DistillArgs& a) {
   const int c = a.classes, k = a.k;
   const double t = a.temperature, alpha = a.alpha;
   const double factor = c > 1 ? static_cast<double>(c) / (c - 1) : 1.0;
   const bool rest = a.teacher_rest.data != nullptr;
-#pragma omp parallel
+  const std::vector<double> wide(c + kApart), few(k + 1 + kApart);
+  auto scratch = ScratchOf(a.rows, DistillScratch{wide, wide, wide, few, few,
+                                                  std::vector<int>(c + kApart, -1),
+                                                  std::vector<int>(k + kApart)});
+#pragma omp parallel num_threads(static_cast<int>(scratch.size()))
   {
-    std::vector<double> z(c), e(c), e1(c), log_p(k + 1), p(k);
-    std::vector<int> slot(c, -1), cls(k);
+    DistillScratch& mine = scratch[omp_get_thread_num()];
+    double *const z = mine.z.data(), *const e = mine.e.data(), *const e1 = mine.e1.data();
+    double *const log_p = mine.log_p.data(), *const p = mine.p.data();
+    int *const slot = mine.slot.data(), *const cls = mine.cls.data();
 #pragma omp for schedule(static)
     for (int64_t i = 0; i < a.rows; ++i) {
       const double w = a.weight.data ? LoadFloat(a.weight, i * a.weight.stride[0]) : 1.0;
@@ -239,7 +266,7 @@ void DistillHost(const LGBM_DistillArgs& a) {
       const double r_read = rest ? LoadFloat(a.teacher_rest, i * a.teacher_rest.stride[0]) : -kInf;
       const double r = r_read == -kInf || !some ? r_read : r_read - top / t;
       log_p[n] = r;
-      const double norm = LogSumExp(log_p.data(), n + 1);
+      const double norm = LogSumExp(log_p, n + 1);
       bool nan = std::isnan(r) || norm == kInf;  // of infinite weights none is a share
       for (int j = 0; j < n; ++j) nan |= std::isnan(log_p[j]);
       const double lse = nan ? std::nan("") : norm;
@@ -305,14 +332,14 @@ void DistillHost(const LGBM_DistillArgs& a) {
 /*! what counts as probability: NaN, infinities and negative values are none */
 double Mass(double v) { return v > 0 && v <= DBL_MAX ? v : 0.0; }
 
-int DrawClass(const std::vector<double>& mass, double total, double v) {
+int DrawClass(const double* mass, int classes, double total, double v) {
   const double goal = v * total;
   double reach = 0;
   int last = -1;
-  for (size_t j = 0; j < mass.size(); ++j) {
+  for (int j = 0; j < classes; ++j) {
     if (mass[j] <= 0) continue;
     reach += mass[j];
-    last = static_cast<int>(j);
+    last = j;
     if (reach > goal) break;
   }
   return last;
@@ -320,9 +347,10 @@ int DrawClass(const std::vector<double>& mass, double total, double v) {
 
 void VerifyHost(const LGBM_VerifyArgs& a) {
   const int c = a.classes, t = a.drafts;
-#pragma omp parallel
+  auto scratch = ScratchOf(a.rows, std::vector<double>(c + kApart));
+#pragma omp parallel num_threads(static_cast<int>(scratch.size()))
   {
-    std::vector<double> mass(c);
+    double* const mass = scratch[omp_get_thread_num()].data();
 #pragma omp for schedule(static)
     for (int64_t i = 0; i < a.rows; ++i) {
       auto p = [&](int s, int64_t j) {
@@ -369,7 +397,7 @@ void VerifyHost(const LGBM_VerifyArgs& a) {
       if (total == 0) {
         for (int j = 0; j < c; ++j) total += mass[j] = p(s, j);
       }
-      out(s) = DrawClass(mass, total, LoadFloat(a.sample, i * a.sample.stride[0]));
+      out(s) = DrawClass(mass, c, total, LoadFloat(a.sample, i * a.sample.stride[0]));
       for (int j = s + 1; j <= t; ++j) out(j) = -1;
     }
   }

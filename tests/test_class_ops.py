@@ -1502,3 +1502,24 @@ def test_hessians_of_many_rows(rows, classes, dtype):
     labels = rng.integers(0, classes, 3)
     for t, alpha in ((2.0, 0.5), (1.0, 1.0)):
         _gradient_case("gpu", z, teacher, dtype, labels=labels, t=t, alpha=alpha, rows=rows)
+
+
+@pytest.mark.parametrize("call", [
+    "ops.top_logits(z, 1)",
+    "ops.distill_loss(z, (ids, f(64, 1)))",
+    "ops.verify_drafts(f(64, 2, 1 << 20), ids, None, f(64, 1), f(64))"])
+def test_host_memory_that_is_not_there(call):
+    """Scratch of a call that does not fit is a LightGBMError, not the end of the process."""
+    code = (
+        "import resource, numpy as np, lightgbm_amd as lgb\n"
+        "from lightgbm_amd import ops\n"
+        "f = lambda *s: np.broadcast_to(np.float32(0.5), s)\n"
+        "ids, z = np.zeros((64, 1), np.int32), f(64, 1 << 20)\n"
+        "ops.distill_loss(f(64, 4), (ids, f(64, 1)))  # the threads are there\n"
+        "size = int(open('/proc/self/statm').read().split()[0]) * 4096\n"
+        "resource.setrlimit(resource.RLIMIT_AS, (size + (6 << 20),) * 2)\n"
+        f"try:\n    {call}\nexcept lgb.LightGBMError:\n    print('refused')\n")
+    root = Path(__file__).resolve().parent.parent
+    got = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=100)
+    assert got.returncode == 0 and "refused" in got.stdout, got.stderr[-2000:]
