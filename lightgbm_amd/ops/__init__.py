@@ -88,19 +88,20 @@ _forward = None  # torch.autograd.forward_ad; its level is -1 where no tangents 
 def _is_tensor(x):
     global _torch, _Tensor, _raw_stream, _forward
     if _torch is None:
-        _torch = sys.modules.get("torch")
-        if _torch is None:
+        torch = sys.modules.get("torch")
+        if torch is None:
             return False
-        _Tensor = _torch.Tensor
-        _forward = _torch.autograd.forward_ad
         for code, name in ((_F32, "float32"), (_F64, "float64"), (_I32, "int32"),
                            (_I64, "int64"), (_F16, "float16"), (_BF16, "bfloat16")):
-            _TORCH_TYPES[getattr(_torch, name)] = code
-            _TORCH_OF[code] = getattr(_torch, name)
+            _TORCH_TYPES[getattr(torch, name)] = code
+            _TORCH_OF[code] = getattr(torch, name)
         # the current stream of a device as a pointer, where torch has it without an object
-        _raw_stream = getattr(_torch._C, "_cuda_getCurrentRawStream", None) or (
-            lambda index: _torch.cuda.current_stream(index).cuda_stream)
-    return isinstance(x, _Tensor)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+        _forward = torch.autograd.forward_ad
+        _torch = torch
+        _Tensor = torch.Tensor  # last, as another thread's call looks at it first
+    return isinstance(x, _torch.Tensor)
 
 
 class _Place:
@@ -112,7 +113,7 @@ class _Place:
         self.made = []  # arrays that stand for other objects, alive as long as the call
         self.device = -1
         self.on = None
-        self.tensor = isinstance(x, _Tensor)  # _shaped has seen it
+        self.tensor = isinstance(x, _Tensor) or _is_tensor(x)
         if self.tensor:
             self.on = x.device
             if x.is_cuda:

@@ -1229,8 +1229,8 @@ def test_distill_large_rows_with_an_offset(place, classes, dtype, offset):
     """Rows of which a part is read again: what is held and what is not have sums of their own. A
     term that matters, 2^-x with x below 64, is off by (3 * 64 + 4) eps, a sum of a thread's 200
     terms in chunks and the tree by 64 more; a quotient has two of them."""
-    if place == "numpy" and dtype == "bf16":
-        pytest.skip("numpy has no bfloat16")
+    if place != "gpu" and classes > 100000:
+        pytest.skip("of the device's shapes; the host has one way")
     rng = np.random.default_rng(classes)
     teacher = _teacher(rng, 3, classes, 20, True)
     z = 3 * rng.standard_normal((3, classes)) + offset
@@ -1368,6 +1368,8 @@ def test_distill_loss_of_the_lowest(place, classes):
 def test_top_logits_masked_by_the_lowest(place, classes):
     """Masks of the type's lowest value are scores: they are chosen after all others, and what is
     not chosen of them has a logarithm of their size. Exactly k others, fewer, none, one more."""
+    if place != "gpu" and classes > 50000:
+        pytest.skip("of the device's shapes; the host has one way")
     rng = np.random.default_rng(classes)
     k = 5
     for dtype in _types(place):
@@ -1385,6 +1387,8 @@ def test_top_logits_masked_by_the_lowest(place, classes):
 def test_top_logits_of_small_temperature(place, classes):
     """Large scores over a small temperature, and scores with a large offset: the rest's logarithm
     is that of a size, with the same few roundings."""
+    if place != "gpu" and classes > 50000:
+        pytest.skip("of the device's shapes; the host has one way")
     rng = np.random.default_rng(classes)
     for dtype in _types(place):
         x = rng.standard_normal((3, classes))
@@ -1433,8 +1437,8 @@ LARGE = [(90001, "f32"), (200003, "f32"), (200003, "f16"), (200003, "bf16")]
 @pytest.mark.parametrize("classes,dtype", LARGE)
 def test_distill_large_rows_masked(place, classes, dtype):
     """Masks, NaN and infinities, a rest that underflows, in what is held and in what is read again."""
-    if place == "numpy" and dtype == "bf16":
-        pytest.skip("numpy has no bfloat16")
+    if place != "gpu" and classes > 100000:
+        pytest.skip("of the device's shapes; the host has one way")
     rng = np.random.default_rng(classes)
     rows = 10
     ids, logits, rest = _teacher(rng, rows, classes, 9, True)
@@ -1473,8 +1477,8 @@ def test_distill_large_rows_masked(place, classes, dtype):
 @pytest.mark.parametrize("classes,dtype", LARGE)
 def test_top_logits_large_rows(place, classes, dtype):
     """Ties, masks and NaN, scores that stand out at the row's ends, and a rest that underflows."""
-    if place == "numpy" and dtype == "bf16":
-        pytest.skip("numpy has no bfloat16")
+    if place != "gpu" and classes > 100000:
+        pytest.skip("of the device's shapes; the host has one way")
     rng = np.random.default_rng(classes)
     x = rng.standard_normal((9, classes))
     x[0] = 1.5
@@ -1523,3 +1527,105 @@ def test_host_memory_that_is_not_there(call):
     got = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
                          timeout=100)
     assert got.returncode == 0 and "refused" in got.stdout, got.stderr[-2000:]
+
+
+def test_first_calls_at_once(monkeypatch):
+    """A call of another thread, while the first one looks torch up, finds all of it or looks it up
+    itself."""
+    z = torch.arange(6.0).reshape(2, 3)
+    want = ops.top_logits(z, 2)
+
+    class Types(dict):
+        def __setitem__(self, key, value):
+            super().__setitem__(key, value)
+            if not seen:
+                seen.append(0)
+                _same(ops.top_logits(z, 2), want)
+
+    seen = []
+    for name, value in (("_torch", None), ("_Tensor", ()), ("_raw_stream", None),
+                        ("_forward", None), ("_TORCH_TYPES", Types()), ("_TORCH_OF", {})):
+        monkeypatch.setattr(ops, name, value)
+    _same(ops.top_logits(z, 2), want)
+    assert seen
+
+
+# ------------------------------------------------------------------ the largest sizes
+MOST = 1 << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f64", "f32", "f16", "bf16"])
+@pytest.mark.parametrize("step", [1, 2])
+def test_most_classes(dtype, step):
+    """2^20 classes, next to each other and every second one; one row and as many as share units."""
+    rng = np.random.default_rng(MOST + step)
+    z = _round(3 * rng.standard_normal((2, MOST)), dtype)
+    wide = torch.zeros((2, MOST * step), dtype=TORCH[dtype], device="cuda")
+    x = wide[:, ::step]
+    x.copy_(_put("gpu", z, dtype))
+    for rows in (1, 2):
+        got = ops.top_logits(x[:rows], 100, temperature=2.0)
+        classes, logits, rest = _plain_top(z[:rows], 100, 2.0)
+        np.testing.assert_array_equal(_get(got.classes), classes)
+        np.testing.assert_array_equal(_get(got.logits), logits)
+        assert np.all(np.abs(_get(got.log_rest) - rest) <=
+                      _rel(MOST, dtype) * (1 + np.abs(rest)))
+    ids, logits, rest = _teacher(rng, 2, MOST, 256, True)
+    ids[1, 0] = MOST - 1
+    labels = np.array([MOST - 1, 0])
+    mix = {"labels": _put("gpu", labels, "i32"), "temperature": 2.0, "alpha": 0.5}
+    got = ops.distill_gradients(x, (_put("gpu", ids, "i32"), _put("gpu", logits, "f32"),
+                                    _put("gpu", rest, "f32")), hessian=True, loss=True, **mix)
+    grad, hess, size = _plain_gradient(z, ids, logits.astype(float), rest.astype(float), labels,
+                                       2.0, 0.5)
+    loss = _plain_loss(z, ids, logits.astype(float), rest.astype(float), labels, 2.0, 0.5)
+    out = "f32" if dtype == "f64" else dtype
+    rel = 3 * _rel(MOST, "f32")
+    for a, b in ((got.gradient, grad), (got.hessian, hess)):
+        far = 2 * rel * size + (1 + rel) * HALF_STEP[out] * np.abs(b) + TINY[out]
+        assert np.all(np.abs(_get(a) - b) <= far)
+    assert np.all(np.abs(_get(got.loss) - loss) <= 3 * _rel(MOST, dtype) * (20 + loss))
+    p = torch.softmax(x.double(), 1)[None]
+    drafts = torch.tensor([[MOST - 1]], device="cuda")
+    p[0, 0, MOST - 1] = 0.25
+    p = p.to(TORCH[dtype])
+    u, v = torch.zeros((1, 1), device="cuda"), torch.full((1,), 0.999, device="cuda")
+    for accept in (u, u + 0.999):
+        got = ops.verify_drafts(p, drafts, None, accept, v)
+        classes, accepted = _plain_verify(_get(p), _get(drafts), None, _get(accept), _get(v), None)
+        np.testing.assert_array_equal(_get(got.accepted), accepted)
+        # next to a border the order of the sums decides: the class's own sum is the check
+        mass = np.where(np.arange(MOST) == (MOST - 1 if not accepted[0] else -1), 0.0,
+                        _get(p)[0, accepted[0]])
+        reach, at = np.cumsum(mass), int(_get(got.classes)[0, accepted[0]])
+        goal, slack = float(_get(v)[0]) * reach[-1], MOST * HALF_STEP["f64"] * reach[-1]
+        assert mass[at] > 0 and reach[at] > goal - slack and reach[at] - mass[at] <= goal + slack
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("classes", [3, 64, 300, 2500])
+def test_most_drafts(place, classes):
+    """1024 drafts a sequence, refused nowhere, at the end, in the middle, at once."""
+    rng = np.random.default_rng(classes)
+    p = _softmax(rng.standard_normal((4, 1025, classes)))
+    drafts = p[:, :-1].argmax(-1)
+    u = np.zeros((4, 1024))
+    u[1, 1023] = u[2, 500] = u[3, 0] = 2.0
+    v = rng.random(4)
+    _verify_case(place, p, drafts, None, u, v, None, "f32")
+    _verify_case(place, p, drafts, p[:, :-1], u, v, np.array([1024, 1024, 700, 5]), "f64", "i64")
+
+
+@pytest.mark.parametrize("place", ["numpy", "torch"])
+def test_more_than_the_most_is_refused(place):
+    wide = np.broadcast_to(np.float32(1.0), (1, MOST + 1))
+    z = wide if place == "numpy" else torch.ones(1, 1).expand(1, MOST + 1)
+    teacher = _put(place, np.zeros((1, 1), np.int32)), _put(place, np.ones((1, 1), np.float32))
+    with pytest.raises(LightGBMError):
+        ops.top_logits(z, 1)
+    with pytest.raises(LightGBMError):
+        ops.distill_loss(z, teacher)
+    p = np.broadcast_to(np.float32(0.5), (1, 1026, 2))
+    with pytest.raises(LightGBMError):
+        ops.verify_drafts(p, np.zeros((1, 1025), np.int32), None, p[:, :-1, 0], p[:, 0, 0])
