@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(kBlock) k_distill_any(LGBM_DistillArgs a, doub
   const bool rest = a.teacher_rest.data != nullptr;
   const TeacherScale teacher(
       BlockMax<kBlock>(logit, s_top),
-      rest ? LoadFloat<double>(a.teacher_rest, row * a.teacher_rest.stride[0]) : NegInf<double>(), by);
+      rest ? LoadFloat<double>(a.teacher_rest, row * a.teacher_rest.stride[0]) : NegInf<double>(),
+      by);
 
   // sums
   const A z_slot = cls >= 0 ? static_cast<A>(z[cls * zs]) : NegInf<A>();
@@ -553,7 +554,8 @@ __global__ void __launch_bounds__(256) k_distill_tile(LGBM_DistillArgs a, double
   };
   double t_top = NegInf<double>();
   for_slots([&](int, double t, W*) { t_top = Max(t_top, t); });
-  const TeacherScale teacher(team.Max(t_top, red_top), rest && teach ? rest_read : NegInf<double>(), by);
+  const TeacherScale teacher(team.Max(t_top, red_top), rest && teach ? rest_read : NegInf<double>(),
+                             by);
   S t_sum = 0;
   for_slots([&](int, double t, W*) { t_sum += exp2_of(teacher.template Slot<S>(t)); });
   const S log_u_rest = teacher.template Rest<S>(), u_rest = exp2_of(log_u_rest);
@@ -952,7 +954,8 @@ k_distill_row(LGBM_DistillArgs a, double by, int lds_chunks) {
     t_own = cls >= 0 ? At<double>(a.teacher_logit, logit_at) : NegInf<double>();
     t_top = BlockMax<kBlock>(t_own, s_top);
   }
-  if (rest && a.teacher_rest.type == C_API_DTYPE_FLOAT64) t_rest = At<double>(a.teacher_rest, rest_at);
+  if (rest && a.teacher_rest.type == C_API_DTYPE_FLOAT64)
+    t_rest = At<double>(a.teacher_rest, rest_at);
   const TeacherScale teacher(t_top, t_rest, by);
   const A log_u = teacher.template Slot<A>(t_own), log_u_rest = teacher.template Rest<A>();
 
@@ -1127,7 +1130,8 @@ __device__ __forceinline__ void PickDigit(const int* hist, int take, int* digit,
  * digit by digit (eight bits a pass, counted in LDS), its equals are cut by class the same
  * way, and what is chosen is put in order by counting how many precede it. Eight to fourteen
  * passes over memory: 4096 x 50021 bfloat16, k = 64, of every second column 2507 us; of
- * neighbours, by the rows' kernel, 129. Rows of many equal scores and float64 rows of more than 512 classes come here.
+ * neighbours, by the rows' kernel, 129. Rows of many equal scores and float64 rows of more than
+ * 512 classes come here.
  */
 template <typename T, int kBlock>
 __device__ __forceinline__ void TopAny(const LGBM_TopLogitsArgs& a, int64_t row) {

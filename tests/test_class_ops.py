@@ -1436,7 +1436,7 @@ LARGE = [(90001, "f32"), (200003, "f32"), (200003, "f16"), (200003, "bf16")]
 @pytest.mark.parametrize("place", PLACES)
 @pytest.mark.parametrize("classes,dtype", LARGE)
 def test_distill_large_rows_masked(place, classes, dtype):
-    """Masks, NaN and infinities, a rest that underflows, in what is held and in what is read again."""
+    """Masks, NaN and infinities, a rest that underflows, in what is held and what is read again."""
     if place != "gpu" and classes > 100000:
         pytest.skip("of the device's shapes; the host has one way")
     rng = np.random.default_rng(classes)
